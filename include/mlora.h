@@ -325,6 +325,33 @@ int mlora_embed(void* out, int out_dtype, const void* table, const int32_t* ids,
  * Replaces: the host-side np.argmax over D2H-copied logits (tvm/llama_auto_batcher/llama_exec_graph.py:92,134-137). */
 int mlora_argmax(int32_t* ids, const float* logits, int B, int V, void* stream);
 
+/* The greedy token of every row under its request's rules.  With c[v] the times token v was generated and seen[v] whether it stands
+ * in the row's prompt or was generated,
+ *     z'[v] = (seen[v] ? (z > 0 ? z / repetition : z * repetition) : z) - (frequency * c[v] + presence * [c[v] > 0]) + the sum of the row's biases of v
+ *     z'[v] = -inf where the row has a mask without the bit of v;     ids[b] = lowest index of the maximum of z', -1 where no token is above -inf
+ * Every step is rounded to fp32 in this order.  NaN is never the maximum.  out (or NULL; may be `logits` itself): z', rows of ld_out.
+ * history [B, cap] int32 holds a row's prompt and generated tokens, lengths [B] of them in use, from gen_start [B] on (NULL: all)
+ * the generated ones; tokens outside 0..V-1 count for nothing.  NULL parameter arrays: 1, 0, 0.  bias_ids, bias [B, n_bias]: entries
+ * outside 0..V-1 are none.  masks [n_masks, ceil(V / 32)]: bit v % 32 of word v / 32; mask_row [B]: outside 0..n_masks-1 the row has
+ * none.  append: a chosen token is stored at history[b][lengths[b]++] where there is room.
+ * No counterpart in the reference, whose decode loop takes the argmax of the model's own logits. */
+typedef struct mlora_logit_rules {
+  int32_t* history;
+  int32_t* lengths;
+  const int32_t* gen_start;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;
+  const float* bias;
+  const int32_t* masks;
+  const int32_t* mask_row;
+  int cap, n_bias, n_masks, append;
+} mlora_logit_rules;
+size_t mlora_constrained_argmax_workspace_bytes(int B, int V);
+int mlora_constrained_argmax(int32_t* ids, float* out, long ld_out, const float* logits, long ld, const mlora_logit_rules* rules, int B, int V,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Paged KV cache (16-token pages) - replaces TVM's TIRPagedKVCache as configured at
  * llama_for_causal_lm.py:148-174 (RoPE applied inside the cache op, rotary_dim = head_dim, scale 1,

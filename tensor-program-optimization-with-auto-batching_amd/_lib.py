@@ -136,6 +136,15 @@ SIGNATURES["mlora_prefill_workspace_bytes"] = (_z, [C.POINTER(PrefillPass)])
 SIGNATURES["mlora_prefill"] = (_i, [C.POINTER(PrefillPass), _p])
 
 
+class LogitRulesArgs(C.Structure):
+    _fields_ = [(n, _p) for n in ("history", "lengths", "gen_start", "repetition", "presence", "frequency", "bias_ids", "bias", "masks", "mask_row")] + \
+               [(n, _i) for n in ("cap", "n_bias", "n_masks", "append")]
+
+
+SIGNATURES["mlora_constrained_argmax_workspace_bytes"] = (_z, [_i, _i])
+SIGNATURES["mlora_constrained_argmax"] = (_i, [_p, _p, _l, _p, _l, C.POINTER(LogitRulesArgs), _i, _i, _p, _z, _p])
+
+
 class TanhNorm(C.Structure):
     _fields_ = [("w", _p), ("b", _p), ("alpha", _f)]
 

@@ -66,6 +66,15 @@ def _dev(t: torch.Tensor, dtype=None, name="tensor") -> int:
     return t.data_ptr()
 
 
+def _here(device, who):
+    """`device`, where work queued on the current stream runs."""
+    if device.type != "cuda":
+        raise ValueError(f"{who}: tensors must live on the GPU (no CPU path)")
+    if device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{who}: tensors on {device} while cuda:{torch._C._cuda_getDevice()} is current")
+    return device
+
+
 def _dt(t: torch.Tensor) -> int:
     if t.dtype in (torch.float16, torch.bfloat16):
         return F16
@@ -699,6 +708,88 @@ def argmax(logits, out=None):
         return out
     check(_lib.loaded().mlora_argmax(_dev(out, torch.int32), _dev(logits, torch.float32), B, V, _stream()))
     return out
+
+
+class LogitRules:
+    """What the rows of a batch may answer with, for `constrained_argmax` (formulas at mlora_constrained_argmax in include/mlora.h).
+    history [B, cap] int32: a row's prompt and generated tokens, lengths [B] of them, from gen_start [B] on the generated ones;
+    repetition, presence, frequency [B] fp32; bias_ids [B, n] int32 (outside the vocabulary: none) and bias [B, n] fp32; masks
+    [m, ceil(V / 32)] int32, bit v % 32 of word v / 32 for token v, and mask_row [B] int32 (outside 0..m-1: no mask).  append: a
+    chosen token goes behind its row's history.  The tensors are the caller's, contiguous and on one device; what a call reads
+    of them is what they hold when it runs."""
+
+    def __init__(self, history=None, lengths=None, gen_start=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias=None,
+                 masks=None, mask_row=None, append=False):
+        i32, f32 = torch.int32, torch.float32
+        given = {"history": (history, i32, 2), "lengths": (lengths, i32, 1), "gen_start": (gen_start, i32, 1), "repetition": (repetition, f32, 1),
+                 "presence": (presence, f32, 1), "frequency": (frequency, f32, 1), "bias_ids": (bias_ids, i32, 2), "bias": (bias, f32, 2),
+                 "masks": (masks, i32, 2), "mask_row": (mask_row, i32, 1)}
+        given = {n: g for n, g in given.items() if g[0] is not None}
+        self.rows, self.device = None, None
+        self._args = _lib.LogitRulesArgs(append=int(bool(append)))
+        for n, (t, dt, dims) in given.items():
+            if t.dim() != dims:
+                raise ValueError(f"LogitRules: {n}{tuple(t.shape)} needs {dims} dimensions")
+            if n != "masks":
+                if self.rows not in (None, t.shape[0]):
+                    raise ValueError(f"LogitRules: {n} has {t.shape[0]} rows, others {self.rows}")
+                self.rows = t.shape[0]
+            if self.device not in (None, t.device):
+                raise ValueError(f"LogitRules: {n} lies on {t.device}, others on {self.device}")
+            self.device = t.device
+            p = _dev(t, dt, n)
+            setattr(self, n, t)
+            setattr(self._args, n, p if t.numel() else None)
+        for a, b in (("history", "lengths"), ("bias_ids", "bias"), ("masks", "mask_row")):
+            if (a in given) != (b in given):
+                raise ValueError(f"LogitRules: {a} and {b} come together")
+        if "history" not in given and (append or any(n in given for n in ("gen_start", "repetition", "presence", "frequency"))):
+            raise ValueError("LogitRules: penalties and append need a history")
+        if "bias" in given:
+            if bias.shape != bias_ids.shape:
+                raise ValueError(f"LogitRules: bias{tuple(bias.shape)} for bias_ids{tuple(bias_ids.shape)}")
+            self._args.n_bias = bias.shape[1] if bias.numel() else 0
+        if "masks" in given:
+            self._args.n_masks = masks.shape[0] if masks.numel() else 0
+        if "history" in given:
+            self._args.cap = history.shape[1]
+            if not history.numel() and self.rows:
+                raise ValueError("LogitRules: a history without room")
+
+
+def constrained_argmax(logits, rules: LogitRules, out=None, ids=None):
+    """The greedy token [B] int32 of logits [B, V] fp32 (any row stride) under `rules`, -1 for a row that has none left; out [B, V]
+    fp32 (or None; may be `logits`) takes the logits after penalties, biases and masks."""
+    B, V = logits.shape
+    dev = _here(logits.device, "constrained_argmax")
+    if rules.rows not in (None, B) or rules.device not in (None, dev):
+        raise ValueError(f"constrained_argmax: rules of {rules.rows} rows on {rules.device} for {B} on {dev}")
+    if rules._args.n_masks and rules.masks.shape[1] != -(-V // 32):
+        raise ValueError(f"constrained_argmax: masks of {rules.masks.shape[1]} words for {V} tokens")
+    lds = []
+    for t, name in ((logits, "logits"), (out, "out")):
+        if t is not None and (not t.is_cuda or t.device != dev or t.dtype != torch.float32 or t.shape != (B, V) or (t.stride(1) != 1 and V > 1)
+                              or (B > 1 and t.stride(0) < V)):
+            raise ValueError(f"constrained_argmax: {name} must be fp32 [{B}, {V}] on the GPU with unit inner stride")
+        lds.append(0 if t is None else t.stride(0) if B > 1 else max(V, t.stride(0)))
+    if ids is None:
+        ids = torch.empty((B,), dtype=torch.int32, device=dev)
+    elif ids.shape != (B,):
+        raise ValueError(f"constrained_argmax: ids{tuple(ids.shape)} for {B} rows")
+    if B == 0:
+        return ids
+    if out is not None and (out.data_ptr(), lds[1]) != (logits.data_ptr(), lds[0]):
+        a, b = ((t.data_ptr(), t.data_ptr() + 4 * ((B - 1) * ld + V)) for t, ld in ((logits, lds[0]), (out, lds[1])))
+        if a[0] < b[1] and b[0] < a[1]:
+            raise ValueError("constrained_argmax: out overlaps the logits without being them")
+    L = _lib.loaded()
+    nb = L.mlora_constrained_argmax_workspace_bytes(B, V)
+    ws = torch.empty(nb // 8, dtype=torch.int64, device=dev) if nb else None
+    code = L.mlora_constrained_argmax(_dev(ids, torch.int32), None if out is None else out.data_ptr(), lds[1], logits.data_ptr(), lds[0],
+                                      ctypes.byref(rules._args), B, V, None if ws is None else ws.data_ptr(), nb, _stream())
+    if code:
+        raise _lib.MloraError(code, L.mlora_last_error().decode())
+    return ids
 
 
 def rope_kv_append(qkv, k_cache, v_cache, block_table, tok_seq, tok_pos, rope_cos, rope_sin, Hq, Hkv, D):
