@@ -371,10 +371,102 @@ class PackedWeight:
         return v.permute(0, 3, 1, 2, 4).reshape(nt * 16, self.K)[: self.N].contiguous()
 
 
+class QuantWeight:
+    """A [N, K] weight scale * (q - zero) of 4-bit q, one fp16 scale and one 4-bit zero per `group` (32, 64 or 128) neighbours along K, in
+    the layout of mlora_linear4."""
+
+    dtype = torch.float16
+
+    def __init__(self, q, scale, zero):
+        """q [N, K] and zero [N, K / group] uint8 of 0 .. 15, scale [N, K / group] fp16."""
+        N, K = q.shape
+        n, G = scale.shape
+        if n != N or zero.shape != scale.shape or G == 0 or K % G or K // G not in (32, 64, 128):
+            raise ValueError(f"QuantWeight: q{tuple(q.shape)} scale{tuple(scale.shape)} zero{tuple(zero.shape)}: one scale and zero per 32, 64 or 128 columns")
+        if q.dtype != torch.uint8 or zero.dtype != torch.uint8 or scale.dtype != torch.float16:
+            raise TypeError("QuantWeight: q and zero are uint8, scale is float16")
+        _here(q.device, "QuantWeight")
+        if q.device != scale.device or q.device != zero.device:
+            raise ValueError("QuantWeight: q, scale and zero on one device")
+        if N and bool((q.amax() > 15) | (zero.amax() > 15)):
+            raise ValueError("QuantWeight: q and zero of 4 bits")
+        self.N, self.K, self.group = N, K, K // G
+        tiles, blocks, gb = -(-N // 16), -(-K // 128), 128 // self.group
+        if (tiles * 16, blocks * 128) != (N, K):
+            q, full = torch.zeros((tiles * 16, blocks * 128), dtype=torch.uint8, device=q.device), q
+            q[:N, :K] = full
+            scale, zero = (torch.nn.functional.pad(t, (0, blocks * gb - G, 0, tiles * 16 - N)) for t in (scale, zero))
+        # [tile][row][block][step][kg][p][2] -> [tile][block][kg][row][step] words of nibbles (p, 4 + p)
+        v = q.view(tiles, 16, blocks, 4, 4, 4, 2).permute(0, 2, 4, 1, 3, 5, 6)
+        low, high = ((v[..., h].contiguous().view(-1, 4) << torch.tensor([0, 4, 0, 4], device=q.device, dtype=torch.uint8)) for h in (0, 1))
+        self.q = torch.stack([low[:, 0] | low[:, 1], low[:, 2] | low[:, 3], high[:, 0] | high[:, 1], high[:, 2] | high[:, 3]], 1).reshape(-1)
+        self.scale, self.zero = (t.view(tiles, 16, blocks, gb).permute(0, 2, 1, 3).contiguous().view(-1) for t in (scale, zero))
+
+    @property
+    def shape(self):
+        return (self.N, self.K)
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def dequantize(self) -> torch.Tensor:
+        """The weight [N, K] in fp32 (for inspection)."""
+        tiles, blocks = -(-self.N // 16), -(-self.K // 128)
+        b = self.q.view(-1, 4)
+        nib = torch.stack([torch.stack([b[:, h * 2 + p // 2] >> (4 * (p % 2)) & 15 for h in (0, 1)], 1) for p in range(4)], 1)       # [words][p][2]
+        q = nib.view(tiles, blocks, 4, 16, 4, 4, 2).permute(0, 3, 1, 4, 2, 5, 6).reshape(tiles * 16, blocks, 128 // self.group, self.group)
+        s, z = (t.view(tiles, blocks, 16, -1).permute(0, 2, 1, 3).reshape(tiles * 16, blocks, -1, 1).float() for t in (self.scale, self.zero))
+        return ((q.float() - z) * s).reshape(tiles * 16, blocks * 128)[: self.N, : self.K].contiguous()
+
+
+def quantize(W: torch.Tensor, group: int = 128) -> QuantWeight:
+    """W [N, K] rounded to 4 bits: per group the 16 steps between its least and its greatest value, 0 among them."""
+    N, K = W.shape
+    if K % group or group not in (32, 64, 128):
+        raise ValueError(f"quantize: groups of {group} for K={K}")
+    w = W.float().view(N, K // group, group)
+    lo, hi = w.amin(2).clamp_max(0.0), w.amax(2).clamp_min(0.0)
+    scale = ((hi - lo) / 15).clamp_min(2.0 ** -24).to(torch.float16)
+    s = scale.float()
+    zero = (-lo / s).round().clamp_(0, 15)
+    q = ((w / s[:, :, None]).round() + zero[:, :, None]).clamp_(0, 15)
+    return QuantWeight(q.view(N, K).to(torch.uint8), scale, zero.to(torch.uint8))
+
+
+def _linear4(x, W, out, out_dtype, accumulate):
+    T, K = x.shape
+    N, K2 = W.shape
+    dev = _here(x.device, "linear")
+    if K2 != K or x.dtype != torch.float16 or W.device != dev:
+        raise ValueError(f"linear: x{tuple(x.shape)} {x.dtype} on {dev} vs a 4-bit weight {W.shape} on {W.device} (fp16 activations)")
+    if accumulate and out is None:
+        raise ValueError("linear: accumulate needs out")
+    if out is None:
+        out = torch.empty((T, N), dtype=out_dtype, device=dev)
+    if out.shape != (T, N) or out.device != dev:
+        raise ValueError(f"linear: out{tuple(out.shape)} on {out.device}, expected {(T, N)} on {dev}")
+    if T == 0:
+        return out
+    if isinstance(x, FragActivation):
+        xp, lay, ldx = x.data.data_ptr(), FRAG, 0
+    else:
+        ldx = x.stride(0) if T > 1 else K
+        if x.stride(1) != 1 or ldx < K or ldx % 8 or x.data_ptr() % 16:
+            x = x.contiguous().clone() if x.is_contiguous() else x.contiguous()       # rows on 16 bytes
+            ldx = K
+        xp, lay = x.data_ptr(), ROWMAJOR
+    check(lib().mlora_linear4(_dev(out), _dt(out), ACCUMULATE if accumulate else STORE, xp, lay, ldx, W.q.data_ptr(), W.scale.data_ptr(), W.zero.data_ptr(),
+                              W.group, T, K, N, _stream()))
+    return out
+
+
 def linear(x, W, out=None, out_dtype=None, accumulate=False, kernel="auto"):
     """y (=|+=) x @ W.T.  x [T,K] (row stride may exceed K) or a FragActivation, W [N,K] of the same type or a
-    PackedWeight; f16, bf16 (fragment order or packed) or f32 (plain); y has their type unless out_dtype says f32.  accumulate=True adds into the fp32 tensor `out`.  kernel: "auto" | "gemv" | "gemm"."""
+    PackedWeight, or a QuantWeight (f16 x); f16, bf16 (fragment order or packed) or f32 (plain); y has their type unless out_dtype says f32.  accumulate=True adds into the fp32 tensor `out`.  kernel: "auto" | "gemv" | "gemm"."""
     out_dtype = out_dtype or W.dtype
+    if isinstance(W, QuantWeight):
+        return _linear4(x, W, out, out_dtype, accumulate)
     if isinstance(x, FragActivation):
         return _linear_frag(x, W, out, out_dtype, accumulate)
     T, K = x.shape
