@@ -939,6 +939,79 @@ def paged_attn_decode(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, Hq, 
     return out
 
 
+class SharedPrefixPlan:
+    """Which rows of a decode batch share their first pages, for `paged_attn_decode_shared`: made once for a batch, good for all its
+    layers and steps while its rows stay.  groups: (rows, pages) - batch rows whose block tables begin with the same `pages` pages, all
+    within their contexts; a row is in one group at most.  lens: the rows' context lengths now, which choose how the work is cut."""
+
+    def __init__(self, groups, lens, Hq, Hkv, D, device):
+        B, G = len(lens), Hq // Hkv
+        if Hq % Hkv or not 1 <= G <= 16:
+            raise ValueError(f"SharedPrefixPlan: {Hq} query heads over {Hkv}")
+        groups = [([int(r) for r in rows], int(pages)) for rows, pages in groups]
+        members = [r for rows, _ in groups for r in rows]
+        if len(set(members)) != len(members) or any(not 0 <= r < B for r in members):
+            raise ValueError(f"SharedPrefixPlan: rows {members} of {B}, each in one group at most")
+        if any(not rows or pages <= 0 for rows, pages in groups) or any(16 * pages > lens[r] for rows, pages in groups for r in rows):
+            raise ValueError("SharedPrefixPlan: a group has rows and pages, and its pages lie within their contexts")
+        self.B, self.Hq, self.Hkv, self.D, self.n_members = B, Hq, Hkv, D, len(members)
+        row_pages, row_slots = [0] * B, [0] * B
+        for rows, pages in groups:
+            for r in rows:
+                row_pages[r] = pages
+        most = lib().mlora_shared_attn_unit_rows() // G                  # members of a unit
+        own = [-(-n // 16) - p for n, p in zip(lens, row_pages)]
+        per = self._pages_per_unit(sum(-(-len(rows) // most) * pages for rows, pages in groups) + sum(own), Hkv)
+        units, first = [], 0
+        for rows, pages in groups:
+            n = -(-pages // per)
+            cut = [pages * i // n for i in range(n + 1)]
+            for r in rows:
+                row_slots[r] = n
+            for m in range(0, len(rows), most):
+                units += [(first + m, min(most, len(rows) - m), a, b - a, i, 0, 0, 0) for i, (a, b) in enumerate(zip(cut, cut[1:]))]
+            first += len(rows)
+        self.own_splits = max(1, min(-(-max(own, default=0) // per), 65535 // max(B, 1) - len(units) // max(B, 1) - 1))
+        units.sort(key=lambda u: -u[3] * u[1])
+        self.n_units, self.slots = len(units), max(row_slots, default=0) + self.own_splits
+        flat = torch.tensor([x for u in units for x in u] + members + row_pages + row_slots, dtype=torch.int32)
+        self.data = upload(flat, device)
+        at = [0, 8 * len(units), 8 * len(units) + len(members)]
+        self.units, self.members, self.row_pages, self.row_slots = (self.data[a:b] for a, b in zip(at + [at[2] + B], at[1:] + [at[2] + B, at[2] + 2 * B]))
+
+    @staticmethod
+    def _pages_per_unit(pages, Hkv):
+        return max(8, -(-pages * Hkv // 1024))
+
+
+def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, plan: SharedPrefixPlan, Hq, Hkv, D, out=None, frag=False):
+    """`paged_attn_decode` for a batch whose rows share prefixes as `plan` says: shared pages are read once for all their rows."""
+    B = qkv.shape[0]
+    n_seq, max_blocks = block_table.shape
+    dev = _here(qkv.device, "paged_attn_decode_shared")
+    if (plan.B, plan.Hq, plan.Hkv, plan.D) != (B, Hq, Hkv, D) or plan.data.device != dev:
+        raise ValueError(f"paged_attn_decode_shared: a plan of {(plan.B, plan.Hq, plan.Hkv, plan.D)} on {plan.data.device} for {(B, Hq, Hkv, D)} on {dev}")
+    if qkv.numel() != B * (Hq + 2 * Hkv) * D or seq_ids.shape != (B,) or ctx_len.shape != (B,) or k_cache.shape != (k_cache.shape[0], Hkv, D // 32, 4, 16, 8) \
+            or v_cache.shape != (k_cache.shape[0], Hkv, D, 16):
+        raise ValueError(f"paged_attn_decode_shared: qkv{tuple(qkv.shape)} rows{tuple(seq_ids.shape)} contexts{tuple(ctx_len.shape)} k{tuple(k_cache.shape)} "
+                         f"v{tuple(v_cache.shape)}")
+    if out is not None and (tuple(out.shape) != (B, Hq * D) or isinstance(out, FragActivation) != frag):
+        raise ValueError(f"paged_attn_decode_shared: out{tuple(out.shape)}")
+    out, optr, lay = _out_arg(out, B, Hq * D, frag, dev)
+    if B == 0:
+        return out
+    L = lib()
+    nb = L.mlora_shared_attn_workspace_bytes(B, Hq, D, plan.slots)
+    ws = torch.empty(nb // 4, dtype=torch.float32, device=dev)
+    f16, i32 = torch.float16, torch.int32
+    check(L.mlora_paged_attn_decode_shared(optr, lay, _dev(qkv, f16, "qkv"), _dev(k_cache, f16, "k_cache"), _dev(v_cache, f16, "v_cache"),
+                                           _dev(block_table, i32, "block_table"), max_blocks, _dev(seq_ids, i32, "seq_ids"), _dev(ctx_len, i32, "ctx_len"),
+                                           plan.units.data_ptr(), plan.n_units, plan.members.data_ptr(), plan.n_members, plan.row_pages.data_ptr(),
+                                           plan.row_slots.data_ptr(), plan.own_splits, plan.slots, B, Hq, Hkv, D, k_cache.shape[0], n_seq, ws.data_ptr(), nb,
+                                           _stream()))
+    return out
+
+
 def rope_attn_decode(qkv, k_cache, v_cache, block_table, seq_ids, tok_pos, ctx_len, rope_cos, rope_sin, Hq, Hkv, D,
                      out=None, frag=False, o_shrink=None):
     """rope_kv_append + paged_attn_decode of one decode step in one launch (no LoRA on q, k, v); qkv is left unrotated.

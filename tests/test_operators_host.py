@@ -36,3 +36,18 @@ def test_linear4_refusals():
     assert call(mode=1) == -2 and call(mode=2) == -2 and call(ldx=120) == -1 and call(ldx=132) == -1 and call(lay=2) == -1
     assert call(x=24) == -1 and call(y=17) == -1 and call(dt=1, y=18) == -1
     assert call(T=0) == 0
+
+
+def test_shared_attention_refusals():
+    lib = load_pkg("_lib").lib()
+    assert lib.mlora_shared_attn_unit_rows() == 128
+    need = lib.mlora_shared_attn_workspace_bytes(4, 8, 128, 3)
+    assert need == 4 * 8 * 3 * 130 * 4 and lib.mlora_shared_attn_workspace_bytes(0, 8, 128, 3) == 0
+    def call(out=16, lay=0, units=16, n_units=1, members=16, n_members=2, row_pages=16, own=2, slots=3, B=4, Hq=8, Hkv=8, D=128, ws=16, nb=need):
+        return lib.mlora_paged_attn_decode_shared(out, lay, 16, 16, 16, 16, 4, 16, 16, units, n_units, members, n_members, row_pages, 16, own, slots, B, Hq, Hkv, D,
+                                                  5, 4, ws, nb, None)
+    assert call(out=None) == -1 and call(row_pages=None) == -1 and call(units=None) == -1 and call(n_members=0) == -1 and call(n_units=-1) == -1
+    assert call(D=96) == -2 and call(Hkv=3) == -1 and call(Hq=34, Hkv=2) == -2 and call(lay=5) == -1
+    assert call(own=0) == -1 and call(slots=1) == -1 and call(B=-1) == -1 and call(B=40000) == -1
+    assert call(ws=None) == -3 and call(nb=need - 1) == -3 and call(ws=24) == -3
+    assert call(B=0) == 0
