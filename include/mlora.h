@@ -324,12 +324,14 @@ int mlora_embed(void* out, int out_dtype, const void* table, const int32_t* ids,
 /* Linear with 4-bit weights and group scales (fp16 library):
  *     y[t, n] (=|+=) sum over groups g of K of  s[n, g] sum_{k in g} x[t, k] (q[n, k] - z[n, g]),     q, z = 0 .. 15,
  * products over the exact integers, sums and scales in fp32.  group: 32, 64 or 128, K a multiple of it.  x [T, K] f16 in rows
- * of ldx or in fragment order, any T; y [T, N] f16 or f32; mode as for mlora_linear.  q, scale (f16) and zero (bytes) in the
- * layouts at the top of linear4.hip, with the sizes that mlora_linear4_sizes gives (outputs may be NULL); x, q, scale and zero 16-byte aligned.
+ * of ldx or in fragment order, any T; y [T, N] f16 or f32; mode as for mlora_linear.  q and meta (scales and zeros) in the
+ * layouts at the top of linear4.hip, with the sizes that mlora_linear4_sizes gives (outputs may be NULL); x, q, meta and workspace
+ * 16-byte aligned.
  * No counterpart in the reference, whose linears are fp16. */
-int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, size_t* scale_bytes, size_t* zero_bytes);
-int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* scale, const void* zero, int group,
-                  int T, int K, int N, void* stream);
+int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, size_t* meta_bytes);
+size_t mlora_linear4_workspace_bytes(int T, int K, int N);
+int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* meta, int group,
+                  int T, int K, int N, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ids[b] = argmax_v logits[b, v], lowest index on ties (numpy.argmax).
  * Replaces: the host-side np.argmax over D2H-copied logits (tvm/llama_auto_batcher/llama_exec_graph.py:92,134-137). */

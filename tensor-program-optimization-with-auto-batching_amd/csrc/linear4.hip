@@ -5,15 +5,18 @@
 // rounding but those of fp32 sums and the result's.  For up to 64 tokens the weight stream from HBM is the bound (N K / 2 bytes and 3
 // N K / group of scales and zeros).
 //
-// Layout (mlora_linear4_bytes; K in blocks of 128, N in tiles of 16 rows, both padded with zeros):
+// Layout (sizes: mlora_linear4_sizes; K in blocks of 128, N in tiles of 16 rows, both padded with zeros):
 //   q     [tile][block][lane 64][k-step 4] words: lane (kg, row) = lane / 16, lane % 16 holds k = 32 step + 8 kg + e of its row in word
 //         `step`, e = 2 p in bits 4 p .., e = 2 p + 1 in bits 16 + 4 p ..: a tile's block is 1 KiB that a wave reads with one load a
 //         lane, and pairs of neighbouring k come out of a word with one mask-and-or each
-//   scale [tile][block][row 16][128 / group] fp16,  zero likewise in bytes
+//   meta  [tile][block] {scale [row 16][128 / group] fp16, zero likewise in bytes}: 48 bytes a group and tile
+#include <type_traits>
+
 #include "lora_device.h"
 
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int L4_WAVES = 8;
 constexpr int L4_BLOCK = 128;
 enum { L4_F16 = 0, L4_F32 = 1, L4_ACC = 2 };
@@ -22,22 +25,29 @@ struct Linear4 {
   void* y;
   const f16* x;
   const uint32_t* q;
-  const f16* scale;
-  const uint8_t* zero;
+  const char* meta;
   int ldx, frag_tt, T, K, N;       // frag_tt: token tiles of a fragment-ordered x, 0: rows of ldx
   bool wide;                       // rows of y take four columns at a time
 };
 
-// The eight weights of a word as fp16 integers q - z; zz = 1024 + z twice.  An fp16 of 1024 .. 2047 holds an integer in its low bits, so
-// 1024 + q is the nibble with an exponent put above it, and 1024 + 16 q the one four bits higher.
-__device__ __forceinline__ f16x8 l4_weights(uint32_t w, f16x2 zz, f16x2 zs) {
-  const uint32_t ex = 0x64006400u, lo = 0x000f000fu, hi = 0x00f000f0u;
+// The eight weights of a word as fp16 integers q - z; zz = 1024 + z, zs = -(64 + z), twice.  An fp16 of 1024 .. 2047 holds an integer in its low
+// bits, so 1024 + q is the nibble with an exponent put above it, and 1024 + 16 q the one four bits higher.  Mask and exponent come in
+// registers (nibble_consts): as literals each pair of and / or would be two instructions, 13 a word instead of 9.
+struct NibbleConsts {
+  uint32_t lo, hi, ex;
+};
+__device__ __forceinline__ NibbleConsts nibble_consts() {
+  NibbleConsts c = {0x000f000fu, 0x00f000f0u, 0x64006400u};
+  asm("" : "+s"(c.lo), "+s"(c.hi), "+v"(c.ex));
+  return c;
+}
+__device__ __forceinline__ f16x8 l4_weights(uint32_t w, const NibbleConsts& k, f16x2 zz, f16x2 zs) {
   union { uint32_t u; f16x2 h; } a, b, c, d;
-  a.u = (w & lo) | ex;
-  b.u = (w & hi) | ex;
+  a.u = (w & k.lo) | k.ex;
+  b.u = (w & k.hi) | k.ex;
   w >>= 8;
-  c.u = (w & lo) | ex;
-  d.u = (w & hi) | ex;
+  c.u = (w & k.lo) | k.ex;
+  d.u = (w & k.hi) | k.ex;
   const f16x2 s = f16x2{(f16)0.0625f, (f16)0.0625f};
   a.h = a.h - zz;
   b.h = __builtin_elementwise_fma(b.h, s, zs);               // (1024 + 16 q) / 16 - (64 + z)
@@ -46,165 +56,390 @@ __device__ __forceinline__ f16x8 l4_weights(uint32_t w, f16x2 zz, f16x2 zs) {
   return f16x8{a.h[0], a.h[1], b.h[0], b.h[1], c.h[0], c.h[1], d.h[0], d.h[1]};
 }
 
-// Workgroup: NT tiles of rows and up to 16 TT tokens; its waves take every eighth block of K and their sums meet in LDS, in wave order.
-template <int NT, int TT, int GB, int OUT>      // GB: groups per block
-__global__ __launch_bounds__(L4_WAVES * WAVE) void linear4_kernel(Linear4 a) {
-  constexpr int TILES = NT * TT;
-  constexpr int HT = TILES > 8 ? 8 : TILES;     // tiles summed per pass through LDS
-  __shared__ f32x4 red[L4_WAVES][HT][WAVE];
+// Four columns n .. of a token's result
+template <int OUT>
+__device__ __forceinline__ void l4_store(const Linear4& a, int t, int n, f32x4 s) {
+  const size_t at = (size_t)t * a.N + n;
+  if (a.wide) {
+    if constexpr (OUT == L4_F16) *reinterpret_cast<f16x4*>((f16*)a.y + at) = f16x4{(f16)s[0], (f16)s[1], (f16)s[2], (f16)s[3]};
+    else if constexpr (OUT == L4_F32) *reinterpret_cast<f32x4*>((float*)a.y + at) = s;
+    else *reinterpret_cast<f32x4*>((float*)a.y + at) += s;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.N) {
+      if constexpr (OUT == L4_F16) ((f16*)a.y)[at + e] = (f16)s[e];
+      else if constexpr (OUT == L4_F32) ((float*)a.y)[at + e] = s[e];
+      else ((float*)a.y)[at + e] += s[e];
+    }
+}
+
+// Up to 16 tokens: a workgroup has NT tiles of rows, its waves take every eighth block of K and their sums meet in LDS, in wave order.
+template <int NT, int GB, int OUT>      // GB: groups per block
+__global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kernel(Linear4 a) {
+  __shared__ f32x4 red[L4_WAVES][NT][WAVE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r16 = lane & 15, kg = lane >> 4;
   const int nb = (a.K + L4_BLOCK - 1) / L4_BLOCK, KB = a.K / 32, tiles = (a.N + 15) / 16;
-  const int tile0 = blockIdx.x * NT, t0 = blockIdx.y * (16 * TT);
+  const NibbleConsts nc = nibble_consts();
+  const int tile0 = blockIdx.x * NT;
   size_t row_block[NT];                         // first block of a tile
 #pragma unroll
   for (int i = 0; i < NT; ++i) row_block[i] = (size_t)(tile0 + i < tiles ? tile0 + i : tiles - 1) * nb;
-  const f16* xp[TT];
-#pragma unroll
-  for (int j = 0; j < TT; ++j) {
-    if (a.frag_tt) {
-      const int tt = t0 / 16 + j;
-      xp[j] = a.x + (size_t)(tt < a.frag_tt ? tt : a.frag_tt - 1) * 512 + lane * 8;
-    } else {
-      const int t = t0 + j * 16 + r16;
-      xp[j] = a.x + (size_t)(t < a.T ? t : a.T - 1) * a.ldx + kg * 8;
-    }
-  }
+  // (rows behind the last token: the last one again, whose results are dropped)
+  const f16* xp = a.x + (a.frag_tt ? (size_t)lane * 8 : (size_t)(r16 < a.T ? r16 : a.T - 1) * a.ldx + kg * 8);
   const size_t xstep = a.frag_tt ? (size_t)a.frag_tt * 512 : 32;
-  f32x4 acc[NT][TT];
+  f32x4 acc[NT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < TT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Stage {
-    uint4 q[NT];
+    u32x4 q[NT];
     f16 s[NT][4 * GB];
     uint8_t z[NT][GB];
+    f16x8 x[4];
   };
   auto load = [&](Stage& st, int b) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const size_t rb = row_block[i] + b;
-      st.q[i] = *reinterpret_cast<const uint4*>(a.q + rb * 256 + lane * 4);
-      __builtin_memcpy(st.s[i], __builtin_assume_aligned(a.scale + (rb * 16 + kg * 4) * GB, 8), sizeof(st.s[i]));
-      __builtin_memcpy(st.z[i], __builtin_assume_aligned(a.zero + (rb * 16 + r16) * GB, GB), sizeof(st.z[i]));
+      st.q[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.q + rb * 256 + lane * 4));
+      __builtin_memcpy(st.s[i], __builtin_assume_aligned(a.meta + rb * (48 * GB) + kg * 8 * GB, 8), sizeof(st.s[i]));
+      __builtin_memcpy(st.z[i], __builtin_assume_aligned(a.meta + rb * (48 * GB) + 32 * GB + r16 * GB, GB), sizeof(st.z[i]));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int ks = b * 4 + k;
+      st.x[k] = ks < KB ? ld8(xp + (size_t)ks * xstep) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
     }
   };
-  Stage st;
-  for (int b = wave; b < nb; b += L4_WAVES) {
-    load(st, b);
-    f16x8 x[4][TT];
+  auto multiply = [&](const Stage& st) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int j = 0; j < TT; ++j) {
-        const int ks = b * 4 + k;
-        x[k][j] = ks < KB ? ld8(xp[j] + (size_t)ks * xstep) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const uint32_t w[4] = {st.q[i].x, st.q[i].y, st.q[i].z, st.q[i].w};
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int g = 0; g < GB; ++g) {
         const f16 z = (f16)(float)st.z[i][g];
         const f16x2 zz = f16x2{(f16)1024.f + z, (f16)1024.f + z}, zs = f16x2{-((f16)64.f + z), -((f16)64.f + z)};
-        f32x4 sum[TT];
+        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < TT; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = g * (4 / GB); k < (g + 1) * (4 / GB); ++k) sum = mfma_16x16x32(l4_weights(st.q[i][k], nc, zz, zs), st.x[k], sum);
 #pragma unroll
-        for (int k = g * (4 / GB); k < (g + 1) * (4 / GB); ++k) {
-          const f16x8 wf = l4_weights(w[k], zz, zs);
+        for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(sum[e], (float)st.s[i][e * GB + g], acc[i][e]);
+      }
+  };
+  Stage st;
+  for (int b = wave; b < nb; b += L4_WAVES) {
+    load(st, b);
+    multiply(st);
+  }
 #pragma unroll
-          for (int j = 0; j < TT; ++j) sum[j] = mfma_16x16x32(wf, x[k][j], sum[j]);
+  for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
+  __syncthreads();
+  for (int o = threadIdx.x; o < NT * WAVE; o += L4_WAVES * WAVE) {
+    const int sl = o % WAVE, n = (tile0 + o / WAVE) * 16 + (sl >> 4) * 4, t = sl & 15;
+    f32x4 s = red[0][o / WAVE][sl];
+#pragma unroll
+    for (int w = 1; w < L4_WAVES; ++w) s += red[w][o / WAVE][sl];
+    if (t < a.T && n < a.N) l4_store<OUT>(a, t, n, s);
+  }
+}
+
+// More tokens: the waves of a workgroup split its rows (MID_NT tiles each) and share the token block, which comes block of K by block of K straight
+// into an LDS ring together with the weights and their scales; a wave's share of a stage is the same number of requests for all, so that
+// a counted wait leaves the later stages in flight.  Rows of x lie in LDS as 256 bytes each, their sixteen 16-byte pieces exchanged by
+// the row's number: the lanes that fetch a fragment of 16 rows then touch every bank once.  Few rows of W: K is cut into slices that leave
+// fp32 partial sums for a second launch.
+constexpr int MID_WAVES = 4, MID_NT = 2, MID_RING = 3, MID_ROWS = MID_WAVES * MID_NT * 16;
+constexpr int MID_WBYTES = 1024 + 256;          // a tile's block: words, then scales and zeros (padded to a request of 4 bytes a lane)
+constexpr int mid_stage_bytes(int TT) { return TT * 4096 + MID_WAVES * MID_NT * MID_WBYTES; }
+
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void to_lds16(const void* g, char* l) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+}
+__device__ __forceinline__ void to_lds4(const void* g, char* l) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 4, 0, 0);
+}
+
+template <int TT, int GB, int OUT, bool XFRAG>
+__global__ __launch_bounds__(MID_WAVES * WAVE, 2) void linear4_mid_kernel(Linear4 a, float* __restrict__ part) {
+  constexpr int RING = MID_RING, STAGE = mid_stage_bytes(TT), XQ = TT * 4 / MID_WAVES, LOADS = XQ + 2 * MID_NT;   // requests of a wave per stage
+  extern __shared__ __align__(16) char ring[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r16 = lane & 15, kg = lane >> 4;
+  const int nb = (a.K + L4_BLOCK - 1) / L4_BLOCK, KB = a.K / 32, tiles = (a.N + 15) / 16;
+  const NibbleConsts nc = nibble_consts();
+  const int tile0 = (blockIdx.x * MID_WAVES + wave) * MID_NT, t0 = blockIdx.z * (16 * TT);
+  const int b0 = (int)((long)nb * blockIdx.y / gridDim.y), b1 = (int)((long)nb * (blockIdx.y + 1) / gridDim.y);
+
+  // uniform bases, and 32-bit offsets of the lanes
+  const char* wsrc[MID_NT];
+  const char* msrc[MID_NT];
+#pragma unroll
+  for (int i = 0; i < MID_NT; ++i) {
+    const size_t rb = (size_t)(tile0 + i < tiles ? tile0 + i : tiles - 1) * nb;
+    wsrc[i] = (const char*)a.q + rb * 1024;
+    msrc[i] = a.meta + rb * (48 * GB);
+  }
+  const uint32_t woff = lane * 16, moff = (lane < 12 * GB ? lane : 12 * GB - 1) * 4;
+  uint32_t xoff[XQ], xend[XQ];                  // of a whole block, and of a last one of fewer than four k-steps
+  const char* xbase = (const char*)a.x + (XFRAG ? 0 : (size_t)t0 * a.ldx * 2);
+  const size_t xblock = XFRAG ? (size_t)a.frag_tt * 4096 : 256;        // bytes from a block to the next
+#pragma unroll
+  for (int q = 0; q < XQ; ++q) {
+    const int f = wave + MID_WAVES * q;
+    if constexpr (XFRAG) {
+      const int tt = t0 / 16 + f % TT, ks = f / TT, last = (KB - 1) & 3;
+      const uint32_t o = (uint32_t)(tt < a.frag_tt ? tt : a.frag_tt - 1) * 1024 + lane * 16;
+      xoff[q] = o + (uint32_t)ks * a.frag_tt * 1024;
+      xend[q] = o + (uint32_t)(ks < last ? ks : last) * a.frag_tt * 1024;
+    } else {
+      const int row = 4 * f + kg, k = (r16 ^ (row & 15)) * 8, last = (a.K - 8) & 127;
+      const uint32_t o = (uint32_t)(t0 + row < a.T ? row : a.T - 1 - t0) * a.ldx * 2;
+      xoff[q] = o + k * 2;
+      xend[q] = o + (k < last ? k : last) * 2;
+    }
+  }
+  const int whole = KB / 4;                     // blocks of four k-steps
+  // Workgroups begin at different blocks of their slice, so that they do not all ask for the same lines of x at a time.
+  const int n_own = b1 - b0;
+  int next = blockIdx.x % n_own;
+  auto issue = [&](int slot) {
+    char* st = ring + slot * STAGE;
+    const int b = b0 + next;                    // past the slice: once more from the front, and not multiplied
+    next = next + 1 == n_own ? 0 : next + 1;
+    const char* xb = xbase + b * xblock;
+    if (b < whole) {                            // uniform
+#pragma unroll
+      for (int q = 0; q < XQ; ++q) to_lds16(xb + xoff[q], st + (wave + MID_WAVES * q) * 1024);
+    } else {
+#pragma unroll
+      for (int q = 0; q < XQ; ++q) to_lds16(xb + xend[q], st + (wave + MID_WAVES * q) * 1024);
+    }
+    char* w = st + TT * 4096 + wave * (MID_NT * MID_WBYTES);
+#pragma unroll
+    for (int i = 0; i < MID_NT; ++i) {
+      to_lds16(wsrc[i] + (size_t)b * 1024 + woff, w + i * MID_WBYTES);
+      to_lds4(msrc[i] + (size_t)b * (48 * GB) + moff, w + i * MID_WBYTES + 1024);
+    }
+  };
+  f32x4 acc[MID_NT][TT];
+#pragma unroll
+  for (int i = 0; i < MID_NT; ++i)
+#pragma unroll
+    for (int j = 0; j < TT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < RING - 1; ++u) issue(u);
+  int rd = 0, wr = RING - 1, at = blockIdx.x % n_own;
+  for (int n = 0; n < n_own; ++n) {
+    const int b = b0 + at;
+    at = at + 1 == n_own ? 0 : at + 1;
+    wait_loads<(RING - 2) * LOADS>();           // this wave's pieces of block b have landed, its reads of the block before are done
+    bare_barrier();
+    issue(wr);
+    const char* st = ring + rd * STAGE;
+    const char* w = st + TT * 4096 + wave * (MID_NT * MID_WBYTES);
+    rd = rd + 1 == RING ? 0 : rd + 1;
+    wr = wr + 1 == RING ? 0 : wr + 1;
+    u32x4 q[MID_NT];
+    f16 sc[MID_NT][4 * GB];
+    uint8_t zr[MID_NT][GB];
+#pragma unroll
+    for (int i = 0; i < MID_NT; ++i) {
+      q[i] = *reinterpret_cast<const u32x4*>(w + i * MID_WBYTES + lane * 16);
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        const f16x4 v = *reinterpret_cast<const f16x4*>(w + i * MID_WBYTES + 1024 + kg * 8 * GB + g * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[i][g * 4 + e] = v[e];
+        zr[i][g] = *reinterpret_cast<const uint8_t*>(w + i * MID_WBYTES + 1024 + 32 * GB + r16 * GB + g);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const int nks = KB - b * 4;                 // k-steps of the block: 4, or fewer at the end of K
+    auto block = [&](auto WHOLE) {
+#pragma unroll
+    for (int g = 0; g < GB; ++g) {
+      f32x4 sum[MID_NT][TT];
+      f16x2 zz[MID_NT], zs[MID_NT];
+#pragma unroll
+      for (int i = 0; i < MID_NT; ++i) {
+        const f16 z = (f16)(float)zr[i][g];
+        zz[i] = f16x2{(f16)1024.f + z, (f16)1024.f + z};
+        zs[i] = f16x2{-((f16)64.f + z), -((f16)64.f + z)};
+#pragma unroll
+        for (int j = 0; j < TT; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int k = g * (4 / GB); k < (g + 1) * (4 / GB); ++k) {
+        if (!decltype(WHOLE)::value && k >= nks) break;       // uniform
+        f16x8 wf[MID_NT];
+#pragma unroll
+        for (int i = 0; i < MID_NT; ++i) wf[i] = l4_weights(q[i][k], nc, zz[i], zs[i]);
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
+          const f16x8 x = *reinterpret_cast<const f16x8*>(XFRAG ? st + (k * TT + j) * 1024 + lane * 16
+                                                                : st + (j * 16 + r16) * 256 + (((k * 4 + kg) ^ r16) * 16));
+#pragma unroll
+          for (int i = 0; i < MID_NT; ++i) sum[i][j] = mfma_16x16x32(wf[i], x, sum[i][j]);
         }
+      }
+#pragma unroll
+      for (int i = 0; i < MID_NT; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[j][e], (float)st.s[i][e * GB + g], acc[i][j][e]);
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[i][j][e], (float)sc[i][e * GB + g], acc[i][j][e]);
+    }
+    };
+    if (nks >= 4) block(std::true_type());
+    else block(std::false_type());
+  }
+  wait_loads<0>();                              // nothing is in flight into LDS that another workgroup may get
+#pragma unroll
+  for (int i = 0; i < MID_NT; ++i)
+#pragma unroll
+    for (int j = 0; j < TT; ++j) {
+      const int n = (tile0 + i) * 16 + kg * 4, t = t0 + j * 16 + r16;
+      if (part) {                               // whole tiles in the lanes' order: 1 KiB a store, where rows of y would be 16 pieces of 64 bytes
+        if (tile0 + i < tiles && t0 + j * 16 < a.T)
+          reinterpret_cast<f32x4*>(part)[(((size_t)blockIdx.y * tiles + tile0 + i) * ((a.T + 15) / 16) + t0 / 16 + j) * WAVE + lane] = acc[i][j];
+      } else if (t < a.T && n < a.N) {
+        l4_store<OUT>(a, t, n, acc[i][j]);
       }
     }
-  }
-#pragma unroll
-  for (int h = 0; h < TILES / HT; ++h) {
-    if (h) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < TT; ++j)
-        if ((i * TT + j) / HT == h) red[wave][(i * TT + j) % HT][lane] = acc[i][j];
-    __syncthreads();
-    for (int o = threadIdx.x; o < HT * WAVE; o += L4_WAVES * WAVE) {
-      const int tile = h * HT + o / WAVE, sl = o % WAVE;
-      f32x4 s = red[0][o / WAVE][sl];
-#pragma unroll
-      for (int w = 1; w < L4_WAVES; ++w) s += red[w][o / WAVE][sl];
-      const int n = (tile0 + tile / TT) * 16 + (sl >> 4) * 4, t = t0 + (tile % TT) * 16 + (sl & 15);
-      if (t >= a.T || n >= a.N) continue;
-      const size_t at = (size_t)t * a.N + n;
-      if (a.wide) {
-        if constexpr (OUT == L4_F16) *reinterpret_cast<f16x4*>((f16*)a.y + at) = f16x4{(f16)s[0], (f16)s[1], (f16)s[2], (f16)s[3]};
-        else if constexpr (OUT == L4_F32) *reinterpret_cast<f32x4*>((float*)a.y + at) = s;
-        else *reinterpret_cast<f32x4*>((float*)a.y + at) += s;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < a.N) {
-            if constexpr (OUT == L4_F16) ((f16*)a.y)[at + e] = (f16)s[e];
-            else if constexpr (OUT == L4_F32) ((float*)a.y)[at + e] = s[e];
-            else ((float*)a.y)[at + e] += s[e];
-          }
-      }
-    }
-  }
 }
 
-template <int NT, int TT, int GB>
+// y from the slices' partial sums, in slice order
+template <int OUT>
+__global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, const float* __restrict__ part, int slices) {
+  const int tts = (a.T + 15) / 16, tiles = (a.N + 15) / 16;
+  const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6), n_tiles = (size_t)tiles * tts;
+  if (i >= n_tiles) return;
+  const int lane = threadIdx.x & 63, n = (int)(i / tts) * 16 + (lane >> 4) * 4, t = (int)(i % tts) * 16 + (lane & 15);
+  const f32x4* __restrict__ p = reinterpret_cast<const f32x4*>(part) + i * WAVE + lane;
+  f32x4 s = p[0];
+#pragma unroll 4
+  for (int k = 1; k < slices; ++k) s += p[k * n_tiles * WAVE];
+  if (t < a.T && n < a.N) l4_store<OUT>(a, t, n, s);
+}
+
+template <int NT, int GB>
 void launch(const Linear4& a, int out, hipStream_t s) {
-  const dim3 grid(ceil_div(ceil_div(a.N, 16), NT), ceil_div(a.T, 16 * TT)), block(L4_WAVES * WAVE);
-  if (out == L4_F16) hipLaunchKernelGGL((linear4_kernel<NT, TT, GB, L4_F16>), grid, block, 0, s, a);
-  else if (out == L4_F32) hipLaunchKernelGGL((linear4_kernel<NT, TT, GB, L4_F32>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((linear4_kernel<NT, TT, GB, L4_ACC>), grid, block, 0, s, a);
+  const dim3 grid(ceil_div(ceil_div(a.N, 16), NT)), block(L4_WAVES * WAVE);
+  if (out == L4_F16) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F16>), grid, block, 0, s, a);
+  else if (out == L4_F32) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F32>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_ACC>), grid, block, 0, s, a);
+}
+
+template <int TT, int GB, int OUT, bool XFRAG>
+int launch_mid_as(const Linear4& a, int slices, float* part, hipStream_t s) {
+  constexpr int lds = MID_RING * mid_stage_bytes(TT);
+  static const hipError_t configured = hipFuncSetAttribute((const void*)linear4_mid_kernel<TT, GB, OUT, XFRAG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (configured != hipSuccess) return mlora_set_error(MLORA_ERR_LAUNCH, "linear4: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(configured));
+  hipLaunchKernelGGL((linear4_mid_kernel<TT, GB, OUT, XFRAG>), dim3(ceil_div(a.N, MID_ROWS), slices, ceil_div(a.T, 16 * TT)), dim3(MID_WAVES * WAVE), lds, s, a,
+                     slices > 1 ? part : nullptr);
+  if (int e = mlora_launch_status("linear4")) return e;
+  if (slices > 1)
+    hipLaunchKernelGGL(linear4_join_kernel<OUT>, dim3((unsigned)(((long)ceil_div(a.T, 16) * ceil_div(a.N, 16) + 3) / 4)), dim3(256), 0, s, a, (const float*)part, slices);
+  return mlora_launch_status("linear4");
+}
+
+template <int TT, int GB>
+int launch_mid(const Linear4& a, int out, int slices, float* part, hipStream_t s) {
+  if (a.frag_tt) {
+    if (out == L4_F16) return launch_mid_as<TT, GB, L4_F16, true>(a, slices, part, s);
+    if (out == L4_F32) return launch_mid_as<TT, GB, L4_F32, true>(a, slices, part, s);
+    return launch_mid_as<TT, GB, L4_ACC, true>(a, slices, part, s);
+  }
+  if (out == L4_F16) return launch_mid_as<TT, GB, L4_F16, false>(a, slices, part, s);
+  if (out == L4_F32) return launch_mid_as<TT, GB, L4_F32, false>(a, slices, part, s);
+  return launch_mid_as<TT, GB, L4_ACC, false>(a, slices, part, s);
+}
+
+int mid_tt(int T) { return T <= 32 ? 2 : 4; }
+
+// How a product is cut: slices of K (0: the kernel whose waves split K).
+int mid_slices(int T, int K, int N) {
+  if (T <= 16) return 0;
+  const int nb = ceil_div(K, L4_BLOCK);
+  const int tt = mid_tt(T);
+  const long wgs = (long)ceil_div(N, MID_ROWS) * ceil_div(T, 16 * tt);
+  long s = 512 / wgs;
+  if (s > nb / 4) s = nb / 4;
+  return s < 1 ? 1 : s > 16 ? 16 : (int)s;
+}
+
+// Tiles of a workgroup up to 16 tokens: as many as leave the most loaded compute unit the fewest; of equal counts the larger, whose fewer
+// workgroups read x less often.
+int row_tiles(int tiles) {
+  int best = 1;
+  long least = 0;
+  for (int nt : {1, 2, 3, 4, 6, 8}) {
+    const long most = (long)nt * ceil_div(ceil_div(tiles, nt), 256);
+    if (nt == 1 || most <= least) {
+      best = nt;
+      least = most;
+    }
+  }
+  return best;
 }
 
 template <int GB>
-void launch_shape(const Linear4& a, int out, hipStream_t s) {
-  const int tiles = ceil_div(a.N, 16);
-  if (a.T <= 16) {
-    if (tiles <= 512) launch<1, 1, GB>(a, out, s);
-    else launch<2, 1, GB>(a, out, s);
-  } else if (a.T <= 32) launch<1, 2, GB>(a, out, s);
-  else launch<1, 4, GB>(a, out, s);
+int launch_shape(const Linear4& a, int out, float* part, hipStream_t s) {
+  const int tiles = ceil_div(a.N, 16), slices = mid_slices(a.T, a.K, a.N);
+  if (slices > 0) {
+    if (a.T <= 32) return launch_mid<2, GB>(a, out, slices, part, s);
+    return launch_mid<4, GB>(a, out, slices, part, s);
+  }
+  switch (row_tiles(tiles)) {
+    case 1: launch<1, GB>(a, out, s); break;
+    case 2: launch<2, GB>(a, out, s); break;
+    case 3: launch<3, GB>(a, out, s); break;
+    case 4: launch<4, GB>(a, out, s); break;
+    case 6: launch<6, GB>(a, out, s); break;
+    default: launch<8, GB>(a, out, s);
+  }
+  return mlora_launch_status("linear4");
 }
 
 }  // namespace
 
-extern "C" int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, size_t* scale_bytes, size_t* zero_bytes) {
+extern "C" int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, size_t* meta_bytes) {
   MLORA_CHECK(N > 0 && K > 0 && K % 32 == 0 && (group == 32 || group == 64 || group == 128) && K % group == 0, MLORA_ERR_UNSUPPORTED,
               "linear4: N=%d K=%d in groups of %d (K a multiple of the group: 32, 64 or 128)", N, K, group);
   const size_t blocks = (size_t)ceil_div(N, 16) * ceil_div(K, L4_BLOCK);
   if (q_bytes) *q_bytes = blocks * 1024;
-  if (scale_bytes) *scale_bytes = blocks * 16 * (L4_BLOCK / group) * 2;
-  if (zero_bytes) *zero_bytes = blocks * 16 * (L4_BLOCK / group);
+  if (meta_bytes) *meta_bytes = blocks * 48 * (L4_BLOCK / group);
   return MLORA_OK;
 }
 
-extern "C" int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* scale, const void* zero, int group,
-                             int T, int K, int N, void* stream) {
-  MLORA_CHECK(y && x && q && scale && zero, MLORA_ERR_INVALID, "linear4: null pointer");
-  if (int e = mlora_linear4_sizes(N, K, group, nullptr, nullptr, nullptr)) return e;
-  MLORA_CHECK(T >= 0 && T <= 65535 * 16, MLORA_ERR_INVALID, "linear4: bad T=%d", T);
+extern "C" size_t mlora_linear4_workspace_bytes(int T, int K, int N) {
+  const int slices = T > 0 && K > 0 && N > 0 ? mid_slices(T, K, N) : 0;
+  return slices > 1 ? (size_t)slices * ceil_div(T, 16) * ceil_div(N, 16) * 256 * sizeof(float) : 0;
+}
+
+extern "C" int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* meta, int group,
+                             int T, int K, int N, void* workspace, size_t workspace_bytes, void* stream) {
+  MLORA_CHECK(y && x && q && meta, MLORA_ERR_INVALID, "linear4: null pointer");
+  if (int e = mlora_linear4_sizes(N, K, group, nullptr, nullptr)) return e;
+  MLORA_CHECK(T >= 0 && T <= 65535 * 16 && N <= 1 << 30, MLORA_ERR_INVALID, "linear4: bad T=%d", T);
   MLORA_CHECK(y_dtype == MLORA_F16 || y_dtype == MLORA_F32, MLORA_ERR_INVALID, "linear4: bad y_dtype %d", y_dtype);
   MLORA_CHECK(mode == MLORA_STORE || (mode == MLORA_ACCUMULATE && y_dtype == MLORA_F32), MLORA_ERR_UNSUPPORTED, "linear4: results are added to fp32 alone (mode=%d)", mode);
-  MLORA_CHECK(x_layout == MLORA_FRAG || (x_layout == MLORA_ROWMAJOR && ldx >= K && ldx % 8 == 0), MLORA_ERR_INVALID, "linear4: bad x (layout=%d ldx=%d K=%d)", x_layout,
+  MLORA_CHECK(x_layout == MLORA_FRAG || (x_layout == MLORA_ROWMAJOR && ldx >= K && ldx % 8 == 0 && ldx <= 1 << 24), MLORA_ERR_INVALID, "linear4: bad x (layout=%d ldx=%d K=%d)", x_layout,
               ldx, K);
-  MLORA_CHECK((((uintptr_t)x | (uintptr_t)q | (uintptr_t)scale | (uintptr_t)zero) & 15) == 0, MLORA_ERR_INVALID, "linear4: operands not 16-byte aligned");
+  MLORA_CHECK((((uintptr_t)x | (uintptr_t)q | (uintptr_t)meta) & 15) == 0, MLORA_ERR_INVALID, "linear4: operands not 16-byte aligned");
   MLORA_CHECK(((uintptr_t)y & (y_dtype == MLORA_F32 ? 3 : 1)) == 0, MLORA_ERR_INVALID, "linear4: y not aligned to its elements");
   if (T == 0) return MLORA_OK;
-  Linear4 a = {y, (const f16*)x, (const uint32_t*)q, (const f16*)scale, (const uint8_t*)zero, ldx, x_layout == MLORA_FRAG ? mlora_frag_tiles(T) : 0, T, K, N, N % 4 == 0 && ((uintptr_t)y & 15) == 0};
+  Linear4 a = {y, (const f16*)x, (const uint32_t*)q, (const char*)meta, ldx, x_layout == MLORA_FRAG ? mlora_frag_tiles(T) : 0, T, K, N, N % 4 == 0 && ((uintptr_t)y & 15) == 0};
   const int out = mode == MLORA_ACCUMULATE ? L4_ACC : y_dtype == MLORA_F32 ? L4_F32 : L4_F16;
   hipStream_t s = (hipStream_t)stream;
-  if (group == 128) launch_shape<1>(a, out, s);
-  else if (group == 64) launch_shape<2>(a, out, s);
-  else launch_shape<4>(a, out, s);
-  return mlora_launch_status("linear4");
+  const size_t need = mlora_linear4_workspace_bytes(T, K, N);
+  MLORA_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), MLORA_ERR_WORKSPACE,
+              "linear4: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (group == 128) return launch_shape<1>(a, out, (float*)workspace, s);
+  if (group == 64) return launch_shape<2>(a, out, (float*)workspace, s);
+  return launch_shape<4>(a, out, (float*)workspace, s);
 }

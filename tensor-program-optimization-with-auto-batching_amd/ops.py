@@ -400,7 +400,8 @@ class QuantWeight:
         v = q.view(tiles, 16, blocks, 4, 4, 4, 2).permute(0, 2, 4, 1, 3, 5, 6)
         low, high = ((v[..., h].contiguous().view(-1, 4) << torch.tensor([0, 4, 0, 4], device=q.device, dtype=torch.uint8)) for h in (0, 1))
         self.q = torch.stack([low[:, 0] | low[:, 1], low[:, 2] | low[:, 3], high[:, 0] | high[:, 1], high[:, 2] | high[:, 3]], 1).reshape(-1)
-        self.scale, self.zero = (t.view(tiles, 16, blocks, gb).permute(0, 2, 1, 3).contiguous().view(-1) for t in (scale, zero))
+        scale, zero = (t.reshape(tiles, 16, blocks, gb).permute(0, 2, 1, 3).reshape(tiles, blocks, 16 * gb) for t in (scale, zero))
+        self.meta = torch.cat([scale.contiguous().view(torch.uint8), zero], 2).reshape(-1)
 
     @property
     def shape(self):
@@ -416,7 +417,10 @@ class QuantWeight:
         b = self.q.view(-1, 4)
         nib = torch.stack([torch.stack([b[:, h * 2 + p // 2] >> (4 * (p % 2)) & 15 for h in (0, 1)], 1) for p in range(4)], 1)       # [words][p][2]
         q = nib.view(tiles, blocks, 4, 16, 4, 4, 2).permute(0, 3, 1, 4, 2, 5, 6).reshape(tiles * 16, blocks, 128 // self.group, self.group)
-        s, z = (t.view(tiles, blocks, 16, -1).permute(0, 2, 1, 3).reshape(tiles * 16, blocks, -1, 1).float() for t in (self.scale, self.zero))
+        meta = self.meta.view(tiles, blocks, -1)
+        cut = meta.shape[2] // 3 * 2
+        s, z = (t.reshape(tiles, blocks, 16, -1).permute(0, 2, 1, 3).reshape(tiles * 16, blocks, -1, 1).float()
+                for t in (meta[:, :, :cut].contiguous().view(torch.float16), meta[:, :, cut:]))
         return ((q.float() - z) * s).reshape(tiles * 16, blocks * 128)[: self.N, : self.K].contiguous()
 
 
@@ -456,8 +460,10 @@ def _linear4(x, W, out, out_dtype, accumulate):
             x = x.contiguous().clone() if x.is_contiguous() else x.contiguous()       # rows on 16 bytes
             ldx = K
         xp, lay = x.data_ptr(), ROWMAJOR
-    check(lib().mlora_linear4(_dev(out), _dt(out), ACCUMULATE if accumulate else STORE, xp, lay, ldx, W.q.data_ptr(), W.scale.data_ptr(), W.zero.data_ptr(),
-                              W.group, T, K, N, _stream()))
+    nb = _size(torch.float16, "mlora_linear4_workspace_bytes", T, K, N)
+    ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
+    check(lib().mlora_linear4(_dev(out), _dt(out), ACCUMULATE if accumulate else STORE, xp, lay, ldx, W.q.data_ptr(), W.meta.data_ptr(),
+                              W.group, T, K, N, None if ws is None else ws.data_ptr(), nb, _stream()))
     return out
 
 

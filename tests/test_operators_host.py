@@ -24,17 +24,21 @@ def test_constrained_argmax_refusals():
 
 def test_linear4_refusals():
     lib = load_pkg("_lib").lib()
-    sizes = [C.c_size_t() for _ in range(3)]
+    sizes = [C.c_size_t() for _ in range(2)]
     assert lib.mlora_linear4_sizes(40, 352, 32, *(C.byref(s) for s in sizes)) == 0
-    assert [s.value for s in sizes] == [9 * 1024, 9 * 16 * 4 * 2, 9 * 16 * 4]
-    assert lib.mlora_linear4_sizes(40, 352, 32, None, None, None) == 0
-    assert lib.mlora_linear4_sizes(40, 352, 64, None, None, None) == -2 and lib.mlora_linear4_sizes(40, 96, 96, None, None, None) == -2
-    assert lib.mlora_linear4_sizes(0, 32, 32, None, None, None) == -2 and lib.mlora_linear4_sizes(1, 0, 32, None, None, None) == -2
-    def call(y=16, dt=0, mode=0, x=16, lay=0, ldx=128, q=16, s=16, z=16, group=128, T=4, K=128, N=32):
-        return lib.mlora_linear4(y, dt, mode, x, lay, ldx, q, s, z, group, T, K, N, None)
-    assert call(y=None) == -1 and call(z=None) == -1 and call(group=16) == -2 and call(T=-1) == -1 and call(dt=3) == -1
+    assert [s.value for s in sizes] == [9 * 1024, 9 * 16 * 4 * 3]
+    assert lib.mlora_linear4_sizes(40, 352, 32, None, None) == 0
+    assert lib.mlora_linear4_sizes(40, 352, 64, None, None) == -2 and lib.mlora_linear4_sizes(40, 96, 96, None, None) == -2
+    assert lib.mlora_linear4_sizes(0, 32, 32, None, None) == -2 and lib.mlora_linear4_sizes(1, 0, 32, None, None) == -2
+    def call(y=16, dt=0, mode=0, x=16, lay=0, ldx=128, q=16, m=16, group=128, T=4, K=128, N=32, ws=None, nb=0):
+        return lib.mlora_linear4(y, dt, mode, x, lay, ldx, q, m, group, T, K, N, ws, nb, None)
+    assert call(y=None) == -1 and call(m=None) == -1 and call(group=16) == -2 and call(T=-1) == -1 and call(dt=3) == -1
     assert call(mode=1) == -2 and call(mode=2) == -2 and call(ldx=120) == -1 and call(ldx=132) == -1 and call(lay=2) == -1
     assert call(x=24) == -1 and call(y=17) == -1 and call(dt=1, y=18) == -1
+    need = lib.mlora_linear4_workspace_bytes(64, 4096, 4096)
+    assert need % (64 * 4096 * 4) == 0 and need > 0 and lib.mlora_linear4_workspace_bytes(1, 4096, 4096) == 0
+    big = dict(T=64, K=4096, N=4096, ldx=4096)
+    assert call(**big) == -3 and call(ws=16, nb=need - 1, **big) == -3 and call(ws=24, nb=need, **big) == -3
     assert call(T=0) == 0
 
 
