@@ -127,10 +127,26 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
         for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(sum[e], (float)st.s[i][e * GB + g], acc[i][e]);
       }
   };
-  Stage st;
-  for (int b = wave; b < nb; b += L4_WAVES) {
-    load(st, b);
-    multiply(st);
+  if constexpr (NT == 1) {                      // few rows: two blocks in flight (4096 x 4096, one token: 5.3 to 4.8 us; with more tiles it costs registers)
+    Stage st[2];
+    load(st[0], wave < nb ? wave : 0);
+    load(st[1], wave + L4_WAVES < nb ? wave + L4_WAVES : 0);
+    for (int b = wave; b < nb; b += 2 * L4_WAVES) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int next = b + (2 + u) * L4_WAVES;
+        if (b + u * L4_WAVES < nb) {            // uniform
+          multiply(st[u]);
+          if (next < nb) load(st[u], next);
+        }
+      }
+    }
+  } else {
+    Stage st;
+    for (int b = wave; b < nb; b += L4_WAVES) {
+      load(st, b);
+      multiply(st);
+    }
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];

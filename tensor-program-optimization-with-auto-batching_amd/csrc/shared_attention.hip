@@ -4,20 +4,24 @@
 //
 // A softmax over a union of ranges of tokens joins from each range's maximum m, sum l = sum exp(s - m) and o = sum exp(s - m) v:
 //   M = max m_i,   out = sum exp(m_i - M) o_i / sum exp(m_i - M) l_i.
-// So the work is cut into units - (rows, range of pages, kv head) - that a workgroup each attends over, and a second launch joins a row's units.
-// A unit of a prefix has up to 128 query rows (the G = Hq / Hkv heads of every request of the group), one of the pages behind it the G
-// of a single request.  Bound by the pages read, 4 D bytes a token and kv head, as long as a page serves no more than some hundred query rows.
+// So the work is cut into units - (query rows, range of pages, kv head) - and a second launch joins a row's units.  Bound by the pages
+// read, 4 D bytes a token and kv head.
 //
-// A wave holds a tile of 16 query rows and the matrix-core layouts are those of the decode kernel in attention.hip: S^T = K . Q^T, with a
-// lane's four probabilities as the operand of O^T += V^T . P^T (as two fp16 halves, so that they enter with 22 bits).  The waves of a
-// workgroup are R row tiles times 8 / R shares of the unit's pages.
+// Everywhere a wave holds a tile of 16 query rows (the G = Hq / Hkv heads of one or more requests) in the matrix-core layouts of the decode
+// kernel in attention.hip: S^T = K . Q^T, then O^T += V^T . P^T, where a lane's probabilities are already the operand that it must supply
+// - as two fp16 halves, so that they enter with 22 bits - and the keys of two pages fill a k-step.
+//   block units  17 to 64 query rows of a group: four waves share pages that come straight into an LDS ring
+//   wave units   up to 16 query rows - a small group, or the pages of a single request behind its prefix: a wave for itself, the next two
+//                pages on their way to registers
 #include "lora_device.h"
 
 namespace {
 
 constexpr int PAGE = MLORA_PAGE_SIZE;
-constexpr int SA_WAVES = 8;
-constexpr int SA_ROWS = 16 * SA_WAVES;        // query rows of a unit
+constexpr int SA_WAVES = 4;
+constexpr int SA_ROWS = 16 * SA_WAVES;        // query rows of a block unit
+constexpr int SA_RING = 3;                    // stages of two pages
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct SharedAttn {
   f16* out;
@@ -27,14 +31,14 @@ struct SharedAttn {
   const int32_t* block_table;
   const int32_t* seq_ids;
   const int32_t* ctx_len;
-  const int32_t* units;        // [n_units][8] {first member, members, first page, pages, slot}
+  const int32_t* units;        // [n_units][8] {first member, members, first page, pages, slot}, the n_block block units first
   const int32_t* members;      // batch rows, group after group
   const int32_t* row_pages;    // [B] shared pages ahead of a row's own
   const int32_t* row_slots;    // [B] units over those
   float* acc;                  // [B][Hq][slots][D]
   float* ml;                   // [B][Hq][slots][2]
-  int max_blocks, B, Hq, Hkv, n_pages, n_seq, n_units, n_members, own_splits, slots, frag_tt;
-  float scale;
+  int max_blocks, B, Hq, Hkv, n_pages, n_seq, n_block, n_units, own_splits, slots, frag_tt;
+  float scale;                 // of scores, with log2 e: weights are powers of two
 };
 
 __device__ __forceinline__ int context_of(const SharedAttn& a, int row, int& seq) {
@@ -47,178 +51,354 @@ __device__ __forceinline__ int context_of(const SharedAttn& a, int row, int& seq
   return c < 0 ? 0 : c > a.max_blocks * PAGE ? a.max_blocks * PAGE : c;
 }
 
-template <int D>
-__global__ __launch_bounds__(SA_WAVES * WAVE, 4) void shared_attn_kernel(SharedAttn a) {
-  constexpr int NKB = D / 32, NDB = D / 16;
-  __shared__ float sm[SA_WAVES][16], sl[SA_WAVES][16];
-  extern __shared__ __align__(16) float sacc[];             // [SA_WAVES][16][D]
-  const int kh = blockIdx.x, G = a.Hq / a.Hkv;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int col = lane & 15, g = lane >> 4;
-  int rows, first_member = -1, own_row = 0, page0, page1, slot, seq;
-  if ((int)blockIdx.y < a.n_units) {
-    const int32_t* u = a.units + 8 * blockIdx.y;
-    first_member = u[0];
-    rows = u[1] * G;
-    page0 = u[2];
-    page1 = u[2] + u[3];
-    slot = u[4];
-    context_of(a, a.members[first_member], seq);
-  } else {
-    const int i = blockIdx.y - a.n_units, part = i % a.own_splits;
-    own_row = i / a.own_splits;
-    rows = G;
-    const int have = (context_of(a, own_row, seq) + PAGE - 1) / PAGE, from = a.row_pages[own_row];
-    const int n = have > from ? have - from : 0, per = (n + a.own_splits - 1) / a.own_splits;
-    page0 = from + part * per;
-    page1 = page0 + per < from + n ? page0 + per : from + n;
-    slot = a.row_slots[own_row] + part;
-  }
-  const int tiles = (rows + 15) / 16;
-  const int R = tiles <= 1 ? 1 : tiles <= 2 ? 2 : tiles <= 4 ? 4 : 8;
-  const int tile = wave & (R - 1), share = wave / R, shares = SA_WAVES / R;
-  const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
-  if (page1 > a.max_blocks) page1 = a.max_blocks;
+// the sequence whose table names the pages of a unit's members: the first that is one
+__device__ __forceinline__ int sequence_of(const SharedAttn& a, int first, int n) {
+  const int lane = threadIdx.x & 63;
+  const int seq = lane < n ? a.seq_ids[a.members[first + lane]] : -1;
+  const unsigned long long ok = __ballot(seq >= 0 && seq < a.n_seq);
+  return ok ? __builtin_amdgcn_readlane(seq, __builtin_ctzll(ok)) : 0;
+}
 
-  // the lane's query row
-  const int r = tile * 16 + col;
-  const bool live = r < rows;
-  const int row = first_member < 0 ? own_row : a.members[first_member + (live ? r / G : 0)];
-  const int head = kh * G + (live ? r % G : 0);
+// a tile of 16 query rows: lane (g, col) has row col, its dims 16 db + 4 g .. + 3 of the output and a quarter of its sum
+template <int D>
+struct Tile {
+  f16x8 q[D / 32];
+  f32x4 o[D / 16];
+  float m, l;
+  int row, head, ctx, least, most;     // batch row and head (row < 0: no query row), context; shortest and longest context of the tile
+};
+
+template <int D>
+__device__ __forceinline__ void tile_begin(Tile<D>& t, const SharedAttn& a, int row, int head) {
+  const int g = (threadIdx.x & 63) >> 4;
+  t.row = row;
+  t.head = head;
   int unused;
-  const int ctx = live ? context_of(a, row, unused) : 0;
-  f16x8 qf[NKB];
+  t.ctx = row >= 0 ? context_of(a, row, unused) : 0;
+  t.least = row >= 0 ? t.ctx : 0x7fffffff;
+  t.most = t.ctx;
+  const f16* qp = a.qkv + ((size_t)(row >= 0 ? row : 0) * (a.Hq + 2 * a.Hkv) + head) * D + g * 8;
 #pragma unroll
-  for (int kb = 0; kb < NKB; ++kb) qf[kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-  if (live) {
-    const f16* qp = a.qkv + ((size_t)row * (a.Hq + 2 * a.Hkv) + head) * D + g * 8;
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) qf[kb] = ld8(qp + kb * 32);
-  }
-  int most = ctx;                                           // the longest context of the tile
+  for (int kb = 0; kb < D / 32; ++kb) t.q[kb] = row >= 0 ? ld8(qp + kb * 32) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) {
-    const int other = __shfl_xor(most, o, WAVE);
-    most = other > most ? other : most;
+    const int lo = __shfl_xor(t.least, o, WAVE), hi = __shfl_xor(t.most, o, WAVE);
+    t.least = lo < t.least ? lo : t.least;
+    t.most = hi > t.most ? hi : t.most;
   }
+  t.least = __builtin_amdgcn_readfirstlane(t.least);
+  t.most = __builtin_amdgcn_readfirstlane(t.most);
+  t.m = -INFINITY;
+  t.l = 0.f;
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) t.o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
 
-  float m = -INFINITY, l = 0.f;
-  f32x4 O[NDB];
+// P pages pg, pg + 1, ..: keys k(p, kb) in fragment order, values v(p, db) of tokens 4 g .. + 3
+template <int D, int P, class K, class V>
+__device__ __forceinline__ void tile_step(Tile<D>& t, float scale, int pg, K k, V v) {
+  const int g = (threadIdx.x & 63) >> 4;
+  f32x4 st[P];
 #pragma unroll
-  for (int db = 0; db < NDB; ++db) O[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (tile < tiles) {
-    for (int pg = page0 + share; pg < page1; pg += shares) {
-      const int page = bt[pg];
-      if (page < 0 || page >= a.n_pages) continue;          // uniform
-      const f16* kp = a.k_cache + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 8;
-      const f16* vp = a.v_cache + (((size_t)page * a.Hkv + kh) * D + col) * PAGE + g * 4;
-      f16x8 kf[NKB];
-      f16x4 vf[NDB];
+  for (int p = 0; p < P; ++p) {
+    st[p] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) kf[kb] = ld8(kp + kb * 512);
+    for (int kb = 0; kb < D / 32; ++kb) st[p] = mfma_16x16x32(k(p, kb), t.q[kb], st[p]);
+  }
+  const bool edge = (pg + P) * PAGE > t.least;              // uniform: some row ends within these pages
+  float pm = -INFINITY;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) vf[db] = *reinterpret_cast<const f16x4*>(vp + db * 16 * PAGE);
-      f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb], qf[kb], st, 0, 0, 0);
-      const int tok = pg * PAGE + 4 * g;
-      if (pg * PAGE + PAGE > most) {                        // slots behind every context hold anything
+    for (int e = 0; e < 4; ++e) {
+      st[p][e] *= scale;
+      if (edge && (pg + p) * PAGE + 4 * g + e >= t.ctx) st[p][e] = -INFINITY;
+      pm = fmaxf(pm, st[p][e]);
+    }
+  pm = fmaxf(pm, __shfl_xor(pm, 16, WAVE));
+  pm = fmaxf(pm, __shfl_xor(pm, 32, WAVE));
+  if (__any(pm > t.m)) {                                    // (after the first pages seldom)
+    const float m = fmaxf(t.m, pm), alpha = __builtin_amdgcn_exp2f(t.m - (m == -INFINITY ? 0.f : m));
+    t.l *= alpha;
+    t.m = m;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) t.o[db] *= alpha;
+  }
+  const float base = t.m == -INFINITY ? 0.f : t.m;          // a row with no token yet
+  f16 hi[P * 4], lo[P * 4];
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float w = __builtin_amdgcn_exp2f(st[p][e] - base);
+      t.l += w;
+      hi[p * 4 + e] = (f16)w;
+      lo[p * 4 + e] = (f16)(w - (float)hi[p * 4 + e]);
+    }
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) {
+    f16x4 x[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      x[p] = v(p, db);
+      if (edge && (pg + p + 1) * PAGE > t.most)             // slots behind every context hold anything
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (tok + e >= most)
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) vf[db][e] = (f16)0.f;
-      }
-      float pm = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        st[e] = tok + e >= ctx ? -INFINITY : st[e] * a.scale;
-        pm = fmaxf(pm, st[e]);
-      }
-      pm = fmaxf(pm, __shfl_xor(pm, 16, WAVE));
-      pm = fmaxf(pm, __shfl_xor(pm, 32, WAVE));
-      const float m_new = fmaxf(m, pm);
-      const float base = m_new == -INFINITY ? 0.f : m_new;  // a row with no token yet
-      const float alpha = __expf(m - base);
-      f16x8 pa;
-      float ps = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = __expf(st[e] - base);
-        ps += p;
-        const f16 hi = (f16)p;
-        pa[e] = hi;
-        pa[4 + e] = (f16)(p - (float)hi);
-      }
-      l = l * alpha + ps;
-      m = m_new;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        O[db] *= alpha;
-        const f16x8 vv = f16x8{vf[db][0], vf[db][1], vf[db][2], vf[db][3], vf[db][0], vf[db][1], vf[db][2], vf[db][3]};
-        O[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pa, O[db], 0, 0, 0);
-      }
+          if ((pg + p) * PAGE + 4 * g + e >= t.most) x[p][e] = (f16)0.f;
     }
-  }
-  l += __shfl_xor(l, 16, WAVE);
-  l += __shfl_xor(l, 32, WAVE);
-  if (shares == 1) {                                        // uniform
-    if (live) {
-      const size_t at = ((size_t)row * a.Hq + head) * a.slots + slot;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(a.acc + at * D + db * 16 + 4 * g) = O[db];
-      if (g == 0) {
-        a.ml[2 * at] = m;
-        a.ml[2 * at + 1] = l;
-      }
-    }
-    return;
-  }
-  if (live) {
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(&sacc[(wave * 16 + col) * D + db * 16 + 4 * g]) = O[db];
-    if (g == 0) {
-      sm[wave][col] = m;
-      sl[wave][col] = l;
-    }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < rows * (D / 4); e += SA_WAVES * WAVE) {
-    const int rr = e / (D / 4), d = e % (D / 4) * 4, c = rr & 15, w0 = rr >> 4;
-    float M = -INFINITY;
-    for (int w = w0; w < SA_WAVES; w += R) M = fmaxf(M, sm[w][c]);
-    float L = 0.f;
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int w = w0; w < SA_WAVES; w += R) {
-      const float f = sm[w][c] == -INFINITY ? 0.f : __expf(sm[w][c] - M);
-      L += sl[w][c] * f;
-      o += *reinterpret_cast<const f32x4*>(&sacc[(w * 16 + c) * D + d]) * f;
-    }
-    const int orow = first_member < 0 ? own_row : a.members[first_member + rr / G];
-    const size_t at = ((size_t)orow * a.Hq + kh * G + rr % G) * a.slots + slot;
-    *reinterpret_cast<f32x4*>(a.acc + at * D + d) = o;
-    if (d == 0) {
-      a.ml[2 * at] = M;
-      a.ml[2 * at + 1] = L;
+    if constexpr (P == 1) {
+      const f16x8 both = f16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[0][0], x[0][1], x[0][2], x[0][3]};
+      t.o[db] = mfma_16x16x32(both, f16x8{hi[0], hi[1], hi[2], hi[3], lo[0], lo[1], lo[2], lo[3]}, t.o[db]);
+    } else {
+      const f16x8 both = f16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+      t.o[db] = mfma_16x16x32(both, f16x8{hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]}, t.o[db]);
+      t.o[db] = mfma_16x16x32(both, f16x8{lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]}, t.o[db]);
     }
   }
 }
 
-// a row's units joined: four heads a workgroup, a wave each
 template <int D>
+__device__ __forceinline__ void tile_end(Tile<D>& t) {
+  t.l += __shfl_xor(t.l, 16, WAVE);
+  t.l += __shfl_xor(t.l, 32, WAVE);
+}
+
+template <int D>
+__device__ __forceinline__ void tile_store(const Tile<D>& t, const SharedAttn& a, int slot) {
+  if (t.row < 0) return;
+  const int g = (threadIdx.x & 63) >> 4;
+  const size_t at = ((size_t)t.row * a.Hq + t.head) * a.slots + slot;
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(a.acc + at * D + db * 16 + 4 * g) = t.o[db];
+  if (g == 0) *reinterpret_cast<f32x2*>(a.ml + 2 * at) = f32x2{t.m, t.l};
+}
+
+// A page's id; -1 where the table names none
+__device__ __forceinline__ int page_id(const SharedAttn& a, int id) { return id >= 0 && id < a.n_pages ? id : -1; }
+
+template <int D>
+__device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
+  constexpr int NKB = D / 32, NDB = D / 16;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, G = a.Hq / a.Hkv;
+  int seq, page0, page1, slot, row;
+  if (u < a.n_units) {
+    const int32_t* d = a.units + 8 * u;
+    const int first = d[0], n = d[1];
+    page0 = d[2];
+    page1 = d[2] + d[3];
+    slot = d[4];
+    seq = sequence_of(a, first, n);
+    row = col < n * G ? a.members[first + col / G] : -1;
+  } else {
+    const int i = u - a.n_units, part = i % a.own_splits, b = i / a.own_splits;
+    const int have = (context_of(a, b, seq) + PAGE - 1) / PAGE, from = a.row_pages[b];
+    const int n = have > from ? have - from : 0, per = (n + a.own_splits - 1) / a.own_splits;
+    page0 = from + part * per;
+    page1 = page0 + per < from + n ? page0 + per : from + n;
+    slot = a.row_slots[b] + part;
+    row = col < G ? b : -1;
+  }
+  if (page1 > a.max_blocks) page1 = a.max_blocks;
+  const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
+  f16x8 k[2][2][NKB];
+  f16x4 v[2][2][NDB];
+  int id[2][2];
+  auto load = [&](int s, int pg, int own) {                 // pages pg, pg + 1 into set s; own: the lane's page id of the chunk
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      id[s][p] = pg + p < page1 ? page_id(a, __builtin_amdgcn_readlane(own, (pg + p - page0) & 63)) : -1;
+      if (id[s][p] < 0) continue;                           // uniform
+      const f16* kp = a.k_cache + ((size_t)id[s][p] * a.Hkv + kh) * (PAGE * D) + lane * 8;
+      const f16* vp = a.v_cache + (((size_t)id[s][p] * a.Hkv + kh) * D + col) * PAGE + g * 4;
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) k[s][p][kb] = ld8(kp + kb * 512);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) v[s][p][db] = *reinterpret_cast<const f16x4*>(vp + db * 16 * PAGE);
+    }
+  };
+  int own = page0 + lane < page1 ? bt[page0 + lane] : -1;   // the ids of up to 64 pages, one a lane
+  load(0, page0, own);
+  Tile<D> t;
+  tile_begin(t, a, row, kh * G + (row >= 0 ? col % G : 0));
+  auto work = [&](int s, int pg) {
+    auto kf = [&](int p) { return [&, p](int q, int kb) { return k[s][p + q][kb]; }; };
+    auto vf = [&](int p) { return [&, p](int q, int db) { return v[s][p + q][db]; }; };
+    if (id[s][0] >= 0 && id[s][1] >= 0) tile_step<D, 2>(t, a.scale, pg, kf(0), vf(0));
+    else if (id[s][0] >= 0) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
+    else if (id[s][1] >= 0) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
+  };
+  for (int pg = page0; pg < page1; pg += 4) {
+    load(1, pg + 2, own);
+    work(0, pg);
+    if (((pg + 4 - page0) & 63) == 0) own = pg + 4 + lane < page1 ? bt[pg + 4 + lane] : -1;
+    load(0, pg + 4, own);
+    work(1, pg + 2);
+  }
+  tile_end(t);
+  tile_store(t, a, slot);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+// R row tiles (2 or 4) times 4 / R shares of the pages.  A stage is two pages, of which a wave fetches the keys or the values of one.
+template <int D, int R>
+__device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* __restrict__ d, int kh, f16* ring) {
+  constexpr int KP = D / 32, PE = PAGE * D, STAGE = 4 * PE;       // pieces of 1 KiB a wave fetches; elements of a page's keys; of a stage
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int G = a.Hq / a.Hkv, first = d[0], rows = d[1] * G, page0 = d[2], slot = d[4];
+  const int page1 = page0 + d[3] < a.max_blocks ? page0 + d[3] : a.max_blocks;
+  const int seq = sequence_of(a, first, d[1]);
+  const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
+  const f16* src = (wave & 1 ? a.v_cache : a.k_cache) + (size_t)kh * PE + lane * 8;
+  int own = page0 + lane < page1 ? bt[page0 + lane] : -1;
+  int chunk = 0;                                            // pages ahead of `own`
+  int next = page0;
+  auto issue = [&](int slot_) {
+    const int pg = next + (wave >> 1);
+    if (next - page0 - chunk >= 64) {                       // uniform
+      chunk += 64;
+      own = page0 + chunk + lane < page1 ? bt[page0 + chunk + lane] : -1;
+    }
+    int id = pg < page1 ? page_id(a, __builtin_amdgcn_readlane(own, (pg - page0) & 63)) : -1;
+    id = id < 0 ? 0 : id;                                   // a page that is none: a valid address, and not multiplied
+    const f16* p = src + (size_t)id * a.Hkv * PE;
+    f16* l = ring + slot_ * STAGE + wave * PE;
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p + j * 512), (__attribute__((address_space(3))) void*)(l + j * 512), 16, 0, 0);
+    next += 2;
+  };
+#pragma unroll
+  for (int i = 0; i < SA_RING - 1; ++i) issue(i);
+  const int tile = wave % R, share = wave / R, r = tile * 16 + col;
+  Tile<D> t;
+  tile_begin(t, a, r < rows ? a.members[first + r / G] : -1, kh * G + (r < rows ? r % G : 0));
+  int ids = page0 + lane < page1 ? bt[page0 + lane] : -1;   // of the pages that are multiplied
+  int rd = 0, wr = SA_RING - 1;
+  for (int pg = page0; pg < page1; pg += 2) {
+    wait_loads<KP*(SA_RING - 2)>();                         // this wave's part of the stage has landed, its reads of the one before are done
+    bare_barrier();
+    issue(wr);
+    const f16* st = ring + rd * STAGE;
+    rd = rd + 1 == SA_RING ? 0 : rd + 1;
+    wr = wr + 1 == SA_RING ? 0 : wr + 1;
+    if (((pg - page0) & 63) == 0 && pg > page0) ids = pg + lane < page1 ? bt[pg + lane] : -1;
+    if (tile * 16 >= rows) continue;                        // uniform: no row of this wave exists; it takes its part in the loads
+    const bool one = page_id(a, __builtin_amdgcn_readlane(ids, (pg - page0) & 63)) >= 0;
+    const bool two = pg + 1 < page1 && page_id(a, __builtin_amdgcn_readlane(ids, (pg + 1 - page0) & 63)) >= 0;
+    auto kf = [&](int p) { return [=](int q, int kb) { return ld8(st + (p + q) * 2 * PE + kb * 512 + lane * 8); }; };
+    auto vf = [&](int p) { return [=](int q, int db) { return *reinterpret_cast<const f16x4*>(st + (p + q) * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); }; };
+    if constexpr (R == 4) {
+      if (one && two) tile_step<D, 2>(t, a.scale, pg, kf(0), vf(0));
+      else if (one) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
+      else if (two) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
+    } else {
+      if (share == 0 ? one : two) tile_step<D, 1>(t, a.scale, pg + share, kf(share), vf(share));
+    }
+  }
+  tile_end(t);
+  wait_loads<0>();                                          // the requests past the end, too, ahead of the end or of what the ring holds next
+  if constexpr (R == 2) {                                   // the second share's rows join the first's
+    float* o = reinterpret_cast<float*>(ring) + tile * (16 * D);
+    float* ml = reinterpret_cast<float*>(ring) + 2 * 16 * D + tile * 32;
+    bare_barrier();
+    if (share == 1) {
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(o + db * 256 + lane * 4) = t.o[db];
+      if (g == 0) {
+        ml[col] = t.m;
+        ml[16 + col] = t.l;
+      }
+    }
+    __syncthreads();
+    if (share == 1) return;
+    const float m1 = ml[col], m = fmaxf(t.m, m1), base = m == -INFINITY ? 0.f : m;
+    const float f0 = __builtin_amdgcn_exp2f(t.m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
+    t.l = t.l * f0 + ml[16 + col] * f1;
+    t.m = m;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) t.o[db] = t.o[db] * f0 + *reinterpret_cast<const f32x4*>(o + db * 256 + lane * 4) * f1;
+  }
+  tile_store(t, a, slot);
+}
+
+template <int D>
+__global__ __launch_bounds__(SA_WAVES * WAVE, 2) void shared_attn_kernel(SharedAttn a) {
+  __shared__ __align__(16) f16 ring[SA_RING * 4 * PAGE * D];
+  int i = blockIdx.x;
+  if (i < a.n_block * a.Hkv) {
+    const int32_t* __restrict__ d = a.units + 8 * (i / a.Hkv);
+    if (d[1] * (a.Hq / a.Hkv) > 32) block_unit<D, 4>(a, d, i % a.Hkv, ring);
+    else block_unit<D, 2>(a, d, i % a.Hkv, ring);
+    return;
+  }
+  i -= a.n_block * a.Hkv;
+  const int per = (a.Hkv + SA_WAVES - 1) / SA_WAVES;
+  const int kh = i % per * SA_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (kh < a.Hkv) wave_unit<D>(a, a.n_block + i / per, kh);
+}
+
+// A row's units joined: W waves for a (row, head), each taking every W-th unit
+template <int D, int W>
 __global__ __launch_bounds__(4 * WAVE) void shared_attn_join_kernel(SharedAttn a) {
-  const int h = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
-  if (h >= a.Hq) return;
+  constexpr int PER = D / WAVE;
+  __shared__ float so[W > 1 ? W : 1][D], sm[W], sl[W];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = blockIdx.y;
+  const int h = W > 1 ? blockIdx.x : blockIdx.x * 4 + wave, w0 = W > 1 ? wave : 0;
+  if (h >= a.Hq) return;                                    // (whole workgroups where waves meet)
   const int n = a.row_slots[b] + a.own_splits;
   const size_t at = ((size_t)b * a.Hq + h) * a.slots;
-  constexpr int PER = D / WAVE;
   float M = -INFINITY, L = 0.f, o[PER] = {};
-  for (int s = 0; s < n; ++s) M = fmaxf(M, a.ml[2 * (at + s)]);
-  for (int s = 0; s < n; ++s) {
-    const float m = a.ml[2 * (at + s)], f = m == -INFINITY ? 0.f : __expf(m - M);
-    L += a.ml[2 * (at + s) + 1] * f;
+  for (int s0 = w0; s0 < n; s0 += 4 * W) {                  // four units at a time, requested together
+    f32x2 ml[4];
+    float x[4][PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] += a.acc[(at + s) * D + lane * PER + e] * f;
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * W;
+      ml[u] = s < n ? *reinterpret_cast<const f32x2*>(a.ml + 2 * (at + s)) : f32x2{-INFINITY, 0.f};
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[u][e] = s < n ? a.acc[(at + s) * D + lane * PER + e] : 0.f;
+    }
+    float m = M;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) m = fmaxf(m, ml[u][0]);
+    const float base = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(M - base);
+    M = m;
+    L *= f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float fu = __builtin_amdgcn_exp2f(ml[u][0] - base);
+      L += ml[u][1] * fu;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] += x[u][e] * fu;
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) so[wave][lane * PER + e] = o[e];
+    if (lane == 0) {
+      sm[wave] = M;
+      sl[wave] = L;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float m = sm[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) m = fmaxf(m, sm[w]);
+    const float base = m == -INFINITY ? 0.f : m;
+    L = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w] - base);
+      L += sl[w] * f;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] += so[w][lane * PER + e] * f;
+    }
   }
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
@@ -239,14 +419,14 @@ extern "C" size_t mlora_shared_attn_workspace_bytes(int B, int Hq, int D, int sl
 }
 
 extern "C" int mlora_paged_attn_decode_shared(void* out, int out_layout, const void* qkv, const void* k_cache, const void* v_cache, const int32_t* block_table,
-                                              int max_blocks, const int32_t* seq_ids, const int32_t* ctx_len, const int32_t* units, int n_units,
-                                              const int32_t* members, int n_members, const int32_t* row_pages, const int32_t* row_slots, int own_splits,
+                                              int max_blocks, const int32_t* seq_ids, const int32_t* ctx_len, const int32_t* units, int n_block,
+                                              int n_units, const int32_t* members, int n_members, const int32_t* row_pages, const int32_t* row_slots, int own_splits,
                                               int slots, int B, int Hq, int Hkv, int D, int n_pages, int n_seq, void* workspace, size_t workspace_bytes,
                                               void* stream) {
   if (int e = mlora_check_attn("paged_attn_decode_shared", Hq, Hkv, D, n_pages, n_seq, max_blocks)) return e;
   MLORA_CHECK(out && qkv && k_cache && v_cache && block_table && seq_ids && ctx_len && row_pages && row_slots, MLORA_ERR_INVALID, "paged_attn_decode_shared: null pointer");
-  MLORA_CHECK(n_units >= 0 && n_members >= 0 && (n_units == 0 || (units && members && n_members > 0)), MLORA_ERR_INVALID, "paged_attn_decode_shared: bad plan");
-  MLORA_CHECK(B >= 0 && own_splits > 0 && slots >= own_splits && (long)B * own_splits + n_units <= 65535, MLORA_ERR_INVALID,
+  MLORA_CHECK(n_block >= 0 && n_units >= n_block && n_members >= 0 && (n_units == 0 || (units && members && n_members > 0)), MLORA_ERR_INVALID, "paged_attn_decode_shared: bad plan");
+  MLORA_CHECK(B >= 0 && B <= 65535 && own_splits > 0 && slots >= own_splits && ((long)B * own_splits + n_units) * Hkv <= 0x7fffffff, MLORA_ERR_INVALID,
               "paged_attn_decode_shared: B=%d with %d units and %d shares of a row's own pages", B, n_units, own_splits);
   MLORA_CHECK(Hq / Hkv <= 16, MLORA_ERR_UNSUPPORTED, "paged_attn_decode_shared: more than 16 query heads per kv head (%d)", Hq / Hkv);
   MLORA_CHECK(out_layout == MLORA_ROWMAJOR || out_layout == MLORA_FRAG, MLORA_ERR_INVALID, "paged_attn_decode_shared: bad out_layout %d", out_layout);
@@ -254,19 +434,17 @@ extern "C" int mlora_paged_attn_decode_shared(void* out, int out_layout, const v
   MLORA_CHECK(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= mlora_shared_attn_workspace_bytes(B, Hq, D, slots), MLORA_ERR_WORKSPACE,
               "paged_attn_decode_shared: workspace of %zu bytes, %zu needed", workspace_bytes, mlora_shared_attn_workspace_bytes(B, Hq, D, slots));
   SharedAttn a = {(f16*)out, (const f16*)qkv, (const f16*)k_cache, (const f16*)v_cache, block_table, seq_ids, ctx_len, units, members, row_pages, row_slots,
-                  (float*)workspace, (float*)workspace + (size_t)B * Hq * slots * D, max_blocks, B, Hq, Hkv, n_pages, n_seq, n_units, n_members, own_splits, slots,
-                  out_layout == MLORA_FRAG ? mlora_frag_tiles(B) : 0, 1.f / sqrtf((float)D)};
+                  (float*)workspace, (float*)workspace + (size_t)B * Hq * slots * D, max_blocks, B, Hq, Hkv, n_pages, n_seq, n_block, n_units, own_splits, slots,
+                  out_layout == MLORA_FRAG ? mlora_frag_tiles(B) : 0, LOG2E / sqrtf((float)D)};
   hipStream_t s = (hipStream_t)stream;
-#define MLORA_SHARED(DD)                                                                                                                         \
-  do {                                                                                                                                           \
-    constexpr size_t lds = (size_t)SA_WAVES * 16 * DD * sizeof(float);                                                                           \
-    static const hipError_t configured =                                                                                                         \
-        hipFuncSetAttribute((const void*)shared_attn_kernel<DD>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                          \
-    if (configured != hipSuccess)                                                                                                                \
-      return mlora_set_error(MLORA_ERR_LAUNCH, "paged_attn_decode_shared: cannot reserve %zu bytes of LDS: %s", lds, hipGetErrorString(configured)); \
-    hipLaunchKernelGGL(shared_attn_kernel<DD>, dim3(Hkv, n_units + B * own_splits), dim3(SA_WAVES * WAVE), lds, s, a);                           \
-    if (int e = mlora_launch_status("paged_attn_decode_shared")) return e;                                                                       \
-    hipLaunchKernelGGL(shared_attn_join_kernel<DD>, dim3(ceil_div(Hq, 4), B), dim3(4 * WAVE), 0, s, a);                                          \
+  const unsigned grid = (unsigned)(n_block * Hkv + ((long)B * own_splits + n_units - n_block) * ceil_div(Hkv, SA_WAVES));
+  const bool many = slots > 8;                              // units of a row: a wave joins up to eight in two rounds
+#define MLORA_SHARED(DD)                                                                                                                          \
+  do {                                                                                                                                            \
+    hipLaunchKernelGGL(shared_attn_kernel<DD>, dim3(grid), dim3(SA_WAVES * WAVE), 0, s, a);                                                       \
+    if (int e = mlora_launch_status("paged_attn_decode_shared")) return e;                                                                        \
+    if (many) hipLaunchKernelGGL((shared_attn_join_kernel<DD, 4>), dim3(Hq, B), dim3(4 * WAVE), 0, s, a);                                         \
+    else hipLaunchKernelGGL((shared_attn_join_kernel<DD, 1>), dim3(ceil_div(Hq, 4), B), dim3(4 * WAVE), 0, s, a);                                 \
   } while (0)
   if (D == 128) MLORA_SHARED(128);
   else MLORA_SHARED(64);

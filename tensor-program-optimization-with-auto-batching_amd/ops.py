@@ -965,29 +965,35 @@ class SharedPrefixPlan:
         for rows, pages in groups:
             for r in rows:
                 row_pages[r] = pages
-        most = lib().mlora_shared_attn_unit_rows() // G                  # members of a unit
         own = [-(-n // 16) - p for n, p in zip(lens, row_pages)]
-        per = self._pages_per_unit(sum(-(-len(rows) // most) * pages for rows, pages in groups) + sum(own), Hkv)
+        large = [(rows, pages) for rows, pages in groups if len(rows) * G > 16]
+        small = [(rows, pages) for rows, pages in groups if len(rows) * G <= 16]
+        groups = large + small
+        members = [r for rows, _ in groups for r in rows]
+        most = lib().mlora_shared_attn_unit_rows() // G                  # members of a block unit
+        # pages of a unit: block units for two workgroups on each compute unit, wave units for eight waves - no shorter than some pages, and no
+        # more units of a row than its second launch joins cheaply
+        per_block = max(8, -(-sum(-(-len(rows) // most) * pages for rows, pages in large) * Hkv // 512))
+        per_wave = max(4, -(-(sum(p for _, p in small) + sum(own)) * Hkv // 2048))
         units, first = [], 0
-        for rows, pages in groups:
-            n = -(-pages // per)
+        for i, (rows, pages) in enumerate(groups):
+            block = i < len(large)
+            n = min(-(-pages // (per_block if block else per_wave)), 64)
             cut = [pages * i // n for i in range(n + 1)]
+            parts = -(-len(rows) // most) if block else 1
+            edge = [len(rows) * i // parts for i in range(parts + 1)]
             for r in rows:
                 row_slots[r] = n
-            for m in range(0, len(rows), most):
-                units += [(first + m, min(most, len(rows) - m), a, b - a, i, 0, 0, 0) for i, (a, b) in enumerate(zip(cut, cut[1:]))]
+            units += [(not block, first + a, b - a, lo, hi - lo, j) for a, b in zip(edge, edge[1:]) for j, (lo, hi) in enumerate(zip(cut, cut[1:]))]
             first += len(rows)
-        self.own_splits = max(1, min(-(-max(own, default=0) // per), 65535 // max(B, 1) - len(units) // max(B, 1) - 1))
-        units.sort(key=lambda u: -u[3] * u[1])
+        units = [(*u[1:], 0, 0, 0) for u in sorted(units, key=lambda u: (u[0], -u[4]))]
+        self.n_block = sum(u[1] * G > 16 for u in units)
+        self.own_splits = max(1, min(-(-max(own, default=0) // per_wave), 64))
         self.n_units, self.slots = len(units), max(row_slots, default=0) + self.own_splits
         flat = torch.tensor([x for u in units for x in u] + members + row_pages + row_slots, dtype=torch.int32)
         self.data = upload(flat, device)
         at = [0, 8 * len(units), 8 * len(units) + len(members)]
         self.units, self.members, self.row_pages, self.row_slots = (self.data[a:b] for a, b in zip(at + [at[2] + B], at[1:] + [at[2] + B, at[2] + 2 * B]))
-
-    @staticmethod
-    def _pages_per_unit(pages, Hkv):
-        return max(8, -(-pages * Hkv // 1024))
 
 
 def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, plan: SharedPrefixPlan, Hq, Hkv, D, out=None, frag=False):
@@ -1012,7 +1018,7 @@ def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_le
     f16, i32 = torch.float16, torch.int32
     check(L.mlora_paged_attn_decode_shared(optr, lay, _dev(qkv, f16, "qkv"), _dev(k_cache, f16, "k_cache"), _dev(v_cache, f16, "v_cache"),
                                            _dev(block_table, i32, "block_table"), max_blocks, _dev(seq_ids, i32, "seq_ids"), _dev(ctx_len, i32, "ctx_len"),
-                                           plan.units.data_ptr(), plan.n_units, plan.members.data_ptr(), plan.n_members, plan.row_pages.data_ptr(),
+                                           plan.units.data_ptr(), plan.n_block, plan.n_units, plan.members.data_ptr(), plan.n_members, plan.row_pages.data_ptr(),
                                            plan.row_slots.data_ptr(), plan.own_splits, plan.slots, B, Hq, Hkv, D, k_cache.shape[0], n_seq, ws.data_ptr(), nb,
                                            _stream()))
     return out

@@ -44,14 +44,14 @@ def test_linear4_refusals():
 
 def test_shared_attention_refusals():
     lib = load_pkg("_lib").lib()
-    assert lib.mlora_shared_attn_unit_rows() == 128
+    assert lib.mlora_shared_attn_unit_rows() == 64
     need = lib.mlora_shared_attn_workspace_bytes(4, 8, 128, 3)
     assert need == 4 * 8 * 3 * 130 * 4 and lib.mlora_shared_attn_workspace_bytes(0, 8, 128, 3) == 0
-    def call(out=16, lay=0, units=16, n_units=1, members=16, n_members=2, row_pages=16, own=2, slots=3, B=4, Hq=8, Hkv=8, D=128, ws=16, nb=need):
-        return lib.mlora_paged_attn_decode_shared(out, lay, 16, 16, 16, 16, 4, 16, 16, units, n_units, members, n_members, row_pages, 16, own, slots, B, Hq, Hkv, D,
+    def call(out=16, lay=0, units=16, n_block=1, n_units=1, members=16, n_members=2, row_pages=16, own=2, slots=3, B=4, Hq=8, Hkv=8, D=128, ws=16, nb=need):
+        return lib.mlora_paged_attn_decode_shared(out, lay, 16, 16, 16, 16, 4, 16, 16, units, n_block, n_units, members, n_members, row_pages, 16, own, slots, B, Hq, Hkv, D,
                                                   5, 4, ws, nb, None)
-    assert call(out=None) == -1 and call(row_pages=None) == -1 and call(units=None) == -1 and call(n_members=0) == -1 and call(n_units=-1) == -1
+    assert call(out=None) == -1 and call(row_pages=None) == -1 and call(units=None) == -1 and call(n_members=0) == -1 and call(n_units=-1) == -1 and call(n_block=2) == -1 and call(n_block=-1) == -1
     assert call(D=96) == -2 and call(Hkv=3) == -1 and call(Hq=34, Hkv=2) == -2 and call(lay=5) == -1
-    assert call(own=0) == -1 and call(slots=1) == -1 and call(B=-1) == -1 and call(B=40000) == -1
+    assert call(own=0) == -1 and call(slots=1) == -1 and call(B=-1) == -1 and call(B=70000) == -1
     assert call(ws=None) == -3 and call(nb=need - 1) == -3 and call(ws=24) == -3
     assert call(B=0) == 0

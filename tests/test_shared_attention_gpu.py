@@ -170,6 +170,10 @@ def test_invalid_rows_and_pages(ops):
     got = call(ops, c)
     assert torch.equal(got[[0, 2]], want[[0, 2]]) and bool((got[[1, 3, 4]] == 0).all())
     c["rows"].copy_(keep)
+    c["rows"][0] = -1                                                  # the first of its group
+    got = call(ops, c)
+    assert torch.equal(got[1:], want[1:]) and bool((got[0] == 0).all())
+    c["rows"].copy_(keep)
     c["ctx"].copy_(torch.tensor([70, 80, -5, 2 ** 30, 20], dtype=torch.int32))
     c["table"][int(keep[3]), 1:] = 2 ** 30
     got = call(ops, c)
