@@ -203,10 +203,11 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
   f16x8 k[2][2][NKB];
   f16x4 v[2][2][NDB];
   int id[2][2];
-  auto load = [&](int s, int pg, int own) {                 // pages pg, pg + 1 into set s; own: the lane's page id of the chunk
+  int own = -1, from = page0, to = page0;                   // the ids of up to 64 pages from .. to - 1, one a lane
+  auto load = [&](int s, int pg) {                          // pages pg, pg + 1 into set s
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      id[s][p] = pg + p < page1 ? page_id(a, __builtin_amdgcn_readlane(own, (pg + p - page0) & 63)) : -1;
+      id[s][p] = pg + p < to ? page_id(a, __builtin_amdgcn_readlane(own, pg + p - from)) : -1;
       if (id[s][p] < 0) continue;                           // uniform
       const f16* kp = a.k_cache + ((size_t)id[s][p] * a.Hkv + kh) * (PAGE * D) + lane * 8;
       const f16* vp = a.v_cache + (((size_t)id[s][p] * a.Hkv + kh) * D + col) * PAGE + g * 4;
@@ -216,10 +217,7 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
       for (int db = 0; db < NDB; ++db) v[s][p][db] = *reinterpret_cast<const f16x4*>(vp + db * 16 * PAGE);
     }
   };
-  int own = page0 + lane < page1 ? bt[page0 + lane] : -1;   // the ids of up to 64 pages, one a lane
-  load(0, page0, own);
   Tile<D> t;
-  tile_begin(t, a, row, kh * G + (row >= 0 ? col % G : 0));
   auto work = [&](int s, int pg) {
     auto kf = [&](int p) { return [&, p](int q, int kb) { return k[s][p + q][kb]; }; };
     auto vf = [&](int p) { return [&, p](int q, int db) { return v[s][p + q][db]; }; };
@@ -227,13 +225,22 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
     else if (id[s][0] >= 0) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
     else if (id[s][1] >= 0) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
   };
-  for (int pg = page0; pg < page1; pg += 4) {
-    load(1, pg + 2, own);
-    work(0, pg);
-    if (((pg + 4 - page0) & 63) == 0) own = pg + 4 + lane < page1 ? bt[pg + 4 + lane] : -1;
-    load(0, pg + 4, own);
-    work(1, pg + 2);
-  }
+  // 64 pages at a time: the wait for ids loaded inside the loop would be one for every page on its way
+  bool begun = false;
+  do {
+    to = from + 64 < page1 ? from + 64 : page1;
+    own = from + lane < to ? bt[from + lane] : -1;
+    load(0, from);
+    if (!begun) tile_begin(t, a, row, kh * G + (row >= 0 ? col % G : 0));
+    begun = true;
+    for (int pg = from; pg < to; pg += 4) {
+      load(1, pg + 2);
+      work(0, pg);
+      load(0, pg + 4);
+      work(1, pg + 2);
+    }
+    from = to;
+  } while (from < page1);
   tile_end(t);
   tile_store(t, a, slot);
 }
@@ -251,54 +258,52 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
   const int seq = sequence_of(a, first, d[1]);
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
   const f16* src = (wave & 1 ? a.v_cache : a.k_cache) + (size_t)kh * PE + lane * 8;
-  int own = page0 + lane < page1 ? bt[page0 + lane] : -1;
-  int chunk = 0;                                            // pages ahead of `own`
-  int next = page0;
-  auto issue = [&](int slot_) {
-    const int pg = next + (wave >> 1);
-    if (next - page0 - chunk >= 64) {                       // uniform
-      chunk += 64;
-      own = page0 + chunk + lane < page1 ? bt[page0 + chunk + lane] : -1;
-    }
-    int id = pg < page1 ? page_id(a, __builtin_amdgcn_readlane(own, (pg - page0) & 63)) : -1;
-    id = id < 0 ? 0 : id;                                   // a page that is none: a valid address, and not multiplied
-    const f16* p = src + (size_t)id * a.Hkv * PE;
-    f16* l = ring + slot_ * STAGE + wave * PE;
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p + j * 512), (__attribute__((address_space(3))) void*)(l + j * 512), 16, 0, 0);
-    next += 2;
-  };
-#pragma unroll
-  for (int i = 0; i < SA_RING - 1; ++i) issue(i);
   const int tile = wave % R, share = wave / R, r = tile * 16 + col;
   Tile<D> t;
-  tile_begin(t, a, r < rows ? a.members[first + r / G] : -1, kh * G + (r < rows ? r % G : 0));
-  int ids = page0 + lane < page1 ? bt[page0 + lane] : -1;   // of the pages that are multiplied
-  int rd = 0, wr = SA_RING - 1;
-  for (int pg = page0; pg < page1; pg += 2) {
-    wait_loads<KP*(SA_RING - 2)>();                         // this wave's part of the stage has landed, its reads of the one before are done
-    bare_barrier();
-    issue(wr);
-    const f16* st = ring + rd * STAGE;
-    rd = rd + 1 == SA_RING ? 0 : rd + 1;
-    wr = wr + 1 == SA_RING ? 0 : wr + 1;
-    if (((pg - page0) & 63) == 0 && pg > page0) ids = pg + lane < page1 ? bt[pg + lane] : -1;
-    if (tile * 16 >= rows) continue;                        // uniform: no row of this wave exists; it takes its part in the loads
-    const bool one = page_id(a, __builtin_amdgcn_readlane(ids, (pg - page0) & 63)) >= 0;
-    const bool two = pg + 1 < page1 && page_id(a, __builtin_amdgcn_readlane(ids, (pg + 1 - page0) & 63)) >= 0;
-    auto kf = [&](int p) { return [=](int q, int kb) { return ld8(st + (p + q) * 2 * PE + kb * 512 + lane * 8); }; };
-    auto vf = [&](int p) { return [=](int q, int db) { return *reinterpret_cast<const f16x4*>(st + (p + q) * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); }; };
-    if constexpr (R == 4) {
-      if (one && two) tile_step<D, 2>(t, a.scale, pg, kf(0), vf(0));
-      else if (one) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
-      else if (two) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
-    } else {
-      if (share == 0 ? one : two) tile_step<D, 1>(t, a.scale, pg + share, kf(share), vf(share));
+  // 64 pages at a time: the wait for ids loaded inside the loop would be one for the whole ring
+  for (int from = page0; from < page1; from += 64) {
+    const int to = from + 64 < page1 ? from + 64 : page1;
+    const int own = from + lane < to ? bt[from + lane] : -1;
+    int next = from;
+    auto issue = [&](int slot_) {
+      const int pg = next + (wave >> 1);
+      int id = pg < to ? page_id(a, __builtin_amdgcn_readlane(own, pg - from)) : -1;
+      id = id < 0 ? 0 : id;                                 // a page that is none: a valid address, and not multiplied
+      const f16* p = src + (size_t)id * a.Hkv * PE;
+      f16* l = ring + slot_ * STAGE + wave * PE;
+#pragma unroll
+      for (int j = 0; j < KP; ++j)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p + j * 512), (__attribute__((address_space(3))) void*)(l + j * 512), 16, 0, 0);
+      next += 2;
+    };
+    if (from > page0) bare_barrier();                       // (everybody is done with the ring)
+#pragma unroll
+    for (int i = 0; i < SA_RING - 1; ++i) issue(i);
+    if (from == page0) tile_begin(t, a, r < rows ? a.members[first + r / G] : -1, kh * G + (r < rows ? r % G : 0));
+    int rd = 0, wr = SA_RING - 1;
+    for (int pg = from; pg < to; pg += 2) {
+      wait_loads<KP*(SA_RING - 2)>();                       // this wave's part of the stage has landed, its reads of the one before are done
+      bare_barrier();
+      issue(wr);
+      const f16* st = ring + rd * STAGE;
+      rd = rd + 1 == SA_RING ? 0 : rd + 1;
+      wr = wr + 1 == SA_RING ? 0 : wr + 1;
+      if (tile * 16 >= rows) continue;                      // uniform: no row of this wave exists; it takes its part in the loads
+      const bool one = page_id(a, __builtin_amdgcn_readlane(own, pg - from)) >= 0;
+      const bool two = pg + 1 < to && page_id(a, __builtin_amdgcn_readlane(own, pg + 1 - from)) >= 0;
+      auto kf = [&](int p) { return [=](int q, int kb) { return ld8(st + (p + q) * 2 * PE + kb * 512 + lane * 8); }; };
+      auto vf = [&](int p) { return [=](int q, int db) { return *reinterpret_cast<const f16x4*>(st + (p + q) * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); }; };
+      if constexpr (R == 4) {
+        if (one && two) tile_step<D, 2>(t, a.scale, pg, kf(0), vf(0));
+        else if (one) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
+        else if (two) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
+      } else {
+        if (share == 0 ? one : two) tile_step<D, 1>(t, a.scale, pg + share, kf(share), vf(share));
+      }
     }
+    wait_loads<0>();                                        // the requests past the end, too, ahead of the end or of what the ring holds next
   }
   tile_end(t);
-  wait_loads<0>();                                          // the requests past the end, too, ahead of the end or of what the ring holds next
   if constexpr (R == 2) {                                   // the second share's rows join the first's
     float* o = reinterpret_cast<float*>(ring) + tile * (16 * D);
     float* ml = reinterpret_cast<float*>(ring) + 2 * 16 * D + tile * 32;
