@@ -408,17 +408,18 @@ int mlora_paged_attn_prefill(void* out, int out_layout, const void* qkv, const v
 
 /* mlora_paged_attn_decode for a batch whose rows share prefixes: groups of rows whose block tables begin with the same pages, which
  * are read once per group.  The same result up to the order of fp32 sums; slots of a page behind a row's context may hold anything.
- * The plan (device arrays): members, the batch rows of the groups one after the other, every row at most once; units [n_units][8]
- * = {first member, members, first page, pages, slot, 0, 0, 0}: rows attended over a range of their group's pages, into that slot of each -
- * first n_block units of at most mlora_shared_attn_unit_rows query rows (members times Hq / Hkv), then units of at most 16; row_pages [B]:
- * shared pages ahead of a row's own (0: none); row_slots [B]: units over those, which have slots 0, 1, ...  A row's own pages are cut into
- * own_splits shares, whose results take the slots behind; slots: most slots of a row.  A row's context does not end within its shared pages.
- * Two launches; workspace of mlora_shared_attn_workspace_bytes, 16-byte aligned. */
+ * The plan (device arrays): units [n_units][mlora_shared_attn_record_ints()] = {rows, first page, pages, slot, four of any value, then
+ * mlora_shared_attn_unit_rows() batch rows, those behind the unit's any row}: rows of a group attended over a range of the group's pages, into
+ * that slot of each - first n_block units of at most mlora_shared_attn_unit_rows query rows (rows times Hq / Hkv), then units of at most 16;
+ * row_pages [B]: shared pages ahead of a row's own (0: none); row_slots [B]: units over those, which have slots 0, 1, ...  A row is in one
+ * group at most.  A row's own pages are cut into own_splits shares, whose results take the slots behind; slots: most slots of a row.  A row's
+ * context does not end within its shared pages.  Two launches; workspace of mlora_shared_attn_workspace_bytes, 16-byte aligned. */
+int mlora_shared_attn_record_ints(void);
 int mlora_shared_attn_unit_rows(void);
 size_t mlora_shared_attn_workspace_bytes(int B, int Hq, int D, int slots);
 int mlora_paged_attn_decode_shared(void* out, int out_layout, const void* qkv, const void* k_cache, const void* v_cache, const int32_t* block_table,
                                    int max_blocks, const int32_t* seq_ids, const int32_t* ctx_len, const int32_t* units, int n_block,
-                                   int n_units, const int32_t* members, int n_members, const int32_t* row_pages, const int32_t* row_slots, int own_splits,
+                                   int n_units, const int32_t* row_pages, const int32_t* row_slots, int own_splits,
                                    int slots, int B, int Hq, int Hkv, int D, int n_pages, int n_seq, void* workspace, size_t workspace_bytes,
                                    void* stream);
 

@@ -93,7 +93,8 @@ SIGNATURES = {
     "mlora_paged_attn_decode": (_i, [_p, _i, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
     "mlora_shared_attn_unit_rows": (_i, []),
     "mlora_shared_attn_workspace_bytes": (_z, [_i, _i, _i, _i]),
-    "mlora_paged_attn_decode_shared": (_i, [_p, _i, _p, _p, _p, _p, _i, _p, _p, _p, _i, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p, _z, _p]),
+    "mlora_shared_attn_record_ints": (_i, []),
+    "mlora_paged_attn_decode_shared": (_i, [_p, _i, _p, _p, _p, _p, _i, _p, _p, _p, _i, _i, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p, _z, _p]),
     "mlora_paged_attn_prefill": (_i, [_p, _i, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
 }
 

@@ -11,8 +11,8 @@
 // kernel in attention.hip: S^T = K . Q^T, then O^T += V^T . P^T, where a lane's probabilities are already the operand that it must supply
 // - as two fp16 halves, so that they enter with 22 bits - and the keys of two pages fill a k-step.
 //   block units  17 to 64 query rows of a group: four waves share pages that come straight into an LDS ring
-//   wave units   up to 16 query rows - a small group, or the pages of a single request behind its prefix: a wave for itself, the next two
-//                pages on their way to registers
+//   wave units   up to 16 query rows - a small group, or the pages of a single request behind its prefix: a wave for itself, the next
+//                page on its way to registers
 #include "lora_device.h"
 
 namespace {
@@ -21,6 +21,7 @@ constexpr int PAGE = MLORA_PAGE_SIZE;
 constexpr int SA_WAVES = 4;
 constexpr int SA_ROWS = 16 * SA_WAVES;        // query rows of a block unit
 constexpr int SA_RING = 3;                    // stages of two pages
+constexpr int SA_RECORD = 8 + SA_ROWS;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct SharedAttn {
@@ -31,8 +32,7 @@ struct SharedAttn {
   const int32_t* block_table;
   const int32_t* seq_ids;
   const int32_t* ctx_len;
-  const int32_t* units;        // [n_units][8] {first member, members, first page, pages, slot}, the n_block block units first
-  const int32_t* members;      // batch rows, group after group
+  const int32_t* units;        // [n_units][SA_RECORD] {rows, first page, pages, slot, 0 .., then up to SA_ROWS batch rows}, the n_block block units first
   const int32_t* row_pages;    // [B] shared pages ahead of a row's own
   const int32_t* row_slots;    // [B] units over those
   float* acc;                  // [B][Hq][slots][D]
@@ -51,12 +51,21 @@ __device__ __forceinline__ int context_of(const SharedAttn& a, int row, int& seq
   return c < 0 ? 0 : c > a.max_blocks * PAGE ? a.max_blocks * PAGE : c;
 }
 
-// the sequence whose table names the pages of a unit's members: the first that is one
-__device__ __forceinline__ int sequence_of(const SharedAttn& a, int first, int n) {
+// the sequence whose table names the pages of a unit's rows (a lane each): the first that is one
+__device__ __forceinline__ int sequence_of(const SharedAttn& a, const int32_t* __restrict__ d) {
   const int lane = threadIdx.x & 63;
-  const int seq = lane < n ? a.seq_ids[a.members[first + lane]] : -1;
+  const int row = d[8 + lane], seq = lane < d[0] ? a.seq_ids[row] : -1;
   const unsigned long long ok = __ballot(seq >= 0 && seq < a.n_seq);
   return ok ? __builtin_amdgcn_readlane(seq, __builtin_ctzll(ok)) : 0;
+}
+
+// the maximum over the lanes of a column, i.e. over the four rows of 16 lanes: each swap exchanges rows (halves) of two copies, which then hold one
+// partner each.  (Through LDS, as a shuffle goes, it is 300 cycles on the way from the scores to the weights.)
+__device__ __forceinline__ float groups_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // a tile of 16 query rows: lane (g, col) has row col, its dims 16 db + 4 g .. + 3 of the output and a quarter of its sum
@@ -94,10 +103,11 @@ __device__ __forceinline__ void tile_begin(Tile<D>& t, const SharedAttn& a, int 
   for (int db = 0; db < D / 16; ++db) t.o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// P pages pg, pg + 1, ..: keys k(p, kb) in fragment order, values v(p, db) of tokens 4 g .. + 3
-template <int D, int P, class K, class V>
-__device__ __forceinline__ void tile_step(Tile<D>& t, float scale, int pg, K k, V v) {
-  const int g = (threadIdx.x & 63) >> 4;
+// P pages pg, pg + 1, ..: keys k(p, kb) in fragment order, values v(p, db) of tokens 4 g .. + 3.  EDGE: some row may end within them, or one of
+// them may be none (pages: bit p).  What then does not count is masked without branches - inside one, every value's operand would wait for
+// its own read.
+template <int D, int P, bool EDGE, class K, class V>
+__device__ __forceinline__ void tile_step(Tile<D>& t, float scale, int pg, int pages, K k, V v) {
   f32x4 st[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -105,26 +115,32 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, float scale, int pg, K k, 
 #pragma unroll
     for (int kb = 0; kb < D / 32; ++kb) st[p] = mfma_16x16x32(k(p, kb), t.q[kb], st[p]);
   }
-  const bool edge = (pg + P) * PAGE > t.least;              // uniform: some row ends within these pages
+  uint32_t keep[P][2];                                      // of a lane's four tokens: slots behind every context hold anything
   float pm = -INFINITY;
 #pragma unroll
-  for (int p = 0; p < P; ++p)
+  for (int p = 0; p < P; ++p) {
+    const int first = (pg + p) * PAGE + 4 * ((int)(threadIdx.x & 63) >> 4), here = pages >> p & 1;
+    if constexpr (EDGE) {
+      const int n = here ? t.most - first : 0;
+      keep[p][0] = n > 1 ? ~0u : n > 0 ? 0xffffu : 0u;
+      keep[p][1] = n > 3 ? ~0u : n > 2 ? 0xffffu : 0u;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       st[p][e] *= scale;
-      if (edge && (pg + p) * PAGE + 4 * g + e >= t.ctx) st[p][e] = -INFINITY;
+      if (EDGE && (first + e >= t.ctx || !here)) st[p][e] = -INFINITY;
       pm = fmaxf(pm, st[p][e]);
     }
-  pm = fmaxf(pm, __shfl_xor(pm, 16, WAVE));
-  pm = fmaxf(pm, __shfl_xor(pm, 32, WAVE));
+  }
+  pm = groups_max(pm);
   if (__any(pm > t.m)) {                                    // (after the first pages seldom)
-    const float m = fmaxf(t.m, pm), alpha = __builtin_amdgcn_exp2f(t.m - (m == -INFINITY ? 0.f : m));
+    const float m = fmaxf(t.m, pm), alpha = __builtin_amdgcn_exp2f(t.m - (EDGE && m == -INFINITY ? 0.f : m));
     t.l *= alpha;
     t.m = m;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) t.o[db] *= alpha;
   }
-  const float base = t.m == -INFINITY ? 0.f : t.m;          // a row with no token yet
+  const float base = EDGE && t.m == -INFINITY ? 0.f : t.m;  // a row with no token yet
   f16 hi[P * 4], lo[P * 4];
 #pragma unroll
   for (int p = 0; p < P; ++p)
@@ -137,20 +153,20 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, float scale, int pg, K k, 
     }
 #pragma unroll
   for (int db = 0; db < D / 16; ++db) {
-    f16x4 x[P];
+    union { f16x4 h; uint32_t u[2]; } x[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      x[p] = v(p, db);
-      if (edge && (pg + p + 1) * PAGE > t.most)             // slots behind every context hold anything
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((pg + p) * PAGE + 4 * g + e >= t.most) x[p][e] = (f16)0.f;
+      x[p].h = v(p, db);
+      if constexpr (EDGE) {
+        x[p].u[0] &= keep[p][0];
+        x[p].u[1] &= keep[p][1];
+      }
     }
+    const f16x4 x0 = x[0].h, x1 = x[P - 1].h;               // (one page: its values twice, for both halves of the weights)
+    const f16x8 both = f16x8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     if constexpr (P == 1) {
-      const f16x8 both = f16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[0][0], x[0][1], x[0][2], x[0][3]};
       t.o[db] = mfma_16x16x32(both, f16x8{hi[0], hi[1], hi[2], hi[3], lo[0], lo[1], lo[2], lo[3]}, t.o[db]);
     } else {
-      const f16x8 both = f16x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
       t.o[db] = mfma_16x16x32(both, f16x8{hi[0], hi[1], hi[2], hi[3], hi[4], hi[5], hi[6], hi[7]}, t.o[db]);
       t.o[db] = mfma_16x16x32(both, f16x8{lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]}, t.o[db]);
     }
@@ -182,13 +198,12 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, G = a.Hq / a.Hkv;
   int seq, page0, page1, slot, row;
   if (u < a.n_units) {
-    const int32_t* d = a.units + 8 * u;
-    const int first = d[0], n = d[1];
-    page0 = d[2];
-    page1 = d[2] + d[3];
-    slot = d[4];
-    seq = sequence_of(a, first, n);
-    row = col < n * G ? a.members[first + col / G] : -1;
+    const int32_t* __restrict__ d = a.units + (size_t)SA_RECORD * u;
+    page0 = d[1];
+    page1 = d[1] + d[2];
+    slot = d[3];
+    row = col < d[0] * G ? d[8 + col / G] : -1;
+    seq = sequence_of(a, d);
   } else {
     const int i = u - a.n_units, part = i % a.own_splits, b = i / a.own_splits;
     const int have = (context_of(a, b, seq) + PAGE - 1) / PAGE, from = a.row_pages[b];
@@ -200,44 +215,36 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
   }
   if (page1 > a.max_blocks) page1 = a.max_blocks;
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
-  f16x8 k[2][2][NKB];
-  f16x4 v[2][2][NDB];
-  int id[2][2];
+  f16x8 k[2][NKB];
+  f16x4 v[2][NDB];
+  int id[2];
   int own = -1, from = page0, to = page0;                   // the ids of up to 64 pages from .. to - 1, one a lane
-  auto load = [&](int s, int pg) {                          // pages pg, pg + 1 into set s
+  auto load = [&](int s, int pg) {                          // page pg into set s
+    id[s] = pg < to ? page_id(a, __builtin_amdgcn_readlane(own, (pg - from) & 63)) : -1;
+    if (id[s] < 0) return;                                  // uniform
+    const f16* kp = a.k_cache + ((size_t)id[s] * a.Hkv + kh) * (PAGE * D) + lane * 8;
+    const f16* vp = a.v_cache + (((size_t)id[s] * a.Hkv + kh) * D + col) * PAGE + g * 4;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      id[s][p] = pg + p < to ? page_id(a, __builtin_amdgcn_readlane(own, pg + p - from)) : -1;
-      if (id[s][p] < 0) continue;                           // uniform
-      const f16* kp = a.k_cache + ((size_t)id[s][p] * a.Hkv + kh) * (PAGE * D) + lane * 8;
-      const f16* vp = a.v_cache + (((size_t)id[s][p] * a.Hkv + kh) * D + col) * PAGE + g * 4;
+    for (int kb = 0; kb < NKB; ++kb) k[s][kb] = ld8(kp + kb * 512);
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) k[s][p][kb] = ld8(kp + kb * 512);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) v[s][p][db] = *reinterpret_cast<const f16x4*>(vp + db * 16 * PAGE);
-    }
+    for (int db = 0; db < NDB; ++db) v[s][db] = *reinterpret_cast<const f16x4*>(vp + db * 16 * PAGE);
   };
   Tile<D> t;
+  tile_begin(t, a, row, kh * G + (row >= 0 ? col % G : 0));
   auto work = [&](int s, int pg) {
-    auto kf = [&](int p) { return [&, p](int q, int kb) { return k[s][p + q][kb]; }; };
-    auto vf = [&](int p) { return [&, p](int q, int db) { return v[s][p + q][db]; }; };
-    if (id[s][0] >= 0 && id[s][1] >= 0) tile_step<D, 2>(t, a.scale, pg, kf(0), vf(0));
-    else if (id[s][0] >= 0) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
-    else if (id[s][1] >= 0) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
+    if (id[s] >= 0) tile_step<D, 1, true>(t, a.scale, pg, 1, [&](int, int kb) { return k[s][kb]; }, [&](int, int db) { return v[s][db]; });   // uniform
   };
   // 64 pages at a time: the wait for ids loaded inside the loop would be one for every page on its way
-  bool begun = false;
   do {
     to = from + 64 < page1 ? from + 64 : page1;
     own = from + lane < to ? bt[from + lane] : -1;
     load(0, from);
-    if (!begun) tile_begin(t, a, row, kh * G + (row >= 0 ? col % G : 0));
-    begun = true;
-    for (int pg = from; pg < to; pg += 4) {
-      load(1, pg + 2);
+    load(1, from + 1);
+    for (int pg = from; pg < to; pg += 2) {
       work(0, pg);
-      load(0, pg + 4);
-      work(1, pg + 2);
+      load(0, pg + 2);
+      work(1, pg + 1);
+      load(1, pg + 3);
     }
     from = to;
   } while (from < page1);
@@ -253,13 +260,14 @@ template <int D, int R>
 __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* __restrict__ d, int kh, f16* ring) {
   constexpr int KP = D / 32, PE = PAGE * D, STAGE = 4 * PE;       // pieces of 1 KiB a wave fetches; elements of a page's keys; of a stage
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int G = a.Hq / a.Hkv, first = d[0], rows = d[1] * G, page0 = d[2], slot = d[4];
-  const int page1 = page0 + d[3] < a.max_blocks ? page0 + d[3] : a.max_blocks;
-  const int seq = sequence_of(a, first, d[1]);
+  const int G = a.Hq / a.Hkv, rows = d[0] * G, page0 = d[1], slot = d[3];
+  const int page1 = page0 + d[2] < a.max_blocks ? page0 + d[2] : a.max_blocks;
+  const int seq = sequence_of(a, d);
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
   const f16* src = (wave & 1 ? a.v_cache : a.k_cache) + (size_t)kh * PE + lane * 8;
   const int tile = wave % R, share = wave / R, r = tile * 16 + col;
-  Tile<D> t;
+  Tile<D> t;                                                // (ahead of the first pages: loads return in order)
+  tile_begin(t, a, r < rows ? d[8 + r / G] : -1, kh * G + (r < rows ? r % G : 0));
   // 64 pages at a time: the wait for ids loaded inside the loop would be one for the whole ring
   for (int from = page0; from < page1; from += 64) {
     const int to = from + 64 < page1 ? from + 64 : page1;
@@ -279,7 +287,6 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
     if (from > page0) bare_barrier();                       // (everybody is done with the ring)
 #pragma unroll
     for (int i = 0; i < SA_RING - 1; ++i) issue(i);
-    if (from == page0) tile_begin(t, a, r < rows ? a.members[first + r / G] : -1, kh * G + (r < rows ? r % G : 0));
     int rd = 0, wr = SA_RING - 1;
     for (int pg = from; pg < to; pg += 2) {
       wait_loads<KP*(SA_RING - 2)>();                       // this wave's part of the stage has landed, its reads of the one before are done
@@ -291,15 +298,12 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
       if (tile * 16 >= rows) continue;                      // uniform: no row of this wave exists; it takes its part in the loads
       const bool one = page_id(a, __builtin_amdgcn_readlane(own, pg - from)) >= 0;
       const bool two = pg + 1 < to && page_id(a, __builtin_amdgcn_readlane(own, pg + 1 - from)) >= 0;
-      auto kf = [&](int p) { return [=](int q, int kb) { return ld8(st + (p + q) * 2 * PE + kb * 512 + lane * 8); }; };
-      auto vf = [&](int p) { return [=](int q, int db) { return *reinterpret_cast<const f16x4*>(st + (p + q) * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); }; };
-      if constexpr (R == 4) {
-        if (one && two) tile_step<D, 2>(t, a.scale, pg, kf(0), vf(0));
-        else if (one) tile_step<D, 1>(t, a.scale, pg, kf(0), vf(0));
-        else if (two) tile_step<D, 1>(t, a.scale, pg + 1, kf(1), vf(1));
-      } else {
-        if (share == 0 ? one : two) tile_step<D, 1>(t, a.scale, pg + share, kf(share), vf(share));
-      }
+      const int shift = R == 4 ? 0 : share, pages = R == 4 ? one | two << 1 : share ? two : one;
+      auto kf = [=](int p, int kb) { return ld8(st + (p + shift) * 2 * PE + kb * 512 + lane * 8); };
+      auto vf = [=](int p, int db) { return *reinterpret_cast<const f16x4*>(st + (p + shift) * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); };
+      constexpr int P = R == 4 ? 2 : 1;
+      if (pages == (1 << P) - 1 && (pg + 2) * PAGE <= t.least) tile_step<D, P, false>(t, a.scale, pg + shift, pages, kf, vf);       // uniform
+      else if (pages) tile_step<D, P, true>(t, a.scale, pg + shift, pages, kf, vf);
     }
     wait_loads<0>();                                        // the requests past the end, too, ahead of the end or of what the ring holds next
   }
@@ -311,16 +315,14 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
     if (share == 1) {
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(o + db * 256 + lane * 4) = t.o[db];
-      if (g == 0) {
-        ml[col] = t.m;
-        ml[16 + col] = t.l;
-      }
+      if (g == 0) *reinterpret_cast<f32x2*>(ml + col * 2) = f32x2{t.m, t.l};
     }
     __syncthreads();
     if (share == 1) return;
-    const float m1 = ml[col], m = fmaxf(t.m, m1), base = m == -INFINITY ? 0.f : m;
-    const float f0 = __builtin_amdgcn_exp2f(t.m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
-    t.l = t.l * f0 + ml[16 + col] * f1;
+    const f32x2 other = *reinterpret_cast<const f32x2*>(ml + col * 2);
+    const float m = fmaxf(t.m, other[0]), base = m == -INFINITY ? 0.f : m;
+    const float f0 = __builtin_amdgcn_exp2f(t.m - base), f1 = __builtin_amdgcn_exp2f(other[0] - base);
+    t.l = t.l * f0 + other[1] * f1;
     t.m = m;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) t.o[db] = t.o[db] * f0 + *reinterpret_cast<const f32x4*>(o + db * 256 + lane * 4) * f1;
@@ -329,12 +331,12 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
 }
 
 template <int D>
-__global__ __launch_bounds__(SA_WAVES * WAVE, 2) void shared_attn_kernel(SharedAttn a) {
+__global__ __launch_bounds__(SA_WAVES * WAVE, 3) void shared_attn_kernel(SharedAttn a) {
   __shared__ __align__(16) f16 ring[SA_RING * 4 * PAGE * D];
   int i = blockIdx.x;
   if (i < a.n_block * a.Hkv) {
-    const int32_t* __restrict__ d = a.units + 8 * (i / a.Hkv);
-    if (d[1] * (a.Hq / a.Hkv) > 32) block_unit<D, 4>(a, d, i % a.Hkv, ring);
+    const int32_t* __restrict__ d = a.units + (size_t)SA_RECORD * (i / a.Hkv);
+    if (d[0] * (a.Hq / a.Hkv) > 32) block_unit<D, 4>(a, d, i % a.Hkv, ring);      // uniform
     else block_unit<D, 2>(a, d, i % a.Hkv, ring);
     return;
   }
@@ -418,6 +420,7 @@ __global__ __launch_bounds__(4 * WAVE) void shared_attn_join_kernel(SharedAttn a
 int mlora_check_attn(const char* who, int Hq, int Hkv, int D, int n_pages, int n_seq, int max_blocks);
 
 extern "C" int mlora_shared_attn_unit_rows(void) { return SA_ROWS; }
+extern "C" int mlora_shared_attn_record_ints(void) { return SA_RECORD; }
 
 extern "C" size_t mlora_shared_attn_workspace_bytes(int B, int Hq, int D, int slots) {
   return B <= 0 || Hq <= 0 || D <= 0 || slots <= 0 ? 0 : (size_t)B * Hq * slots * (D + 2) * sizeof(float);
@@ -425,12 +428,12 @@ extern "C" size_t mlora_shared_attn_workspace_bytes(int B, int Hq, int D, int sl
 
 extern "C" int mlora_paged_attn_decode_shared(void* out, int out_layout, const void* qkv, const void* k_cache, const void* v_cache, const int32_t* block_table,
                                               int max_blocks, const int32_t* seq_ids, const int32_t* ctx_len, const int32_t* units, int n_block,
-                                              int n_units, const int32_t* members, int n_members, const int32_t* row_pages, const int32_t* row_slots, int own_splits,
+                                              int n_units, const int32_t* row_pages, const int32_t* row_slots, int own_splits,
                                               int slots, int B, int Hq, int Hkv, int D, int n_pages, int n_seq, void* workspace, size_t workspace_bytes,
                                               void* stream) {
   if (int e = mlora_check_attn("paged_attn_decode_shared", Hq, Hkv, D, n_pages, n_seq, max_blocks)) return e;
   MLORA_CHECK(out && qkv && k_cache && v_cache && block_table && seq_ids && ctx_len && row_pages && row_slots, MLORA_ERR_INVALID, "paged_attn_decode_shared: null pointer");
-  MLORA_CHECK(n_block >= 0 && n_units >= n_block && n_members >= 0 && (n_units == 0 || (units && members && n_members > 0)), MLORA_ERR_INVALID, "paged_attn_decode_shared: bad plan");
+  MLORA_CHECK(n_block >= 0 && n_units >= n_block && (n_units == 0 || units), MLORA_ERR_INVALID, "paged_attn_decode_shared: bad plan");
   MLORA_CHECK(B >= 0 && B <= 65535 && own_splits > 0 && slots >= own_splits && ((long)B * own_splits + n_units) * Hkv <= 0x7fffffff, MLORA_ERR_INVALID,
               "paged_attn_decode_shared: B=%d with %d units and %d shares of a row's own pages", B, n_units, own_splits);
   MLORA_CHECK(Hq / Hkv <= 16, MLORA_ERR_UNSUPPORTED, "paged_attn_decode_shared: more than 16 query heads per kv head (%d)", Hq / Hkv);
@@ -438,7 +441,7 @@ extern "C" int mlora_paged_attn_decode_shared(void* out, int out_layout, const v
   if (B == 0) return MLORA_OK;
   MLORA_CHECK(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= mlora_shared_attn_workspace_bytes(B, Hq, D, slots), MLORA_ERR_WORKSPACE,
               "paged_attn_decode_shared: workspace of %zu bytes, %zu needed", workspace_bytes, mlora_shared_attn_workspace_bytes(B, Hq, D, slots));
-  SharedAttn a = {(f16*)out, (const f16*)qkv, (const f16*)k_cache, (const f16*)v_cache, block_table, seq_ids, ctx_len, units, members, row_pages, row_slots,
+  SharedAttn a = {(f16*)out, (const f16*)qkv, (const f16*)k_cache, (const f16*)v_cache, block_table, seq_ids, ctx_len, units, row_pages, row_slots,
                   (float*)workspace, (float*)workspace + (size_t)B * Hq * slots * D, max_blocks, B, Hq, Hkv, n_pages, n_seq, n_block, n_units, own_splits, slots,
                   out_layout == MLORA_FRAG ? mlora_frag_tiles(B) : 0, LOG2E / sqrtf((float)D)};
   hipStream_t s = (hipStream_t)stream;

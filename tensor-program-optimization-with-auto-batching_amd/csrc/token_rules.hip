@@ -184,18 +184,20 @@ __global__ __launch_bounds__(WAVE) void token_rules_join_kernel(int32_t* __restr
   if (threadIdx.x == 0) finish(ids, r, row, best, history_of(r, row));
 }
 
-constexpr int CHUNK_THREADS = 256, CHUNK_QUADS = 4, CHUNK = CHUNK_THREADS * 4 * CHUNK_QUADS;
-constexpr int ROW_THREADS = 1024, ROW_QUADS = 8, ROW = ROW_THREADS * 4 * ROW_QUADS;
+#ifndef V_T
+#define V_T 256
+#define V_Q 4
+#endif
+constexpr int CHUNK_THREADS = V_T, CHUNK_QUADS = V_Q, CHUNK = CHUNK_THREADS * 4 * CHUNK_QUADS;
 constexpr int MAX_BIAS = 1024;
 
-bool whole_row(int B, int V) { return V + 3 <= ROW; }
 int chunks_of(int V) { return (int)(((long)V + 3 + CHUNK - 1) / CHUNK); }
 
 }  // namespace
 
 extern "C" size_t mlora_constrained_argmax_workspace_bytes(int B, int V) {
-  if (B <= 0 || V <= 0 || whole_row(B, V)) return 0;
-  return (size_t)B * chunks_of(V) * sizeof(Best);
+  const int chunks = B > 0 && V > 0 ? chunks_of(V) : 0;
+  return chunks > 1 ? (size_t)B * chunks * sizeof(Best) : 0;
 }
 
 extern "C" int mlora_constrained_argmax(int32_t* ids, float* out, long ld_out, const float* logits, long ld, const mlora_logit_rules* rules, int B, int V,
@@ -212,20 +214,12 @@ extern "C" int mlora_constrained_argmax(int32_t* ids, float* out, long ld_out, c
   MLORA_CHECK(!r.masks || (r.mask_row && r.n_masks > 0), MLORA_ERR_INVALID, "constrained_argmax: masks without their rows");
   if (B == 0) return MLORA_OK;
   hipStream_t s = (hipStream_t)stream;
-  if (whole_row(B, V)) {
-    const size_t lds = (ROW + 2 * (size_t)r.n_bias) * 4;
-    static const hipError_t configured = hipFuncSetAttribute((const void*)token_rules_kernel<ROW_THREADS, ROW_QUADS>,
-                                                             hipFuncAttributeMaxDynamicSharedMemorySize, (ROW + 2 * MAX_BIAS) * 4);
-    if (configured != hipSuccess)
-      return mlora_set_error(MLORA_ERR_LAUNCH, "constrained_argmax: cannot reserve LDS: %s", hipGetErrorString(configured));
-    hipLaunchKernelGGL((token_rules_kernel<ROW_THREADS, ROW_QUADS>), dim3(1, B), dim3(ROW_THREADS), lds, s, ids, out, ld_out, logits, ld, r, V, (Best*)nullptr);
-    return mlora_launch_status("constrained_argmax");
-  }
   const int chunks = chunks_of(V);
-  MLORA_CHECK(workspace && workspace_bytes >= mlora_constrained_argmax_workspace_bytes(B, V) && ((uintptr_t)workspace & 7) == 0, MLORA_ERR_WORKSPACE,
+  MLORA_CHECK(chunks == 1 || (workspace && workspace_bytes >= mlora_constrained_argmax_workspace_bytes(B, V) && ((uintptr_t)workspace & 7) == 0), MLORA_ERR_WORKSPACE,
               "constrained_argmax: workspace of %zu bytes, %zu needed", workspace_bytes, mlora_constrained_argmax_workspace_bytes(B, V));
   hipLaunchKernelGGL((token_rules_kernel<CHUNK_THREADS, CHUNK_QUADS>), dim3(chunks, B), dim3(CHUNK_THREADS), (CHUNK + 2 * (size_t)r.n_bias) * 4, s, ids, out,
-                     ld_out, logits, ld, r, V, (Best*)workspace);
+                     ld_out, logits, ld, r, V, chunks > 1 ? (Best*)workspace : nullptr);
+  if (chunks == 1) return mlora_launch_status("constrained_argmax");
   if (int e = mlora_launch_status("constrained_argmax")) return e;
   hipLaunchKernelGGL(token_rules_join_kernel, dim3(B), dim3(WAVE), 0, s, ids, r, (const Best*)workspace, chunks);
   return mlora_launch_status("constrained_argmax");

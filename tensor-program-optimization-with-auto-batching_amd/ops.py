@@ -960,7 +960,7 @@ class SharedPrefixPlan:
             raise ValueError(f"SharedPrefixPlan: rows {members} of {B}, each in one group at most")
         if any(not rows or pages <= 0 for rows, pages in groups) or any(16 * pages > lens[r] for rows, pages in groups for r in rows):
             raise ValueError("SharedPrefixPlan: a group has rows and pages, and its pages lie within their contexts")
-        self.B, self.Hq, self.Hkv, self.D, self.n_members = B, Hq, Hkv, D, len(members)
+        self.B, self.Hq, self.Hkv, self.D = B, Hq, Hkv, D
         row_pages, row_slots = [0] * B, [0] * B
         for rows, pages in groups:
             for r in rows:
@@ -968,32 +968,30 @@ class SharedPrefixPlan:
         own = [-(-n // 16) - p for n, p in zip(lens, row_pages)]
         large = [(rows, pages) for rows, pages in groups if len(rows) * G > 16]
         small = [(rows, pages) for rows, pages in groups if len(rows) * G <= 16]
-        groups = large + small
-        members = [r for rows, _ in groups for r in rows]
-        most = lib().mlora_shared_attn_unit_rows() // G                  # members of a block unit
-        # pages of a unit: block units for two workgroups on each compute unit, wave units for eight waves - no shorter than some pages, and no
-        # more units of a row than its second launch joins cheaply
+        most = lib().mlora_shared_attn_unit_rows() // G                  # rows of a block unit
+        # pages of a unit: block units for two workgroups on each compute unit, a row's own pages for eight waves - but no shorter than some
+        # pages, and no more units of a row than its second launch joins cheaply
         per_block = max(8, -(-sum(-(-len(rows) // most) * pages for rows, pages in large) * Hkv // 512))
-        per_wave = max(4, -(-(sum(p for _, p in small) + sum(own)) * Hkv // 2048))
-        units, first = [], 0
-        for i, (rows, pages) in enumerate(groups):
-            block = i < len(large)
+        per_wave = max(4, -(-sum(pages for _, pages in small) * Hkv // 2048))
+        self.own_splits = max(1, min(-(-max(own, default=0) // 4), 2048 // max(B * Hkv, 1), 64))
+        units = []
+        for rows, pages in large + small:
+            block = len(rows) * G > 16
             n = min(-(-pages // (per_block if block else per_wave)), 64)
             cut = [pages * i // n for i in range(n + 1)]
             parts = -(-len(rows) // most) if block else 1
             edge = [len(rows) * i // parts for i in range(parts + 1)]
             for r in rows:
                 row_slots[r] = n
-            units += [(not block, first + a, b - a, lo, hi - lo, j) for a, b in zip(edge, edge[1:]) for j, (lo, hi) in enumerate(zip(cut, cut[1:]))]
-            first += len(rows)
-        units = [(*u[1:], 0, 0, 0) for u in sorted(units, key=lambda u: (u[0], -u[4]))]
-        self.n_block = sum(u[1] * G > 16 for u in units)
-        self.own_splits = max(1, min(-(-max(own, default=0) // per_wave), 64))
+            units += [(not block, lo - hi, rows[a:b], lo, j) for a, b in zip(edge, edge[1:]) for j, (lo, hi) in enumerate(zip(cut, cut[1:]))]
+        units.sort(key=lambda u: u[:2])                                  # block units first, the longest first
+        self.n_block = sum(not u[0] for u in units)
         self.n_units, self.slots = len(units), max(row_slots, default=0) + self.own_splits
-        flat = torch.tensor([x for u in units for x in u] + members + row_pages + row_slots, dtype=torch.int32)
-        self.data = upload(flat, device)
-        at = [0, 8 * len(units), 8 * len(units) + len(members)]
-        self.units, self.members, self.row_pages, self.row_slots = (self.data[a:b] for a, b in zip(at + [at[2] + B], at[1:] + [at[2] + B, at[2] + 2 * B]))
+        size = lib().mlora_shared_attn_record_ints()
+        records = [x for _, less, rows, lo, j in units for x in (len(rows), lo, -less, j, 0, 0, 0, 0, *rows, *([rows[0]] * (size - 8 - len(rows))))]
+        self.data = upload(torch.tensor(records + row_pages + row_slots, dtype=torch.int32), device)
+        n = len(records)
+        self.units, self.row_pages, self.row_slots = self.data[:n], self.data[n:n + B], self.data[n + B:]
 
 
 def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, plan: SharedPrefixPlan, Hq, Hkv, D, out=None, frag=False):
@@ -1018,7 +1016,7 @@ def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_le
     f16, i32 = torch.float16, torch.int32
     check(L.mlora_paged_attn_decode_shared(optr, lay, _dev(qkv, f16, "qkv"), _dev(k_cache, f16, "k_cache"), _dev(v_cache, f16, "v_cache"),
                                            _dev(block_table, i32, "block_table"), max_blocks, _dev(seq_ids, i32, "seq_ids"), _dev(ctx_len, i32, "ctx_len"),
-                                           plan.units.data_ptr(), plan.n_block, plan.n_units, plan.members.data_ptr(), plan.n_members, plan.row_pages.data_ptr(),
+                                           plan.units.data_ptr(), plan.n_block, plan.n_units, plan.row_pages.data_ptr(),
                                            plan.row_slots.data_ptr(), plan.own_splits, plan.slots, B, Hq, Hkv, D, k_cache.shape[0], n_seq, ws.data_ptr(), nb,
                                            _stream()))
     return out

@@ -10,7 +10,7 @@ def test_constrained_argmax_refusals():
     def call(B=2, V=50000, ld=50000, out=None, ld_out=0, ws=16, nb=1 << 20, **kw):
         r = lm.LogitRulesArgs(**kw)
         return lib.mlora_constrained_argmax(16, out, ld_out, 16, ld, C.byref(r), B, V, ws, nb, None)
-    assert lib.mlora_constrained_argmax_workspace_bytes(2, 50000) == 2 * 13 * 8 and lib.mlora_constrained_argmax_workspace_bytes(2, 32000) == 0
+    assert lib.mlora_constrained_argmax_workspace_bytes(2, 50000) == 2 * 13 * 8 and lib.mlora_constrained_argmax_workspace_bytes(2, 4000) == 0
     assert lib.mlora_constrained_argmax(16, None, 0, None, 10, C.byref(lm.LogitRulesArgs()), 1, 10, None, 0, None) == -1
     assert call(B=-1) == -1 and call(B=65536) == -1 and call(V=0) == -1 and call(ld=49999) == -1
     assert call(out=16, ld_out=100) == -1
@@ -44,13 +44,13 @@ def test_linear4_refusals():
 
 def test_shared_attention_refusals():
     lib = load_pkg("_lib").lib()
-    assert lib.mlora_shared_attn_unit_rows() == 64
+    assert lib.mlora_shared_attn_unit_rows() == 64 and lib.mlora_shared_attn_record_ints() == 72
     need = lib.mlora_shared_attn_workspace_bytes(4, 8, 128, 3)
     assert need == 4 * 8 * 3 * 130 * 4 and lib.mlora_shared_attn_workspace_bytes(0, 8, 128, 3) == 0
-    def call(out=16, lay=0, units=16, n_block=1, n_units=1, members=16, n_members=2, row_pages=16, own=2, slots=3, B=4, Hq=8, Hkv=8, D=128, ws=16, nb=need):
-        return lib.mlora_paged_attn_decode_shared(out, lay, 16, 16, 16, 16, 4, 16, 16, units, n_block, n_units, members, n_members, row_pages, 16, own, slots, B, Hq, Hkv, D,
+    def call(out=16, lay=0, units=16, n_block=1, n_units=1, row_pages=16, own=2, slots=3, B=4, Hq=8, Hkv=8, D=128, ws=16, nb=need):
+        return lib.mlora_paged_attn_decode_shared(out, lay, 16, 16, 16, 16, 4, 16, 16, units, n_block, n_units, row_pages, 16, own, slots, B, Hq, Hkv, D,
                                                   5, 4, ws, nb, None)
-    assert call(out=None) == -1 and call(row_pages=None) == -1 and call(units=None) == -1 and call(n_members=0) == -1 and call(n_units=-1) == -1 and call(n_block=2) == -1 and call(n_block=-1) == -1
+    assert call(out=None) == -1 and call(row_pages=None) == -1 and call(units=None) == -1 and call(n_units=-1) == -1 and call(n_block=2) == -1 and call(n_block=-1) == -1
     assert call(D=96) == -2 and call(Hkv=3) == -1 and call(Hq=34, Hkv=2) == -2 and call(lay=5) == -1
     assert call(own=0) == -1 and call(slots=1) == -1 and call(B=-1) == -1 and call(B=70000) == -1
     assert call(ws=None) == -3 and call(nb=need - 1) == -3 and call(ws=24) == -3
