@@ -23,10 +23,27 @@ struct Best {
 // the greater value, the lower index of equal ones; NaN never wins
 __device__ __forceinline__ Best better(Best a, Best b) { return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a; }
 
+// A wave's maximum and the lowest index that has it: rotations within the rows of 16 lanes, then exchanges of rows and halves (through LDS, as
+// shuffles go, the two reductions of a chunk were a third of its time)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+
+template <class F>
+__device__ __forceinline__ uint32_t wave_all(uint32_t v, F f) {
+  v = f(v, dpp<0x128>(v));                                   // row_ror:8, 4, 2, 1
+  v = f(v, dpp<0x124>(v));
+  v = f(v, dpp<0x122>(v));
+  v = f(v, dpp<0x121>(v));
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = f(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f(r[0], r[1]);
+}
+
 __device__ __forceinline__ Best wave_best(Best a) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a = better(a, Best{__shfl_xor(a.v, o, WAVE), __shfl_xor(a.i, o, WAVE)});
-  return a;
+  const float v = __uint_as_float(wave_all(__float_as_uint(a.v), [](uint32_t x, uint32_t y) { return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y))); }));
+  const uint32_t i = wave_all(a.v == v ? (uint32_t)a.i : 0x7fffffffu, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+  return Best{v, (int)i};
 }
 
 __device__ __forceinline__ int history_of(const mlora_logit_rules& r, int row) {
@@ -184,19 +201,18 @@ __global__ __launch_bounds__(WAVE) void token_rules_join_kernel(int32_t* __restr
   if (threadIdx.x == 0) finish(ids, r, row, best, history_of(r, row));
 }
 
-#ifndef V_T
-#define V_T 256
-#define V_Q 4
-#endif
-constexpr int CHUNK_THREADS = V_T, CHUNK_QUADS = V_Q, CHUNK = CHUNK_THREADS * 4 * CHUNK_QUADS;
+constexpr int CHUNK_THREADS = 256;
 constexpr int MAX_BIAS = 1024;
 
-int chunks_of(int V) { return (int)(((long)V + 3 + CHUNK - 1) / CHUNK); }
+// Quadruples of a thread: four while that leaves the device eight workgroups a compute unit or more, two below (one row of 32000: 7.5 to 6.3 us;
+// 256 rows of 128256 with two: 62 to 73 us, each chunk reading the row's history anew)
+int quads_of(int B, int V) { return (long)B * V >= 2048l * CHUNK_THREADS * 16 ? 4 : 2; }
+int chunks_of(int V, int quads) { return (int)(((long)V + 3 + CHUNK_THREADS * 4 * quads - 1) / (CHUNK_THREADS * 4 * quads)); }
 
 }  // namespace
 
 extern "C" size_t mlora_constrained_argmax_workspace_bytes(int B, int V) {
-  const int chunks = B > 0 && V > 0 ? chunks_of(V) : 0;
+  const int chunks = B > 0 && V > 0 ? chunks_of(V, quads_of(B, V)) : 0;
   return chunks > 1 ? (size_t)B * chunks * sizeof(Best) : 0;
 }
 
@@ -214,11 +230,13 @@ extern "C" int mlora_constrained_argmax(int32_t* ids, float* out, long ld_out, c
   MLORA_CHECK(!r.masks || (r.mask_row && r.n_masks > 0), MLORA_ERR_INVALID, "constrained_argmax: masks without their rows");
   if (B == 0) return MLORA_OK;
   hipStream_t s = (hipStream_t)stream;
-  const int chunks = chunks_of(V);
+  const int quads = quads_of(B, V), chunks = chunks_of(V, quads);
   MLORA_CHECK(chunks == 1 || (workspace && workspace_bytes >= mlora_constrained_argmax_workspace_bytes(B, V) && ((uintptr_t)workspace & 7) == 0), MLORA_ERR_WORKSPACE,
               "constrained_argmax: workspace of %zu bytes, %zu needed", workspace_bytes, mlora_constrained_argmax_workspace_bytes(B, V));
-  hipLaunchKernelGGL((token_rules_kernel<CHUNK_THREADS, CHUNK_QUADS>), dim3(chunks, B), dim3(CHUNK_THREADS), (CHUNK + 2 * (size_t)r.n_bias) * 4, s, ids, out,
-                     ld_out, logits, ld, r, V, chunks > 1 ? (Best*)workspace : nullptr);
+  const size_t lds = (CHUNK_THREADS * 4 * quads + 2 * (size_t)r.n_bias) * 4;
+  Best* part = chunks > 1 ? (Best*)workspace : nullptr;
+  if (quads == 4) hipLaunchKernelGGL((token_rules_kernel<CHUNK_THREADS, 4>), dim3(chunks, B), dim3(CHUNK_THREADS), lds, s, ids, out, ld_out, logits, ld, r, V, part);
+  else hipLaunchKernelGGL((token_rules_kernel<CHUNK_THREADS, 2>), dim3(chunks, B), dim3(CHUNK_THREADS), lds, s, ids, out, ld_out, logits, ld, r, V, part);
   if (chunks == 1) return mlora_launch_status("constrained_argmax");
   if (int e = mlora_launch_status("constrained_argmax")) return e;
   hipLaunchKernelGGL(token_rules_join_kernel, dim3(B), dim3(WAVE), 0, s, ids, r, (const Best*)workspace, chunks);

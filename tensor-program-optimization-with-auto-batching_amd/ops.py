@@ -440,30 +440,32 @@ def quantize(W: torch.Tensor, group: int = 128) -> QuantWeight:
 
 def _linear4(x, W, out, out_dtype, accumulate):
     T, K = x.shape
-    N, K2 = W.shape
-    dev = _here(x.device, "linear")
-    if K2 != K or x.dtype != torch.float16 or W.device != dev:
-        raise ValueError(f"linear: x{tuple(x.shape)} {x.dtype} on {dev} vs a 4-bit weight {W.shape} on {W.device} (fp16 activations)")
-    if accumulate and out is None:
-        raise ValueError("linear: accumulate needs out")
+    N, dev = W.N, W.q.device
+    if W.K != K or x.dtype != torch.float16 or x.device != dev:
+        raise ValueError(f"linear: x{tuple(x.shape)} {x.dtype} on {x.device} vs a 4-bit weight {W.shape} on {dev} (fp16 activations)")
+    _here(dev, "linear")
     if out is None:
+        if accumulate:
+            raise ValueError("linear: accumulate needs out")
         out = torch.empty((T, N), dtype=out_dtype, device=dev)
-    if out.shape != (T, N) or out.device != dev:
+    elif out.shape != (T, N) or out.device != dev:
         raise ValueError(f"linear: out{tuple(out.shape)} on {out.device}, expected {(T, N)} on {dev}")
     if T == 0:
         return out
     if isinstance(x, FragActivation):
         xp, lay, ldx = x.data.data_ptr(), FRAG, 0
     else:
-        ldx = x.stride(0) if T > 1 else K
-        if x.stride(1) != 1 or ldx < K or ldx % 8 or x.data_ptr() % 16:
-            x = x.contiguous().clone() if x.is_contiguous() else x.contiguous()       # rows on 16 bytes
-            ldx = K
+        ldx, inner = x.stride()
         xp, lay = x.data_ptr(), ROWMAJOR
+        if T == 1:
+            ldx = K
+        if inner != 1 or ldx < K or ldx % 8 or xp % 16:
+            x = x.clone(memory_format=torch.contiguous_format)            # rows on 16 bytes
+            xp, ldx = x.data_ptr(), K
     nb = _size(torch.float16, "mlora_linear4_workspace_bytes", T, K, N)
     ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
-    check(lib().mlora_linear4(_dev(out), _dt(out), ACCUMULATE if accumulate else STORE, xp, lay, ldx, W.q.data_ptr(), W.meta.data_ptr(),
-                              W.group, T, K, N, None if ws is None else ws.data_ptr(), nb, _stream()))
+    check(lib().mlora_linear4(_dev(out), _dt(out), ACCUMULATE if accumulate else STORE, xp, lay, ldx, W.q.data_ptr(), W.meta.data_ptr(), W.group, T, K, N,
+                              None if ws is None else ws.data_ptr(), nb, _stream()))
     return out
 
 
@@ -860,34 +862,44 @@ def constrained_argmax(logits, rules: LogitRules, out=None, ids=None):
     fp32 (or None; may be `logits`) takes the logits after penalties, biases and masks."""
     B, V = logits.shape
     dev = _here(logits.device, "constrained_argmax")
-    if rules.rows not in (None, B) or rules.device not in (None, dev):
+    args = rules._args
+    if rules.device is not None and (rules.rows != B and rules.rows is not None or rules.device != dev):
         raise ValueError(f"constrained_argmax: rules of {rules.rows} rows on {rules.device} for {B} on {dev}")
-    if rules._args.n_masks and rules.masks.shape[1] != -(-V // 32):
+    if args.n_masks and rules.masks.shape[1] != -(-V // 32):
         raise ValueError(f"constrained_argmax: masks of {rules.masks.shape[1]} words for {V} tokens")
-    lds = []
-    for t, name in ((logits, "logits"), (out, "out")):
-        if t is not None and (not t.is_cuda or t.device != dev or t.dtype != torch.float32 or t.shape != (B, V) or (t.stride(1) != 1 and V > 1)
-                              or (B > 1 and t.stride(0) < V)):
-            raise ValueError(f"constrained_argmax: {name} must be fp32 [{B}, {V}] on the GPU with unit inner stride")
-        lds.append(0 if t is None else t.stride(0) if B > 1 else max(V, t.stride(0)))
+    ld, ld_out, p_out = _rows_of(logits, B, V, dev, "logits"), 0, None
+    if out is not None:
+        ld_out, p_out = _rows_of(out, B, V, dev, "out"), out.data_ptr()
+        p, apart = logits.data_ptr(), 4 * (B - 1)
+        if (p != p_out or ld != ld_out) and p < p_out + apart * ld_out + 4 * V and p_out < p + apart * ld + 4 * V:
+            raise ValueError("constrained_argmax: out overlaps the logits without being them")
     if ids is None:
-        ids = torch.empty((B,), dtype=torch.int32, device=dev)
-    elif ids.shape != (B,):
-        raise ValueError(f"constrained_argmax: ids{tuple(ids.shape)} for {B} rows")
+        ids = torch.empty(B, dtype=torch.int32, device=dev)
+    elif ids.shape != (B,) or ids.device != dev:
+        raise ValueError(f"constrained_argmax: ids{tuple(ids.shape)} on {ids.device} for {B} rows on {dev}")
     if B == 0:
         return ids
-    if out is not None and (out.data_ptr(), lds[1]) != (logits.data_ptr(), lds[0]):
-        a, b = ((t.data_ptr(), t.data_ptr() + 4 * ((B - 1) * ld + V)) for t, ld in ((logits, lds[0]), (out, lds[1])))
-        if a[0] < b[1] and b[0] < a[1]:
-            raise ValueError("constrained_argmax: out overlaps the logits without being them")
     L = _lib.loaded()
-    nb = L.mlora_constrained_argmax_workspace_bytes(B, V)
+    nb = _rules_bytes(B, V)
     ws = torch.empty(nb // 8, dtype=torch.int64, device=dev) if nb else None
-    code = L.mlora_constrained_argmax(_dev(ids, torch.int32), None if out is None else out.data_ptr(), lds[1], logits.data_ptr(), lds[0],
-                                      ctypes.byref(rules._args), B, V, None if ws is None else ws.data_ptr(), nb, _stream())
+    code = L.mlora_constrained_argmax(_dev(ids, torch.int32), p_out, ld_out, logits.data_ptr(), ld, ctypes.byref(args), B, V,
+                                      None if ws is None else ws.data_ptr(), nb, _stream())
     if code:
         raise _lib.MloraError(code, L.mlora_last_error().decode())
     return ids
+
+
+@functools.lru_cache(maxsize=256)
+def _rules_bytes(B, V):
+    return _lib.loaded().mlora_constrained_argmax_workspace_bytes(B, V)
+
+
+def _rows_of(t, B, V, dev, name):
+    """Row stride of fp32 rows [B, V] with unit inner stride."""
+    ld, inner = t.stride()
+    if t.dtype != torch.float32 or t.shape != (B, V) or (inner != 1 and V > 1) or (ld < V and B > 1) or t.device != dev:
+        raise ValueError(f"constrained_argmax: {name} must be fp32 [{B}, {V}] on {dev} with unit inner stride")
+    return ld if B > 1 else V if ld < V else ld
 
 
 def rope_kv_append(qkv, k_cache, v_cache, block_table, tok_seq, tok_pos, rope_cos, rope_sin, Hq, Hkv, D):
