@@ -22,8 +22,8 @@ class LlamaAutoBatcherClass:
         self.graph = LlamaExecGraph()
         self.seq_info = LlamaSeqInfo(self.exec_config.max_gen_len)
         self.model = self.tokenizer = self.eos_token_id = self.free_pages = None
-        # a request's sequence id is claimed by its first set_adapter() or generate(); `_open` says that the newest
-        # id has been claimed by set_adapter() and still waits for its generate()
+        # a request's sequence id is claimed by its first set_adapter(), set_rules() or generate(); `_open` says that the newest
+        # id has been claimed by one of the first two and still waits for its generate()
         self._last_sid = -1
         self._open = False
         self.warmup_trials, self.measurement_trials, self.measurements_dest = 3, 0, "measure.txt"
@@ -64,6 +64,12 @@ class LlamaAutoBatcherClass:
         sid = self._claim_sid()
         self._open = True
         self.seq_info.set_adapter(sid, config, wid)
+
+    def set_rules(self, rules):
+        """What the answer of the request whose generate() comes next is held to (token_rules.TokenRules)."""
+        sid = self._claim_sid()
+        self._open = True
+        self.seq_info.set_rules(sid, rules)
 
     def generate(self, input_var, max_gen_len=None):
         sid = self._claim_sid()

@@ -20,16 +20,20 @@ class DecodeSession:
     scratch buffers outside the graph's memory pool - and replayed, so the interpreter is out of the loop; the
     kernels and their order are those of the eager step, hence the same tokens bit for bit."""
 
-    def __init__(self, model, kv, seq_ids, tok_adapter, first_tokens, use_graph=False, longest_first=False):
+    def __init__(self, model, kv, seq_ids, tok_adapter, first_tokens, use_graph=False, longest_first=False, rules=None):
         """seq_ids: sequences already prefilled in `kv`; tok_adapter: {tid: ids [B] int32 (host or device), -1 = the
         row does not use that type}; first_tokens [B]: the tokens produced by prefill.
         longest_first: run the batch internally in order of decreasing context length, so that the attention
         workgroups of the longest sequences start first and the short ones fill the tail of the launch (every
         operator treats rows independently: a sequence's results do not depend on its row); step() still returns
-        the tokens in the caller's order."""
+        the tokens in the caller's order.
+        rules: token_rules.BatchRules of the rows in the caller's order; a row that has no token left gets -1."""
         self.model, self.kv = model, kv
         B = len(seq_ids)
         dev = model.device
+        if rules is not None and (longest_first or len(rules.rules) != B):
+            raise ValueError("DecodeSession: rules for the batch's rows, in the order in which they run")
+        self.rules = rules
         i32 = lambda a: (a if isinstance(a, torch.Tensor) else torch.as_tensor(np.asarray(a, dtype=np.int32))).to(dev, torch.int32)
         self._inv = None
         if longest_first and B > 1:
@@ -55,7 +59,10 @@ class DecodeSession:
     def _enqueue(self):
         m = self.model
         logits = m.forward(m.embed(self.tokens), self.kv, self.tok_adapter)
-        self.tokens.copy_(ops.argmax(logits))
+        if self.rules is not None:
+            self.rules.choose(logits, out=self.tokens)
+        else:
+            self.tokens.copy_(ops.argmax(logits))
         self.pos.add_(1)
         self.ctx.add_(1)
 
@@ -69,6 +76,7 @@ class DecodeSession:
                 with torch.cuda.graph(g):         # records, does not run
                     self._enqueue()
                 self.graph = g
+                self._plan = getattr(kv, "plan", None)       # what the recorded launches read
             self.graph.replay()
         else:
             self._enqueue()
@@ -93,6 +101,8 @@ class NativeDecodeSession:
         step() returns the tokens in the caller's order (`tokens` and `buf` stay in the internal order)."""
         import ctypes as C
         from . import _lib
+        if not model.native_step:
+            raise ValueError("NativeDecodeSession: the model has no C decode step")
         self.model, self.kv = model, kv
         self.seq_ids = list(seq_ids)
         s = model.shape

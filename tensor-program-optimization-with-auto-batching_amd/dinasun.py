@@ -141,6 +141,10 @@ class DinasunForCausalLM(CausalLM):
                                max_blocks=max_blocks, max_pos=max_blocks * page_size, dtype=self.dtype, device=self.device,
                                free_pages=free_pages, page_size=page_size)
 
+    @property
+    def vocab_size(self):
+        return self.config.vocab
+
     # ------------------------------------------------------------------ forward
     def embed(self, input_ids: torch.Tensor) -> LoopHidden:
         ids = ops.upload(input_ids.reshape(-1), self.device, torch.int32).contiguous()

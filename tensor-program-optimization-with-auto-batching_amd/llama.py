@@ -59,9 +59,16 @@ class LoraType:
 class LlamaForCausalLM(CausalLM):
     dtypes = ("float16",)
     native_step = True
+    quant_group = None
 
-    def __init__(self, shape: LlamaShape, device="cuda:0"):
+    def __init__(self, shape: LlamaShape, device="cuda:0", quant_group=None):
+        """quant_group: the layers' linears in 4 bits with a scale and zero per so many neighbours along K (32, 64 or 128; None: fp16).  Adapters,
+        norms, embedding and head stay fp16."""
+        if quant_group not in (None, 32, 64, 128):
+            raise ValueError(f"quant_group {quant_group}: 32, 64, 128 or None")
         self.shape = shape
+        self.quant_group = quant_group
+        self.native_step = quant_group is None         # (the C decode step takes fp16 weights)
         self.device = torch.device(device)
         self.layers = []          # per layer dict: qkv, o, gate_up, down (PackedWeight), ln1, ln2 (fp16 [H])
         self.embed_tokens = None
@@ -79,9 +86,10 @@ class LlamaForCausalLM(CausalLM):
         dev = self.device
         qkv = torch.cat([w["q_proj"], w["k_proj"], w["v_proj"]], 0).to(dev, torch.float16)
         gu = torch.cat([w["gate_proj"], w["up_proj"]], 0).to(dev, torch.float16)
+        packed = ops.PackedWeight if self.quant_group is None else lambda t: ops.quantize(t, self.quant_group)
         self.layers.append({
-            "qkv": ops.PackedWeight(qkv), "o": ops.PackedWeight(w["o_proj"].to(dev, torch.float16)),
-            "gate_up": ops.PackedWeight(gu), "down": ops.PackedWeight(w["down_proj"].to(dev, torch.float16)),
+            "qkv": packed(qkv), "o": packed(w["o_proj"].to(dev, torch.float16)),
+            "gate_up": packed(gu), "down": packed(w["down_proj"].to(dev, torch.float16)),
             "ln1": w["input_layernorm"].to(dev, torch.float16).contiguous(),
             "ln2": w["post_attention_layernorm"].to(dev, torch.float16).contiguous(),
         })
@@ -97,10 +105,10 @@ class LlamaForCausalLM(CausalLM):
         return len(self.lora_types) - 1
 
     @classmethod
-    def from_synthetic(cls, seed: int, shape: LlamaShape, lora_specs=(), device="cuda:0", synth=None):
+    def from_synthetic(cls, seed: int, shape: LlamaShape, lora_specs=(), device="cuda:0", synth=None, quant_group=None):
         """Random-init model generated on the device (bit-identical to the CPU generation of the same seed)."""
         from . import synth as S
-        m = cls(shape, device)
+        m = cls(shape, device, quant_group)
         for l in range(shape.num_hidden_layers):
             w = S.layer_weights(seed, shape, l, torch.float16, device)
             m.load_layer(l, {k.split(".", 2)[2]: v for k, v in w.items()})
@@ -118,8 +126,8 @@ class LlamaForCausalLM(CausalLM):
         return m
 
     @classmethod
-    def from_weights(cls, config: dict, tensors, dtype=torch.float16, device="cuda:0"):
-        """config: a config.json of a Llama checkpoint; tensors(name) -> tensor."""
+    def from_weights(cls, config: dict, tensors, dtype=torch.float16, device="cuda:0", quant_group=None):
+        """config: a config.json of a Llama checkpoint; tensors(name) -> tensor.  quant_group: as for the class."""
         heads = config["num_attention_heads"]
         shape = LlamaShape(hidden_size=config["hidden_size"], intermediate_size=config["intermediate_size"], num_attention_heads=heads,
                            num_key_value_heads=config.get("num_key_value_heads") or heads, num_hidden_layers=config["num_hidden_layers"],
@@ -127,7 +135,7 @@ class LlamaForCausalLM(CausalLM):
                            rms_norm_eps=config["rms_norm_eps"], rope_theta=config.get("rope_theta", 10000.0))
         if config.get("rope_scaling"):
             raise ValueError("rope_scaling is not supported")
-        m = cls(shape, device)
+        m = cls(shape, device, quant_group)
         for l in range(shape.num_hidden_layers):
             n = f"model.layers.{l}."
             w = {p: tensors(f"{n}self_attn.{p}.weight") for p in ("q_proj", "k_proj", "v_proj", "o_proj")}
@@ -141,11 +149,16 @@ class LlamaForCausalLM(CausalLM):
     def interleaved_gate_up(self):
         """Per layer, the gate/up matrix with 16-row tiles of gate and up alternating (for the GEMV whose epilogue
         is the SiLU product).  Cached; one more copy of that matrix."""
+        self._fp16_layers("interleaved_gate_up")
         cache = getattr(self, "_il_cache", None)
         if cache is None:
             cache = [ops.interleave_gate_up(L["gate_up"].unpack()) for L in self.layers]
             self._il_cache = cache
         return cache
+
+    def _fp16_layers(self, what):
+        if self.quant_group is not None:
+            raise ValueError(f"{what}: the layers' linears are in 4 bits")
 
     def lora_union(self, tids):
         """-> (type, {tid: first table row}): one set of tables that serves the adapter types `tids` in one launch.
@@ -198,6 +211,7 @@ class LlamaForCausalLM(CausalLM):
         a tuple of types) appended as extra rows ([n_ad * r, K] per adapted projection; q, k, v slots always present
         for qkv, zero when not adapted), in fragment order.  with_o=False leaves o as the base weight (its delta then
         comes from riders of the GEMV launch).  Cached; costs one more copy of those matrices."""
+        self._fp16_layers("dense_lora_weights")
         cache = getattr(self, "_dense_cache", None)
         if cache is None:
             cache = self._dense_cache = {}
@@ -237,7 +251,11 @@ class LlamaForCausalLM(CausalLM):
         n_pages, max_blocks = self._cache_geometry(max_batch_size, max_total_seq_len, page_size, free_pages, max_seq_len)
         return PagedKVCache(s.num_hidden_layers, n_pages, s.num_key_value_heads, s.head_dim, max_seqs=max_batch_size,
                             max_blocks=max_blocks, rope_theta=s.rope_theta, max_pos=max_blocks * page_size,
-                            device=self.device, free_pages=free_pages, page_size=page_size)
+                            device=self.device, free_pages=free_pages, page_size=page_size, n_q_heads=s.num_attention_heads)
+
+    @property
+    def vocab_size(self):
+        return self.shape.vocab_size
 
     # ------------------------------------------------------------------ forward
     def embed(self, input_ids: torch.Tensor) -> torch.Tensor:
@@ -389,7 +407,8 @@ class LlamaForCausalLM(CausalLM):
         # (a prefill pass only: where the ids are known on the device only, the choice needs a read-back, which a decode
         # step recorded into a graph cannot make)
         fuse = None
-        if (tok_adapter and "multi" not in tok_adapter and frag and T > 64 and not is_decode
+        four_bit = self.quant_group is not None           # its linears have no fused forms: deltas and products behind them
+        if (not four_bit and tok_adapter and "multi" not in tok_adapter and frag and T > 64 and not is_decode
                 and not torch.cuda.is_current_stream_capturing() and ops.gemm_frag_preferred(T, H, H)):
             (tid, ids), = tok_adapter.items()
             lt = self.lora_types[tid]
@@ -404,11 +423,11 @@ class LlamaForCausalLM(CausalLM):
         # below the persistent kernel's sizes the linears themselves take any mix of adapters: a prompt's where the host knows that they are few, and those of up
         # to 16 tokens whatever they are
         near = None
-        if segs or (host_ids is not None and len(tok_adapter) == 1 and "multi" not in tok_adapter and frag and T > 64 and not is_decode):
+        if not four_bit and (segs or host_ids is not None and len(tok_adapter) == 1 and "multi" not in tok_adapter and frag and T > 64 and not is_decode):
             (tid, ids), = tok_adapter.items()
             near = (self.lora_types[tid], ids, 1 if segs else distinct_adapters(host_ids[tid], self.lora_types[tid].n_adapters))
         o_shares = None
-        if tok_adapter and "multi" not in tok_adapter and len(tok_adapter) == 1 and is_decode and T > 64 and frag:
+        if tok_adapter and "multi" not in tok_adapter and len(tok_adapter) == 1 and is_decode and T > 64 and frag and getattr(kv, "plan", None) is None:
             (tid, ids), = tok_adapter.items()
             lt = self.lora_types[tid]
             if ops.o_shrink_served(T, s.num_attention_heads, s.num_key_value_heads, s.head_dim, H, lt.r):
@@ -446,7 +465,7 @@ class LlamaForCausalLM(CausalLM):
                     if tok_adapter:
                         self._lora(resid, attn, l, "o_proj", tok_adapter, segs)
             xn = ops.rmsnorm(resid, L["ln2"], s.rms_norm_eps, frag=frag, parts=parts)
-            if (dec_frag and I % 32 == 0 or T <= 64 and frag and hasattr(self, "_il_cache")) and not (tok_adapter and self._targets(l, "gate_proj", "up_proj")):
+            if not four_bit and (dec_frag and I % 32 == 0 or T <= 64 and frag and hasattr(self, "_il_cache")) and not (tok_adapter and self._targets(l, "gate_proj", "up_proj")):
                 # decode step (or, where one has made that order of the weights, a short prompt) without an adapter on gate / up: the
                 # SiLU product is the epilogue of the GEMV (same bits)
                 act = ops.gate_up_silu(xn, self.interleaved_gate_up()[l])
@@ -585,7 +604,7 @@ class LlamaForCausalLM(CausalLM):
         """Whether `mlora_prefill` takes a pass: not a decode step, activations in fragment order, a cache of at least the model's layers, and `forward` is this
         class's (whose launches it queues)."""
         s = self.shape
-        return (getattr(self.forward, "__func__", None) is LlamaForCausalLM.forward and kv._cur is not None and not kv._cur[2] and h.dim() == 2 and h.shape[0] > 0 and h.is_cuda and h.dtype == torch.float32
+        return (self.quant_group is None and getattr(self.forward, "__func__", None) is LlamaForCausalLM.forward and kv._cur is not None and not kv._cur[2] and h.dim() == 2 and h.shape[0] > 0 and h.is_cuda and h.dtype == torch.float32
                 and h.is_contiguous() and not s.hidden_size % 32 and not s.q_size % 32 and not s.intermediate_size % 32
                 and tuple(h.shape) == (sum(kv._cur[1]), s.hidden_size) and kv.n_layers >= len(self.layers))
 
@@ -708,9 +727,11 @@ class LlamaForCausalLM(CausalLM):
             raise KeyError(f"adapter type a{tid} not loaded")
 
     def weight_bytes_per_step(self):
-        """Algorithmic fp16 weight bytes one decode step streams (all layers + lm_head)."""
+        """Algorithmic weight bytes one decode step streams (all layers + lm_head)."""
         s = self.shape
         per_layer = sum(np.prod(linear_dims(s, p)) for p in LINEARS)
+        if self.quant_group is not None:
+            return int((0.5 + 3 / self.quant_group) * per_layer * s.num_hidden_layers + 2 * s.vocab_size * s.hidden_size)
         return int(2 * (per_layer * s.num_hidden_layers + s.vocab_size * s.hidden_size))
 
 

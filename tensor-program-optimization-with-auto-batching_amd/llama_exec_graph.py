@@ -18,6 +18,7 @@ import torch
 
 from . import ops
 from .exec_graph import ExecGraph
+from .token_rules import BatchRules
 
 
 @dataclasses.dataclass
@@ -42,6 +43,11 @@ class LlamaExecConfig:
     # Same arithmetic per token, but larger token counts take other GEMM kernels and summation orders, so the first
     # token of a request can differ from the per-request prefill at a near tie.
     batch_prefill: bool = False
+    # Let a request whose prompt begins like that of one prefilled before it, with the same adapter, take over the whole pages of that
+    # beginning instead of prefilling them again (not in a batch_prefill pass, whose prompts run at once).  Decode steps then read what
+    # their requests share once, where that pays; a batch for which it does runs through the recorded per-operator step.  Shorter
+    # prefills take other kernels and summation orders, so a token can differ at a near tie.
+    share_prefix: bool = False
 
 
 class LlamaExecGraph(ExecGraph):
@@ -50,6 +56,7 @@ class LlamaExecGraph(ExecGraph):
         self.measure = False
         self.measure_file = None
         self.step_ms = []
+        self._ended = set()           # sequences of a decode that had no token left
 
     def set_exec_vars(self, vm, dev, params, tokenizer, seq_info, exec_config, eos_token_id=None, free_pages=None):
         self.vm = vm                  # a LlamaForCausalLM: entry points by name
@@ -62,11 +69,13 @@ class LlamaExecGraph(ExecGraph):
         self.free_pages = free_pages
         self.measure = False
         self.kv_cache = None
+        self._prompts = {}            # sequence -> its prompt's tokens, of those prefilled
         self.set_kv_cache(False)
 
     def set_kv_cache(self, delete_prev=True):
         if delete_prev:
             self.kv_cache = None
+        self._prompts = {}
         n = self.seq_info.get_num_sequences()
         c = self.exec_config
         self.kv_cache = self.vm["create_paged_kv_cache"](
@@ -118,6 +127,8 @@ class LlamaExecGraph(ExecGraph):
         sid = op.seqids[0]
         tokens = op.input_vars[0].var
         self.kv_cache.add_sequence(sid)
+        self._prompts[sid] = tokens.reshape(-1)
+        tokens = tokens[:, self._share_prefix(sid):]
         hidden = self.vm["embed"](torch.from_numpy(np.ascontiguousarray(tokens)))
         adapter = self.seq_info.get_adapter_info(sid)
         ev = self._tic()
@@ -128,7 +139,39 @@ class LlamaExecGraph(ExecGraph):
             logits, _ = self.vm[f"prefill_a{adapter['tid']}"](hidden, self.kv_cache, [adapter["wid"]])
         self.kv_cache.end_forward()
         self._toc(ev)
-        op.output_vars[0].var = int(ops.argmax(logits).cpu()[0])
+        op.output_vars[0].var = int(self._choose_first([sid], logits)[0])
+
+    def _share_prefix(self, sid):
+        """Tokens of the prompt that the sequence takes over from one prefilled before (`LlamaExecConfig.share_prefix`): all but the
+        last at most, which the pass needs."""
+        if not getattr(self.exec_config, "share_prefix", False) or not self.kv_cache.shares_pages:
+            return 0
+        mine, best, most = self._prompts[sid], None, 0
+        adapter = self.seq_info.get_adapter_info(sid)
+        for other, tokens in self._prompts.items():
+            if other == sid or other not in self.kv_cache.slot or self.seq_info.get_adapter_info(other) != adapter:
+                continue
+            n = min(len(tokens), len(mine) - 1)
+            differ = np.flatnonzero(tokens[:n] != mine[:n])
+            n = int(differ[0]) if differ.size else n
+            if n > most:
+                best, most = other, n
+        return self.kv_cache.share_prefix(sid, best, most) if best is not None else 0
+
+    def _choose_first(self, sids, logits):
+        """The tokens behind the prompts, on the host."""
+        rules = [self.seq_info.get_rules(sid) for sid in sids]
+        if not any(r is not None for r in rules):
+            return ops.argmax(logits).cpu().numpy()
+        batch = BatchRules(rules, [self._prompts[s] for s in sids], [[] for _ in sids], 1, logits.shape[1], logits.device)
+        return batch.choose(logits).cpu().numpy()
+
+    def _batch_rules(self, seqs, outputs, room):
+        """The rules of a decode batch, or None where no request has any."""
+        rules = [self.seq_info.get_rules(sid) for sid in seqs]
+        if not any(r is not None for r in rules):
+            return None
+        return BatchRules(rules, [self._prompts[s] for s in seqs], [outputs[s] for s in seqs], room, self.vm.vocab_size, self.vm.device)
 
     def _prefill_batch(self, op):
         """The prompts of several requests in one forward pass (`LlamaExecConfig.batch_prefill`; the reference
@@ -142,8 +185,9 @@ class LlamaExecGraph(ExecGraph):
         T = sum(lens)
         per_type = {}                                           # adapter type -> weight id per token, -1 elsewhere
         start = 0
-        for sid, L in zip(op.seqids, lens):
+        for sid, L, prompt in zip(op.seqids, lens, prompts):
             self.kv_cache.add_sequence(sid)
+            self._prompts[sid] = prompt
             adapter = self.seq_info.get_adapter_info(sid)
             if adapter is not None:
                 per_type.setdefault(adapter["tid"], np.full(T, -1, dtype=np.int32))[start:start + L] = adapter["wid"]
@@ -155,13 +199,18 @@ class LlamaExecGraph(ExecGraph):
         logits = self.vm.forward(hidden, self.kv_cache, ids, self.vm._last_rows(self.kv_cache))
         self.kv_cache.end_forward()
         self._toc(ev)
-        first = ops.argmax(logits).cpu().numpy()
+        first = self._choose_first(op.seqids, logits)
         for i in range(n):
             op.output_vars[i].var = int(first[i])
 
     def check_seqs_finished(self, seqs_2_decode, outputs):
-        return [sid for sid in seqs_2_decode
-                if outputs[sid][-1] != self.eos_token_id and len(outputs[sid]) < self.seq_info.get_max_gen_len(sid)]
+        """The sequences that go on.  One that had no token left (-1) has ended ahead of it."""
+        for sid in seqs_2_decode:
+            if -1 in outputs[sid]:
+                del outputs[sid][outputs[sid].index(-1):]
+                self._ended.add(sid)
+        return [sid for sid in seqs_2_decode if sid not in self._ended and outputs[sid][-1] != self.eos_token_id
+                and len(outputs[sid]) < self.seq_info.get_max_gen_len(sid)]
 
     def execute_decode(self, op):
         assert len(op.input_vars) == len(op.output_vars), "decode node needs as many output vars as input vars"
@@ -169,12 +218,19 @@ class LlamaExecGraph(ExecGraph):
         seqs, original_positions = self.seq_info.order_seqs(op.seqids)
         outputs = {sid: [int(op.input_vars[original_positions[i]].var)] for i, sid in enumerate(seqs)}
         ordered = list(seqs)
+        self._ended = set()
+        if any(outputs[sid][0] < 0 for sid in seqs):        # nothing was left ahead of the first step
+            seqs = [sid for sid in seqs if outputs[sid][0] >= 0]
+            self.check_seqs_finished([sid for sid in ordered if outputs[sid][0] < 0], outputs)
         # As in the reference (`:102-141`), the finish rule (`:94-100`) is applied only after a decode step: every
         # sequence takes at least one step after its prefill, also when its first token is EOS or max_gen_len is 1.
         while seqs:
             method, params = self.seq_info.get_decode_method(seqs)
+            ruled = any(self.seq_info.get_rules(sid) is not None for sid in seqs)
             if getattr(self.exec_config, "native_decode", False):
-                if not self.vm.native_step:               # a model without the C decode step: graph-replayed operators
+                # a model without the C decode step, rules, which it does not apply, or shared pages, which it reads for every request:
+                # graph-replayed operators
+                if not self.vm.native_step or ruled or self._shared_pays(seqs):
                     seqs = self._decode_session(seqs, outputs, method, params)
                     continue
                 dense = len(seqs) <= 64 and self._dense_ok(method)       # the dense shrink serves at most 64 sequences
@@ -188,7 +244,8 @@ class LlamaExecGraph(ExecGraph):
             logits, _ = self.vm[method](hidden, self.kv_cache, *params)
             self.kv_cache.end_forward()
             self._toc(ev)
-            nxt = ops.argmax(logits).cpu().numpy()
+            rules = self._batch_rules(seqs, outputs, 1)
+            nxt = (ops.argmax(logits) if rules is None else rules.choose(logits)).cpu().numpy()
             for i, sid in enumerate(seqs):
                 outputs[sid].append(int(nxt[i]))
             seqs = self.check_seqs_finished(seqs, outputs)
@@ -230,6 +287,11 @@ class LlamaExecGraph(ExecGraph):
             if len(left) != len(seqs):
                 return left
 
+    def _shared_pays(self, seqs):
+        """Whether the batch shares pages that its attention reads once, and those are enough to give up the native step's fused launches."""
+        plan = self.kv_cache.shared_plan(seqs) if hasattr(self.kv_cache, "shared_plan") else None
+        return plan is not None and plan.saved_bytes >= 512e6
+
     @staticmethod
     def _method_tids(method):
         return [int(t) for t in re.findall(r"_a(\d+)", method)]
@@ -242,16 +304,22 @@ class LlamaExecGraph(ExecGraph):
                     and len({lt.scaling for lt in types}) == 1)
 
     def _decode_session(self, seqs, outputs, method, params):
-        """A batch that mixes adapter types (`mixed_decode_a{i}_a{j}...`): the per-operator step with the tokens,
-        positions and context lengths kept on the device, replayed from a graph when enough steps lie ahead.  Same
-        kernels in the same order as the call-per-step path, so the same tokens."""
+        """A batch that the native step does not serve - of several adapter types (`mixed_decode_a{i}_a{j}...`), under rules, or with
+        shared pages that pay: the per-operator step with the tokens, positions and context lengths kept on the device,
+        replayed from a graph when enough steps lie ahead.  Same kernels in the same order as the call-per-step path,
+        so the same tokens."""
         from .decode_session import DecodeSession
         tids = self._method_tids(method)
-        pairs = {tid: (params[2 * i], params[2 * i + 1]) for i, tid in enumerate(tids)}
+        if method.startswith("mixed_decode"):
+            pairs = {tid: (params[2 * i], params[2 * i + 1]) for i, tid in enumerate(tids)}
+        else:
+            pairs = {tid: (None, params[0]) for tid in tids}
         last = [outputs[sid][-1] for sid in seqs]
         ahead = max(1, min(self.seq_info.get_max_gen_len(sid) - len(outputs[sid]) for sid in seqs))
-        sess = DecodeSession(self.vm, self.kv_cache, seqs, self.vm._ids(len(seqs), pairs), last, use_graph=ahead >= 8)
-        if self.eos_token_id is None and not self.measure:
+        rules = self._batch_rules(seqs, outputs, ahead)
+        sess = DecodeSession(self.vm, self.kv_cache, seqs, self.vm._ids(len(seqs), pairs), last, use_graph=ahead >= 8, rules=rules)
+        held = rules is not None and rules.held            # a grammar is asked between two steps
+        if self.eos_token_id is None and not self.measure and not held:
             for _ in range(ahead):
                 sess.step(keep_history=True)
             toks = torch.stack(sess.history).cpu().numpy()             # [ahead, batch]
@@ -268,6 +336,8 @@ class LlamaExecGraph(ExecGraph):
             left = self.check_seqs_finished(seqs, outputs)
             if len(left) != len(seqs):
                 return left
+            if held:
+                rules.allow([outputs[sid] for sid in seqs])
 
     def execute_decode_answer(self, op):
         assert len(op.input_vars) == 1 and len(op.output_vars) == 1 and len(op.seqids) == 1, \

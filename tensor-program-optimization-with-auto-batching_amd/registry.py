@@ -58,11 +58,12 @@ class Tensors:
         return self._file_of[name].get_tensor(name)
 
 
-def load_model(folder: str, dtype: str = None, device="cuda:0"):
-    """The model of a folder in one of its element types (default: its first)."""
+def load_model(folder: str, dtype: str = None, device="cuda:0", **options):
+    """The model of a folder in one of its element types (default: its first).  options: what else its class takes (Llama: quant_group,
+    for linears in 4 bits)."""
     config = read_config(folder)
     cls = model_class(config)
     dtype = dtype or cls.dtypes[0]
     if dtype not in cls.dtypes:
         raise ValueError(f"{cls.__name__} runs in {cls.dtypes}, not in {dtype}")
-    return cls.from_weights(config, Tensors(folder), getattr(torch, dtype), device)
+    return cls.from_weights(config, Tensors(folder), getattr(torch, dtype), device, **options)

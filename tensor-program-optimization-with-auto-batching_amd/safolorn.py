@@ -136,6 +136,10 @@ class SafolornForCausalLM(CausalLM):
         return PagedLatentCache(layers, n_pages, max_seqs=max_batch_size, max_blocks=max_blocks, max_pos=max_blocks * page_size,
                                 dtype=self.dtype, device=self.device, free_pages=free_pages, page_size=page_size)
 
+    @property
+    def vocab_size(self):
+        return self.config.vocab
+
     # ------------------------------------------------------------------ forward
     def embed(self, input_ids: torch.Tensor) -> TokenHidden:
         ids = ops.upload(input_ids.reshape(-1), self.device, torch.int32).contiguous()

@@ -19,6 +19,7 @@ class _Request:
     max_gen_len: int
     tid: Optional[int] = None     # adapter type, None = no adapter
     wid: Optional[int] = None     # weight id inside the type
+    rules: Optional[object] = None    # token_rules.TokenRules
 
 
 class LlamaSeqInfo:
@@ -56,6 +57,9 @@ class LlamaSeqInfo:
                   f"{{'tid': {tid}, 'wid': {int(wid)}}}")
         req.tid, req.wid = tid, int(wid)
 
+    def set_rules(self, sid: int, rules) -> None:
+        self._requests[sid].rules = rules
+
     # ------------------------------------------------------------------ queries
     def get_num_sequences(self) -> int:
         return len(self._requests)
@@ -66,6 +70,9 @@ class LlamaSeqInfo:
     def get_adapter_info(self, sid: int) -> Optional[dict]:
         req = self._requests[sid]
         return None if req.tid is None else {"tid": req.tid, "wid": req.wid}
+
+    def get_rules(self, sid: int):
+        return self._requests[sid].rules
 
     def get_adapter_configs(self) -> list:
         return self._types

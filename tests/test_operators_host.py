@@ -55,3 +55,105 @@ def test_shared_attention_refusals():
     assert call(own=0) == -1 and call(slots=1) == -1 and call(B=-1) == -1 and call(B=70000) == -1
     assert call(ws=None) == -3 and call(nb=need - 1) == -3 and call(ws=24) == -3
     assert call(B=0) == 0
+
+
+def _cache(**kw):
+    kvc = load_pkg("kv_cache")
+    return kvc.PagedKVCache(1, 40, 2, 64, max_seqs=8, max_blocks=12, rope_theta=1e4, max_pos=192, device="cpu", **kw)
+
+
+def _fill(kv, sid, n):
+    kv.add_sequence(sid)
+    kv.begin_forward([sid], [n])
+    kv.end_forward()
+
+
+def test_shared_pages_have_owners_and_go_back_with_the_last():
+    kv = _cache()
+    free = set(kv.free)
+    _fill(kv, "a", 70)
+    kv.add_sequence("b")
+    assert kv.share_prefix("b", "a", 69) == 64 and kv.lens["b"] == 64 and kv.pages_of("b") == kv.pages_of("a")[:4]
+    kv.add_sequence("c")
+    assert kv.share_prefix("c", "b") == 64
+    kv.add_sequence("d")
+    assert kv.share_prefix("d", "a", 15) == 0 and kv.lens["d"] == 0 and kv.pages_of("d") == []
+    kv.begin_forward(["b", "c", "a"], [3, 20, 1])
+    kv.end_forward()
+    shared, own_a = kv.pages_of("a")[:4], kv.pages_of("a")[4:]
+    assert kv.pages_of("b")[:4] == shared and kv.pages_of("c")[:4] == shared and kv.lens["c"] == 84
+    assert len({*kv.pages_of("a"), *kv.pages_of("b"), *kv.pages_of("c")}) == 4 + 1 + 1 + 2
+    assert (kv.block_table[kv.slot["c"], :4] == kv.block_table[kv.slot["a"], :4]).all()
+    kv.free_sequence("a")
+    assert set(own_a) <= set(kv.free) and not set(shared) & set(kv.free)
+    kv.free_sequence("c")
+    assert not set(shared) & set(kv.free)
+    kv.free_sequence("b")
+    kv.free_sequence("d")
+    assert set(kv.free) == free and len(kv.free) == len(free) and not kv._owners
+
+
+def test_share_prefix_refusals():
+    import pytest
+    kv = _cache()
+    _fill(kv, 0, 40)
+    _fill(kv, 1, 5)
+    kv.add_sequence(2)
+    for sid, of in ((1, 0), (0, 0), (2, 2)):
+        with pytest.raises(ValueError):
+            kv.share_prefix(sid, of)
+    with pytest.raises(KeyError):
+        kv.share_prefix(2, 7)
+    kv.begin_forward([1], [1])
+    with pytest.raises(RuntimeError):
+        kv.share_prefix(2, 0)
+    kv.end_forward()
+    assert kv.share_prefix(2, 0, -3) == 0 and kv.share_prefix(2, 0, 1000) == 32
+    time_mix = load_pkg("time_mix")
+    state = load_pkg("kv_cache").PagedStateCache([time_mix.TimeMixSpec(2, 8)], 64, 4, 2, 4, 64, dtype=__import__("torch").float32, device="cpu")
+    state.add_sequence(0)
+    state.add_sequence(1)
+    with pytest.raises(ValueError):
+        state.share_prefix(1, 0)
+
+
+def test_prefix_groups_save_most():
+    kv = _cache()
+    _fill(kv, 0, 16 * 6)
+    for sid, of, n in ((1, 0, 16 * 6), (2, 0, 16 * 2), (3, 0, 16 * 5)):
+        kv.add_sequence(sid)
+        kv.share_prefix(sid, of, n)
+    _fill(kv, 4, 20)
+    kv.begin_forward([0, 1, 2, 3], [1, 1, 40, 1])
+    kv.end_forward()
+    # all four share two pages (saves 6); 0, 1 and 3 share five (saves 10)
+    assert kv.prefix_groups([0, 1, 2, 3, 4]) == [([0, 1, 3], 5)]
+    assert kv.prefix_groups([4, 2, 0]) == [([1, 2], 2)]
+    assert kv.prefix_groups([4]) == [] and kv.prefix_groups([0]) == [] and kv.prefix_groups([]) == []
+    for sid in (5, 6):
+        kv.add_sequence(sid)
+        kv.share_prefix(sid, 4)
+    assert sorted(kv.prefix_groups([5, 0, 6, 3, 1])) == [([0, 2], 1), ([1, 3, 4], 5)]
+
+
+def test_plans_of_a_cache_live_with_their_sequences():
+    kv = _cache(n_q_heads=2)
+    _fill(kv, 0, 33)
+    kv.add_sequence(1)
+    kv.share_prefix(1, 0)
+    assert kv.shared_plan([0, 1]) is None and (0, 1) in kv._plans          # two pages do not pay
+    kv.free_sequence(1)
+    assert not kv._plans and kv.shared_plan([0]) is None
+
+
+def test_grammar_masks_and_rules_on_the_host():
+    import pytest
+    tr = load_pkg("token_rules")
+    with pytest.raises(ValueError):
+        tr.TokenRules(repetition=0.0)
+    si = load_pkg("seq_info").LlamaSeqInfo(4)
+    si.add_sequence(0)
+    assert si.get_rules(0) is None
+    r = tr.TokenRules(bias={3: 1.0})
+    si.set_rules(0, r)
+    assert si.get_rules(0) is r
