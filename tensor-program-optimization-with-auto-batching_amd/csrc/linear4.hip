@@ -75,6 +75,12 @@ __device__ __forceinline__ void l4_store(const Linear4& a, int t, int n, f32x4 s
     }
 }
 
+__device__ __forceinline__ void l4_store(const Linear4& a, int out, int t, int n, f32x4 s) {
+  if (out == L4_F16) l4_store<L4_F16>(a, t, n, s);                          // uniform
+  else if (out == L4_F32) l4_store<L4_F32>(a, t, n, s);
+  else l4_store<L4_ACC>(a, t, n, s);
+}
+
 // Up to 16 tokens: a workgroup has NT tiles of rows, its waves take every eighth block of K and their sums meet in LDS, in wave order.
 template <int NT, int GB, int OUT>      // GB: groups per block
 __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kernel(Linear4 a) {
@@ -160,14 +166,17 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
   }
 }
 
-// More tokens: the waves of a workgroup split its rows (MID_NT tiles each) and share the token block, which comes block of K by block of K straight
-// into an LDS ring together with the weights and their scales; a wave's share of a stage is the same number of requests for all, so that
-// a counted wait leaves the later stages in flight.  Rows of x lie in LDS as 256 bytes each, their sixteen 16-byte pieces exchanged by
-// the row's number: the lanes that fetch a fragment of 16 rows then touch every bank once.  Few rows of W: K is cut into slices that leave
-// fp32 partial sums for a second launch.
-constexpr int MID_WAVES = 4, MID_NT = 2, MID_RING = 3, MID_ROWS = MID_WAVES * MID_NT * 16;
+// More tokens: two groups of four waves take every second block of a slice of K each; a group's waves split the workgroup's rows (NT tiles each)
+// and share the token block, which comes block of K by block of K straight into the group's LDS ring together with the weights and
+// their scales; a wave's share of a stage is the same number of requests for all, so that a counted wait leaves the later stages in
+// flight.  The groups take turns: one reads its next block from LDS into registers, the other multiplies.  (Both at a time, as four
+// waves a group or eight, took 5% longer; LDS, the matrix cores and what unpacks and scales the weights each need a third of the time.)
+// Rows of x lie in LDS as 256 bytes each, their sixteen 16-byte pieces exchanged by the row's number: the lanes that fetch a fragment of
+// 16 rows then touch every bank once.  The groups' sums meet in LDS; more slices of K leave fp32 partial sums for a second launch.
+constexpr int MID_WAVES = 4, MID_GROUPS = 2, MID_THREADS = MID_GROUPS * MID_WAVES * WAVE;
 constexpr int MID_WBYTES = 1024 + 256;          // a tile's block: words, then scales and zeros (padded to a request of 4 bytes a lane)
-constexpr int mid_stage_bytes(int TT) { return TT * 4096 + MID_WAVES * MID_NT * MID_WBYTES; }
+constexpr int mid_stage_bytes(int TT, int NT) { return TT * 4096 + MID_WAVES * NT * MID_WBYTES; }
+constexpr int mid_ring(int TT, int NT) { return MID_GROUPS * 3 * mid_stage_bytes(TT, NT) <= 160 * 1024 ? 3 : 2; }      // stages
 
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
@@ -179,22 +188,26 @@ __device__ __forceinline__ void to_lds4(const void* g, char* l) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 4, 0, 0);
 }
 
-template <int TT, int GB, int OUT, bool XFRAG>
-__global__ __launch_bounds__(MID_WAVES * WAVE, 2) void linear4_mid_kernel(Linear4 a, float* __restrict__ part) {
-  constexpr int RING = MID_RING, STAGE = mid_stage_bytes(TT), XQ = TT * 4 / MID_WAVES, LOADS = XQ + 2 * MID_NT;   // requests of a wave per stage
-  extern __shared__ __align__(16) char ring[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+template <int TT, int NT, int GB, bool XFRAG>
+__global__ __launch_bounds__(MID_THREADS, 2) void linear4_mid_kernel(Linear4 a, int out, float* __restrict__ part) {
+  constexpr int RING = mid_ring(TT, NT), STAGE = mid_stage_bytes(TT, NT), XQ = TT * 4 / MID_WAVES, LOADS = XQ + 2 * NT;   // requests of a wave per stage
+  constexpr int HELD = NT * TT > 8 ? GB < 4 ? 3 : 2 : 4;     // k-steps whose x waits in registers: all, where they are enough
+  using zeros_t = std::conditional_t<GB == 1, uint8_t, std::conditional_t<GB == 2, uint16_t, uint32_t>>;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % MID_WAVES;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / MID_WAVES;
+  char* ring = lds + group * (RING * STAGE);
   const int r16 = lane & 15, kg = lane >> 4;
   const int nb = (a.K + L4_BLOCK - 1) / L4_BLOCK, KB = a.K / 32, tiles = (a.N + 15) / 16;
   const NibbleConsts nc = nibble_consts();
-  const int tile0 = (blockIdx.x * MID_WAVES + wave) * MID_NT, t0 = blockIdx.z * (16 * TT);
+  const int tile0 = (blockIdx.x * MID_WAVES + wave) * NT, t0 = blockIdx.z * (16 * TT);
   const int b0 = (int)((long)nb * blockIdx.y / gridDim.y), b1 = (int)((long)nb * (blockIdx.y + 1) / gridDim.y);
 
   // uniform bases, and 32-bit offsets of the lanes
-  const char* wsrc[MID_NT];
-  const char* msrc[MID_NT];
+  const char* wsrc[NT];
+  const char* msrc[NT];
 #pragma unroll
-  for (int i = 0; i < MID_NT; ++i) {
+  for (int i = 0; i < NT; ++i) {
     const size_t rb = (size_t)(tile0 + i < tiles ? tile0 + i : tiles - 1) * nb;
     wsrc[i] = (const char*)a.q + rb * 1024;
     msrc[i] = a.meta + rb * (48 * GB);
@@ -220,11 +233,12 @@ __global__ __launch_bounds__(MID_WAVES * WAVE, 2) void linear4_mid_kernel(Linear
   }
   const int whole = KB / 4;                     // blocks of four k-steps
   // Workgroups begin at different blocks of their slice, so that they do not all ask for the same lines of x at a time.
-  const int n_own = b1 - b0;
+  const int n_own = (b1 - b0 + MID_GROUPS - 1) / MID_GROUPS;            // of a group: block i is b0 + group + 2 i; the second's last may be none
   int next = blockIdx.x % n_own;
   auto issue = [&](int slot) {
     char* st = ring + slot * STAGE;
-    const int b = b0 + next;                    // past the slice: once more from the front, and not multiplied
+    int b = b0 + group + MID_GROUPS * next;     // past the slice: once more from the front, and not multiplied
+    b = b < b1 ? b : b0;
     next = next + 1 == n_own ? 0 : next + 1;
     const char* xb = xbase + b * xblock;
     if (b < whole) {                            // uniform
@@ -234,103 +248,144 @@ __global__ __launch_bounds__(MID_WAVES * WAVE, 2) void linear4_mid_kernel(Linear
 #pragma unroll
       for (int q = 0; q < XQ; ++q) to_lds16(xb + xend[q], st + (wave + MID_WAVES * q) * 1024);
     }
-    char* w = st + TT * 4096 + wave * (MID_NT * MID_WBYTES);
+    char* w = st + TT * 4096 + wave * (NT * MID_WBYTES);
 #pragma unroll
-    for (int i = 0; i < MID_NT; ++i) {
+    for (int i = 0; i < NT; ++i) {
       to_lds16(wsrc[i] + (size_t)b * 1024 + woff, w + i * MID_WBYTES);
       to_lds4(msrc[i] + (size_t)b * (48 * GB) + moff, w + i * MID_WBYTES + 1024);
     }
   };
-  f32x4 acc[MID_NT][TT];
+  f32x4 acc[NT][TT];
 #pragma unroll
-  for (int i = 0; i < MID_NT; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < TT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < RING - 1; ++u) issue(u);
   int rd = 0, wr = RING - 1, at = blockIdx.x % n_own;
+  wait_loads<(RING - 2) * LOADS>();
+  bare_barrier();
+  if (group == 1) bare_barrier();               // one group reads LDS while the other multiplies
   for (int n = 0; n < n_own; ++n) {
-    const int b = b0 + at;
+    const int b = b0 + group + MID_GROUPS * at;
     at = at + 1 == n_own ? 0 : at + 1;
-    wait_loads<(RING - 2) * LOADS>();           // this wave's pieces of block b have landed, its reads of the block before are done
-    bare_barrier();
     issue(wr);
     const char* st = ring + rd * STAGE;
-    const char* w = st + TT * 4096 + wave * (MID_NT * MID_WBYTES);
+    const char* w = st + TT * 4096 + wave * (NT * MID_WBYTES);
     rd = rd + 1 == RING ? 0 : rd + 1;
     wr = wr + 1 == RING ? 0 : wr + 1;
-    u32x4 q[MID_NT];
-    f16 sc[MID_NT][4 * GB];
-    uint8_t zr[MID_NT][GB];
+    u32x4 q[NT];
+    f16 sc[NT][4 * GB];
+    zeros_t zr[NT];
+    f16x8 x[HELD][TT];
+    auto fetch = [&](int k) {                   // the fragments of k-step k
 #pragma unroll
-    for (int i = 0; i < MID_NT; ++i) {
+      for (int j = 0; j < TT; ++j)
+        x[k % HELD][j] = *reinterpret_cast<const f16x8*>(XFRAG ? st + (k * TT + j) * 1024 + lane * 16 : st + (j * 16 + r16) * 256 + (((k * 4 + kg) ^ r16) * 16));
+    };
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
       q[i] = *reinterpret_cast<const u32x4*>(w + i * MID_WBYTES + lane * 16);
 #pragma unroll
       for (int g = 0; g < GB; ++g) {
         const f16x4 v = *reinterpret_cast<const f16x4*>(w + i * MID_WBYTES + 1024 + kg * 8 * GB + g * 8);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[i][g * 4 + e] = v[e];
-        zr[i][g] = *reinterpret_cast<const uint8_t*>(w + i * MID_WBYTES + 1024 + 32 * GB + r16 * GB + g);
       }
+      zr[i] = *reinterpret_cast<const zeros_t*>(w + i * MID_WBYTES + 1024 + 32 * GB + r16 * GB);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    const int nks = KB - b * 4;                 // k-steps of the block: 4, or fewer at the end of K
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) fetch(k);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    bare_barrier();
+    const int nks = b < b1 ? KB - b * 4 : 0;    // k-steps of the block: 4, or fewer at the end of K
     auto block = [&](auto WHOLE) {
+      constexpr int PER = 4 / GB;
+      constexpr bool LATE = HELD == 4;       // a group's sums are scaled between the next one's products, where registers hold both
+      f32x4 sum[NT][TT];
+      f16x8 wf[2][NT];
+      auto weights = [&](int k) {
 #pragma unroll
-    for (int g = 0; g < GB; ++g) {
-      f32x4 sum[MID_NT][TT];
-      f16x2 zz[MID_NT], zs[MID_NT];
+        for (int i = 0; i < NT; ++i) {
+          const f16 z = (f16)(float)(zr[i] >> 8 * (k / PER) & 0xff);
+          wf[k & 1][i] = l4_weights(q[i][k], nc, f16x2{(f16)1024.f + z, (f16)1024.f + z}, f16x2{-((f16)64.f + z), -((f16)64.f + z)});
+        }
+      };
+      auto multiply = [&](int k, int j) {
 #pragma unroll
-      for (int i = 0; i < MID_NT; ++i) {
-        const f16 z = (f16)(float)zr[i][g];
-        zz[i] = f16x2{(f16)1024.f + z, (f16)1024.f + z};
-        zs[i] = f16x2{-((f16)64.f + z), -((f16)64.f + z)};
+        for (int i = 0; i < NT; ++i) sum[i][j] = mfma_16x16x32(wf[k & 1][i], x[k % HELD][j], k % PER == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[i][j]);
+      };
+      auto scale = [&](int g, int j) {
 #pragma unroll
-        for (int j = 0; j < TT; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int k = g * (4 / GB); k < (g + 1) * (4 / GB); ++k) {
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[i][j][e], (float)sc[i][e * GB + g], acc[i][j][e]);
+      };
+      weights(0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
         if (!decltype(WHOLE)::value && k >= nks) break;       // uniform
-        f16x8 wf[MID_NT];
-#pragma unroll
-        for (int i = 0; i < MID_NT; ++i) wf[i] = l4_weights(q[i][k], nc, zz[i], zs[i]);
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-          const f16x8 x = *reinterpret_cast<const f16x8*>(XFRAG ? st + (k * TT + j) * 1024 + lane * 16
-                                                                : st + (j * 16 + r16) * 256 + (((k * 4 + kg) ^ r16) * 16));
+          if (LATE && k % PER == 0 && k > 0) scale(k / PER - 1, j);
+          multiply(k, j);
+        }
+        if (k + HELD < 4) {
+          __builtin_amdgcn_sched_barrier(0);
+          fetch(k + HELD);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (k < 3) weights(k + 1);
+        // a product occupies the matrix cores for the time of four other instructions
 #pragma unroll
-          for (int i = 0; i < MID_NT; ++i) sum[i][j] = mfma_16x16x32(wf[i], x, sum[i][j]);
+        for (int j = 0; j < NT * TT; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!LATE && k % PER == PER - 1) {
+#pragma unroll
+          for (int j = 0; j < TT; ++j) scale(k / PER, j);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
 #pragma unroll
-      for (int i = 0; i < MID_NT; ++i)
+      for (int k = PER; k <= 4; k += PER)
+        if (LATE && k == (decltype(WHOLE)::value ? 4 : nks)) {
 #pragma unroll
-        for (int j = 0; j < TT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[i][j][e], (float)sc[i][e * GB + g], acc[i][j][e]);
-    }
+          for (int j = 0; j < TT; ++j) scale(k / PER - 1, j);
+        }
     };
     if (nks >= 4) block(std::true_type());
-    else block(std::false_type());
+    else if (nks > 0) block(std::false_type());
+    wait_loads<(RING - 2) * LOADS>();           // this wave's pieces of the next block have landed
+    bare_barrier();
   }
-  wait_loads<0>();                              // nothing is in flight into LDS that another workgroup may get
+  if (group == 0) bare_barrier();
+  wait_loads<0>();                              // nothing is in flight into LDS that is used otherwise now
+  bare_barrier();
+  f32x4* meet = reinterpret_cast<f32x4*>(lds) + wave * (NT * TT * WAVE) + lane;
+  constexpr int GROUP = MID_WAVES * NT * TT * WAVE;
 #pragma unroll
-  for (int i = 0; i < MID_NT; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int j = 0; j < TT; ++j) {
-      const int n = (tile0 + i) * 16 + kg * 4, t = t0 + j * 16 + r16;
-      if (part) {                               // whole tiles in the lanes' order: 1 KiB a store, where rows of y would be 16 pieces of 64 bytes
-        if (tile0 + i < tiles && t0 + j * 16 < a.T)
-          reinterpret_cast<f32x4*>(part)[(((size_t)blockIdx.y * tiles + tile0 + i) * ((a.T + 15) / 16) + t0 / 16 + j) * WAVE + lane] = acc[i][j];
-      } else if (t < a.T && n < a.N) {
-        l4_store<OUT>(a, t, n, acc[i][j]);
-      }
+    for (int j = 0; j < TT; ++j) meet[group * GROUP + (i * TT + j) * WAVE] = acc[i][j];
+  __syncthreads();
+#pragma unroll 1
+  for (int o = group; o < NT * TT; o += MID_GROUPS) {
+    const f32x4 sum = meet[o * WAVE] + meet[GROUP + o * WAVE];
+    const int tile = tile0 + o / TT, j = o % TT, n = tile * 16 + kg * 4, t = t0 + j * 16 + r16;
+    if (part) {                                 // whole tiles in the lanes' order: 1 KiB a store, where rows of y would be 16 pieces of 64 bytes
+      if (tile < tiles && t0 + j * 16 < a.T)
+        reinterpret_cast<f32x4*>(part)[(((size_t)blockIdx.y * tiles + tile) * ((a.T + 15) / 16) + t0 / 16 + j) * WAVE + lane] = sum;
+    } else if (t < a.T && n < a.N) {
+      l4_store(a, out, t, n, sum);
     }
+  }
 }
 
 // y from the slices' partial sums, in slice order
-template <int OUT>
-__global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, const float* __restrict__ part, int slices) {
+__global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, int out, const float* __restrict__ part, int slices) {
   const int tts = (a.T + 15) / 16, tiles = (a.N + 15) / 16;
   const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6), n_tiles = (size_t)tiles * tts;
   if (i >= n_tiles) return;
@@ -339,7 +394,7 @@ __global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, const floa
   f32x4 s = p[0];
 #pragma unroll 4
   for (int k = 1; k < slices; ++k) s += p[k * n_tiles * WAVE];
-  if (t < a.T && n < a.N) l4_store<OUT>(a, t, n, s);
+  if (t < a.T && n < a.N) l4_store(a, out, t, n, s);
 }
 
 template <int NT, int GB>
@@ -350,42 +405,55 @@ void launch(const Linear4& a, int out, hipStream_t s) {
   else hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_ACC>), grid, block, 0, s, a);
 }
 
-template <int TT, int GB, int OUT, bool XFRAG>
-int launch_mid_as(const Linear4& a, int slices, float* part, hipStream_t s) {
-  constexpr int lds = MID_RING * mid_stage_bytes(TT);
-  static const hipError_t configured = hipFuncSetAttribute((const void*)linear4_mid_kernel<TT, GB, OUT, XFRAG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (configured != hipSuccess) return mlora_set_error(MLORA_ERR_LAUNCH, "linear4: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(configured));
-  hipLaunchKernelGGL((linear4_mid_kernel<TT, GB, OUT, XFRAG>), dim3(ceil_div(a.N, MID_ROWS), slices, ceil_div(a.T, 16 * TT)), dim3(MID_WAVES * WAVE), lds, s, a,
-                     slices > 1 ? part : nullptr);
-  if (int e = mlora_launch_status("linear4")) return e;
-  if (slices > 1)
-    hipLaunchKernelGGL(linear4_join_kernel<OUT>, dim3((unsigned)(((long)ceil_div(a.T, 16) * ceil_div(a.N, 16) + 3) / 4)), dim3(256), 0, s, a, (const float*)part, slices);
-  return mlora_launch_status("linear4");
-}
-
-template <int TT, int GB>
-int launch_mid(const Linear4& a, int out, int slices, float* part, hipStream_t s) {
-  if (a.frag_tt) {
-    if (out == L4_F16) return launch_mid_as<TT, GB, L4_F16, true>(a, slices, part, s);
-    if (out == L4_F32) return launch_mid_as<TT, GB, L4_F32, true>(a, slices, part, s);
-    return launch_mid_as<TT, GB, L4_ACC, true>(a, slices, part, s);
-  }
-  if (out == L4_F16) return launch_mid_as<TT, GB, L4_F16, false>(a, slices, part, s);
-  if (out == L4_F32) return launch_mid_as<TT, GB, L4_F32, false>(a, slices, part, s);
-  return launch_mid_as<TT, GB, L4_ACC, false>(a, slices, part, s);
-}
+// How a product of more than 16 tokens is cut: row tiles of a wave, and slices of K (0 slices: the kernel for 16 tokens).
+struct MidCut {
+  int tiles, slices;
+};
 
 int mid_tt(int T) { return T <= 32 ? 2 : 4; }
 
-// How a product is cut: slices of K (0: the kernel whose waves split K).
-int mid_slices(int T, int K, int N) {
-  if (T <= 16) return 0;
-  const int nb = ceil_div(K, L4_BLOCK);
-  const int tt = mid_tt(T);
-  const long wgs = (long)ceil_div(N, MID_ROWS) * ceil_div(T, 16 * tt);
-  long s = 512 / wgs;
-  if (s > nb / 4) s = nb / 4;
-  return s < 1 ? 1 : s > 16 ? 16 : (int)s;
+// The cut of the least estimated time: rounds of the 256 compute units, which hold one workgroup each, times 3 us and what a step costs - a block
+// for either group, (1 + tiles) / 2 us for 64 tokens and a third less for 32 -, and for more than one slice the partial sums' write and read
+// and the second launch.  Measured, us with 1, 2 and 3 tiles, then 1 tile in 2 and in 4 slices (groups of 64):
+//   64 tokens, 4096 x 4096    18.1  24.7  33.1  14.4  12.9        200 tokens, 4096 x 12288   52.2  49.3  36.7  66.4  84.5
+//   64 tokens, 4096 x 12288   18.9  25.4  33.8  25.2  26.4        32 tokens, 11008 x 4096    31.1  49.7  62.4  20.4  14.6
+//   128 tokens, 4096 x 16384  36.6  28.3  35.9  47.1  61.2        64 tokens, 11008 x 4096    35.1  50.2  64.8  23.0  16.3
+MidCut mid_cut(int T, int K, int N) {
+  if (T <= 16) return {0, 0};
+  const int nb = ceil_div(K, L4_BLOCK), tt = mid_tt(T);
+  MidCut best = {1, 1};
+  double least = 0;
+  for (int tiles = 1; tiles <= 3; ++tiles)
+    for (int slices = 1; slices <= 16 && (slices == 1 || 4 * slices <= nb); ++slices) {
+      const long wgs = (long)ceil_div(N, 16 * MID_WAVES * tiles) * ceil_div(T, 16 * tt) * slices;
+      const int steps = ceil_div(ceil_div(nb, slices), MID_GROUPS);
+      const double us = (double)((wgs + 255) / 256) * (3 + steps * (tt == 4 ? 0.5 : 0.33) * (1 + tiles)) + (slices > 1 ? 2.5 + 3e-6 * slices * T * N : 0);
+      if (least == 0 || us < least) {
+        best = {tiles, slices};
+        least = us;
+      }
+    }
+  return best;
+}
+
+template <int TT, int NT, int GB, bool XFRAG>
+int launch_mid_as(const Linear4& a, int out, int slices, float* part, hipStream_t s) {
+  constexpr int ring = MID_GROUPS * mid_ring(TT, NT) * mid_stage_bytes(TT, NT), meet = MID_THREADS * NT * TT * 16, lds = ring > meet ? ring : meet;
+  static const hipError_t configured = hipFuncSetAttribute((const void*)linear4_mid_kernel<TT, NT, GB, XFRAG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (configured != hipSuccess) return mlora_set_error(MLORA_ERR_LAUNCH, "linear4: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(configured));
+  hipLaunchKernelGGL((linear4_mid_kernel<TT, NT, GB, XFRAG>), dim3(ceil_div(a.N, 16 * MID_WAVES * NT), slices, ceil_div(a.T, 16 * TT)), dim3(MID_THREADS), lds, s, a,
+                     out, slices > 1 ? part : nullptr);
+  if (int e = mlora_launch_status("linear4")) return e;
+  if (slices > 1)
+    hipLaunchKernelGGL(linear4_join_kernel, dim3((unsigned)(((long)ceil_div(a.T, 16) * ceil_div(a.N, 16) + 3) / 4)), dim3(256), 0, s, a, out, (const float*)part, slices);
+  return mlora_launch_status("linear4");
+}
+
+template <int TT, int GB, bool XFRAG>
+int launch_mid(const Linear4& a, int out, MidCut cut, float* part, hipStream_t s) {
+  if (cut.tiles == 1) return launch_mid_as<TT, 1, GB, XFRAG>(a, out, cut.slices, part, s);
+  if (cut.tiles == 2) return launch_mid_as<TT, 2, GB, XFRAG>(a, out, cut.slices, part, s);
+  return launch_mid_as<TT, 3, GB, XFRAG>(a, out, cut.slices, part, s);
 }
 
 // Tiles of a workgroup up to 16 tokens: as many as leave the most loaded compute unit the fewest; of equal counts the larger, whose fewer
@@ -404,11 +472,11 @@ int row_tiles(int tiles) {
 }
 
 template <int GB>
-int launch_shape(const Linear4& a, int out, float* part, hipStream_t s) {
-  const int tiles = ceil_div(a.N, 16), slices = mid_slices(a.T, a.K, a.N);
-  if (slices > 0) {
-    if (a.T <= 32) return launch_mid<2, GB>(a, out, slices, part, s);
-    return launch_mid<4, GB>(a, out, slices, part, s);
+int launch_shape(const Linear4& a, int out, MidCut cut, float* part, hipStream_t s) {
+  const int tiles = ceil_div(a.N, 16);
+  if (cut.slices > 0) {
+    if (a.T <= 32) return a.frag_tt ? launch_mid<2, GB, true>(a, out, cut, part, s) : launch_mid<2, GB, false>(a, out, cut, part, s);
+    return a.frag_tt ? launch_mid<4, GB, true>(a, out, cut, part, s) : launch_mid<4, GB, false>(a, out, cut, part, s);
   }
   switch (row_tiles(tiles)) {
     case 1: launch<1, GB>(a, out, s); break;
@@ -432,9 +500,10 @@ extern "C" int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, siz
   return MLORA_OK;
 }
 
+static size_t partial_bytes(int slices, int T, int N) { return slices > 1 ? (size_t)slices * ceil_div(T, 16) * ceil_div(N, 16) * 256 * sizeof(float) : 0; }
+
 extern "C" size_t mlora_linear4_workspace_bytes(int T, int K, int N) {
-  const int slices = T > 0 && K > 0 && N > 0 ? mid_slices(T, K, N) : 0;
-  return slices > 1 ? (size_t)slices * ceil_div(T, 16) * ceil_div(N, 16) * 256 * sizeof(float) : 0;
+  return T > 0 && K > 0 && N > 0 ? partial_bytes(mid_cut(T, K, N).slices, T, N) : 0;
 }
 
 extern "C" int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* meta, int group,
@@ -452,10 +521,11 @@ extern "C" int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int 
   Linear4 a = {y, (const f16*)x, (const uint32_t*)q, (const char*)meta, ldx, x_layout == MLORA_FRAG ? mlora_frag_tiles(T) : 0, T, K, N, N % 4 == 0 && ((uintptr_t)y & 15) == 0};
   const int out = mode == MLORA_ACCUMULATE ? L4_ACC : y_dtype == MLORA_F32 ? L4_F32 : L4_F16;
   hipStream_t s = (hipStream_t)stream;
-  const size_t need = mlora_linear4_workspace_bytes(T, K, N);
+  const MidCut cut = mid_cut(T, K, N);
+  const size_t need = partial_bytes(cut.slices, T, N);
   MLORA_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), MLORA_ERR_WORKSPACE,
               "linear4: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  if (group == 128) return launch_shape<1>(a, out, (float*)workspace, s);
-  if (group == 64) return launch_shape<2>(a, out, (float*)workspace, s);
-  return launch_shape<4>(a, out, (float*)workspace, s);
+  if (group == 128) return launch_shape<1>(a, out, cut, (float*)workspace, s);
+  if (group == 64) return launch_shape<2>(a, out, cut, (float*)workspace, s);
+  return launch_shape<4>(a, out, cut, (float*)workspace, s);
 }
