@@ -54,7 +54,7 @@ __device__ __forceinline__ int context_of(const SharedAttn& a, int row, int& seq
 // the sequence whose table names the pages of a unit's rows (a lane each): the first that is one
 __device__ __forceinline__ int sequence_of(const SharedAttn& a, const int32_t* __restrict__ d) {
   const int lane = threadIdx.x & 63;
-  const int row = d[8 + lane], seq = lane < d[0] ? a.seq_ids[row] : -1;
+  const int row = d[8 + lane], seq = lane < d[0] && (uint32_t)row < (uint32_t)a.B ? a.seq_ids[row] : -1;
   const unsigned long long ok = __ballot(seq >= 0 && seq < a.n_seq);
   return ok ? __builtin_amdgcn_readlane(seq, __builtin_ctzll(ok)) : 0;
 }
@@ -80,6 +80,7 @@ struct Tile {
 template <int D>
 __device__ __forceinline__ void tile_begin(Tile<D>& t, const SharedAttn& a, int row, int head) {
   const int g = (threadIdx.x & 63) >> 4;
+  if (row >= a.B) row = -1;
   t.row = row;
   t.head = head;
   int unused;
@@ -181,7 +182,7 @@ __device__ __forceinline__ void tile_end(Tile<D>& t) {
 
 template <int D>
 __device__ __forceinline__ void tile_store(const Tile<D>& t, const SharedAttn& a, int slot) {
-  if (t.row < 0) return;
+  if (t.row < 0 || (uint32_t)slot >= (uint32_t)a.slots) return;
   const int g = (threadIdx.x & 63) >> 4;
   const size_t at = ((size_t)t.row * a.Hq + t.head) * a.slots + slot;
 #pragma unroll
@@ -206,13 +207,14 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
     seq = sequence_of(a, d);
   } else {
     const int i = u - a.n_units, part = i % a.own_splits, b = i / a.own_splits;
-    const int have = (context_of(a, b, seq) + PAGE - 1) / PAGE, from = a.row_pages[b];
+    const int have = (context_of(a, b, seq) + PAGE - 1) / PAGE, from = a.row_pages[b] > 0 ? a.row_pages[b] : 0;
     const int n = have > from ? have - from : 0, per = (n + a.own_splits - 1) / a.own_splits;
     page0 = from + part * per;
     page1 = page0 + per < from + n ? page0 + per : from + n;
     slot = a.row_slots[b] + part;
     row = col < G ? b : -1;
   }
+  if (page0 < 0) page0 = 0;
   if (page1 > a.max_blocks) page1 = a.max_blocks;
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
   f16x8 k[2][NKB];
@@ -260,8 +262,8 @@ template <int D, int R>
 __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* __restrict__ d, int kh, f16* ring) {
   constexpr int KP = D / 32, PE = PAGE * D, STAGE = 4 * PE;       // pieces of 1 KiB a wave fetches; elements of a page's keys; of a stage
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int G = a.Hq / a.Hkv, rows = d[0] * G, page0 = d[1], slot = d[3];
-  const int page1 = page0 + d[2] < a.max_blocks ? page0 + d[2] : a.max_blocks;
+  const int G = a.Hq / a.Hkv, rows = d[0] * G, page0 = d[1] > 0 ? d[1] : 0, slot = d[3];
+  const int page1 = d[1] + d[2] < a.max_blocks ? d[1] + d[2] : a.max_blocks;
   const int seq = sequence_of(a, d);
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
   const f16* src = (wave & 1 ? a.v_cache : a.k_cache) + (size_t)kh * PE + lane * 8;
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(4 * WAVE) void shared_attn_join_kernel(SharedAttn a
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = blockIdx.y;
   const int h = W > 1 ? blockIdx.x : blockIdx.x * 4 + wave, w0 = W > 1 ? wave : 0;
   if (h >= a.Hq) return;                                    // (whole workgroups where waves meet)
-  const int n = a.row_slots[b] + a.own_splits;
+  const int n = a.row_slots[b] + a.own_splits < a.slots ? a.row_slots[b] + a.own_splits : a.slots;
   const size_t at = ((size_t)b * a.Hq + h) * a.slots;
   float M = -INFINITY, L = 0.f, o[PER] = {};
   for (int s0 = w0; s0 < n; s0 += 4 * W) {                  // four units at a time, requested together

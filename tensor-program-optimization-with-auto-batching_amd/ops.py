@@ -1004,33 +1004,33 @@ class SharedPrefixPlan:
         self.data = upload(torch.tensor(records + row_pages + row_slots, dtype=torch.int32), device)
         n = len(records)
         self.units, self.row_pages, self.row_slots = self.data[:n], self.data[n:n + B], self.data[n + B:]
+        self.workspace_bytes = lib().mlora_shared_attn_workspace_bytes(B, Hq, D, self.slots)
+        # what the C call takes of a plan, whose arrays live as long as it does
+        self._heads, self._page = (Hq, Hkv, D), ((Hkv, D // 32, 4, 16, 8), (Hkv, D, 16))
+        self._args = (self.units.data_ptr(), self.n_block, self.n_units, self.row_pages.data_ptr(), self.row_slots.data_ptr(), self.own_splits, self.slots)
 
 
 def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, plan: SharedPrefixPlan, Hq, Hkv, D, out=None, frag=False):
     """`paged_attn_decode` for a batch whose rows share prefixes as `plan` says: shared pages are read once for all their rows."""
-    B = qkv.shape[0]
-    n_seq, max_blocks = block_table.shape
+    B, (n_seq, max_blocks), (n_pages, *page_k), (pages_v, *page_v) = qkv.shape[0], block_table.shape, k_cache.shape, v_cache.shape
     dev = _here(qkv.device, "paged_attn_decode_shared")
-    if (plan.B, plan.Hq, plan.Hkv, plan.D) != (B, Hq, Hkv, D) or plan.data.device != dev:
+    if plan.B != B or plan._heads != (Hq, Hkv, D) or plan.data.device != dev:
         raise ValueError(f"paged_attn_decode_shared: a plan of {(plan.B, plan.Hq, plan.Hkv, plan.D)} on {plan.data.device} for {(B, Hq, Hkv, D)} on {dev}")
-    if qkv.numel() != B * (Hq + 2 * Hkv) * D or seq_ids.shape != (B,) or ctx_len.shape != (B,) or k_cache.shape != (k_cache.shape[0], Hkv, D // 32, 4, 16, 8) \
-            or v_cache.shape != (k_cache.shape[0], Hkv, D, 16):
+    if qkv.numel() != B * (Hq + 2 * Hkv) * D or seq_ids.shape != (B,) or ctx_len.shape != (B,) or pages_v != n_pages or (tuple(page_k), tuple(page_v)) != plan._page:
         raise ValueError(f"paged_attn_decode_shared: qkv{tuple(qkv.shape)} rows{tuple(seq_ids.shape)} contexts{tuple(ctx_len.shape)} k{tuple(k_cache.shape)} "
                          f"v{tuple(v_cache.shape)}")
     if out is not None and (tuple(out.shape) != (B, Hq * D) or isinstance(out, FragActivation) != frag):
         raise ValueError(f"paged_attn_decode_shared: out{tuple(out.shape)}")
+    if any(t.device != dev for t in (k_cache, v_cache, block_table, seq_ids, ctx_len)) or out is not None and out.device != dev:
+        raise ValueError(f"paged_attn_decode_shared: all tensors on {dev}")
     out, optr, lay = _out_arg(out, B, Hq * D, frag, dev)
     if B == 0:
         return out
-    L = lib()
-    nb = L.mlora_shared_attn_workspace_bytes(B, Hq, D, plan.slots)
+    nb, f16, i32 = plan.workspace_bytes, torch.float16, torch.int32
     ws = torch.empty(nb // 4, dtype=torch.float32, device=dev)
-    f16, i32 = torch.float16, torch.int32
-    check(L.mlora_paged_attn_decode_shared(optr, lay, _dev(qkv, f16, "qkv"), _dev(k_cache, f16, "k_cache"), _dev(v_cache, f16, "v_cache"),
-                                           _dev(block_table, i32, "block_table"), max_blocks, _dev(seq_ids, i32, "seq_ids"), _dev(ctx_len, i32, "ctx_len"),
-                                           plan.units.data_ptr(), plan.n_block, plan.n_units, plan.row_pages.data_ptr(),
-                                           plan.row_slots.data_ptr(), plan.own_splits, plan.slots, B, Hq, Hkv, D, k_cache.shape[0], n_seq, ws.data_ptr(), nb,
-                                           _stream()))
+    check(lib().mlora_paged_attn_decode_shared(optr, lay, _dev(qkv, f16, "qkv"), _dev(k_cache, f16, "k_cache"), _dev(v_cache, f16, "v_cache"),
+                                               _dev(block_table, i32, "block_table"), max_blocks, _dev(seq_ids, i32, "seq_ids"), _dev(ctx_len, i32, "ctx_len"),
+                                               *plan._args, B, Hq, Hkv, D, n_pages, n_seq, ws.data_ptr(), nb, _stream()))
     return out
 
 
