@@ -275,6 +275,11 @@ class PagedKVCache(PageTable):
         super().free_sequence(sid)
         self._plans = {b: p for b, p in self._plans.items() if sid not in b}
 
+    def share_prefix(self, sid, of, tokens=None):
+        n = super().share_prefix(sid, of, tokens)
+        self._plans = {b: p for b, p in self._plans.items() if sid not in b}
+        return n
+
     def shared_plan(self, seq_ids):
         """The plan by which a decode step of these sequences reads the pages they share once, or None where none are shared or it does
         not pay.  Kept while all of them live (a recorded step reads it).  us of attention without / with, 50 own tokens a row:

@@ -450,6 +450,8 @@ def _linear4(x, W, out, out_dtype, accumulate):
         out = torch.empty((T, N), dtype=out_dtype, device=dev)
     elif out.shape != (T, N) or out.device != dev:
         raise ValueError(f"linear: out{tuple(out.shape)} on {out.device}, expected {(T, N)} on {dev}")
+    if out.dtype not in (torch.float16, torch.float32):
+        raise TypeError(f"linear: a 4-bit weight gives float16 or float32, not {out.dtype}")
     if T == 0:
         return out
     if isinstance(x, FragActivation):

@@ -144,6 +144,10 @@ def test_plans_of_a_cache_live_with_their_sequences():
     assert kv.shared_plan([0, 1]) is None and (0, 1) in kv._plans          # two pages do not pay
     kv.free_sequence(1)
     assert not kv._plans and kv.shared_plan([0]) is None
+    kv.add_sequence(2)
+    kv._plans[(0, 2)] = None                                             # asked before there was anything to share
+    kv.share_prefix(2, 0)
+    assert not kv._plans
 
 
 def test_grammar_masks_and_rules_on_the_host():

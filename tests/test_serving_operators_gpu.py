@@ -336,3 +336,79 @@ def test_all_together_in_a_recorded_session(four_bit):
         for a, t in zip(answers, plain_ids(z, rules, prompts, answers)):
             a.append(t)
     assert [a[1:] for a in answers] == eager.T.tolist()
+
+
+def test_four_bit_decode_of_wide_mixed_batches():
+    """More than 64 requests of two adapter types and none on a 4-bit base: rows as alone."""
+    print("case wide mixed", flush=True)
+    synth = load_pkg("synth")
+    wl = synth.config1()
+    specs = [wl.lora, synth.LoraSpec(r=8, alpha=16.0, n_adapters=3, targets=("q_proj", "o_proj", "gate_proj", "down_proj"))]
+    model = load_pkg("llama").LlamaForCausalLM.from_synthetic(5, wl.shape, specs, DEV, quant_group=32)
+    rng = np.random.default_rng(5)
+    rows = 70
+    prompts = [rng.integers(0, wl.shape.vocab_size, 3 + i % 9).astype(np.int32) for i in range(rows)]
+    who = [(None, 0)[i % 2] if i % 3 else 1 for i in range(rows)]
+    kv = model.create_paged_kv_cache(2 * rows, 2 * rows * 16, 16, 16)
+    for copy in range(2):
+        for i, p in enumerate(prompts):
+            sid = copy * rows + i
+            kv.add_sequence(sid)
+            kv.begin_forward([sid], [len(p)])
+            h = model.embed(torch.from_numpy(p))
+            _ = model["prefill_no_adapter"](h, kv) if who[i] is None else model[f"prefill_a{who[i]}"](h, kv, [i % 3])
+            kv.end_forward()
+    tokens = rng.integers(0, wl.shape.vocab_size, rows)
+    pairs = []
+    for tid in (0, 1):
+        at = [i for i in range(rows) if who[i] == tid]
+        pairs += [at, [i % 3 for i in at]]
+    kv.begin_forward(list(range(rows)), [1] * rows)
+    wide, _ = model["mixed_decode_a0_a1"](model.embed(torch.from_numpy(tokens.astype(np.int32))), kv, *pairs)
+    kv.end_forward()
+    for i in range(rows):
+        sid = rows + i
+        kv.begin_forward([sid], [1])
+        h = model.embed(torch.as_tensor(tokens[i:i + 1].astype(np.int32)))
+        alone, _ = model["decode_no_adapter"](h, kv) if who[i] is None else model[f"decode_a{who[i]}"](h, kv, np.array([i % 3], dtype=np.int32))
+        kv.end_forward()
+        assert err(wide[i].cpu().numpy(), alone[0].cpu().numpy()) <= 1e-2          # (whole-model bound, as against the oracle)
+
+
+def test_latent_pages_are_shared_too():
+    """A cache of latents: a sequence on another's pages has the logits of the whole prompt."""
+    print("case latent", flush=True)
+    import safolorn_cases as C
+    from oracle import safolorn_ref as R
+    name, cfg = next(iter(C.CONFIGS.items()))
+    weights = C.weights(cfg, 3, 1.0)
+    model = load_pkg("safolorn").SafolornForCausalLM.from_weights(cfg, C.tensors(weights), torch.float32, DEV)
+    rng = np.random.default_rng(9)
+    head, tails = rng.integers(0, cfg["vocab"], 70), [rng.integers(0, cfg["vocab"], n) for n in (5, 20)]
+    kv = model.create_paged_kv_cache(4, 1024, 1024, 16)
+    def run(sid, t):
+        kv.begin_forward([sid], [len(t)])
+        out = model.forward(model.embed(torch.from_numpy(np.asarray(t).astype(np.int32))), kv, None)
+        kv.end_forward()
+        return out.double().cpu().numpy()
+    kv.add_sequence(0)
+    run(0, np.concatenate([head, tails[0]]))
+    kv.add_sequence(1)
+    skip = kv.share_prefix(1, 0, len(head))
+    assert skip == 64
+    prompt = np.concatenate([head, tails[1]])
+    got = run(1, prompt[skip:])
+    kv.free_sequence(0)
+    got = np.concatenate([got, run(1, [int(tails[0][0])])])
+    want = R.forward(np.concatenate([prompt, tails[0][:1]]), cfg, weights)[skip:]
+    d = got - want
+    assert np.abs(d).max() <= 2e-5 * 5 * want.std()          # rms 2e-5 of the logits' scale (the model's bound in fp32), five times that at most
+
+
+def test_four_bit_linear_refuses_other_results():
+    ops = load_pkg("ops")
+    w = ops.quantize(torch.randn(32, 64, device=DEV), 32)
+    x = torch.randn(3, 64, device=DEV).half()
+    for kw in ({"out_dtype": torch.bfloat16}, {"out": torch.empty(3, 32, dtype=torch.bfloat16, device=DEV)}):
+        with pytest.raises(TypeError):
+            ops.linear(x, w, **kw)
