@@ -56,6 +56,14 @@ __device__ __forceinline__ f16x8 l4_weights(uint32_t w, const NibbleConsts& k, f
   return f16x8{a.h[0], a.h[1], b.h[0], b.h[1], c.h[0], c.h[1], d.h[0], d.h[1]};
 }
 
+// A uniform address that stays in scalar registers: lanes then add a 32-bit offset to it, where the compiler would carry 64 bits a lane for every
+// pointer of a loop.  It costs scalar instructions ahead of each load (16 tokens, 22016 x 4096: 12.9 to 13.5 us), and pays where the vector
+// registers would run out (the same in groups of 32: 32 to 17.7 us).
+__device__ __forceinline__ const char* uniform(const char* p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
 // Four columns n .. of a token's result
 template <int OUT>
 __device__ __forceinline__ void l4_store(const Linear4& a, int t, int n, f32x4 s) {
@@ -82,7 +90,7 @@ __device__ __forceinline__ void l4_store(const Linear4& a, int out, int t, int n
 }
 
 // Up to 16 tokens: a workgroup has NT tiles of rows, its waves take every eighth block of K and their sums meet in LDS, in wave order.
-template <int NT, int GB, int OUT>      // GB: groups per block
+template <int NT, int GB, int OUT, int DEPTH>      // GB: groups per block; DEPTH: blocks of a wave on their way
 __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kernel(Linear4 a) {
   __shared__ f32x4 red[L4_WAVES][NT][WAVE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -96,6 +104,7 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
   // (rows behind the last token: the last one again, whose results are dropped)
   const f16* xp = a.x + (a.frag_tt ? (size_t)lane * 8 : (size_t)(r16 < a.T ? r16 : a.T - 1) * a.ldx + kg * 8);
   const size_t xstep = a.frag_tt ? (size_t)a.frag_tt * 512 : 32;
+  const uint32_t qoff = lane * 16, soff = kg * 8 * GB, zoff = 32 * GB + r16 * GB;
   f32x4 acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -105,18 +114,20 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
     uint8_t z[NT][GB];
     f16x8 x[4];
   };
-  auto load = [&](Stage& st, int b) {
+  auto load = [&](Stage& st, int b, auto WHOLE) {          // (no branch where four k-steps are sure: behind one, a block on its way is waited for)
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const size_t rb = row_block[i] + b;
-      st.q[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.q + rb * 256 + lane * 4));
-      __builtin_memcpy(st.s[i], __builtin_assume_aligned(a.meta + rb * (48 * GB) + kg * 8 * GB, 8), sizeof(st.s[i]));
-      __builtin_memcpy(st.z[i], __builtin_assume_aligned(a.meta + rb * (48 * GB) + 32 * GB + r16 * GB, GB), sizeof(st.z[i]));
+      const char *m = a.meta + rb * (48 * GB), *q = (const char*)a.q + rb * 1024;
+      if constexpr (GB >= 2 && (NT == 3 || NT * GB >= 16)) m = uniform(m), q = uniform(q);
+      st.q[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(q + qoff));
+      __builtin_memcpy(st.s[i], __builtin_assume_aligned(m + soff, 8), sizeof(st.s[i]));
+      __builtin_memcpy(st.z[i], __builtin_assume_aligned(m + zoff, GB), sizeof(st.z[i]));
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int ks = b * 4 + k;
-      st.x[k] = ks < KB ? ld8(xp + (size_t)ks * xstep) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      st.x[k] = decltype(WHOLE)::value || ks < KB ? ld8(xp + (size_t)ks * xstep) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
     }
   };
   auto multiply = [&](const Stage& st) {
@@ -133,26 +144,32 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
         for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(sum[e], (float)st.s[i][e * GB + g], acc[i][e]);
       }
   };
-  if constexpr (NT == 1) {                      // few rows: two blocks in flight (4096 x 4096, one token: 5.3 to 4.8 us; with more tiles it costs registers)
-    Stage st[2];
-    load(st[0], wave < nb ? wave : 0);
-    load(st[1], wave + L4_WAVES < nb ? wave + L4_WAVES : 0);
-    for (int b = wave; b < nb; b += 2 * L4_WAVES) {
+  const int whole = KB / 4, own = (whole - wave + L4_WAVES - 1) / L4_WAVES;      // whole blocks, those of this wave
+  Stage st[DEPTH];
+  if (own > 0) {                                // uniform
+    auto at = [&](int i) { return wave + i * L4_WAVES; };
+    constexpr std::true_type sure;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int next = b + (2 + u) * L4_WAVES;
-        if (b + u * L4_WAVES < nb) {            // uniform
-          multiply(st[u]);
-          if (next < nb) load(st[u], next);
-        }
+    for (int u = 0; u < DEPTH; ++u) load(st[u], at(u < own ? u : own - 1), sure);
+    int i = 0;
+    for (; i + 2 * DEPTH <= own; i += DEPTH)
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        multiply(st[u]);
+        load(st[u], at(i + DEPTH + u), sure);
       }
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      if (i + u < own) multiply(st[u]);
+      if (i + DEPTH + u < own) load(st[u], at(i + DEPTH + u), sure);
     }
-  } else {
-    Stage st;
-    for (int b = wave; b < nb; b += L4_WAVES) {
-      load(st, b);
-      multiply(st);
-    }
+#pragma unroll
+    for (int u = 0; u < DEPTH - 1; ++u)
+      if (i + DEPTH + u < own) multiply(st[u]);
+  }
+  if (whole < nb && whole % L4_WAVES == wave) { // the end of K
+    load(st[0], whole, std::false_type());
+    multiply(st[0]);
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
@@ -240,7 +257,7 @@ __global__ __launch_bounds__(MID_THREADS, 2) void linear4_mid_kernel(Linear4 a, 
     int b = b0 + group + MID_GROUPS * next;     // past the slice: once more from the front, and not multiplied
     b = b < b1 ? b : b0;
     next = next + 1 == n_own ? 0 : next + 1;
-    const char* xb = xbase + b * xblock;
+    const char* xb = uniform(xbase + b * xblock);
     if (b < whole) {                            // uniform
 #pragma unroll
       for (int q = 0; q < XQ; ++q) to_lds16(xb + xoff[q], st + (wave + MID_WAVES * q) * 1024);
@@ -251,8 +268,8 @@ __global__ __launch_bounds__(MID_THREADS, 2) void linear4_mid_kernel(Linear4 a, 
     char* w = st + TT * 4096 + wave * (NT * MID_WBYTES);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      to_lds16(wsrc[i] + (size_t)b * 1024 + woff, w + i * MID_WBYTES);
-      to_lds4(msrc[i] + (size_t)b * (48 * GB) + moff, w + i * MID_WBYTES + 1024);
+      to_lds16(uniform(wsrc[i] + (size_t)b * 1024) + woff, w + i * MID_WBYTES);
+      to_lds4(uniform(msrc[i] + (size_t)b * (48 * GB)) + moff, w + i * MID_WBYTES + 1024);
     }
   };
   f32x4 acc[NT][TT];
@@ -397,12 +414,16 @@ __global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, int out, c
   if (t < a.T && n < a.N) l4_store(a, out, t, n, s);
 }
 
+// Blocks of a wave on their way: two of one tile (one token, 11008 x 4096, one, two, three: 11.7, 9.4, 10.2 us); with more tiles they cost the registers of
+// a second workgroup on the compute unit (16 tokens, 12288 x 4096: 8.9 to 14.8 us).
+constexpr int depth_of(int NT) { return NT == 1 ? 2 : 1; }
+
 template <int NT, int GB>
 void launch(const Linear4& a, int out, hipStream_t s) {
   const dim3 grid(ceil_div(ceil_div(a.N, 16), NT)), block(L4_WAVES * WAVE);
-  if (out == L4_F16) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F16>), grid, block, 0, s, a);
-  else if (out == L4_F32) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F32>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_ACC>), grid, block, 0, s, a);
+  if (out == L4_F16) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F16, depth_of(NT)>), grid, block, 0, s, a);
+  else if (out == L4_F32) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F32, depth_of(NT)>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_ACC, depth_of(NT)>), grid, block, 0, s, a);
 }
 
 // How a product of more than 16 tokens is cut: row tiles of a wave, and slices of K (0 slices: the kernel for 16 tokens).
@@ -457,7 +478,9 @@ int launch_mid(const Linear4& a, int out, MidCut cut, float* part, hipStream_t s
 }
 
 // Tiles of a workgroup up to 16 tokens: as many as leave the most loaded compute unit the fewest; of equal counts the larger, whose fewer
-// workgroups read x less often.
+// workgroups read x less often.  Measured, us with 1, 2, 3, 4, 6 and 8 tiles (groups of 128; the choice in brackets):
+//   1 token, 4096 x 4096    [5.2]  5.9   7.2   8.3  10.4  12.5      16 tokens, 22016 x 4096  27.9  18.6  16.1  17.4  [13.6]  16.1
+//   8 tokens, 32003 x 4096  26.9  20.4  18.8  [17.5]  20.7  18.6    16 tokens, 12288 x 4096  15.7  12.9  [9.3]  9.7  11.7  14.0
 int row_tiles(int tiles) {
   int best = 1;
   long least = 0;
