@@ -219,13 +219,16 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
   f16x8 k[2][NKB];
   f16x4 v[2][NDB];
-  int id[2];
+  bool live[2];
   int own = -1, from = page0, to = page0;                   // the ids of up to 64 pages from .. to - 1, one a lane
-  auto load = [&](int s, int pg) {                          // page pg into set s
-    id[s] = pg < to ? page_id(a, __builtin_amdgcn_readlane(own, (pg - from) & 63)) : -1;
-    if (id[s] < 0) return;                                  // uniform
-    const f16* kp = a.k_cache + ((size_t)id[s] * a.Hkv + kh) * (PAGE * D) + lane * 8;
-    const f16* vp = a.v_cache + (((size_t)id[s] * a.Hkv + kh) * D + col) * PAGE + g * 4;
+  // page pg into set s; behind the last that one again, for a page that is none the first: loads without a branch, behind which the next page
+  // would be waited for as well
+  auto load = [&](int s, int pg) {
+    int id = page_id(a, __builtin_amdgcn_readlane(own, (pg < to ? pg : to - 1) - from));
+    live[s] = pg < to && id >= 0;
+    id = id < 0 ? 0 : id;
+    const f16* kp = a.k_cache + ((size_t)id * a.Hkv + kh) * (PAGE * D) + lane * 8;
+    const f16* vp = a.v_cache + (((size_t)id * a.Hkv + kh) * D + col) * PAGE + g * 4;
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) k[s][kb] = ld8(kp + kb * 512);
 #pragma unroll
@@ -234,10 +237,10 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
   Tile<D> t;
   tile_begin(t, a, row, kh * G + (row >= 0 ? col % G : 0));
   auto work = [&](int s, int pg) {
-    if (id[s] >= 0) tile_step<D, 1, true>(t, a.scale, pg, 1, [&](int, int kb) { return k[s][kb]; }, [&](int, int db) { return v[s][db]; });   // uniform
+    if (live[s]) tile_step<D, 1, true>(t, a.scale, pg, 1, [&](int, int kb) { return k[s][kb]; }, [&](int, int db) { return v[s][db]; });   // uniform
   };
   // 64 pages at a time: the wait for ids loaded inside the loop would be one for every page on its way
-  do {
+  while (from < page1) {
     to = from + 64 < page1 ? from + 64 : page1;
     own = from + lane < to ? bt[from + lane] : -1;
     load(0, from);
@@ -249,7 +252,7 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
       load(1, pg + 3);
     }
     from = to;
-  } while (from < page1);
+  }
   tile_end(t);
   tile_store(t, a, slot);
 }
