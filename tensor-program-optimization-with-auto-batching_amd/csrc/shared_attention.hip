@@ -276,12 +276,13 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
   // 64 pages at a time: the wait for ids loaded inside the loop would be one for the whole ring
   for (int from = page0; from < page1; from += 64) {
     const int to = from + 64 < page1 ? from + 64 : page1;
-    const int own = from + lane < to ? bt[from + lane] : -1;
+    int own = from + lane < to ? bt[from + lane] : -1;
+    asm volatile("" : "+v"(own));                           // (waited for here, not again with each of the first stages)
     int next = from;
     auto issue = [&](int slot_) {
       const int pg = next + (wave >> 1);
-      int id = pg < to ? page_id(a, __builtin_amdgcn_readlane(own, pg - from)) : -1;
-      id = id < 0 ? 0 : id;                                 // a page that is none: a valid address, and not multiplied
+      int id = page_id(a, __builtin_amdgcn_readlane(own, (pg < to ? pg : to - 1) - from));
+      id = id < 0 ? 0 : id;                                 // a page that is none, or behind the last: a valid address, and not multiplied
       const f16* p = src + (size_t)id * a.Hkv * PE;
       f16* l = ring + slot_ * STAGE + wave * PE;
 #pragma unroll
