@@ -283,8 +283,9 @@ class PagedKVCache(PageTable):
     def shared_plan(self, seq_ids):
         """The plan by which a decode step of these sequences reads the pages they share once, or None where none are shared or it does
         not pay.  Kept while all of them live (a recorded step reads it).  us of attention without / with, 50 own tokens a row:
-        32 heads of 128 over 32, 32 rows, 16 shared pages 16.3 / 15.0, 64 pages 36 / 17, 256 pages 135 / 32; 2 rows, 64 pages 11.2 / 11.8, 256 pages
-        39 / 25; 128 rows, 4 pages 37 / 42; 32 heads over 8, 32 rows, 64 pages 12.9 / 15.1, 256 pages 33 / 23, 64 rows, 64 pages 20 / 18."""
+        32 heads of 128 over 32, 32 rows, 16 shared pages 16.4 / 14.2, 64 pages 35 / 16, 256 pages 133 / 29; 2 rows, 64 pages 11.2 / 10.4, 256 pages
+        38 / 22; 128 rows, 4 pages 36 / 35; 32 heads over 8, 32 rows, 64 pages (130 MB) 12.8 / 14.6, 256 pages 32 / 23, 128 rows, 16 pages (133 MB) 18 / 16,
+        64 rows, 64 pages 20 / 17."""
         if not self._owners or not self.n_q_heads or not 1 <= self.n_q_heads // self.Hkv <= 16:
             return None
         batch = tuple(seq_ids)
@@ -292,7 +293,7 @@ class PagedKVCache(PageTable):
             groups = self.prefix_groups(batch)
             saved = sum((len(m) - 1) * p for m, p in groups) * self.Hkv * self.D * 4 * PAGE
             plan = None
-            if saved >= 256e6 or any(p >= 128 for _, p in groups):
+            if saved >= 132e6 or any(p >= 128 for _, p in groups):
                 plan = ops.SharedPrefixPlan(groups, [self.lens[s] + 1 for s in batch], self.n_q_heads, self.Hkv, self.D, self.device)
                 plan.saved_bytes = saved
                 self._stage()

@@ -983,11 +983,13 @@ class SharedPrefixPlan:
         large = [(rows, pages) for rows, pages in groups if len(rows) * G > 16]
         small = [(rows, pages) for rows, pages in groups if len(rows) * G <= 16]
         most = lib().mlora_shared_attn_unit_rows() // G                  # rows of a block unit
-        # pages of a unit: block units for two workgroups on each compute unit, a row's own pages for eight waves - but no shorter than some
-        # pages, and no more units of a row than its second launch joins cheaply
+        # pages of a unit: block units for two workgroups on each compute unit (16 rows behind 32752 tokens, 32 heads of 128 over 8, for one / two /
+        # three: 50 / 46 / 46.5 us, three services of 20 rows behind 4096 tokens 44 / 44 / 49), units of single waves for four (the three
+        # services, for two / four / eight / sixteen: 47 / 42 / 44.5 / 46, 32 rows behind 1024 tokens 22.7 / 22.7 / 22.7 / 26) - but no shorter than some pages
+        # (own ones two / four / eight: the first 46.4 / 46.2 / 45.2), and no more units of a row than its second launch joins cheaply
         per_block = max(8, -(-sum(-(-len(rows) // most) * pages for rows, pages in large) * Hkv // 512))
-        per_wave = max(4, -(-sum(pages for _, pages in small) * Hkv // 2048))
-        self.own_splits = max(1, min(-(-max(own, default=0) // 4), 2048 // max(B * Hkv, 1), 64))
+        per_wave = max(4, -(-sum(pages for _, pages in small) * Hkv // 1024))
+        self.own_splits = max(1, min(-(-max(own, default=0) // 8), 1024 // max(B * Hkv, 1), 64))
         units = []
         for rows, pages in large + small:
             block = len(rows) * G > 16
