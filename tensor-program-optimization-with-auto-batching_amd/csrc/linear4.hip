@@ -2,8 +2,11 @@
 //   y[t, n] (=|+=) sum over groups g of K:  s[n, g] sum_{k in g} x[t, k] (q[n, k] - z[n, g]),   q, z = 0 .. 15
 //
 // The matrix cores multiply fp16 activations with the integers q - z, which fp16 holds exactly, and a group's sum is scaled in fp32: no
-// rounding but those of fp32 sums and the result's.  For up to 64 tokens the weight stream from HBM is the bound (N K / 2 bytes and 3
-// N K / group of scales and zeros).
+// rounding but those of fp32 sums and the result's.  Up to 16 tokens the weight stream from HBM is the bound (N K / 2 bytes and 3 N K /
+// group of scales and zeros): 8 tokens, 32003 x 4096, groups of 128: 17.4 us, 4.0 TB/s, what a plain read of 2 GiB reaches on the same card;
+// 16 tokens, 22016 x 4096: 12.7 us, 3.8 TB/s; one token, 4096 x 4096: 4.8 us, a launch and two rounds to memory.  With more tokens it is the
+// unpacking and scaling on the vector units beside the products and the reads of LDS: 200 tokens, 12288 x 4096, groups of 64: 35 us, 570 TFLOP/s
+// (a plain fp16 product of 8192^3: 1.17 PFLOP/s).
 //
 // Layout (sizes: mlora_linear4_sizes; K in blocks of 128, N in tiles of 16 rows, both padded with zeros):
 //   q     [tile][block][lane 64][k-step 4] words: lane (kg, row) = lane / 16, lane % 16 holds k = 32 step + 8 kg + e of its row in word
@@ -414,7 +417,7 @@ __global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, int out, c
   if (t < a.T && n < a.N) l4_store(a, out, t, n, s);
 }
 
-// Blocks of a wave on their way: two of one tile (one token, 11008 x 4096, one, two, three: 11.7, 9.4, 10.2 us); with more tiles they cost the registers of
+// Blocks of a wave on their way: two of one tile (one token, 4096 x 11008, one, two, three: 11.7, 9.4, 10.2 us); with more tiles they cost the registers of
 // a second workgroup on the compute unit (16 tokens, 12288 x 4096: 8.9 to 14.8 us).
 constexpr int depth_of(int NT) { return NT == 1 ? 2 : 1; }
 
@@ -435,10 +438,11 @@ int mid_tt(int T) { return T <= 32 ? 2 : 4; }
 
 // The cut of the least estimated time: rounds of the 256 compute units, which hold one workgroup each, times 3 us and what a step costs - a block
 // for either group, (1 + tiles) / 2 us for 64 tokens and a third less for 32 -, and for more than one slice the partial sums' write and read
-// and the second launch.  Measured, us with 1, 2 and 3 tiles, then 1 tile in 2 and in 4 slices (groups of 64):
-//   64 tokens, 4096 x 4096    18.1  24.7  33.1  14.4  12.9        200 tokens, 4096 x 12288   52.2  49.3  36.7  66.4  84.5
-//   64 tokens, 4096 x 12288   18.9  25.4  33.8  25.2  26.4        32 tokens, 11008 x 4096    31.1  49.7  62.4  20.4  14.6
-//   128 tokens, 4096 x 16384  36.6  28.3  35.9  47.1  61.2        64 tokens, 11008 x 4096    35.1  50.2  64.8  23.0  16.3
+// and the second launch.  Measured, us with 1, 2 and 3 tiles, then 1 tile in 2 and in 4 slices and 2 in 4 (N x K,
+// groups of 64; the choice in brackets, which was the best of these in all of 27 such products):
+//   64 tokens, 4096 x 4096      17.7  25.3  31.8  14.3  [12.9]  15.2      200 tokens, 12288 x 4096    52.5  50.6  [36.6]  66.0  82.6  66.2
+//   64 tokens, 12288 x 4096    [18.6]  26.1  32.7  24.8  26.0  25.5      32 tokens, 4096 x 11008     29.6  43.5  56.8  19.5  [14.2]  17.7
+//   128 tokens, 16384 x 4096    36.2  [28.5]  34.4  46.8  60.2  51.4      64 tokens, 4096 x 11008     39.2  59.0  75.8  25.1  [17.4]  22.6
 MidCut mid_cut(int T, int K, int N) {
   if (T <= 16) return {0, 0};
   const int nb = ceil_div(K, L4_BLOCK), tt = mid_tt(T);
@@ -479,8 +483,9 @@ int launch_mid(const Linear4& a, int out, MidCut cut, float* part, hipStream_t s
 
 // Tiles of a workgroup up to 16 tokens: as many as leave the most loaded compute unit the fewest; of equal counts the larger, whose fewer
 // workgroups read x less often.  Measured, us with 1, 2, 3, 4, 6 and 8 tiles (groups of 128; the choice in brackets):
-//   1 token, 4096 x 4096    [5.2]  5.9   7.2   8.3  10.4  12.5      16 tokens, 22016 x 4096  27.9  18.6  16.1  17.4  [13.6]  16.1
-//   8 tokens, 32003 x 4096  26.9  20.4  18.8  [17.5]  20.7  18.6    16 tokens, 12288 x 4096  15.7  12.9  [9.3]  9.7  11.7  14.0
+//   1 token, 4096 x 4096    [4.7]  5.8   7.1   8.1  10.3  12.3      16 tokens, 22016 x 4096   27.7  17.4  15.1  16.2  [12.3]  14.5
+//   8 tokens, 8192 x 4096    8.3  [6.4]  7.4   8.6  10.7  12.7      8 tokens, 32003 x 4096    26.1  18.6  17.9  17.1  21.0  [17.7]
+//   16 tokens, 12288 x 4096 15.6  12.3  [8.6]  9.1  11.3  13.3      16 tokens, 128256 x 4096   133  81.5  69.8  66.2  63.5  [60.6]
 int row_tiles(int tiles) {
   int best = 1;
   long least = 0;
