@@ -69,6 +69,8 @@ class DecodeSession:
     def step(self, keep_history=False):
         """One decode step for the whole batch; returns the device tensor of new token ids (updated in place)."""
         kv = self.kv
+        if self.rules is not None:
+            self.rules.take()
         kv.begin_forward(self.seq_ids, [1] * len(self.seq_ids), device_meta=(self.rows, self.pos, self.ctx))
         if self.use_graph and self._eager_steps >= 1:
             if self.graph is None:

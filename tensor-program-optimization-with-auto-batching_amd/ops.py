@@ -476,6 +476,8 @@ def linear(x, W, out=None, out_dtype=None, accumulate=False, kernel="auto"):
     PackedWeight, or a QuantWeight (f16 x); f16, bf16 (fragment order or packed) or f32 (plain); y has their type unless out_dtype says f32.  accumulate=True adds into the fp32 tensor `out`.  kernel: "auto" | "gemv" | "gemm"."""
     out_dtype = out_dtype or W.dtype
     if isinstance(W, QuantWeight):
+        if kernel != "auto":
+            raise ValueError(f"linear: a 4-bit weight has one kernel family, not {kernel!r}")
         return _linear4(x, W, out, out_dtype, accumulate)
     if isinstance(x, FragActivation):
         return _linear_frag(x, W, out, out_dtype, accumulate)

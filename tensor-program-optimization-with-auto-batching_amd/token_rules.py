@@ -31,8 +31,9 @@ class BatchRules:
     """The rules of a batch's rows (None: a row without), whose chosen tokens go on behind their histories."""
 
     def __init__(self, rules, prompts, answers, room, vocab, device):
-        """prompts, answers: token ids per row; room: tokens a row may still be given; vocab: columns of the logits."""
-        self.rules, self.vocab, self.device = [r or TokenRules() for r in rules], vocab, device
+        """prompts, answers: token ids per row; room: tokens a row may still be given (its history has no place for more); vocab: columns
+        of the logits."""
+        self.rules, self.vocab, self.device, self.left = [r or TokenRules() for r in rules], vocab, device, max(room, 1)
         for r in self.rules:
             if r.bias and not all(0 <= int(v) < vocab for v in r.bias):
                 raise ValueError(f"TokenRules: a bias for a token outside 0..{vocab - 1}")
@@ -76,6 +77,12 @@ class BatchRules:
         if self.held:
             self.masks.copy_(torch.from_numpy(self._words.view(np.int32)))
             self.mask_row.copy_(torch.from_numpy(rows))
+
+    def take(self):
+        """Ahead of a step, recorded or not, that chooses tokens: a place of the histories is used."""
+        if self.left <= 0:
+            raise RuntimeError("BatchRules: no room for another token")
+        self.left -= 1
 
     def choose(self, logits, out=None):
         """The rows' tokens [B] int32, -1 where none is left; they go behind the rows' histories."""

@@ -63,6 +63,26 @@ def test_linear4_against_64_bits(ops, T, K, N, group):
     assert torch.equal(buf[3:3 + T * N].view(T, N), ops.linear(x, W, out_dtype=torch.float32)) and bool((buf[:3] == 3).all()) and bool((buf[3 + T * N:] == 3).all())
 
 
+# every cut of the kernel for more than 16 tokens: one to three row tiles a wave, K in slices, whole and broken last blocks for either group of
+# waves, token blocks of 32 and 64 that are not full; and of the other one tiles of every count, waves with and without the end of K
+CUTS = [(200, 160, 12200, 32), (193, 192, 12250, 64), (250, 256, 12288, 128), (100, 160, 16300, 32), (20, 1056, 12300, 32), (64, 2080, 300, 32), (48, 4160, 70, 64),
+        (25, 2048, 700, 128), (17, 128, 40000, 128), (16, 1056, 4100, 32), (9, 288, 8200, 32), (5, 320, 12290, 64), (16, 192, 16400, 64), (3, 96, 24600, 32), (2, 128, 33000, 128),
+        (1, 2016, 50, 32), (8, 1152, 33000, 64)]
+
+
+@pytest.mark.parametrize("T,K,N,group", CUTS)
+def test_every_cut(ops, T, K, N, group):
+    print("case cut", T, K, N, group, flush=True)
+    x, q, scale, zero = make(T + K + N, T, K, N, group)
+    W = ops.QuantWeight(q, scale, zero)
+    y, mag = exact(x, q, scale, zero, group)
+    for a in (x, ops.FragActivation.pack(x)):
+        for out in (torch.float16, torch.float32):
+            got = ops.linear(a, W, out_dtype=out)
+            assert bool(((got.double() - y).abs() <= bound(y, mag, K, group, out)).all())
+            assert torch.equal(got, ops.linear(a, W, out_dtype=out))
+
+
 def _shifted(x):
     flat = torch.zeros(x.numel() + 1, dtype=x.dtype, device=x.device)
     flat[1:] = x.reshape(-1)

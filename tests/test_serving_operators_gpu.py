@@ -329,6 +329,8 @@ def test_all_together_in_a_recorded_session(four_bit):
     again, replayed, batch = run(True)
     assert again == firsts and np.array_equal(eager, replayed)
     assert batch.args.lengths.tolist() == [len(p) + 1 + steps for p in prompts]
+    with pytest.raises(RuntimeError):                        # the histories have no place for another token
+        batch.take()
     kv, _ = start()
     answers = [[f] for f in firsts]
     for step in range(steps):
@@ -412,3 +414,5 @@ def test_four_bit_linear_refuses_other_results():
     for kw in ({"out_dtype": torch.bfloat16}, {"out": torch.empty(3, 32, dtype=torch.bfloat16, device=DEV)}):
         with pytest.raises(TypeError):
             ops.linear(x, w, **kw)
+    with pytest.raises(ValueError):
+        ops.linear(x, w, kernel="gemm")
