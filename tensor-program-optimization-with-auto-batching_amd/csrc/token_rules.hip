@@ -202,18 +202,42 @@ __global__ __launch_bounds__(WAVE) void token_rules_join_kernel(int32_t* __restr
   if (threadIdx.x == 0) finish(ids, r, row, best, history_of(r, row));
 }
 
-constexpr int CHUNK_THREADS = 256;
+constexpr int CHUNK_THREADS = 256, ROW_THREADS = 1024;
 constexpr int MAX_BIAS = 1024;
 
-// Quadruples of a thread: four while that leaves the device eight workgroups a compute unit or more, two below (one row of 32000: 7.5 to 6.3 us;
-// 256 rows of 128256 with two: 62 to 73 us, each chunk reading the row's history anew)
-int quads_of(int B, int V) { return (long)B * V >= 2048l * CHUNK_THREADS * 16 ? 4 : 2; }
-int chunks_of(int V, int quads) { return (int)(((long)V + 3 + CHUNK_THREADS * 4 * quads - 1) / (CHUNK_THREADS * 4 * quads)); }
+// How rows are cut: threads of a workgroup, quadruples of a thread, workgroups of a row.
+struct RowCut {
+  int threads, quads, chunks;
+};
+
+// A row that 16384 columns hold is one workgroup's, and needs no second launch; so is one of up to 32768 where rows are many; us of GPU time (of an eager
+// call) in chunks / whole: 8 rows of 8000 7.6 / 6.0 (10.8 / 7.8), of 16000 7.4 / 8.1 (11.1 / 7.8), of 32000 7.3 / 12.1; 128 rows of 16000 9.6 / 9.5 (10.6 /
+// 9.0), of 32000 13.2 / 15.4; 256 rows of 32000 21.1 / 18.4.  Chunks: four quadruples a thread while that leaves the device eight workgroups a
+// compute unit or more, two below (one row of 32000: 7.5 to 6.3 us; 256 rows of 128256 with two: 62 to 73 us, each chunk reading the row's history anew).
+RowCut row_cut(int B, int V) {
+  auto chunks = [&](int threads, int quads) { return (int)(((long)V + 3 + threads * 4 * quads - 1) / (threads * 4 * quads)); };
+  if (chunks(CHUNK_THREADS, 2) == 1) return {CHUNK_THREADS, 2, 1};
+  for (int quads : {2, 4, 8})
+    if (chunks(ROW_THREADS, quads) == 1 && (quads < 8 || B >= 192)) return {ROW_THREADS, quads, 1};
+  const int quads = (long)B * V >= 2048l * CHUNK_THREADS * 16 ? 4 : 2;
+  return {CHUNK_THREADS, quads, chunks(CHUNK_THREADS, quads)};
+}
+
+template <int NTH, int E>
+int launch(dim3 grid, hipStream_t s, int32_t* ids, float* out, long ld_out, const float* logits, long ld, const mlora_logit_rules& r, int V, Best* part) {
+  constexpr int counts = NTH * 4 * E * 4, most = counts + 2 * MAX_BIAS * 4;
+  if constexpr (most > 64 * 1024) {
+    static const hipError_t configured = hipFuncSetAttribute((const void*)token_rules_kernel<NTH, E>, hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (configured != hipSuccess) return mlora_set_error(MLORA_ERR_LAUNCH, "constrained_argmax: cannot reserve %d bytes of LDS: %s", most, hipGetErrorString(configured));
+  }
+  hipLaunchKernelGGL((token_rules_kernel<NTH, E>), grid, dim3(NTH), counts + 8 * (size_t)r.n_bias, s, ids, out, ld_out, logits, ld, r, V, part);
+  return mlora_launch_status("constrained_argmax");
+}
 
 }  // namespace
 
 extern "C" size_t mlora_constrained_argmax_workspace_bytes(int B, int V) {
-  const int chunks = B > 0 && V > 0 ? chunks_of(V, quads_of(B, V)) : 0;
+  const int chunks = B > 0 && V > 0 ? row_cut(B, V).chunks : 0;
   return chunks > 1 ? (size_t)B * chunks * sizeof(Best) : 0;
 }
 
@@ -231,15 +255,21 @@ extern "C" int mlora_constrained_argmax(int32_t* ids, float* out, long ld_out, c
   MLORA_CHECK(!r.masks || (r.mask_row && r.n_masks > 0), MLORA_ERR_INVALID, "constrained_argmax: masks without their rows");
   if (B == 0) return MLORA_OK;
   hipStream_t s = (hipStream_t)stream;
-  const int quads = quads_of(B, V), chunks = chunks_of(V, quads);
-  MLORA_CHECK(chunks == 1 || (workspace && workspace_bytes >= mlora_constrained_argmax_workspace_bytes(B, V) && ((uintptr_t)workspace & 7) == 0), MLORA_ERR_WORKSPACE,
-              "constrained_argmax: workspace of %zu bytes, %zu needed", workspace_bytes, mlora_constrained_argmax_workspace_bytes(B, V));
-  const size_t lds = (CHUNK_THREADS * 4 * quads + 2 * (size_t)r.n_bias) * 4;
-  Best* part = chunks > 1 ? (Best*)workspace : nullptr;
-  if (quads == 4) hipLaunchKernelGGL((token_rules_kernel<CHUNK_THREADS, 4>), dim3(chunks, B), dim3(CHUNK_THREADS), lds, s, ids, out, ld_out, logits, ld, r, V, part);
-  else hipLaunchKernelGGL((token_rules_kernel<CHUNK_THREADS, 2>), dim3(chunks, B), dim3(CHUNK_THREADS), lds, s, ids, out, ld_out, logits, ld, r, V, part);
-  if (chunks == 1) return mlora_launch_status("constrained_argmax");
-  if (int e = mlora_launch_status("constrained_argmax")) return e;
-  hipLaunchKernelGGL(token_rules_join_kernel, dim3(B), dim3(WAVE), 0, s, ids, r, (const Best*)workspace, chunks);
+  const RowCut cut = row_cut(B, V);
+  const size_t need = cut.chunks > 1 ? (size_t)B * cut.chunks * sizeof(Best) : 0;
+  MLORA_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 7) == 0), MLORA_ERR_WORKSPACE,
+              "constrained_argmax: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const dim3 grid(cut.chunks, B);
+  Best* part = need ? (Best*)workspace : nullptr;
+  int e;
+  if (cut.threads == CHUNK_THREADS) {
+    e = cut.quads == 4 ? launch<CHUNK_THREADS, 4>(grid, s, ids, out, ld_out, logits, ld, r, V, part) : launch<CHUNK_THREADS, 2>(grid, s, ids, out, ld_out, logits, ld, r, V, part);
+  } else {
+    e = cut.quads == 2 ? launch<ROW_THREADS, 2>(grid, s, ids, out, ld_out, logits, ld, r, V, part)
+      : cut.quads == 4 ? launch<ROW_THREADS, 4>(grid, s, ids, out, ld_out, logits, ld, r, V, part)
+                       : launch<ROW_THREADS, 8>(grid, s, ids, out, ld_out, logits, ld, r, V, part);
+  }
+  if (e || cut.chunks == 1) return e;
+  hipLaunchKernelGGL(token_rules_join_kernel, dim3(B), dim3(WAVE), 0, s, ids, r, (const Best*)workspace, cut.chunks);
   return mlora_launch_status("constrained_argmax");
 }

@@ -73,6 +73,7 @@ def show(*what):
 @pytest.mark.parametrize("B,V,cap,n_bias,n_masks,pad", [
     (1, 1, 1, 1, 1, 0), (3, 5, 7, 2, 2, 0), (2, 33, 64, 3, 1, 1), (1, 32000, 64, 4, 1, 0), (5, 32003, 900, 16, 3, 0), (4, 32765, 100, 0, 0, 3),
     (3, 32766, 300, 5, 2, 0), (2, 40961, 2000, 40, 2, 2), (7, 128256, 3001, 300, 4, 0), (3, 50257, 1, 1024, 2, 1), (70, 1023, 5000, 7, 5, 0),
+    (2, 2045, 500, 5, 1, 0), (2, 2046, 500, 5, 1, 0), (9, 8189, 700, 9, 2, 1), (3, 8190, 700, 9, 2, 2), (4, 16381, 1200, 0, 3, 3), (4, 16382, 1200, 30, 0, 0), (192, 32765, 40, 3, 2, 1), (192, 32766, 40, 0, 1, 0),
 ])
 def test_rules_bit_for_bit_and_against_64_bits(ops, B, V, cap, n_bias, n_masks, pad):
     show("rules", B, V, cap, n_bias, n_masks, pad)
