@@ -146,6 +146,38 @@ def test_shared_prefixes_in_the_cache(fp16, monkeypatch, rows, shared):
     assert err(again.cpu().numpy(), decode(model, apart, left, tokens[1:]).cpu().numpy()) <= 1e-2
 
 
+def test_shared_prefixes_of_wide_batches_with_adapters():
+    """More than 64 rows, whose o deltas otherwise ride on the attention, in two groups and alone: as without a plan."""
+    print("case wide shared", flush=True)
+    synth = load_pkg("synth")
+    wl = synth.config1()
+    model = load_pkg("llama").LlamaForCausalLM.from_synthetic(6, wl.shape, [synth.LoraSpec(r=16, alpha=8.0, n_adapters=4)], DEV)
+    rng = np.random.default_rng(4)
+    rows, heads = 80, [rng.integers(0, wl.shape.vocab_size, n * 16).astype(np.int32) for n in (130, 20)]
+    who = [(0, 1, None, 0)[i % 4] for i in range(rows)]
+    wids = np.array([-1 if i % 7 == 3 else (2 if who[i] else 1) for i in range(rows)], dtype=np.int32)
+    kv = model.create_paged_kv_cache(rows, 3000 + rows * 100, 2200, 16, max_seq_len=2200)
+    first = {}
+    for i in range(rows):
+        g = who[i]
+        prompt = np.concatenate([heads[g] if g is not None else heads[1][:9], rng.integers(0, wl.shape.vocab_size, 1 + i % 30).astype(np.int32)])
+        kv.add_sequence(i)
+        skip = 0 if g is None or g not in first else kv.share_prefix(i, first[g], len(heads[g]))
+        first.setdefault(g, i)
+        prefill(model, kv, i, prompt, 1, skip)
+    sids, tokens = list(range(rows)), rng.integers(0, wl.shape.vocab_size, rows)
+    def step():
+        kv.begin_forward(sids, [1] * rows)
+        z = model.forward(model.embed(torch.as_tensor(tokens.astype(np.int32))), kv, {0: torch.from_numpy(wids).to(DEV)})
+        plan, kv._cur = kv.plan, None                        # the same step again: its keys and values are written anew
+        return z.cpu().numpy(), plan
+    got, plan = step()
+    assert plan is not None and sorted(len(r) for r, _ in kv.prefix_groups(sids)) == [20, 40]
+    kv._plans[tuple(sids)] = None
+    want, plan = step()
+    assert plan is None and err(got, want) <= 1e-2           # (whole-model bound, as against the oracle)
+
+
 def plain_ids(logits, rules, prompts, answers):
     """The rules evaluated on the host, in the operator's order of roundings."""
     out = []
@@ -345,7 +377,7 @@ def test_four_bit_decode_of_wide_mixed_batches():
     print("case wide mixed", flush=True)
     synth = load_pkg("synth")
     wl = synth.config1()
-    specs = [wl.lora, synth.LoraSpec(r=8, alpha=16.0, n_adapters=3, targets=("q_proj", "o_proj", "gate_proj", "down_proj"))]
+    specs = [synth.LoraSpec(r=16, alpha=8.0, n_adapters=4), synth.LoraSpec(r=8, alpha=16.0, n_adapters=3, targets=("q_proj", "o_proj", "gate_proj", "down_proj"))]
     model = load_pkg("llama").LlamaForCausalLM.from_synthetic(5, wl.shape, specs, DEV, quant_group=32)
     rng = np.random.default_rng(5)
     rows = 70
@@ -375,6 +407,9 @@ def test_four_bit_decode_of_wide_mixed_batches():
         alone, _ = model["decode_no_adapter"](h, kv) if who[i] is None else model[f"decode_a{who[i]}"](h, kv, np.array([i % 3], dtype=np.int32))
         kv.end_forward()
         assert err(wide[i].cpu().numpy(), alone[0].cpu().numpy()) <= 1e-2          # (whole-model bound, as against the oracle)
+    wide = decode(model, kv, list(range(rows)), tokens, np.arange(rows) % 4)       # all of one type
+    for i in range(0, rows, 7):
+        assert err(wide[i].cpu().numpy(), decode(model, kv, [rows + i], tokens[i:i + 1], np.array([i % 4]))[0].cpu().numpy()) <= 1e-2
 
 
 def test_latent_pages_are_shared_too():
