@@ -225,3 +225,47 @@ def test_refusals(ops):
         call(ops, c, out=torch.zeros((2, 100), dtype=torch.float16, device=DEV))
     empty = ops.SharedPrefixPlan([], [], 8, 8, 64, DEV)
     assert ops.paged_attn_decode_shared(c["qkv"][:0], c["k"], c["v"], c["table"], c["rows"][:0], c["ctx"][:0], empty, 8, 8, 64).shape == (0, 512)
+
+
+@pytest.mark.parametrize("Hq,Hkv,groups,lens", [(32, 8, [(list(range(8)), 40)], [640 + 30 * i for i in range(8)]), (8, 8, [([0, 1], 9), ([2, 3, 4], 5)], [150, 160, 80, 99, 200])])
+def test_pages_far_into_a_cache(ops, Hq, Hkv, groups, lens):
+    """Page ids whose elements lie beyond 32 bits give the bits of near ones."""
+    print("case far", Hq, Hkv, flush=True)
+    D = 128
+    c = build(ops, 9, groups, lens, Hq, Hkv, D)
+    want = call(ops, c)
+    n = c["k"].shape[0]
+    base = 2 ** 31 // (Hkv * D * PAGE) + 1000                  # (an element of page `base` has a number of 32 bits)
+    far = {}
+    for name in ("k", "v"):
+        far[name] = torch.empty((base + n, *c[name].shape[1:]), dtype=torch.float16, device=DEV)
+        far[name][0], far[name][base:] = float("nan"), c[name]
+    table = torch.where(c["table"] >= 0, c["table"] + base, -1).to(torch.int32)
+    assert torch.equal(call(ops, {**c, **far, "table": table}), want)
+
+
+def test_plans_out_of_bounds_stay_within_the_call(ops):
+    """A plan's arrays are bounded by the kernels: what they name outside the batch, the pages or the workspace counts for nothing, and other rows keep
+    their results."""
+    print("case damaged plan", flush=True)
+    Hq, Hkv, D = (8, 2, 64)
+    groups, lens = [(list(range(10)), 6), ([11, 12], 3)], [100 + i for i in range(10)] + [30, 60, 70]
+    c = build(ops, 2, groups, lens, Hq, Hkv, D)
+    want = call(ops, c)
+    plan, n = c["plan"], c["plan"].units.numel() // 72
+    keep = plan.data.clone()
+    units = plan.units.view(n, 72)
+    small = [u for u in range(plan.n_block, n)]                # the units of rows 11 and 12
+    for at, value in ((1, 2 ** 20), (1, -5), (2, 2 ** 30), (3, 1000), (3, -1), (8, 10 ** 6), (8, -7), (0, -1)):
+        units[small, at] = value
+        got = call(ops, c)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:11], want[:11])
+        plan.data.copy_(keep)
+    for name, value in (("row_slots", 10 ** 6), ("row_slots", -3), ("row_pages", 2 ** 30), ("row_pages", -1)):
+        getattr(plan, name)[11:] = value
+        got = call(ops, c)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:11], want[:11])
+        plan.data.copy_(keep)
+    assert torch.equal(call(ops, c), want)
