@@ -413,7 +413,7 @@ int mlora_paged_attn_prefill(void* out, int out_layout, const void* qkv, const v
  * that slot of each - first n_block units of at most mlora_shared_attn_unit_rows query rows (rows times Hq / Hkv), then units of at most 16;
  * row_pages [B]: shared pages ahead of a row's own (0: none); row_slots [B]: units over those, which have slots 0, 1, ...  A row is in one
  * group at most.  A row's own pages are cut into own_splits shares, whose results take the slots behind; slots: most slots of a row.  A row's
- * context does not end within its shared pages.  Two launches; workspace of mlora_shared_attn_workspace_bytes, 16-byte aligned. */
+ * context does not end within its shared pages.  What a plan names outside the batch, the block table or the slots counts for nothing.  Two launches; workspace of mlora_shared_attn_workspace_bytes, 16-byte aligned. */
 int mlora_shared_attn_record_ints(void);
 int mlora_shared_attn_unit_rows(void);
 size_t mlora_shared_attn_workspace_bytes(int B, int Hq, int D, int slots);

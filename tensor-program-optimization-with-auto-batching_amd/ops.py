@@ -1044,16 +1044,24 @@ def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_le
     if k_cache.device != dev or v_cache.device != dev or block_table.device != dev or seq_ids.device != dev or ctx_len.device != dev \
             or out is not None and out.device != dev:
         raise ValueError(f"paged_attn_decode_shared: all tensors on {dev}")
+    f16, i32 = torch.float16, torch.int32
+    if not (qkv.dtype is f16 and k_cache.dtype is f16 and v_cache.dtype is f16 and block_table.dtype is i32 and seq_ids.dtype is i32 and ctx_len.dtype is i32
+            and qkv.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous() and seq_ids.is_contiguous()
+            and ctx_len.is_contiguous()):                                  # (says which)
+        for t, dt, name in ((qkv, f16, "qkv"), (k_cache, f16, "k_cache"), (v_cache, f16, "v_cache"), (block_table, i32, "block_table"), (seq_ids, i32, "seq_ids"),
+                            (ctx_len, i32, "ctx_len")):
+            _dev(t, dt, name)
     if out is None and not frag:
-        out = _empty_strided_cuda((B, Hq * D), (Hq * D, 1), torch.float16)
-    out, optr, lay = _out_arg(out, B, Hq * D, frag, dev)
+        out, lay = _empty_strided_cuda((B, Hq * D), (Hq * D, 1), f16), ROWMAJOR
+        optr = out.data_ptr()
+    else:
+        out, optr, lay = _out_arg(out, B, Hq * D, frag, dev)
     if B == 0:
         return out
-    nb, f16, i32 = plan.workspace_bytes, torch.float16, torch.int32
+    nb = plan.workspace_bytes
     ws = _empty_strided_cuda((nb // 4,), (1,), torch.float32)
-    code = lib().mlora_paged_attn_decode_shared(optr, lay, _dev(qkv, f16, "qkv"), _dev(k_cache, f16, "k_cache"), _dev(v_cache, f16, "v_cache"),
-                                                _dev(block_table, i32, "block_table"), max_blocks, _dev(seq_ids, i32, "seq_ids"), _dev(ctx_len, i32, "ctx_len"),
-                                                *plan._args, B, Hq, Hkv, D, n_pages, n_seq, ws.data_ptr(), nb, _stream())
+    code = lib().mlora_paged_attn_decode_shared(optr, lay, qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), max_blocks,
+                                                seq_ids.data_ptr(), ctx_len.data_ptr(), *plan._args, B, Hq, Hkv, D, n_pages, n_seq, ws.data_ptr(), nb, _stream())
     if code:
         check(code)
     return out
