@@ -241,7 +241,9 @@ def lib(dtype: str = "float16") -> C.CDLL:
 
 def loaded() -> C.CDLL:
     """A library for what does not depend on the element type: one that is loaded already, else the fp16 one."""
-    return next(iter(_libs.values()), None) or lib()
+    for l in _libs.values():
+        return l
+    return lib()
 
 
 def check(code: int, dtype: str = "float16") -> None:

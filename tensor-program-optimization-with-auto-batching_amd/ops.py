@@ -873,6 +873,7 @@ class LogitRules:
             self._args.cap = history.shape[1]
             if not history.numel() and self.rows:
                 raise ValueError("LogitRules: a history without room")
+        self._words, self._ref = masks.shape[1] if self._args.n_masks else 0, ctypes.byref(self._args)
 
 
 def constrained_argmax(logits, rules: LogitRules, out=None, ids=None):
@@ -880,28 +881,30 @@ def constrained_argmax(logits, rules: LogitRules, out=None, ids=None):
     fp32 (or None; may be `logits`) takes the logits after penalties, biases and masks."""
     B, V = logits.shape
     dev = _here(logits.device, "constrained_argmax")
-    args = rules._args
     if rules.device is not None and (rules.rows != B and rules.rows is not None or rules.device != dev):
         raise ValueError(f"constrained_argmax: rules of {rules.rows} rows on {rules.device} for {B} on {dev}")
-    if args.n_masks and rules.masks.shape[1] != -(-V // 32):
-        raise ValueError(f"constrained_argmax: masks of {rules.masks.shape[1]} words for {V} tokens")
-    ld, ld_out, p_out = _rows_of(logits, B, V, dev, "logits"), 0, None
+    if rules._words and rules._words != -(-V // 32):
+        raise ValueError(f"constrained_argmax: masks of {rules._words} words for {V} tokens")
+    ld, ld_out, p, p_out = _rows_of(logits, B, V, dev, "logits"), 0, logits.data_ptr(), None
     if out is not None:
         ld_out, p_out = _rows_of(out, B, V, dev, "out"), out.data_ptr()
-        p, apart = logits.data_ptr(), 4 * (B - 1)
-        if (p != p_out or ld != ld_out) and p < p_out + apart * ld_out + 4 * V and p_out < p + apart * ld + 4 * V:
-            raise ValueError("constrained_argmax: out overlaps the logits without being them")
+        if p != p_out or ld != ld_out:
+            apart = 4 * (B - 1)
+            if p < p_out + apart * ld_out + 4 * V and p_out < p + apart * ld + 4 * V:
+                raise ValueError("constrained_argmax: out overlaps the logits without being them")
     if ids is None:
         ids = _empty_strided_cuda((B,), (1,), torch.int32)
+        p_ids = ids.data_ptr()
     elif ids.shape != (B,) or ids.device != dev:
         raise ValueError(f"constrained_argmax: ids{tuple(ids.shape)} on {ids.device} for {B} rows on {dev}")
+    else:
+        p_ids = _dev(ids, torch.int32, "ids")
     if B == 0:
         return ids
     L = _lib.loaded()
     nb = _rules_bytes(B, V)
     ws = _empty_strided_cuda((nb // 8,), (1,), torch.int64) if nb else None
-    code = L.mlora_constrained_argmax(_dev(ids, torch.int32), p_out, ld_out, logits.data_ptr(), ld, ctypes.byref(args), B, V,
-                                      None if ws is None else ws.data_ptr(), nb, _stream())
+    code = L.mlora_constrained_argmax(p_ids, p_out, ld_out, p, ld, rules._ref, B, V, None if ws is None else ws.data_ptr(), nb, _stream())
     if code:
         raise _lib.MloraError(code, L.mlora_last_error().decode())
     return ids
