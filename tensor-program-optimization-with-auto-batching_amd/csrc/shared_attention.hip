@@ -262,8 +262,9 @@ __device__ __forceinline__ void wave_unit(const SharedAttn& a, int u, int kh) {
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
-// R row tiles (2 or 4) times 4 / R shares of the pages.  A stage is two pages, of which a wave fetches the keys or the values of one.
-template <int D, int R>
+// A wave has 16 of the query rows (of up to 32 rows two waves with half of the pages each were no faster: 5 rows of 4 heads behind 16384 tokens 25.0 us, this
+// way 24.6) and fetches the keys or the values of one page of a stage, which is two.
+template <int D>
 __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* __restrict__ d, int kh, f16* ring) {
   constexpr int KP = D / 32, PE = PAGE * D, STAGE = 4 * PE;       // pieces of 1 KiB a wave fetches; elements of a page's keys; of a stage
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
@@ -272,7 +273,7 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
   const int seq = sequence_of(a, d);
   const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
   const f16* src = (wave & 1 ? a.v_cache : a.k_cache) + (size_t)kh * PE + lane * 8;
-  const int tile = wave % R, share = wave / R, r = tile * 16 + col;
+  const int r = wave * 16 + col;
   Tile<D> t;                                                // (ahead of the first pages: loads return in order)
   tile_begin(t, a, r < rows ? d[8 + r / G] : -1, kh * G + (r < rows ? r % G : 0));
   // 64 pages at a time: the wait for ids loaded inside the loop would be one for the whole ring
@@ -303,38 +304,18 @@ __device__ __forceinline__ void block_unit(const SharedAttn& a, const int32_t* _
       const f16* st = ring + rd * STAGE;
       rd = rd + 1 == SA_RING ? 0 : rd + 1;
       wr = wr + 1 == SA_RING ? 0 : wr + 1;
-      if (tile * 16 >= rows) continue;                      // uniform: no row of this wave exists; it takes its part in the loads
+      if (wave * 16 >= rows) continue;                      // uniform: no row of this wave exists; it takes its part in the loads
       const bool one = page_id(a, __builtin_amdgcn_readlane(own, pg - from)) >= 0;
       const bool two = pg + 1 < to && page_id(a, __builtin_amdgcn_readlane(own, pg + 1 - from)) >= 0;
-      const int shift = R == 4 ? 0 : share, pages = R == 4 ? one | two << 1 : share ? two : one;
-      auto kf = [=](int p, int kb) { return ld8(st + (p + shift) * 2 * PE + kb * 512 + lane * 8); };
-      auto vf = [=](int p, int db) { return *reinterpret_cast<const f16x4*>(st + (p + shift) * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); };
-      constexpr int P = R == 4 ? 2 : 1;
-      if (pages == (1 << P) - 1 && (pg + 2) * PAGE <= t.least) tile_step<D, P, false>(t, a.scale, pg + shift, pages, kf, vf);       // uniform
-      else if (pages) tile_step<D, P, true>(t, a.scale, pg + shift, pages, kf, vf);
+      const int pages = one | two << 1;
+      auto kf = [=](int p, int kb) { return ld8(st + p * 2 * PE + kb * 512 + lane * 8); };
+      auto vf = [=](int p, int db) { return *reinterpret_cast<const f16x4*>(st + p * 2 * PE + PE + (db * 16 + col) * PAGE + g * 4); };
+      if (pages == 3 && (pg + 2) * PAGE <= t.least) tile_step<D, 2, false>(t, a.scale, pg, pages, kf, vf);       // uniform
+      else if (pages) tile_step<D, 2, true>(t, a.scale, pg, pages, kf, vf);
     }
     wait_loads<0>();                                        // the requests past the end, too, ahead of the end or of what the ring holds next
   }
   tile_end(t);
-  if constexpr (R == 2) {                                   // the second share's rows join the first's
-    float* o = reinterpret_cast<float*>(ring) + tile * (16 * D);
-    float* ml = reinterpret_cast<float*>(ring) + 2 * 16 * D + tile * 32;
-    bare_barrier();
-    if (share == 1) {
-#pragma unroll
-      for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(o + db * 256 + lane * 4) = t.o[db];
-      if (g == 0) *reinterpret_cast<f32x2*>(ml + col * 2) = f32x2{t.m, t.l};
-    }
-    __syncthreads();
-    if (share == 1) return;
-    const f32x2 other = *reinterpret_cast<const f32x2*>(ml + col * 2);
-    const float m = fmaxf(t.m, other[0]), base = m == -INFINITY ? 0.f : m;
-    const float f0 = __builtin_amdgcn_exp2f(t.m - base), f1 = __builtin_amdgcn_exp2f(other[0] - base);
-    t.l = t.l * f0 + other[1] * f1;
-    t.m = m;
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) t.o[db] = t.o[db] * f0 + *reinterpret_cast<const f32x4*>(o + db * 256 + lane * 4) * f1;
-  }
   tile_store(t, a, slot);
 }
 
@@ -343,9 +324,7 @@ __global__ __launch_bounds__(SA_WAVES * WAVE, 3) void shared_attn_kernel(SharedA
   __shared__ __align__(16) f16 ring[SA_RING * 4 * PAGE * D];
   int i = blockIdx.x;
   if (i < a.n_block * a.Hkv) {
-    const int32_t* __restrict__ d = a.units + (size_t)SA_RECORD * (i / a.Hkv);
-    if (d[0] * (a.Hq / a.Hkv) > 32) block_unit<D, 4>(a, d, i % a.Hkv, ring);      // uniform
-    else block_unit<D, 2>(a, d, i % a.Hkv, ring);
+    block_unit<D>(a, a.units + (size_t)SA_RECORD * (i / a.Hkv), i % a.Hkv, ring);
     return;
   }
   i -= a.n_block * a.Hkv;
@@ -454,7 +433,8 @@ extern "C" int mlora_paged_attn_decode_shared(void* out, int out_layout, const v
                   out_layout == MLORA_FRAG ? mlora_frag_tiles(B) : 0, LOG2E / sqrtf((float)D)};
   hipStream_t s = (hipStream_t)stream;
   const unsigned grid = (unsigned)(n_block * Hkv + ((long)B * own_splits + n_units - n_block) * ceil_div(Hkv, SA_WAVES));
-  const bool many = slots > 8;                              // units of a row: a wave joins up to eight in two rounds
+  const bool many = slots > 8;                              // units of a row: a wave joins up to eight in two rounds (us, a wave / four: 2 and 3 units
+                                                            // 12.3 / 12.8, 8.7 / 8.9; 9 units 8.0 / 7.5, 65 units 32.7 / 25.1)
 #define MLORA_SHARED(DD)                                                                                                                          \
   do {                                                                                                                                            \
     hipLaunchKernelGGL(shared_attn_kernel<DD>, dim3(grid), dim3(SA_WAVES * WAVE), 0, s, a);                                                       \
