@@ -12,7 +12,7 @@
 // Everywhere a wave holds a tile of 16 query rows (the G = Hq / Hkv heads of one or more requests) in the matrix-core layouts of the decode
 // kernel in attention.hip: S^T = K . Q^T, then O^T += V^T . P^T, where a lane's probabilities are already the operand that it must supply
 // - as two fp16 halves, so that they enter with 22 bits - and the keys of two pages fill a k-step.
-//   block units  17 to 64 query rows of a group: four waves share pages that come straight into an LDS ring
+//   block units  up to 64 query rows of a group: four waves share pages that come straight into an LDS ring
 //   wave units   up to 16 query rows - a small group, or the pages of a single request behind its prefix: a wave for itself, the next
 //                page on its way to registers
 #include "lora_device.h"

@@ -999,8 +999,11 @@ class SharedPrefixPlan:
             for r in rows:
                 row_pages[r] = pages
         own = [-(-n // 16) - p for n, p in zip(lens, row_pages)]
-        large = [(rows, pages) for rows, pages in groups if len(rows) * G > 16]
-        small = [(rows, pages) for rows, pages in groups if len(rows) * G <= 16]
+        # more than eight query rows are a block's (us as units of single waves / of blocks: 16 rows of 32 heads over 32 behind 256 pages 27.0 / 24.4, behind 64
+        # 14.9 / 13.4; 4 rows of 32 heads over 8 behind 64 pages 10.6 / 9.6, behind 1024 22.7 / 22.9; 4 of 16 over 16 behind 32 7.5 / 8.1, 2 of 32 over 32
+        # behind 64 10.5 / 11.7)
+        in_block = lambda rows: len(rows) * G > 8
+        large, small = [g for g in groups if in_block(g[0])], [g for g in groups if not in_block(g[0])]
         most = lib().mlora_shared_attn_unit_rows() // G                  # rows of a block unit
         # pages of a unit: block units for two workgroups on each compute unit (16 rows behind 32752 tokens, 32 heads of 128 over 8, for one / two /
         # three: 50 / 46 / 46.5 us, three services of 20 rows behind 4096 tokens 44 / 44 / 49), units of single waves for four (the three
@@ -1011,7 +1014,7 @@ class SharedPrefixPlan:
         self.own_splits = max(1, min(-(-max(own, default=0) // 8), 1024 // max(B * Hkv, 1), 64))
         units = []
         for rows, pages in large + small:
-            block = len(rows) * G > 16
+            block = in_block(rows)
             n = min(-(-pages // (per_block if block else per_wave)), 64)
             cut = [pages * i // n for i in range(n + 1)]
             parts = -(-len(rows) // most) if block else 1

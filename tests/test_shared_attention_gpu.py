@@ -262,6 +262,12 @@ def test_plans_out_of_bounds_stay_within_the_call(ops):
         torch.cuda.synchronize()
         assert torch.equal(got[:11], want[:11])
         plan.data.copy_(keep)
+    for at, value in ((1, 2 ** 20), (1, -5), (2, 2 ** 30), (3, 1000), (3, -1), (8, 10 ** 6), (8, -7), (0, -1), (0, 1000)):       # and of the others
+        units[:plan.n_block, at] = value
+        got = call(ops, c)
+        torch.cuda.synchronize()
+        assert torch.equal(got[10:], want[10:])
+        plan.data.copy_(keep)
     for name, value in (("row_slots", 10 ** 6), ("row_slots", -3), ("row_pages", 2 ** 30), ("row_pages", -1)):
         getattr(plan, name)[11:] = value
         got = call(ops, c)
