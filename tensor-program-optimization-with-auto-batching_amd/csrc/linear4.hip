@@ -92,9 +92,9 @@ __device__ __forceinline__ void l4_store(const Linear4& a, int out, int t, int n
   else l4_store<L4_ACC>(a, t, n, s);
 }
 
-// Up to 16 tokens: a workgroup has NT tiles of rows, its waves take every eighth block of K and their sums meet in LDS, in wave order.
-template <int NT, int GB, int OUT, int DEPTH>      // GB: groups per block; DEPTH: blocks of a wave on their way
-__global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kernel(Linear4 a) {
+// Up to 16 TT tokens: a workgroup has NT tiles of rows, its waves take every eighth block of K and their sums meet in LDS, in wave order.
+template <int TT, int NT, int GB, int DEPTH, bool XFRAG>      // GB: groups per block; DEPTH: blocks of a wave on their way
+__global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 || TT > 1 ? 2 : 4) void linear4_kernel(Linear4 a, int out) {
   __shared__ f32x4 red[L4_WAVES][NT][WAVE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r16 = lane & 15, kg = lane >> 4;
@@ -105,24 +105,30 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
 #pragma unroll
   for (int i = 0; i < NT; ++i) row_block[i] = (size_t)(tile0 + i < tiles ? tile0 + i : tiles - 1) * nb;
   // (rows behind the last token: the last one again, whose results are dropped)
-  const f16* xp = a.x + (a.frag_tt ? (size_t)lane * 8 : (size_t)(r16 < a.T ? r16 : a.T - 1) * a.ldx + kg * 8);
-  const size_t xstep = a.frag_tt ? (size_t)a.frag_tt * 512 : 32;
-  const uint32_t qoff = lane * 16, soff = kg * 8 * GB, zoff = 32 * GB + r16 * GB;
-  f32x4 acc[NT];
+  const bool frag = TT == 1 ? a.frag_tt > 0 : XFRAG;            // (one token tile: the same code for either order)
+  const f16* xp[TT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < TT; ++j)
+    xp[j] = a.x + (frag ? (size_t)lane * 8 : (size_t)(j * 16 + r16 < a.T ? j * 16 + r16 : a.T - 1) * a.ldx + kg * 8);
+  const size_t xstep = frag ? (size_t)a.frag_tt * 512 : 32;
+  const uint32_t qoff = lane * 16, soff = kg * 8 * GB, zoff = 32 * GB + r16 * GB;
+  f32x4 acc[NT][TT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < TT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Stage {
     u32x4 q[NT];
     f16 s[NT][4 * GB];
     uint8_t z[NT][GB];
-    f16x8 x[4];
+    f16x8 x[4][TT];
   };
   auto load = [&](Stage& st, int b, auto WHOLE) {          // (no branch where four k-steps are sure: behind one, a block on its way is waited for)
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const size_t rb = row_block[i] + b;
       const char *m = a.meta + rb * (48 * GB), *q = (const char*)a.q + rb * 1024;
-      if constexpr (GB >= 2 && (NT == 3 || NT * GB >= 16)) m = uniform(m), q = uniform(q);
+      if constexpr (GB >= 2 && (NT == 3 || NT * GB >= 16) || TT > 1 && NT * GB >= 12) m = uniform(m), q = uniform(q);
       st.q[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(q + qoff));
       __builtin_memcpy(st.s[i], __builtin_assume_aligned(m + soff, 8), sizeof(st.s[i]));
       __builtin_memcpy(st.z[i], __builtin_assume_aligned(m + zoff, GB), sizeof(st.z[i]));
@@ -130,7 +136,9 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int ks = b * 4 + k;
-      st.x[k] = decltype(WHOLE)::value || ks < KB ? ld8(xp + (size_t)ks * xstep) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < TT; ++j)
+        st.x[k][j] = decltype(WHOLE)::value || ks < KB ? ld8(xp[XFRAG ? 0 : j] + (size_t)ks * xstep + (XFRAG ? j * 512 : 0)) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
     }
   };
   auto multiply = [&](const Stage& st) {
@@ -140,11 +148,19 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
       for (int g = 0; g < GB; ++g) {
         const f16 z = (f16)(float)st.z[i][g];
         const f16x2 zz = f16x2{(f16)1024.f + z, (f16)1024.f + z}, zs = f16x2{-((f16)64.f + z), -((f16)64.f + z)};
-        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 sum[TT];
 #pragma unroll
-        for (int k = g * (4 / GB); k < (g + 1) * (4 / GB); ++k) sum = mfma_16x16x32(l4_weights(st.q[i][k], nc, zz, zs), st.x[k], sum);
+        for (int j = 0; j < TT; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(sum[e], (float)st.s[i][e * GB + g], acc[i][e]);
+        for (int k = g * (4 / GB); k < (g + 1) * (4 / GB); ++k) {
+          const f16x8 w = l4_weights(st.q[i][k], nc, zz, zs);
+#pragma unroll
+          for (int j = 0; j < TT; ++j) sum[j] = mfma_16x16x32(w, st.x[k][j], sum[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < TT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[j][e], (float)st.s[i][e * GB + g], acc[i][j][e]);
       }
   };
   const int whole = KB / 4, own = (whole - wave + L4_WAVES - 1) / L4_WAVES;      // whole blocks, those of this wave
@@ -175,14 +191,18 @@ __global__ __launch_bounds__(L4_WAVES * WAVE, NT > 3 ? 2 : 4) void linear4_kerne
     multiply(st[0]);
   }
 #pragma unroll
-  for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
-  __syncthreads();
-  for (int o = threadIdx.x; o < NT * WAVE; o += L4_WAVES * WAVE) {
-    const int sl = o % WAVE, n = (tile0 + o / WAVE) * 16 + (sl >> 4) * 4, t = sl & 15;
-    f32x4 s = red[0][o / WAVE][sl];
+  for (int j = 0; j < TT; ++j) {
+    if (j > 0) __syncthreads();
 #pragma unroll
-    for (int w = 1; w < L4_WAVES; ++w) s += red[w][o / WAVE][sl];
-    if (t < a.T && n < a.N) l4_store<OUT>(a, t, n, s);
+    for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i][j];
+    __syncthreads();
+    for (int o = threadIdx.x; o < NT * WAVE; o += L4_WAVES * WAVE) {
+      const int sl = o % WAVE, n = (tile0 + o / WAVE) * 16 + (sl >> 4) * 4, t = j * 16 + (sl & 15);
+      f32x4 s = red[0][o / WAVE][sl];
+#pragma unroll
+      for (int w = 1; w < L4_WAVES; ++w) s += red[w][o / WAVE][sl];
+      if (t < a.T && n < a.N) l4_store(a, out, t, n, s);
+    }
   }
 }
 
@@ -421,20 +441,25 @@ __global__ __launch_bounds__(256) void linear4_join_kernel(Linear4 a, int out, c
 // a second workgroup on the compute unit (16 tokens, 12288 x 4096: 8.9 to 14.8 us).
 constexpr int depth_of(int NT) { return NT == 1 ? 2 : 1; }
 
-template <int NT, int GB>
-void launch(const Linear4& a, int out, hipStream_t s) {
+template <int TT, int NT, int GB>
+int launch(const Linear4& a, int out, hipStream_t s) {
   const dim3 grid(ceil_div(ceil_div(a.N, 16), NT)), block(L4_WAVES * WAVE);
-  if (out == L4_F16) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F16, depth_of(NT)>), grid, block, 0, s, a);
-  else if (out == L4_F32) hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_F32, depth_of(NT)>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((linear4_kernel<NT, GB, L4_ACC, depth_of(NT)>), grid, block, 0, s, a);
+  if (TT > 1 && a.frag_tt) hipLaunchKernelGGL((linear4_kernel<TT, NT, GB, depth_of(NT), (TT > 1)>), grid, block, 0, s, a, out);
+  else hipLaunchKernelGGL((linear4_kernel<TT, NT, GB, depth_of(NT), false>), grid, block, 0, s, a, out);
+  return mlora_launch_status("linear4");
 }
 
-// How a product of more than 16 tokens is cut: row tiles of a wave, and slices of K (0 slices: the kernel for 16 tokens).
+// How a product of more tokens is cut: row tiles of a wave, and slices of K (0 slices: the kernel for few tokens).
 struct MidCut {
   int tiles, slices;
 };
 
 int mid_tt(int T) { return T <= 32 ? 2 : 4; }
+
+// Whether the kernel for few tokens takes a product: up to 16 tokens, and up to 32 where K is short and a compute unit has at most six tiles of rows.  us with 32
+// tokens in fragment order (in rows), that kernel / two groups of waves, N x K: 4096 x 4096 7.5 / 10.3 (11.5 / 10.2), 12288 x 4096 10.1 / 13.5 (13.0 / 13.4),
+// 22016 x 4096 15.0 / 18.5 (16.3 / 18.4), 3000 x 1024 4.4 / 5.9 (6.2 / 5.9); 32003 x 4096 22.3 / 21.0 (27.5 / 21.8), 4096 x 11008 15.4 / 14.2 (25.1 / 14.6).
+bool few_tokens(int T, int K, int N) { return T <= 16 || (T <= 32 && K <= 6144 && N <= 6 * 256 * 16); }
 
 // The cut of the least estimated time: rounds of the 256 compute units, which hold one workgroup each, times 3 us and what a step costs - a block
 // for either group, (1 + tiles) / 2 us for 64 tokens and a third less for 32 -, and for more than one slice the partial sums' write and read
@@ -444,7 +469,7 @@ int mid_tt(int T) { return T <= 32 ? 2 : 4; }
 //   64 tokens, 12288 x 4096    [18.6]  26.1  32.7  24.8  26.0  25.5      32 tokens, 4096 x 11008     29.6  43.5  56.8  19.5  [14.2]  17.7
 //   128 tokens, 16384 x 4096    36.2  [28.5]  34.4  46.8  60.2  51.4      64 tokens, 4096 x 11008     39.2  59.0  75.8  25.1  [17.4]  22.6
 MidCut mid_cut(int T, int K, int N) {
-  if (T <= 16) return {0, 0};
+  if (few_tokens(T, K, N)) return {0, 0};
   const int nb = ceil_div(K, L4_BLOCK), tt = mid_tt(T);
   MidCut best = {1, 1};
   double least = 0;
@@ -499,22 +524,23 @@ int row_tiles(int tiles) {
   return best;
 }
 
+template <int TT, int GB>
+int launch_rows(const Linear4& a, int out, hipStream_t s) {
+  switch (row_tiles(ceil_div(a.N, 16))) {
+    case 1: return launch<TT, 1, GB>(a, out, s);
+    case 2: return launch<TT, 2, GB>(a, out, s);
+    case 3: return launch<TT, 3, GB>(a, out, s);
+    case 4: return launch<TT, 4, GB>(a, out, s);
+    case 6: return launch<TT, 6, GB>(a, out, s);
+    default: return launch<TT, (TT > 1 ? 4 : 8), GB>(a, out, s);
+  }
+}
+
 template <int GB>
 int launch_shape(const Linear4& a, int out, MidCut cut, float* part, hipStream_t s) {
-  const int tiles = ceil_div(a.N, 16);
-  if (cut.slices > 0) {
-    if (a.T <= 32) return a.frag_tt ? launch_mid<2, GB, true>(a, out, cut, part, s) : launch_mid<2, GB, false>(a, out, cut, part, s);
-    return a.frag_tt ? launch_mid<4, GB, true>(a, out, cut, part, s) : launch_mid<4, GB, false>(a, out, cut, part, s);
-  }
-  switch (row_tiles(tiles)) {
-    case 1: launch<1, GB>(a, out, s); break;
-    case 2: launch<2, GB>(a, out, s); break;
-    case 3: launch<3, GB>(a, out, s); break;
-    case 4: launch<4, GB>(a, out, s); break;
-    case 6: launch<6, GB>(a, out, s); break;
-    default: launch<8, GB>(a, out, s);
-  }
-  return mlora_launch_status("linear4");
+  if (cut.slices == 0) return a.T <= 16 ? launch_rows<1, GB>(a, out, s) : launch_rows<2, GB>(a, out, s);
+  if (a.T <= 32) return a.frag_tt ? launch_mid<2, GB, true>(a, out, cut, part, s) : launch_mid<2, GB, false>(a, out, cut, part, s);
+  return a.frag_tt ? launch_mid<4, GB, true>(a, out, cut, part, s) : launch_mid<4, GB, false>(a, out, cut, part, s);
 }
 
 }  // namespace
