@@ -67,7 +67,7 @@ def test_linear4_against_64_bits(ops, T, K, N, group):
 # waves, token blocks of 32 and 64 that are not full; and of the other one tiles of every count, waves with and without the end of K
 CUTS = [(200, 160, 12200, 32), (193, 192, 12250, 64), (250, 256, 12288, 128), (100, 160, 16300, 32), (20, 1056, 12300, 32), (64, 2080, 300, 32), (48, 4160, 70, 64),
         (25, 2048, 700, 128), (17, 128, 40000, 128), (16, 1056, 4100, 32), (9, 288, 8200, 32), (5, 320, 12290, 64), (16, 192, 16400, 64), (3, 96, 24600, 32), (2, 128, 33000, 128),
-        (1, 2016, 50, 32), (8, 1152, 33000, 64), (30, 160, 8200, 64), (18, 288, 16400, 32), (32, 96, 22100, 32), (27, 128, 24576, 64), (19, 6144, 40, 128), (17, 6176, 33, 32)]
+        (1, 2016, 50, 32), (8, 1152, 33000, 64), (30, 192, 8200, 64), (18, 288, 16400, 32), (32, 96, 22100, 32), (27, 128, 24576, 64), (19, 6144, 40, 128), (17, 6176, 33, 32)]
 
 
 @pytest.mark.parametrize("T,K,N,group", CUTS)
