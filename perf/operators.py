@@ -7,7 +7,6 @@ cannot do without and `exact` the operator's definition in 64 bits.
 """
 from __future__ import annotations
 
-import functools
 import importlib
 import math
 import zlib
@@ -24,7 +23,6 @@ own = False
 HEADS = {"16x64": (16, 16, 64), "32x128": (32, 32, 128), "32/8x128": (32, 8, 128)}
 
 
-@functools.lru_cache(maxsize=None)                    # (a program imports them once, not with every call)
 def _ops():
     return importlib.import_module(f"{PACKAGE}.ops")
 
