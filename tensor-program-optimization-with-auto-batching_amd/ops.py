@@ -1028,12 +1028,23 @@ class SharedPrefixPlan:
         size = lib().mlora_shared_attn_record_ints()
         records = [x for _, less, rows, lo, j in units for x in (len(rows), lo, -less, j, 0, 0, 0, 0, *rows, *([rows[0]] * (size - 8 - len(rows))))]
         self.data = upload(torch.tensor(records + row_pages + row_slots, dtype=torch.int32), device)
-        n = len(records)
-        self.units, self.row_pages, self.row_slots = self.data[:n], self.data[n:n + B], self.data[n + B:]
         self.workspace_bytes = lib().mlora_shared_attn_workspace_bytes(B, Hq, D, self.slots)
-        # what the C call takes of a plan, whose arrays live as long as it does
         self._heads, self._page = (Hq, Hkv, D), ((Hkv, D // 32, 4, 16, 8), (Hkv, D, 16))
+        self._bind()
+
+    def _bind(self):
+        """The plan's arrays as parts of `data`, and what the C call takes of them: addresses that hold while the plan lives."""
+        n = self.data.numel() - 2 * self.B
+        self.units, self.row_pages, self.row_slots = self.data[:n], self.data[n:n + self.B], self.data[n + self.B:]
         self._args = (self.units.data_ptr(), self.n_block, self.n_units, self.row_pages.data_ptr(), self.row_slots.data_ptr(), self.own_splits, self.slots)
+
+    def __getstate__(self):
+        return {n: v for n, v in self.__dict__.items() if n not in ("units", "row_pages", "row_slots", "_args")}
+
+    def __setstate__(self, state):
+        """A copy has arrays of its own, and their addresses."""
+        self.__dict__.update(state)
+        self._bind()
 
 
 def paged_attn_decode_shared(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, plan: SharedPrefixPlan, Hq, Hkv, D, out=None, frag=False):

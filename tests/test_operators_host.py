@@ -161,3 +161,36 @@ def test_grammar_masks_and_rules_on_the_host():
     r = tr.TokenRules(bias={3: 1.0})
     si.set_rules(0, r)
     assert si.get_rules(0) is r
+
+
+def _on_shared_pages(rows=3, pages=130, own=5):
+    """A cache on the CPU whose sequences share enough pages for a plan, and its batch."""
+    kvc = load_pkg("kv_cache")
+    kv = kvc.PagedKVCache(1, pages + 2 * rows, 2, 64, max_seqs=rows, max_blocks=pages + 4, rope_theta=1e4, max_pos=16 * (pages + 4), device="cpu", n_q_heads=4)
+    for sid in range(rows):
+        kv.add_sequence(sid)
+        skip = kv.share_prefix(sid, 0) if sid else 0
+        kv.begin_forward([sid], [16 * pages + (own if sid else 0) - skip])
+        kv.end_forward()
+    return kv, tuple(range(rows))
+
+
+def test_copies_of_a_cache_with_a_plan_have_its_arrays_for_themselves():
+    """What a copied or unpickled cache hands to the kernels lies in its own arrays and holds the same plan."""
+    import copy
+    import pickle
+    import torch
+    kv, batch = _on_shared_pages()
+    kv.begin_forward(batch, [1] * len(batch))
+    kv.end_forward()
+    plan = kv.shared_plan(batch)
+    assert plan is not None and kv.plan is plan
+    for make in (copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))):
+        other = make(kv)
+        mine = other.shared_plan(batch)
+        assert mine is not plan and other.plan is mine and torch.equal(mine.data, plan.data) and mine.data.data_ptr() != plan.data.data_ptr()
+        for name in ("units", "row_pages", "row_slots"):
+            a, b = getattr(mine, name), getattr(plan, name)
+            assert torch.equal(a, b) and a.untyped_storage().data_ptr() == mine.data.untyped_storage().data_ptr()
+        assert mine._args == (mine.units.data_ptr(), plan.n_block, plan.n_units, mine.row_pages.data_ptr(), mine.row_slots.data_ptr(), plan.own_splits, plan.slots)
+        assert not {mine._args[i] for i in (0, 3, 4)} & {plan._args[i] for i in (0, 3, 4)}
