@@ -106,26 +106,67 @@ class PageTable:
         return n * PAGE
 
     def prefix_groups(self, seq_ids):
-        """(positions in seq_ids, pages): which of the sequences begin with the same pages, cut so that the pages saved are most."""
+        """(positions in seq_ids, pages): which of the sequences begin with the same pages, cut so that the pages saved are most; of equal
+        cuts one with fewer groups.
+
+        The sequences' whole pages make a tree, whose nodes are what several of them begin with.  A group is a node, and every sequence
+        goes with the deepest one that it passes: saved are the depths of the sequences' groups, less every group's own.  So from the leaves up,
+        for each ancestor that may be the deepest group above a node: the most that its sequences save, with a group of their own at the node
+        or without."""
         rows = [self.slot[s] for s in seq_ids]
         full = [self.lens[s] // PAGE for s in seq_ids]
-
-        def cut(members, depth):
-            """members share `depth` pages -> (pages saved, groups)"""
-            first, most = rows[members[0]], min(full[i] for i in members)
-            while depth < most and all(self.table_h[rows[i], depth] == self.table_h[first, depth] for i in members):
-                depth += 1
-            here = ((len(members) - 1) * depth, [(members, depth)] if depth else [])
-            parts = {}
-            for i in members:
-                if full[i] > depth:
-                    parts.setdefault(int(self.table_h[rows[i], depth]), []).append(i)
-            below = [cut(p, depth) for p in parts.values() if 1 < len(p) < len(members)]
-            apart = (sum(s for s, _ in below), [g for _, gs in below for g in gs])
-            return apart if apart[0] > here[0] else here
-
         owned = [i for i, r in enumerate(rows) if full[i] and int(self.table_h[r, 0]) in self._owners]
-        return cut(owned, 0)[1] if len(owned) > 1 else []
+        if len(owned) < 2:
+            return []
+        paths = {i: self.table_h[rows[i], :full[i]] for i in owned}
+        # the tree from the sequences in the order of their pages, where neighbours share most
+        depth, up, ends, below = [0], [0], [[]], [[]]         # of a node: its pages, parent, sequences that end there, children (node 0: no page)
+
+        def node(d, parent):
+            depth.append(d), up.append(parent), ends.append([]), below.append([])
+            below[parent].append(len(depth) - 1)
+            return len(depth) - 1
+
+        last, at = None, 0
+        for i in sorted(owned, key=lambda i: paths[i].tobytes()):
+            n = 0
+            if last is not None:
+                n = min(full[last], full[i])
+                differ = np.flatnonzero(paths[last][:n] != paths[i][:n])
+                n = int(differ[0]) if differ.size else n
+            under = None
+            while depth[at] > n:
+                under, at = at, up[at]
+            if depth[at] < n:                                  # what the two share ends between two nodes
+                mid = node(n, at)
+                below[at].remove(under)
+                below[mid].append(under)
+                up[under], at = mid, mid
+            if full[i] > n:
+                at = node(full[i], at)
+            ends[at].append(i)
+            last = i
+        order = [0]                                            # parents ahead of their children
+        for v in order:
+            order.extend(below[v])
+        above = {0: np.zeros(1, np.int64)}                     # depths of the ancestors that may be the group above (node 0: none)
+        for v in order:
+            if below[v]:
+                above.update(dict.fromkeys(below[v], above[0] if v == 0 else np.append(above[v], depth[v])))
+        without, own, best = {}, {}, {}
+        for v in reversed(order[1:]):
+            without[v] = len(ends[v]) * above[v] + sum(best[c][:-1] for c in below[v])
+            own[v] = (len(ends[v]) - 1) * depth[v] + sum(int(best[c][-1]) for c in below[v])
+            best[v] = np.maximum(without[v], own[v])
+        groups, group, which = [], {0: None}, {0: 0}           # of a node: the group that its sequences go with, its place among the ancestors
+        for v in order[1:]:
+            group[v], which[v] = group[up[v]], which[up[v]]
+            if own[v] > without[v][which[v]]:
+                group[v], which[v] = ([], depth[v]), len(above[v])
+                groups.append(group[v])
+            if group[v] is not None:
+                group[v][0].extend(ends[v])
+        return sorted((sorted(members), pages) for members, pages in groups)
 
     def begin_forward(self, seq_ids, append_lens, device_meta=None):
         """Reserve pages for the appended tokens and stage the per-token (sequence, position) arrays."""

@@ -194,3 +194,79 @@ def test_copies_of_a_cache_with_a_plan_have_its_arrays_for_themselves():
             assert torch.equal(a, b) and a.untyped_storage().data_ptr() == mine.data.untyped_storage().data_ptr()
         assert mine._args == (mine.units.data_ptr(), plan.n_block, plan.n_units, mine.row_pages.data_ptr(), mine.row_slots.data_ptr(), plan.own_splits, plan.slots)
         assert not {mine._args[i] for i in (0, 3, 4)} & {plan._args[i] for i in (0, 3, 4)}
+
+
+def _tree_of_prefixes(seqs):
+    """A cache whose sequences begin like one another: seqs are (of, pages taken over, own pages) in order."""
+    kvc = load_pkg("kv_cache")
+    most = 1 + max(taken + own for _, taken, own in seqs)
+    kv = kvc.PagedKVCache(1, 1 + sum(own + 1 for _, _, own in seqs), 1, 32, max_seqs=len(seqs), max_blocks=most, rope_theta=1e4, max_pos=16 * most, device="cpu")
+    for sid, (of, taken, own) in enumerate(seqs):
+        kv.add_sequence(sid)
+        if of is not None and taken:
+            kv.share_prefix(sid, of, 16 * taken)
+        kv.begin_forward([sid], [16 * own])
+        kv.end_forward()
+    return kv
+
+
+def _pages_saved(kv, seq_ids, groups):
+    """Of groups that are sound: a sequence in one at most, each of several with the same pages."""
+    rows = [r for members, _ in groups for r in members]
+    assert len(rows) == len(set(rows))
+    for members, pages in groups:
+        heads = {tuple(kv.pages_of(seq_ids[r])[:pages]) for r in members}
+        assert len(members) > 1 and pages > 0 and len(heads) == 1 and all(kv.lens[seq_ids[r]] >= 16 * pages for r in members)
+    return sum((len(members) - 1) * pages for members, pages in groups)
+
+
+def test_prefix_groups_keep_those_outside_a_deeper_group():
+    """Eleven sequences share ten pages, two of them 160: the two are one group, the nine others another."""
+    kv = _tree_of_prefixes([(None, 0, 10), (0, 10, 150), (1, 160, 1)] + [(0, 10, 1)] * 8)
+    ids = [0, 2, 3, 4, 5, 6, 7, 8, 9, 10, 1]
+    assert sorted(kv.prefix_groups(ids)) == [([0, 2, 3, 4, 5, 6, 7, 8, 9], 10), ([1, 10], 160)]
+
+
+def test_prefix_groups_against_every_choice():
+    """Small trees of prefixes: the most that any choice of a depth for every sequence saves."""
+    import itertools
+    import random
+    for seed in range(60):
+        rng = random.Random(seed)
+        seqs = [(None, 0, rng.randint(1, 4))]
+        for sid in range(1, rng.randint(2, 6)):
+            of = rng.randrange(sid)
+            has = seqs[of][1] + seqs[of][2]
+            seqs.append((of, rng.randint(0, has), rng.randint(0, max(0, 4 - has) + 1)))
+        seqs = [(of, taken, own if taken + own else 1) for of, taken, own in seqs]
+        kv = _tree_of_prefixes(seqs)
+        ids = list(range(len(seqs)))
+        rng.shuffle(ids)
+        pages = [kv.pages_of(s) for s in ids]
+        most = 0
+        for depths in itertools.product(*(range(min(len(p), 5) + 1) for p in pages)):
+            groups = {}
+            for r, d in enumerate(depths):
+                groups.setdefault(tuple(pages[r][:d]), []).append(r)
+            most = max(most, sum((len(m) - 1) * len(head) for head, m in groups.items()))
+        assert max(map(len, pages)) <= 9 and _pages_saved(kv, ids, kv.prefix_groups(ids)) == max(most, 0)
+
+
+def test_prefix_groups_of_a_long_chain():
+    """Every sequence begins with all of the one before."""
+    kv = _tree_of_prefixes([(None, 0, 1)] + [(i, i + 1, 1) for i in range(1299)])
+    ids = list(range(1300))
+    saved = _pages_saved(kv, ids, kv.prefix_groups(ids))
+    # groups at depths d1 < d2 < .. of a chain: sum over them of d (number of sequences up to the next - 1); one at half the chain saves 650 x 650
+    assert saved >= 650 * 650
+    assert saved == _chain_most(1300)
+
+
+def _chain_most(n):
+    """The most that a chain saves: by a recursion over the deepest group, of sequences d - 1 .. e - 1 at depth d."""
+    import numpy as np
+    most = np.zeros(n + 1, np.int64)                          # of the sequences 0 .. e - 1
+    for e in range(1, n + 1):
+        d = np.arange(1, e + 1)
+        most[e] = max(most[e - 1], int((most[d - 1] + (e - d) * d).max()))
+    return int(most[n])
