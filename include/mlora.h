@@ -326,10 +326,11 @@ int mlora_embed(void* out, int out_dtype, const void* table, const int32_t* ids,
  * products over the exact integers, sums and scales in fp32.  group: 32, 64 or 128, K a multiple of it.  x [T, K] f16 in rows
  * of ldx or in fragment order, any T; y [T, N] f16 or f32; mode as for mlora_linear.  q and meta (scales and zeros) in the
  * layouts at the top of linear4.hip, with the sizes that mlora_linear4_sizes gives (outputs may be NULL); x, q, meta and workspace
- * 16-byte aligned.
+ * 16-byte aligned.  The workspace's size is that of x's layout, or that of either.
  * No counterpart in the reference, whose linears are fp16. */
 int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, size_t* meta_bytes);
 size_t mlora_linear4_workspace_bytes(int T, int K, int N);
+size_t mlora_linear4_workspace_bytes_of(int T, int K, int N, int x_layout);
 int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* meta, int group,
                   int T, int K, int N, void* workspace, size_t workspace_bytes, void* stream);
 

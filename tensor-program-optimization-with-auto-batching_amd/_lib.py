@@ -86,6 +86,7 @@ SIGNATURES = {
     "mlora_silu_mul": (_i, [_p, _i, _p, _p, _i, _i, _i, _p]),
     "mlora_linear4_sizes": (_i, [_i, _i, _i, _p, _p]),
     "mlora_linear4_workspace_bytes": (_z, [_i, _i, _i]),
+    "mlora_linear4_workspace_bytes_of": (_z, [_i, _i, _i, _i]),
     "mlora_linear4": (_i, [_p, _i, _i, _p, _i, _i, _p, _p, _i, _i, _i, _i, _p, _z, _p]),
     "mlora_embed": (_i, [_p, _i, _p, _p, _i, _i, _i, _p]),
     "mlora_argmax": (_i, [_p, _p, _i, _i, _p]),

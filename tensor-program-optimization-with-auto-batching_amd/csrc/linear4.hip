@@ -456,10 +456,23 @@ struct MidCut {
 
 int mid_tt(int T) { return T <= 32 ? 2 : 4; }
 
-// Whether the kernel for few tokens takes a product: up to 16 tokens, and up to 32 where K is short and a compute unit has at most six tiles of rows.  us with 32
-// tokens in fragment order (in rows), that kernel / two groups of waves, N x K: 4096 x 4096 7.5 / 10.3 (11.5 / 10.2), 12288 x 4096 10.1 / 13.5 (13.0 / 13.4),
-// 22016 x 4096 15.0 / 18.5 (16.3 / 18.4), 3000 x 1024 4.4 / 5.9 (6.2 / 5.9); 32003 x 4096 22.3 / 21.0 (27.5 / 21.8), 4096 x 11008 15.4 / 14.2 (25.1 / 14.6).
-bool few_tokens(int T, int K, int N) { return T <= 16 || (T <= 32 && K <= 6144 && N <= 6 * 256 * 16); }
+// Whether the kernel for few tokens takes a product: up to 16 tokens; up to 32, where K is short and a compute unit has at most six tiles of rows, always with
+// x in fragment order, of which a wave's load touches eight lines.  In rows it touches one a token, which costs the more the more tokens and the
+// longer K, and is hidden the better the more rows of the weight a compute unit has.  us with 32 tokens in fragment order (17; 24; 32 in rows), that kernel / two groups
+// of waves, N x K, groups of 64 and 128:
+//   1024 x 1024   4.2 / 5.5 ( 4.7 /  5.5;  5.3 /  5.8;  6.3 /  5.6)     1024 x 2048  4.6 / 7.4 (5.1 /  7.6;  5.9 / 7.6;  6.5 /  7.6)
+//   1024 x 4096   7.0 / 8.2 ( 7.7 /  8.3;  9.3 /  8.4; 10.2 /  8.3)     4096 x 4096  7.3 / 10.3 (7.9 / 10.4;  9.3 / 10.4; 10.5 / 10.3)
+//   8192 x 4096   8.4 / 12.0 (8.7 / 13.8; 10.1 / 13.8; 11.5 / 12.0)    24576 x 4096 16.4 / 20.5 (15.0 / 20.0; 17.8 / 21.3; 17.5 / 20.8)
+//   1024 x 6144   9.1 / 8.8 (10.2 /  9.0; 12.7 /  9.0; 15.0 /  9.0)     8192 x 6144 11.7 / 14.6 (12.2 / 15.3; 14.0 / 15.1; 16.0 / 14.9)
+// and beyond, in fragment order: 32003 x 4096 22.3 / 21.0, 4096 x 11008 15.4 / 14.2.  In rows the rule took the side that was slower by 3 to 5 % in six of 188
+// such products, by more in none.
+bool few_tokens(int T, int K, int N, bool frag) {
+  if (T <= 16) return true;
+  if (T > 32 || K > 6144 || N > 6 * 256 * 16) return false;
+  if (frag) return true;
+  if (K <= 2048) return T <= 24 || N > 4096 || K <= 512 || K > 1024;
+  return K <= 4096 ? (T - 16) * K <= 12 * N : N >= 4096 && (T - 16) * K <= 6 * N;
+}
 
 // The cut of the least estimated time: rounds of the 256 compute units, which hold one workgroup each, times 3 us and what a step costs - a block
 // for either group, (1 + tiles) / 2 us for 64 tokens and a third less for 32 -, and for more than one slice the partial sums' write and read
@@ -468,8 +481,8 @@ bool few_tokens(int T, int K, int N) { return T <= 16 || (T <= 32 && K <= 6144 &
 //   64 tokens, 4096 x 4096      17.7  25.3  31.8  14.3  [12.9]  15.2      200 tokens, 12288 x 4096    52.5  50.6  [36.6]  66.0  82.6  66.2
 //   64 tokens, 12288 x 4096    [18.6]  26.1  32.7  24.8  26.0  25.5      32 tokens, 4096 x 11008     29.6  43.5  56.8  19.5  [14.2]  17.7
 //   128 tokens, 16384 x 4096    36.2  [28.5]  34.4  46.8  60.2  51.4      64 tokens, 4096 x 11008     39.2  59.0  75.8  25.1  [17.4]  22.6
-MidCut mid_cut(int T, int K, int N) {
-  if (few_tokens(T, K, N)) return {0, 0};
+MidCut mid_cut(int T, int K, int N, bool frag) {
+  if (few_tokens(T, K, N, frag)) return {0, 0};
   const int nb = ceil_div(K, L4_BLOCK), tt = mid_tt(T);
   MidCut best = {1, 1};
   double least = 0;
@@ -556,8 +569,13 @@ extern "C" int mlora_linear4_sizes(int N, int K, int group, size_t* q_bytes, siz
 
 static size_t partial_bytes(int slices, int T, int N) { return slices > 1 ? (size_t)slices * ceil_div(T, 16) * ceil_div(N, 16) * 256 * sizeof(float) : 0; }
 
+extern "C" size_t mlora_linear4_workspace_bytes_of(int T, int K, int N, int x_layout) {
+  return T > 0 && K > 0 && N > 0 ? partial_bytes(mid_cut(T, K, N, x_layout == MLORA_FRAG).slices, T, N) : 0;
+}
+
 extern "C" size_t mlora_linear4_workspace_bytes(int T, int K, int N) {
-  return T > 0 && K > 0 && N > 0 ? partial_bytes(mid_cut(T, K, N).slices, T, N) : 0;
+  const size_t rows = mlora_linear4_workspace_bytes_of(T, K, N, MLORA_ROWMAJOR), frag = mlora_linear4_workspace_bytes_of(T, K, N, MLORA_FRAG);
+  return rows > frag ? rows : frag;
 }
 
 extern "C" int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int x_layout, int ldx, const void* q, const void* meta, int group,
@@ -575,7 +593,7 @@ extern "C" int mlora_linear4(void* y, int y_dtype, int mode, const void* x, int 
   Linear4 a = {y, (const f16*)x, (const uint32_t*)q, (const char*)meta, ldx, x_layout == MLORA_FRAG ? mlora_frag_tiles(T) : 0, T, K, N, N % 4 == 0 && ((uintptr_t)y & 15) == 0};
   const int out = mode == MLORA_ACCUMULATE ? L4_ACC : y_dtype == MLORA_F32 ? L4_F32 : L4_F16;
   hipStream_t s = (hipStream_t)stream;
-  const MidCut cut = mid_cut(T, K, N);
+  const MidCut cut = mid_cut(T, K, N, a.frag_tt > 0);
   const size_t need = partial_bytes(cut.slices, T, N);
   MLORA_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), MLORA_ERR_WORKSPACE,
               "linear4: workspace of %zu bytes, %zu needed", workspace_bytes, need);

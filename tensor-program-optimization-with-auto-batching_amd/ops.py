@@ -476,7 +476,7 @@ def _linear4(x, W, out, out_dtype, accumulate):
         if inner != 1 or ldx < K or ldx % 8 or xp % 16:
             x = x.clone(memory_format=torch.contiguous_format)            # rows on 16 bytes
             xp, ldx = x.data_ptr(), K
-    nb = _size(torch.float16, "mlora_linear4_workspace_bytes", T, K, N)
+    nb = _size(torch.float16, "mlora_linear4_workspace_bytes_of", T, K, N, lay)
     ws = _empty_strided_cuda((nb // 4,), (1,), torch.float32) if nb else None
     code = lib().mlora_linear4(_dev(out, name="out"), F16 if out_dtype is torch.float16 else F32, ACCUMULATE if accumulate else STORE, xp, lay, ldx, W.q.data_ptr(),
                                W.meta.data_ptr(), W.group, T, K, N, None if ws is None else ws.data_ptr(), nb, _stream())

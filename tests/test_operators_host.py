@@ -270,3 +270,19 @@ def _chain_most(n):
         d = np.arange(1, e + 1)
         most[e] = max(most[e - 1], int((most[d - 1] + (e - d) * d).max()))
     return int(most[n])
+
+
+def test_linear4_cuts_by_the_order_of_x():
+    """17 to 32 tokens in rows: which kernel takes a product, told by its partial sums; either order finds room in the general size."""
+    lib = load_pkg("_lib").lib()
+    of, either = lib.mlora_linear4_workspace_bytes_of, lib.mlora_linear4_workspace_bytes
+    for T, K, N, slices in ((32, 4096, 4096, True), (24, 4096, 1024, True), (20, 6144, 3000, True), (17, 6144, 1024, True),       # two groups of waves, in slices
+                            (28, 4096, 4096, False), (17, 4096, 1024, False), (32, 4096, 8192, False), (32, 2048, 1024, False), (24, 6144, 8192, False)):
+        rows, frag = of(T, K, N, 0), of(T, K, N, 1)
+        assert (rows > 0) == slices and frag == 0 and either(T, K, N) == rows, (T, K, N)
+    for T, K, N in ((64, 4096, 4096), (33, 11008, 4096), (16, 4096, 4096), (30, 11008, 4096)):
+        assert of(T, K, N, 0) == of(T, K, N, 1) == either(T, K, N)
+    need = of(32, 4096, 4096, 0)
+    def call(lay, ws, nb, T=32, K=4096, N=4096):
+        return lib.mlora_linear4(16, 0, 0, 16, lay, K, 16, 16, 128, T, K, N, ws, nb, None)
+    assert call(0, None, 0) == -3 and call(0, 16, need - 1) == -3
