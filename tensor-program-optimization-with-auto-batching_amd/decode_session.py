@@ -17,8 +17,8 @@ from .llama import share_of
 class DecodeSession:
     """Fixed-batch greedy decode through the per-operator path (any mix of adapter types and ranks).  With
     use_graph the launch sequence of a step is captured once - after one eager step, which also sizes the model's
-    scratch buffers outside the graph's memory pool - and replayed, so the interpreter is out of the loop; the
-    kernels and their order are those of the eager step, hence the same tokens bit for bit."""
+    scratch buffers outside the graph's memory pool, and again when the cache's plan over shared prefixes changes - and replayed,
+    so the interpreter is out of the loop; the kernels and their order are those of the eager step, hence the same tokens bit for bit."""
 
     def __init__(self, model, kv, seq_ids, tok_adapter, first_tokens, use_graph=False, longest_first=False, rules=None):
         """seq_ids: sequences already prefilled in `kv`; tok_adapter: {tid: ids [B] int32 (host or device), -1 = the
@@ -52,7 +52,7 @@ class DecodeSession:
         self.pos = i32([kv.lens[s] for s in self.seq_ids])
         self.ctx = self.pos + 1
         self.use_graph = use_graph
-        self.graph = None
+        self.graph = self._plan = None
         self._eager_steps = 0
         self.history = []
 
@@ -73,12 +73,12 @@ class DecodeSession:
             self.rules.take()
         kv.begin_forward(self.seq_ids, [1] * len(self.seq_ids), device_meta=(self.rows, self.pos, self.ctx))
         if self.use_graph and self._eager_steps >= 1:
-            if self.graph is None:
+            plan = getattr(kv, "plan", None)
+            if self.graph is None or plan is not self._plan:     # (a plan that its rows have outgrown is replaced)
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g):         # records, does not run
+                with torch.cuda.graph(g):         # behind a wait for the device; records, does not run
                     self._enqueue()
-                self.graph = g
-                self._plan = getattr(kv, "plan", None)       # what the recorded launches read
+                self.graph, self._plan = g, plan  # what the recorded launches read
             self.graph.replay()
         else:
             self._enqueue()

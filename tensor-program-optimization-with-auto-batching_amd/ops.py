@@ -981,7 +981,8 @@ def paged_attn_decode(qkv, k_cache, v_cache, block_table, seq_ids, ctx_len, Hq, 
 class SharedPrefixPlan:
     """Which rows of a decode batch share their first pages, for `paged_attn_decode_shared`: made once for a batch, good for all its
     layers and steps while its rows stay.  groups: (rows, pages) - batch rows whose block tables begin with the same `pages` pages, all
-    within their contexts; a row is in one group at most.  lens: the rows' context lengths now, which choose how the work is cut."""
+    within their contexts; a row is in one group at most.  lens: the rows' context lengths now, which choose how the work is cut: a plan
+    that its rows have `outgrown` still gives their results, but slowly."""
 
     def __init__(self, groups, lens, Hq, Hkv, D, device):
         B, G = len(lens), Hq // Hkv
@@ -994,6 +995,7 @@ class SharedPrefixPlan:
         if any(not rows or pages <= 0 for rows, pages in groups) or any(16 * pages > lens[r] for rows, pages in groups for r in rows):
             raise ValueError("SharedPrefixPlan: a group has rows and pages, and its pages lie within their contexts")
         self.B, self.Hq, self.Hkv, self.D = B, Hq, Hkv, D
+        self.earlier = None                                              # a plan that this one replaces, as long as recorded steps may read it
         row_pages, row_slots = [0] * B, [0] * B
         for rows, pages in groups:
             for r in rows:
@@ -1011,7 +1013,8 @@ class SharedPrefixPlan:
         # (own ones two / four / eight: the first 46.4 / 46.2 / 45.2), and no more units of a row than its second launch joins cheaply
         per_block = max(8, -(-sum(-(-len(rows) // most) * pages for rows, pages in large) * Hkv // 512))
         per_wave = max(4, -(-sum(pages for _, pages in small) * Hkv // 1024))
-        self.own_splits = max(1, min(-(-max(own, default=0) // 8), 1024 // max(B * Hkv, 1), 64))
+        self.groups = groups
+        self.own_splits = self._shares(max(own, default=0))
         units = []
         for rows, pages in large + small:
             block = in_block(rows)
@@ -1032,6 +1035,19 @@ class SharedPrefixPlan:
         self._heads, self._page = (Hq, Hkv, D), ((Hkv, D // 32, 4, 16, 8), (Hkv, D, 16))
         self._bind()
 
+    def _shares(self, pages):
+        """How many units share the pages that a row has for itself."""
+        return max(1, min(-(-pages // 8), 1024 // max(self.B * self.Hkv, 1), 64))
+
+    def outgrown(self, lens) -> bool:
+        """Whether a plan made for these contexts would cut the rows' own pages into twice as many shares.  us, a plan of 20 own tokens / a new one / no
+        sharing, 8 rows behind 2048 tokens, 32 heads over 8: 200 own tokens 15.3 / 12.8 / 19.3, 400 20.6 / 13.1 / 20.5, 2000 65 / 19.5 / 31.8."""
+        own = [-(-n // 16) for n in lens]
+        for rows, pages in self.groups:
+            for r in rows:
+                own[r] -= pages
+        return self._shares(max(own, default=0)) >= 2 * self.own_splits
+
     def _bind(self):
         """The plan's arrays as parts of `data`, and what the C call takes of them: addresses that hold while the plan lives."""
         n = self.data.numel() - 2 * self.B
@@ -1039,11 +1055,11 @@ class SharedPrefixPlan:
         self._args = (self.units.data_ptr(), self.n_block, self.n_units, self.row_pages.data_ptr(), self.row_slots.data_ptr(), self.own_splits, self.slots)
 
     def __getstate__(self):
-        return {n: v for n, v in self.__dict__.items() if n not in ("units", "row_pages", "row_slots", "_args")}
+        return {n: v for n, v in self.__dict__.items() if n not in ("units", "row_pages", "row_slots", "_args", "earlier")}
 
     def __setstate__(self, state):
-        """A copy has arrays of its own, and their addresses."""
-        self.__dict__.update(state)
+        """A copy has arrays of its own, and their addresses; no recorded step reads them."""
+        self.__dict__.update(state, earlier=None)
         self._bind()
 
 

@@ -286,3 +286,33 @@ def test_linear4_cuts_by_the_order_of_x():
     def call(lay, ws, nb, T=32, K=4096, N=4096):
         return lib.mlora_linear4(16, 0, 0, 16, lay, K, 16, 16, 128, T, K, N, ws, nb, None)
     assert call(0, None, 0) == -3 and call(0, 16, need - 1) == -3
+
+
+def test_plans_are_cut_anew_when_their_rows_outgrow_them():
+    """As the rows' own pages grow the cache's plan is that of a new batch of these lengths (up to a factor of two in its shares); those before it stay as
+    they are for the steps that were recorded with them, and go with the batch."""
+    kvc, ops = load_pkg("kv_cache"), load_pkg("ops")
+    kv = kvc.PagedKVCache(1, 1000, 8, 64, max_seqs=8, max_blocks=300, rope_theta=1e4, max_pos=4800, device="cpu", n_q_heads=32)
+    batch = tuple(range(8))
+    for sid in batch:
+        kv.add_sequence(sid)
+        skip = kv.share_prefix(sid, 0, 2048) if sid else 0
+        kv.begin_forward([sid], [2048 + 5 + sid - skip])
+        kv.end_forward()
+    seen, before = [], []
+    for step in range(1400):
+        kv.begin_forward(batch, [1] * 8)
+        assert kv.plan is kv.shared_plan(batch)
+        if not seen or kv.plan is not seen[-1]:
+            seen.append(kv.plan)
+            before.append((kv.plan._args, kv.plan.data.clone()))
+        kv.end_forward()
+        new = ops.SharedPrefixPlan([(list(batch), 128)], [kv.lens[s] for s in batch], 32, 8, 64, "cpu")
+        assert kv.plan.own_splits <= new.own_splits and (kv.plan.own_splits * 2 > new.own_splits or (kv.lens[0] - 1) % 16)
+        assert kv.plan.groups == [(list(batch), 128)] and kv.plan.saved_bytes == seen[0].saved_bytes
+    assert [p.own_splits for p in seen] == [1, 2, 4, 8]
+    assert all(b.earlier is a for a, b in zip(seen, seen[1:])) and seen[0].earlier is None
+    for p, (args, data) in zip(seen, before):
+        assert p._args == args and (p.data == data).all() and p.units.data_ptr() == args[0]
+    kv.free_sequence(3)
+    assert not kv._plans

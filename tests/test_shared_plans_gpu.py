@@ -1,0 +1,68 @@
+"""Plans over shared prefixes as batches live: rows that outgrow them, copies of a cache, steps recorded with them."""
+import numpy as np
+import pytest
+import torch
+
+import test_shared_attention_gpu as A
+from conftest import load_pkg
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def model():
+    synth = load_pkg("synth")
+    wl = synth.config1()
+    return load_pkg("llama").LlamaForCausalLM.from_synthetic(wl.seed, wl.shape, [wl.lora], DEV)
+
+
+def behind_one_prefix(model, rows, pages, room, seed=0):
+    """A cache whose sequences share `pages` pages of keys and values, and have a few tokens of their own."""
+    rng = np.random.default_rng(seed)
+    V = model.shape.vocab_size
+    head = rng.integers(0, V, 16 * pages).astype(np.int32)
+    longest = 16 * pages + room
+    kv = model.create_paged_kv_cache(rows, 16 * pages + rows * (room + 32), longest, 16, max_seq_len=longest)
+    for i in range(rows):
+        kv.add_sequence(i)
+        skip = kv.share_prefix(i, 0, len(head)) if i else 0
+        prompt = np.concatenate([head, rng.integers(0, V, 2 + 3 * i).astype(np.int32)])
+        kv.begin_forward([i], [len(prompt) - skip])
+        model["prefill_no_adapter"](model.embed(torch.from_numpy(np.ascontiguousarray(prompt[skip:]))), kv)
+        kv.end_forward()
+    return kv
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,own", [(32, 8, 128, (130, 700, 40, 1)), (8, 8, 64, (2000, 3, 500))])
+def test_plans_of_either_length(ops, Hq, Hkv, D, own):
+    """The plan of the first step and the one for the contexts as they have become give results within their bounds of the definition."""
+    print("case either plan", Hq, Hkv, D, own, flush=True)
+    rows = len(own)
+    lens = [160 + n for n in own]
+    c = A.build(ops, rows, [(list(range(rows)), 10)], lens, Hq, Hkv, D)
+    early = ops.SharedPrefixPlan([(list(range(rows)), 10)], [161] * rows, Hq, Hkv, D, DEV)
+    assert early.outgrown(lens) and early.own_splits == 1 and not c["plan"].outgrown(lens)
+    A.close(A.call(ops, c), c)
+    A.close(A.call(ops, {**c, "plan": early}), c)
+
+
+def test_recorded_sessions_follow_their_plan(model):
+    """A batch that outgrows its plan twice: replayed steps choose what eager ones choose, on the plan that the cache has by then."""
+    print("case outgrown", flush=True)
+    ds = load_pkg("decode_session")
+    rows, steps = 4, 420
+    out, plans = {}, {}
+    for graph in (False, True):
+        kv = behind_one_prefix(model, rows, 128, steps + 40)
+        s = ds.DecodeSession(model, kv, list(range(rows)), {}, [5, 6, 7, 8], use_graph=graph)
+        plans[graph] = []
+        for _ in range(steps):
+            s.step(keep_history=True)
+            if not plans[graph] or kv.plan is not plans[graph][-1]:
+                plans[graph].append(kv.plan)
+            assert not graph or s._eager_steps == 1
+        assert not graph or s._plan is kv.plan
+        out[graph] = torch.stack(s.history).cpu().numpy()
+    assert [p.own_splits for p in plans[True]] == [p.own_splits for p in plans[False]] == [1, 2, 4]
+    assert np.array_equal(out[True], out[False])
