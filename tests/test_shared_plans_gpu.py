@@ -1,4 +1,6 @@
 """Plans over shared prefixes as batches live: rows that outgrow them, copies of a cache, steps recorded with them."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -66,3 +68,26 @@ def test_recorded_sessions_follow_their_plan(model):
         out[graph] = torch.stack(s.history).cpu().numpy()
     assert [p.own_splits for p in plans[True]] == [p.own_splits for p in plans[False]] == [1, 2, 4]
     assert np.array_equal(out[True], out[False])
+
+
+def test_copy_of_a_cache_decodes_when_the_original_is_gone(model):
+    print("case copied cache", flush=True)
+    rows = 3
+    kv = behind_one_prefix(model, rows, 130, 80)
+    sids, tokens = list(range(rows)), torch.tensor([3, 4, 5], dtype=torch.int32)
+
+    def step(cache):
+        cache.begin_forward(sids, [1] * rows)
+        logits, _ = model["decode_no_adapter"](model.embed(tokens), cache)
+        cache.end_forward()
+        assert cache.plan is not None
+        return logits
+
+    step(kv)
+    other = copy.deepcopy(kv)
+    want = step(kv)
+    old = kv.plan.data
+    kv.plan, kv._plans = None, {}
+    old.fill_(-1)                                            # what the original's plan said
+    del kv, old
+    assert torch.equal(step(other), want)
