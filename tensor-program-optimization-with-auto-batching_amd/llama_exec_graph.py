@@ -230,10 +230,10 @@ class LlamaExecGraph(ExecGraph):
             if getattr(self.exec_config, "native_decode", False):
                 # a model without the C decode step, rules, which it does not apply, or shared pages, which it reads for every request:
                 # graph-replayed operators
-                if not self.vm.native_step or ruled or self._shared_pays(seqs):
+                dense = len(seqs) <= 64 and self._dense_ok(method)       # the dense shrink serves at most 64 sequences
+                if not self.vm.native_step or ruled or self._shared_pays(seqs, dense):
                     seqs = self._decode_session(seqs, outputs, method, params)
                     continue
-                dense = len(seqs) <= 64 and self._dense_ok(method)       # the dense shrink serves at most 64 sequences
                 seqs = self._decode_native(seqs, outputs, method, params, dense) if dense or not method.startswith("mixed_decode") \
                     else self._decode_session(seqs, outputs, method, params)
                 continue
@@ -287,13 +287,21 @@ class LlamaExecGraph(ExecGraph):
             if len(left) != len(seqs):
                 return left
 
-    def _shared_pays(self, seqs):
-        """Whether the batch shares pages that its attention reads once, and those are enough to give up the native step's fused launches.
-        Measured on layers of 1024 x 2752 with 16 heads of 64, an adapter per row, us a layer and step, native / once: 32 rows that save
-        260 MB a layer 67 / 86, 520 MB 85 / 90; 64 rows 264 MB 75 / 77, 528 MB 92 / 79; 16 rows 252 MB 65 / 75; 4 rows 101 MB 80 / 66.
-        What the fused launches are worth grows with the rows, so the line is drawn where it holds for all."""
+    def _shared_pays(self, seqs, dense):
+        """Whether the batch shares pages that its attention reads once, and gains more by that than the native step's fused launches are worth.
+        Both are estimates in us a layer and step.  The native step's attention walks the longest prefix, and reads every row's pages from the caches;
+        its fused launches, most of all the dense shrink, are worth the more the more rows there are, until from 48 rows on the operators have forms as good.
+        Measured on layers of 1024 x 2752 with 16 heads of 64, and of 4096 x 11008 with 32 heads of 128 over 32 and over 8, native / once, us a step of two layers:
+          rows, shared pages       dense adapters: 4, 512    16, 256    32, 256    64, 128     none: 2, 256    32, 128    64, 64
+          1024 x 2752                        160 / 129    128 / 146  166 / 177  182 / 154       123 / 110  128 / 117  145 / 129
+          4096 x 11008, 32 over 32           366 / 319    351 / 324  468 / 367  516 / 378       291 / 280  363 / 293  411 / 338
+          4096 x 11008, 32 over 8            330 / 276    286 / 300  299 / 347  333 / 341       280 / 253  273 / 275  305 / 307
+        Of 221 such batches the choice is more than 2 % slower than the other one in two (by 3 %)."""
         plan = self.kv_cache.shared_plan(seqs) if hasattr(self.kv_cache, "shared_plan") else None
-        return plan is not None and plan.saved_bytes >= 512e6
+        if plan is None:
+            return False
+        gain = max(0.055 * (max(pages for _, pages in plan.groups) - 80), 0.04e-6 * plan.saved_bytes / (1 if plan.Hq == plan.Hkv else 2))
+        return gain > (4 if not dense else 13 if len(seqs) >= 48 else 6 + 0.9 * len(seqs))
 
     @staticmethod
     def _method_tids(method):

@@ -316,3 +316,22 @@ def test_plans_are_cut_anew_when_their_rows_outgrow_them():
         assert p._args == args and (p.data == data).all() and p.units.data_ptr() == args[0]
     kv.free_sequence(3)
     assert not kv._plans
+
+
+def test_when_a_batch_gives_up_the_native_step_for_shared_pages():
+    """The choice on measured batches of both sides: rows, longest shared prefix, saved MB a layer, heads, dense adapters."""
+    import types
+    xg = load_pkg("llama_exec_graph").LlamaExecGraph
+    graph = xg.__new__(xg)
+    for rows, pages, mb, heads, dense, pays in ((4, 512, 101, (16, 16), True, True), (2, 1024, 67, (16, 16), True, True), (32, 256, 520, (16, 16), True, False),
+                                                (16, 256, 252, (16, 16), True, False), (64, 128, 528, (16, 16), True, True), (64, 128, 528, (16, 16), False, True),
+                                                (32, 64, 520, (32, 32), True, False), (32, 64, 520, (32, 32), False, True), (16, 256, 1007, (32, 32), True, True),
+                                                (32, 256, 520, (32, 8), True, False), (32, 256, 520, (32, 8), False, True), (8, 128, 59, (32, 8), True, False),
+                                                (8, 512, 235, (32, 8), True, True), (128, 64, 533, (32, 8), False, True)):
+        plan = types.SimpleNamespace(groups=[([0, 1], 3), (list(range(rows)), pages)], saved_bytes=mb * 1e6, Hq=heads[0], Hkv=heads[1])
+        graph.kv_cache = types.SimpleNamespace(shared_plan=lambda seqs: plan)
+        assert graph._shared_pays(list(range(rows)), dense) == pays, (rows, pages, mb, heads, dense)
+    graph.kv_cache = types.SimpleNamespace(shared_plan=lambda seqs: None)
+    assert not graph._shared_pays([0, 1], False)
+    graph.kv_cache = types.SimpleNamespace()
+    assert not graph._shared_pays([0, 1], False)

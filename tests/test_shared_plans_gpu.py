@@ -91,3 +91,48 @@ def test_copy_of_a_cache_decodes_when_the_original_is_gone(model):
     old.fill_(-1)                                            # what the original's plan said
     del kv, old
     assert torch.equal(step(other), want)
+
+
+@pytest.mark.parametrize("adapters,dense,pages,once", [(False, False, 300, True), (True, True, 300, True), (True, False, 300, True), (True, True, 140, False)])
+def test_front_end_reads_shared_pages_once_where_that_pays(model, monkeypatch, adapters, dense, pages, once):
+    """A batch that the native step could serve goes through the attention over shared prefixes where that pays, and there alone; every token is the model's own
+    choice along its path (up to near ties: shorter prefills sum in another order)."""
+    print("case front end once", adapters, dense, pages, flush=True)
+    ab, xg, lora, kvm = load_pkg("auto_batcher"), load_pkg("llama_exec_graph"), load_pkg("lora"), load_pkg("kv_cache")
+    made, shared = [], kvm.ops.paged_attn_decode_shared
+    monkeypatch.setattr(kvm.ops, "paged_attn_decode_shared", lambda *a, **k: made.append(1) or shared(*a, **k))
+    V, steps, rows = model.shape.vocab_size, 10, 4
+    rng = np.random.default_rng(pages)
+    head = rng.integers(0, V, 16 * pages).astype(np.int32)
+    prompts = [np.concatenate([head, rng.integers(0, V, 2 + 7 * i).astype(np.int32)]) for i in range(rows)]
+    longest = 16 * pages + 60
+    lt = model.lora_types[0]
+    batcher = ab.LlamaAutoBatcherClass()
+    batcher.set_model(model)
+    batcher.set_exec_config(xg.LlamaExecConfig(max_prompt_len=longest, max_gen_len=steps, page_size=16, share_prefix=True, dense_lora=dense))
+    out = []
+    for p in prompts:
+        if adapters:
+            batcher.set_adapter(lora.LoraConfig(r=lt.r, alpha=lt.scaling * lt.r), wid=1)
+        out.append(batcher.generate(batcher.create_var(p)))
+    batcher.compile()
+    batcher.execute()
+    assert (len(made) >= model.shape.num_hidden_layers) == once and bool(made) == once
+    kv = model.create_paged_kv_cache(rows, rows * (longest + 32), longest, 16, max_seq_len=longest + 32)
+    def tokens_of(sid, toks, kind):
+        kv.begin_forward([sid], [len(toks)])
+        h = model.embed(torch.from_numpy(np.ascontiguousarray(toks)))
+        if adapters:
+            z, _ = model[f"{kind}_a0"](h, kv, [1] if kind == "prefill" else np.array([1], dtype=np.int32))
+        else:
+            z, _ = model[f"{kind}_no_adapter"](h, kv)
+        kv.end_forward()
+        return z[0]
+    for s, p in enumerate(prompts):
+        kv.add_sequence(s)
+        z = tokens_of(s, p, "prefill")
+        answer = list(map(int, out[s].var))
+        assert len(answer) == steps
+        for t in answer:
+            assert float(z.max() - z[t]) <= 2e-2 * float(z.std())
+            z = tokens_of(s, np.array([t], dtype=np.int32), "decode")
