@@ -203,12 +203,15 @@ class LlamaExecGraph(ExecGraph):
         for i in range(n):
             op.output_vars[i].var = int(first[i])
 
-    def check_seqs_finished(self, seqs_2_decode, outputs):
-        """The sequences that go on.  One that had no token left (-1) has ended ahead of it."""
+    def check_seqs_finished(self, seqs_2_decode, outputs, new=1):
+        """The sequences that go on; new: tokens that each was given since the last look.  One that had no token left (-1) has ended ahead of it."""
         for sid in seqs_2_decode:
-            if -1 in outputs[sid]:
-                del outputs[sid][outputs[sid].index(-1):]
-                self._ended.add(sid)
+            answer = outputs[sid]
+            for i in range(len(answer) - new, len(answer)):
+                if answer[i] < 0:
+                    del answer[i:]
+                    self._ended.add(sid)
+                    break
         return [sid for sid in seqs_2_decode if sid not in self._ended and outputs[sid][-1] != self.eos_token_id
                 and len(outputs[sid]) < self.seq_info.get_max_gen_len(sid)]
 
@@ -336,7 +339,7 @@ class LlamaExecGraph(ExecGraph):
             toks = torch.stack(sess.history).cpu().numpy()             # [ahead, batch]
             for i, sid in enumerate(seqs):
                 outputs[sid].extend(int(t) for t in toks[:, i])
-            return self.check_seqs_finished(seqs, outputs)
+            return self.check_seqs_finished(seqs, outputs, ahead)
         while True:
             ev = self._tic()
             nxt = sess.step()

@@ -335,3 +335,23 @@ def test_when_a_batch_gives_up_the_native_step_for_shared_pages():
     assert not graph._shared_pays([0, 1], False)
     graph.kv_cache = types.SimpleNamespace()
     assert not graph._shared_pays([0, 1], False)
+
+
+def test_finished_sequences_are_told_by_their_new_tokens():
+    """-1 (no token left) ends an answer wherever it stands among the new tokens; the rest of an answer is not looked at again."""
+    import types
+
+    class Answer(list):
+        def __contains__(self, x):
+            raise AssertionError("an answer is searched")
+
+        def index(self, *a):
+            raise AssertionError("an answer is searched")
+
+    xg = load_pkg("llama_exec_graph").LlamaExecGraph
+    graph = xg.__new__(xg)
+    graph.eos_token_id, graph._ended, graph.seq_info = 2, set(), types.SimpleNamespace(get_max_gen_len=lambda sid: 6)
+    out = {0: Answer([5, 6, 7]), 1: Answer([5, 6, -1]), 2: Answer([5, 6, 2]), 3: Answer([-1])}
+    assert graph.check_seqs_finished([0, 1, 2, 3], out) == [0] and out[1] == [5, 6] and out[3] == [] and graph._ended == {1, 3}
+    out = {0: Answer([5, 6, 7, 8]), 4: Answer([5, -1, 9, -1]), 5: Answer([1, 2, 3, 4, 5, 6]), 6: Answer([5, 6, 7, -1])}
+    assert graph.check_seqs_finished([0, 4, 5, 6], out, 3) == [0] and out[4] == [5] and out[6] == [5, 6, 7] and graph._ended == {1, 3, 4, 6}
