@@ -143,7 +143,7 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, float scale, int pg, int p
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) t.o[db] *= alpha;
   }
-  const float base = EDGE && t.m == -INFINITY ? 0.f : t.m;  // a row with no token yet
+  const float base = t.m == -INFINITY ? 0.f : t.m;          // a row with no token yet, or none above -inf
   f16 hi[P * 4], lo[P * 4];
 #pragma unroll
   for (int p = 0; p < P; ++p)
