@@ -408,7 +408,8 @@ int mlora_paged_attn_prefill(void* out, int out_layout, const void* qkv, const v
                              int T, int Hq, int Hkv, int D, int n_pages, int n_seq, void* stream);
 
 /* mlora_paged_attn_decode for a batch whose rows share prefixes: groups of rows whose block tables begin with the same pages, which
- * are read once per group.  The same result up to the order of fp32 sums; slots of a page behind a row's context may hold anything.
+ * are read once per group.  The same result up to the order of fp32 sums (NaN among a row's tokens gives NaN here); slots of a page behind a row's
+ * context may hold anything.
  * The plan (device arrays): units [n_units][mlora_shared_attn_record_ints()] = {rows, first page, pages, slot, four of any value, then
  * mlora_shared_attn_unit_rows() batch rows, those behind the unit's any row}: rows of a group attended over a range of the group's pages, into
  * that slot of each - first n_block units of at most mlora_shared_attn_unit_rows query rows (rows times Hq / Hkv), then units of at most 16;

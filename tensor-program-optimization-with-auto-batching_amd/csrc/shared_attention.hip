@@ -398,7 +398,7 @@ __global__ __launch_bounds__(4 * WAVE) void shared_attn_join_kernel(SharedAttn a
   for (int e = 0; e < PER; ++e) {
     const int d = lane * PER + e;
     const size_t oo = a.frag_tt ? frag_offset(b, h * D + d, a.frag_tt) : ((size_t)b * a.Hq + h) * D + d;
-    a.out[oo] = (f16)(L > 0.f ? o[e] / L : 0.f);
+    a.out[oo] = (f16)(L == 0.f ? 0.f : o[e] / L);           // no token: 0; a sum that is NaN stays so
   }
 }
 

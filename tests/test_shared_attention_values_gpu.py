@@ -44,3 +44,22 @@ def test_scores_of_minus_infinity(ops, Hq, Hkv, D, groups, lens, pages):
     got = A.call(ops, c)
     assert bool(got[some].isfinite().all()) and torch.equal(got[some], want[some])
     assert bool(definition(c)[some].isfinite().all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,groups,lens", SETS)
+@pytest.mark.parametrize("what", ["k", "v", "q"])
+def test_nan_is_not_hidden(ops, Hq, Hkv, D, groups, lens, what):
+    """NaN in a key, a value or a query that counts: NaN where the definition has it, and nowhere else."""
+    print("case nan", Hq, Hkv, D, what, flush=True)
+    c = A.build(ops, 4, groups, lens, Hq, Hkv, D, garbage=False)
+    clean = A.call(ops, c)
+    page = int(c["table"][int(c["rows"][0]), 5])
+    if what == "q":
+        c["qkv"][0, 1, 7] = float("nan")
+    elif what == "k":
+        c["k"][page, 1, 0, 1, 3, 2] = float("nan")
+    else:
+        c["v"][page, 1, 9, 3] = float("nan")
+    got, want = A.call(ops, c), definition(c)
+    assert bool(want.isnan().any()) and torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[~got.isnan()], clean[~got.isnan()])
