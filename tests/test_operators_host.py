@@ -355,3 +355,16 @@ def test_finished_sequences_are_told_by_their_new_tokens():
     assert graph.check_seqs_finished([0, 1, 2, 3], out) == [0] and out[1] == [5, 6] and out[3] == [] and graph._ended == {1, 3}
     out = {0: Answer([5, 6, 7, 8]), 4: Answer([5, -1, 9, -1]), 5: Answer([1, 2, 3, 4, 5, 6]), 6: Answer([5, 6, 7, -1])}
     assert graph.check_seqs_finished([0, 4, 5, 6], out, 3) == [0] and out[4] == [5] and out[6] == [5, 6, 7] and graph._ended == {1, 3, 4, 6}
+
+
+def test_short_allocation_only_where_it_means_what_it_did():
+    import torch
+    ops = load_pkg("ops")
+    right = lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype)
+    cpu = torch.device("cpu")
+    assert ops._short_or_plain(right, cpu) is right
+    for wrong in (None, lambda size, stride: right(size, stride, torch.float16), lambda size, stride, dtype: right(size, stride, torch.float32),
+                  lambda size, stride, dtype: right(size, (1, 2), dtype), lambda size, stride, dtype: right((3, 2), (2, 1), dtype),
+                  lambda size, stride, dtype: right(size, stride, dtype).requires_grad_()):
+        assert ops._short_or_plain(wrong, cpu) is ops._plain_empty
+    assert ops._short_or_plain(right, torch.device("cuda", 0)) is ops._plain_empty
