@@ -32,3 +32,23 @@ def test_either_order_of_x(ops, K, N, group):
         want = acc.double() + y[:T]
         most = L.bound(y[:T], mag[:T] + want.abs() + y[:T].abs(), K, group, torch.float32)
         assert bool(((ops.linear(a, W, out=acc, accumulate=True).double() - want).abs() <= most).all())
+
+
+@pytest.mark.parametrize("N,K", [(256, 384), (250, 352)])
+def test_weights_in_any_order(ops, N, K):
+    """q, scale and zero, or the weight that is rounded, as transposed or cut views: the same packed weight."""
+    print("case strided weights", N, K, flush=True)
+    group = 32
+    x, q, scale, zero = L.make(N, 4, K, N, group)
+    want = ops.QuantWeight(q, scale, zero)
+    turned = [t.t().contiguous().t() for t in (q, scale, zero)]
+    cut = [torch.cat([t, t], 1)[:, :t.shape[1]] for t in (q, scale, zero)]
+    for views in (turned, cut):
+        assert not views[0].is_contiguous()
+        W = ops.QuantWeight(*views)
+        assert torch.equal(W.q, want.q) and torch.equal(W.meta, want.meta)
+    w = torch.randn((N, K), device=L.DEV).half()
+    want = ops.quantize(w, group)
+    for view in (w.t().contiguous().t(), torch.cat([w, w], 1)[:, :K], w.float().t().contiguous().t()):
+        W = ops.quantize(view, group)
+        assert torch.equal(W.q, want.q) and torch.equal(W.meta, want.meta)
