@@ -3,9 +3,9 @@
 //
 // The matrix cores multiply fp16 activations with the integers q - z, which fp16 holds exactly, and a group's sum is scaled in fp32: no
 // rounding but those of fp32 sums and the result's.  Up to 16 tokens the weight stream from HBM is the bound (N K / 2 bytes and 3 N K /
-// group of scales and zeros): 8 tokens, 32003 x 4096, groups of 128: 17.4 us, 4.0 TB/s, what a plain read of 2 GiB reaches on the same card;
-// 16 tokens, 22016 x 4096: 12.7 us, 3.8 TB/s; one token, 4096 x 4096: 4.8 us, a launch and two rounds to memory.  With more tokens it is the
-// unpacking and scaling on the vector units beside the products and the reads of LDS: 200 tokens, 12288 x 4096, groups of 64: 35 us, 570 TFLOP/s
+// group of scales and zeros): 8 tokens, 32003 x 4096, groups of 128: 17.5 us, 4.0 TB/s (the fp16 products of this library stream 5.5); 16 tokens, 22016 x 4096:
+// 13.3 us, 3.6 TB/s; one token, 4096 x 4096: 5.0 us, a launch and two rounds to memory.  With more tokens it is the
+// unpacking and scaling on the vector units beside the products and the reads of LDS: 200 tokens, 12288 x 4096, groups of 64: 38 us, 530 TFLOP/s
 // (a plain fp16 product of 8192^3: 1.17 PFLOP/s).
 //
 // Layout (sizes: mlora_linear4_sizes; K in blocks of 128, N in tiles of 16 rows, both padded with zeros):

@@ -7,7 +7,7 @@
 // So the work is cut into units - (query rows, range of pages, kv head) - and a second launch joins a row's units.  Bound by the pages
 // read, 4 D bytes a token and kv head: 16 rows behind 32752 tokens, 32 heads of 128 over 8: 45 us, 3.2 TB/s (39 for the units, of which 23 are
 // the loads and 20 the products, half of them at a time, and the rest partial results; 6 for the join); 32 rows behind 1024 tokens, 32 heads
-// over 32: 23 us, 3.2 TB/s; four rows of 16 heads of 64 behind 512: 7.5 us, two launches.
+// over 32: 24 us, 3.1 TB/s; four rows of 16 heads of 64 behind 512: 9 us, two launches.
 //
 // Everywhere a wave holds a tile of 16 query rows (the G = Hq / Hkv heads of one or more requests) in the matrix-core layouts of the decode
 // kernel in attention.hip: S^T = K . Q^T, then O^T += V^T . P^T, where a lane's probabilities are already the operand that it must supply

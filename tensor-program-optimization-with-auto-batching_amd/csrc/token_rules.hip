@@ -6,7 +6,7 @@
 //
 // Every step is a separately rounded IEEE fp32 operation in this order, so the results are those of a plain evaluation bit for bit.
 // Bound by the logits (4 V bytes read a row, 4 V more where they are asked for): 256 rows of 128256 with histories of 4096, the logits asked
-// for: 61 us, 4.4 TB/s; for few rows by latency: one row of 32000 6 us, 32 rows 10 us, two launches.  The counts are made from the
+// for: 61 us, 4.4 TB/s; for few rows by latency: one row of 32000 6 us, 32 rows 11 us, two launches.  The counts are made from the
 // row's token history in LDS: a table of counts per row kept in memory would add half as much traffic again to a row of 128256
 // tokens, while a history of 4096 is 16 KiB.  They come from integer atomics, whose order does not matter.  A workgroup's logits and
 // mask words are requested ahead of that and wait in registers.
