@@ -324,21 +324,23 @@ class PagedKVCache(PageTable):
     def shared_plan(self, seq_ids):
         """The plan by which a decode step of these sequences reads the pages they share once, or None where none are shared or it does
         not pay.  Kept while all of them live (recorded steps read it), and cut anew where their own pages have outgrown it (looked at when the
-        first of them has filled a page).  us of attention without / with, 50 own tokens a row:
+        first of them has filled a page).  A pass that is being recorded takes the plan that is there, or none.  us of attention without / with, 50 own tokens a row:
         32 heads of 128 over 32, 32 rows, 16 shared pages 16.4 / 14.2, 64 pages 35 / 16, 256 pages 133 / 29; 2 rows, 64 pages 11.2 / 10.4, 256 pages
         38 / 22; 128 rows, 4 pages 36 / 35; 32 heads over 8, 32 rows, 64 pages (130 MB) 12.8 / 14.6, 256 pages 32 / 23, 128 rows, 16 pages (133 MB) 18 / 16,
         64 rows, 64 pages 20 / 17."""
         if not self._owners or not self.n_q_heads or not 1 <= self.n_q_heads // self.Hkv <= 16:
             return None
         batch = tuple(seq_ids)
+        recorded = self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()      # (a capture takes no arrays from the host)
         if batch not in self._plans:
+            if recorded:
+                return None
             groups = self.prefix_groups(batch)
             saved = sum((len(m) - 1) * p for m, p in groups) * self.Hkv * self.D * 4 * PAGE
             pays = saved >= 132e6 or any(p >= 128 for _, p in groups)
             self._plans[batch] = self._cut(batch, groups, saved) if pays else None
         plan = self._plans[batch]
-        if plan is not None and self.lens[batch[0]] % PAGE == 0 and plan.outgrown([self.lens[s] + 1 for s in batch]) \
-                and not (self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()):
+        if plan is not None and not recorded and self.lens[batch[0]] % PAGE == 0 and plan.outgrown([self.lens[s] + 1 for s in batch]):
             self._plans[batch] = self._cut(batch, plan.groups, plan.saved_bytes)
             self._plans[batch].earlier = plan
         return self._plans[batch]

@@ -368,3 +368,22 @@ def test_short_allocation_only_where_it_means_what_it_did():
                   lambda size, stride, dtype: right(size, stride, dtype).requires_grad_()):
         assert ops._short_or_plain(wrong, cpu) is ops._plain_empty
     assert ops._short_or_plain(right, torch.device("cuda", 0)) is ops._plain_empty
+
+
+def test_a_recorded_pass_makes_no_plan(monkeypatch):
+    """A pass begun inside a capture, with arrays on the device, reads shared pages for every row where no plan is there yet, and takes the one that is."""
+    import torch
+    kv, batch = _on_shared_pages()
+    kv.begin_forward(batch, [1] * len(batch))
+    kv.end_forward()
+    plan, kv._plans = kv.shared_plan(batch), {}
+    assert plan is not None
+    kv.device = torch.device("cuda")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    kv.begin_forward(batch, [1] * len(batch), device_meta=(None, None, None))
+    kv.end_forward()
+    assert kv.plan is None and not kv._plans
+    kv._plans[batch] = plan
+    kv.begin_forward(batch, [1] * len(batch), device_meta=(None, None, None))
+    kv.end_forward()
+    assert kv.plan is plan

@@ -136,3 +136,44 @@ def test_front_end_reads_shared_pages_once_where_that_pays(model, monkeypatch, a
         for t in answer:
             assert float(z.max() - z[t]) <= 2e-2 * float(z.std())
             z = tokens_of(s, np.array([t], dtype=np.int32), "decode")
+
+
+@pytest.mark.parametrize("planned", [False, True])
+def test_pass_begun_inside_a_capture(model, planned):
+    """Recorded with the plan that is there or with none, a step's replays give what an eager step gives."""
+    print("case pass in a capture", planned, flush=True)
+    rows = 3
+    kv = behind_one_prefix(model, rows, 130, 80)
+    sids, tokens = list(range(rows)), torch.tensor([3, 4, 5], dtype=torch.int32, device=DEV)
+
+    def step(meta):
+        kv.begin_forward(sids, [1] * rows, device_meta=meta)
+        logits = model.forward(model.embed(tokens), kv, {})
+        kv._cur = None                                       # the same step again: its keys and values are written anew
+        return logits
+
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=DEV)
+    at = [kv.lens[s] for s in sids]
+    meta = i32([kv.slot[s] for s in sids]), i32(at), i32([n + 1 for n in at])
+    want = step(meta)
+    plan = kv.plan
+    assert plan is not None
+    if not planned:
+        kv._plans.clear()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(meta)
+    assert kv.plan is (plan if planned else None)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        if planned:
+            assert torch.equal(got, want)
+        else:
+            assert float((got - want).abs().max() / want.std()) <= 1e-2          # (whole-model bound, as against the oracle)
+        again = step(meta)
+        assert kv.plan is not None and torch.equal(again, want)
+        if not planned:
+            kv._plans.clear()
