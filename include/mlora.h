@@ -425,6 +425,64 @@ int mlora_paged_attn_decode_shared(void* out, int out_layout, const void* qkv, c
                                    int slots, int B, int Hq, int Hkv, int D, int n_pages, int n_seq, void* workspace, size_t workspace_bytes,
                                    void* stream);
 
+/* Caches that hold more: pages of 8 bits, and sliding windows with sinks over those or over fp16 pages.
+ *
+ * Pages of 8 bits (step != NULL): of a page and kv head, k codes [D/64][4][16][2][8] (element (token, d) at [d/64][(d%32)/8][token][(d%64)/32][d%8]) and
+ * v codes [D/64][4][16][4][4] (at [d/64][token/4][d%16][(d%64)/16][token%4]), int8, and step [n_pages, Hkv, 2] fp32 of keys and values: a code c stands for c * step.  A page
+ * is rounded once, when its 16 tokens are there: step = fp32(a / 127), c = rint(127 x / a) (ties to even), a = the largest magnitude; a = 0: codes 0; where it holds an
+ * infinity or NaN: codes 0 and a step that is NaN.  tail_k, tail_v [n_seq, ...]: a page of each sequence in the layouts of fp16 pages, which holds the tokens of the
+ * sequence's last page unrounded.  Every slot may hold anything ahead of its first use.
+ * A token at position p sees positions j <= p, with window > 0 only those with j > p - window or j < sinks; of pages of 8 bits, its own page unrounded.
+ * Pages that nobody sees need not be there (ids outside [0, n_pages) are not seen either), and what nobody sees may be infinite or NaN.  A sequence or position that is out of
+ * range sees nothing (the result is 0) and is not stored.
+ *
+ * mlora_page_attn_decode: T single tokens of different sequences: rotates q and k (qkv stays as it is), puts the token's k and v in its place - completing its page, where
+ * it is the last -, attends.  The work of a row is cut into `splits` shares (mlora_page_attn_splits names a good number for rows of up to `pages` visible pages);
+ * with more than one: workspace of mlora_page_attn_workspace_bytes, 16-byte aligned, and a second launch.  Hq / Hkv <= 16.
+ * mlora_page_attn_prefill: T tokens of a pass, those of a sequence consecutive with increasing positions.  Pages of 8 bits: rotates, stores and attends, as above
+ * (three launches).  fp16 pages: as mlora_paged_attn_prefill, on rotated queries and stored keys (rope_cos, rope_sin unused). */
+typedef struct {
+  void* out;
+  const void* qkv;
+  void *k, *v;
+  float* step;
+  void *tail_k, *tail_v;
+  const int32_t *block_table, *tok_seq, *tok_pos;
+  const float *rope_cos, *rope_sin;
+  void* workspace;
+  size_t workspace_bytes;
+  int out_layout, max_blocks, max_pos, T, Hq, Hkv, D, n_pages, n_seq, window, sinks, splits;
+} mlora_page_attn;
+int mlora_page_attn_splits(int T, int Hkv, int pages);
+size_t mlora_page_attn_workspace_bytes(int T, int Hq, int D, int splits);
+int mlora_page_attn_decode(const mlora_page_attn* host_args, void* stream);
+int mlora_page_attn_prefill(const mlora_page_attn* host_args, void* stream);
+/* keys, values [n, Hkv, 16, D] f16: what pages ids [n] of 8 bits stand for (rows of ids outside [0, n_pages) are not written) */
+int mlora_page_values(void* keys, void* values, const void* k, const void* v, const float* step, const int32_t* ids, int n, int Hkv, int D, int n_pages, void* stream);
+
+/* Rows src[i] of pools [layers][rows][row_bytes] to rows dst[i], i < n, in every layer of up to 8 pools: one launch.  A row that is written is in no other pair;
+ * indices out of range name no row.  host_pools is read during the call. */
+typedef struct {
+  void* data;
+  long row_bytes;
+  int layers, rows;
+} mlora_page_pool;
+int mlora_copy_pages(const mlora_page_pool* host_pools, int n_pools, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* A step of a beam search over R requests of W <= 16 beams.
+ * mlora_beam_select: the k <= 32 best continuations of every request: candidates (b, v) with value scores[b] + z[b, v] - log sum exp z[b], z = logits [R * W, ld] fp32; a beam
+ * with ended[b] != 0 (ended may be NULL) has the one candidate eos, of value scores[b].  Values are compared in 64 bits, the lowest b V + v of equal ones comes first, -inf
+ * and NaN are none.  out_scores, tokens, parents (beam within the request) [R, k]; where candidates run out -inf, -1, -1.
+ * mlora_beam_reorder: beam i goes on as a child of parents[i].  slots [R, W]: rows of block_table that the beams have, pos [R * W]: of the tokens they appended last.  A parent's
+ * first child keeps the parent's slot; the others (and a beam with a parent outside 0..W-1, which copies nothing) take, in order, the slots of beams without children: new_slots.
+ * For those, row dst_slot of the table takes over row src_slot's pages ahead of the one of the last token, and dst_page is to become a copy of src_page (and whatever else a
+ * slot holds: dst_slot of src_slot); -1 where there is nothing to copy.  Slots are distinct. */
+size_t mlora_beam_select_workspace_bytes(int R, int W, int V, int k);
+int mlora_beam_select(float* out_scores, int32_t* tokens, int32_t* parents, const float* logits, long ld, const float* scores, const int32_t* ended, int eos,
+                      int R, int W, int V, int k, void* workspace, size_t workspace_bytes, void* stream);
+int mlora_beam_reorder(int32_t* new_slots, int32_t* src_slot, int32_t* dst_slot, int32_t* src_page, int32_t* dst_page, const int32_t* parents, const int32_t* slots,
+                       int32_t* block_table, const int32_t* pos, int R, int W, int n_rows, int max_blocks, void* stream);
+
 
 /* ---------------------------------------------------------------------------------------------
  * Decode-step variants that carry the LoRA work of a projection inside a neighbouring launch, so that the

@@ -92,6 +92,15 @@ SIGNATURES = {
     "mlora_argmax": (_i, [_p, _p, _i, _i, _p]),
     "mlora_rope_kv_append": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p]),
     "mlora_paged_attn_decode": (_i, [_p, _i, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
+    "mlora_page_attn_splits": (_i, [_i, _i, _i]),
+    "mlora_page_attn_workspace_bytes": (_z, [_i, _i, _i, _i]),
+    "mlora_page_attn_decode": (_i, [_p, _p]),
+    "mlora_page_attn_prefill": (_i, [_p, _p]),
+    "mlora_page_values": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "mlora_copy_pages": (_i, [_p, _i, _p, _p, _i, _p]),
+    "mlora_beam_select_workspace_bytes": (_z, [_i, _i, _i, _i]),
+    "mlora_beam_select": (_i, [_p, _p, _p, _p, _l, _p, _p, _i, _i, _i, _i, _i, _p, _z, _p]),
+    "mlora_beam_reorder": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
     "mlora_shared_attn_unit_rows": (_i, []),
     "mlora_shared_attn_workspace_bytes": (_z, [_i, _i, _i, _i]),
     "mlora_shared_attn_record_ints": (_i, []),

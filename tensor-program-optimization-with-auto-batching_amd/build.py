@@ -15,13 +15,13 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["api.hip", "gather_mm.hip", "gather_mm_batch.hip", "gemv.hip", "gemm.hip", "rowops.hip", "attention.hip", "decode_step.hip", "prefill.hip", "token_rules.hip", "linear4.hip", "shared_attention.hip"]
+SOURCES = ["api.hip", "gather_mm.hip", "gather_mm_batch.hip", "gemv.hip", "gemm.hip", "rowops.hip", "attention.hip", "decode_step.hip", "prefill.hip", "token_rules.hip", "linear4.hip", "shared_attention.hip", "page_attention.hip", "beams.hip"]
 DECODER_SOURCES = ["stream_ops.hip", "latent_attention.hip", "time_mix.hip", "moe.hip"]
 LIBS = {   # element type -> (library, sources, suffix of the objects, extra flags)
     "float16": (os.path.join(HERE, "libmlora_hip.so"), SOURCES, "", []),
-    "bfloat16": (os.path.join(HERE, "libmlora_bf16.so"), ["api.hip", "gemv.hip", "gemm.hip", "rowops.hip", "token_rules.hip", *DECODER_SOURCES], "_bf16",
+    "bfloat16": (os.path.join(HERE, "libmlora_bf16.so"), ["api.hip", "gemv.hip", "gemm.hip", "rowops.hip", "token_rules.hip", "beams.hip", *DECODER_SOURCES], "_bf16",
                  ["-DMLORA_ELT_BF16"]),
-    "float32": (os.path.join(HERE, "libmlora_f32.so"), ["api.hip", "rowops.hip", "token_rules.hip", "linear_f32.hip", *DECODER_SOURCES], "_f32", ["-DMLORA_ELT_F32"]),
+    "float32": (os.path.join(HERE, "libmlora_f32.so"), ["api.hip", "rowops.hip", "token_rules.hip", "beams.hip", "linear_f32.hip", *DECODER_SOURCES], "_f32", ["-DMLORA_ELT_F32"]),
 }
 LIB = LIBS["float16"][0]
 HEADERS = [os.path.join(CSRC, h) for h in ("common.h", "lora_device.h", "gather_mm_batch.h", "moe.h")] + \

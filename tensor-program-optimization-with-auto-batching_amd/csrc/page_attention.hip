@@ -1,0 +1,1037 @@
+// Attention over paged caches that hold more: pages of 8 bits, and sliding windows with sinks over those or over fp16 pages.
+//
+//   out[t, h] = softmax(scale q[t, h] . K) V  over the tokens that position p sees: j <= p and (j > p - window or j < sinks)
+//
+// Pages of 8 bits: once the 16 tokens of a page are there, its keys and its values are rounded per kv head to code * step, step = fp32(a / 127),
+// a = max |x|, code = rint(127 x / a).  That is exact in fp32: x and a are fp16 numbers, so 127 x / a, where it is below 2^(8 - d), is a ratio whose
+// denominator is below 2^(11 + d): it is half-way between two integers or at least 2^(-12 - d) off, and the division errs by 2^(-16 - d).
+// A page with an infinity or NaN has a step that is NaN.  The tokens of a sequence's last page lie unrounded in its tail.  A query sees its
+// own page unrounded and the pages ahead of it in 8 bits, so results do not depend on how a prompt is cut into passes.
+//
+// Codes enter the matrix cores as fp16 integers (exact), steps multiply scores and a page's weighted values in fp32.
+#include "common.h"
+
+int mlora_check_attn(const char* who, int Hq, int Hkv, int D, int n_pages, int n_seq, int max_blocks);
+
+namespace {
+
+constexpr int PAGE = MLORA_PAGE_SIZE;
+constexpr float LOG2E = 1.4426950408889634f;
+// Weights enter the matrix cores as two fp16 halves, the greatest as 2^14 (2^15 with a page's factor): 22 bits, and none of them is off by more than 2^-39 of the greatest, where
+// fp16 numbers end.  (With 1 for the greatest it is 2^-25: too much where small weights meet values that are 2^25 times those of the others.)
+constexpr float TOP = 14.f;
+
+struct PageAttn {
+  f16* out;
+  const f16* qkv;
+  void *k, *v;                 // fp16 pages as in attention.hip, or codes [n_pages][Hkv][D / 64][4][16][2][8] and [n_pages][Hkv][D / 64][4][16][4][4]
+  float* step;                 // [n_pages][Hkv][2] of keys and values (8 bits)
+  f16 *tail_k, *tail_v;        // [n_seq] pages in the layouts of fp16 pages (8 bits)
+  const int32_t *block_table, *tok_seq, *tok_pos;
+  const float *rope_cos, *rope_sin;
+  float *acc, *ml;             // [T][Hq][splits][D], [T][Hq][splits][2]
+  int max_blocks, max_pos, T, Hq, Hkv, n_pages, n_seq, window, sinks, splits, frag_tt;
+  float scale;                 // of scores, with log2 e: weights are powers of two
+};
+
+// the maximum over the lanes of a column, i.e. over the four rows of 16 lanes
+__device__ __forceinline__ float groups_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Eight codes as fp16 integers: a byte under the exponent of 1024 is 1024 + byte
+__device__ __forceinline__ f16x8 from_codes(uint32_t a, uint32_t b) {
+  union { uint32_t u[4]; f16x8 h; } x;
+  a ^= 0x80808080u;
+  b ^= 0x80808080u;
+  x.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x07010700u);
+  x.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x07030702u);
+  x.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x07010700u);
+  x.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x07030702u);
+  const f16 c = (f16)1152.f;
+  return x.h - f16x8{c, c, c, c, c, c, c, c};
+}
+
+__device__ __forceinline__ f16x4 from_codes(uint32_t a) {
+  union { uint32_t u[2]; f16x4 h; } x;
+  a ^= 0x80808080u;
+  x.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x07010700u);
+  x.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x07030702u);
+  const f16 c = (f16)1152.f;
+  return x.h - f16x4{c, c, c, c};
+}
+
+// A head row of a token as the lane (group g) of an operand holds it - dims 32 kb + 8 g .. + 7 -, rotated.  Separately rounded products, as in
+// attention.hip: the keys are those of the fp16 cache bit for bit.  (Both elements of a pair are the lane's own.)
+template <int D>
+__device__ __forceinline__ void load_rotated(f16x8 (&x)[D / 32], const f16* __restrict__ row, const float* __restrict__ c, const float* __restrict__ s, int g) {
+  constexpr int H = D / 64;
+#pragma unroll
+  for (int kb = 0; kb < D / 32; ++kb) x[kb] = ld8(row + kb * 32 + g * 8);
+#pragma unroll
+  for (int kb = 0; kb < H; ++kb) {
+    const float* cp = c + kb * 32 + g * 8;
+    const float* sp = s + kb * 32 + g * 8;
+    const f32x4 c0 = *reinterpret_cast<const f32x4*>(cp), c1 = *reinterpret_cast<const f32x4*>(cp + 4);
+    const f32x4 s0 = *reinterpret_cast<const f32x4*>(sp), s1 = *reinterpret_cast<const f32x4*>(sp + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float cc = e < 4 ? c0[e & 3] : c1[e & 3], ss = e < 4 ? s0[e & 3] : s1[e & 3], a = (float)x[kb][e], b = (float)x[kb + H][e];
+      float r1, r2;
+      {
+#pragma clang fp contract(off)
+        r1 = a * cc - b * ss;
+        r2 = b * cc + a * ss;
+      }
+      asm volatile("" : "+v"(r1), "+v"(r2));               // the fp32 result exists before the conversion
+      x[kb][e] = (f16)r1;
+      x[kb + H][e] = (f16)r2;
+    }
+  }
+}
+
+__device__ __forceinline__ bool token_ok(const PageAttn& a, int seq, int pos) {
+  return seq >= 0 && seq < a.n_seq && pos >= 0 && pos < a.max_pos && pos / PAGE < a.max_blocks;
+}
+
+__device__ __forceinline__ int8_t code_of(float x, float most) {
+  return (int8_t)(int)rintf(127.f * x / most);
+}
+
+// A whole page of a head from a wave's operands - keys: lane (g, token) dims 32 kb + 8 g ..; values: lane (g, col) tokens 4 g .. of dims 16 db + col -
+// in 8 bits
+template <int D>
+__device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh, const f16x8 (&k)[D / 32], const f16x4 (&v)[D / 16]) {
+  const int lane = threadIdx.x & 63;
+  float mk = 0.f, mv = 0.f, odd_k = 0.f, odd_v = 0.f;       // odd: x - x, which is zero but for infinities and NaN
+#pragma unroll
+  for (int kb = 0; kb < D / 32; ++kb)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = (float)k[kb][e];
+      mk = fmaxf(mk, fabsf(x));
+      odd_k += x - x;
+    }
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = (float)v[db][e];
+      mv = fmaxf(mv, fabsf(x));
+      odd_v += x - x;
+    }
+  mk = wave_max(mk);
+  mv = wave_max(mv);
+  const bool bad_k = __any(odd_k != 0.f), bad_v = __any(odd_v != 0.f);
+  const float dk = mk > 0.f && !bad_k ? mk : INFINITY, dv = mv > 0.f && !bad_v ? mv : INFINITY;      // (x / inf: codes 0)
+  uint8_t* kp = (uint8_t*)a.k + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 16;
+  uint8_t* vp = (uint8_t*)a.v + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 16;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) {
+    union { int8_t b[16]; uint4 u; } x, y;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      x.b[e] = code_of(bad_k ? 0.f : (float)k[2 * j + e / 8][e % 8], dk);
+      y.b[e] = code_of(bad_v ? 0.f : (float)v[4 * j + e / 4][e % 4], dv);
+    }
+    *reinterpret_cast<uint4*>(kp + j * 1024) = x.u;
+    *reinterpret_cast<uint4*>(vp + j * 1024) = y.u;
+  }
+  if (lane == 0)
+    *reinterpret_cast<f32x2*>(a.step + 2 * ((size_t)page * a.Hkv + kh)) = f32x2{bad_k ? NAN : mk / 127.f, bad_v ? NAN : mv / 127.f};
+}
+
+// ---------------------------------------------------------------------------------------------
+// One token a sequence: rotation, the new token's place in the cache, and attention.  A workgroup has a kv head of a sequence, or a share of
+// its pages; its waves take them in turn, in the matrix-core layouts of the decode kernel in attention.hip.
+// ---------------------------------------------------------------------------------------------
+template <int D, bool Q8>
+struct PageRegs {
+  uint4 k[Q8 ? D / 64 : D / 32];
+  uint4 v[Q8 ? D / 64 : D / 32];     // fp16: tokens 4 g .. of dims 16 (2 j) + col, then 16 (2 j + 1) + col
+  f32x2 step;
+  int page;                          // < 0: none
+};
+
+template <int D, bool Q8, int NW>
+__global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
+  constexpr int NKB = D / 32, NDB = D / 16, RING = 2, NL = Q8 ? D / 64 : D / 32;
+  __shared__ float sm[NW][16], sl[NW][16];
+  extern __shared__ float sacc[];                           // [NW][G][D]
+  const int kh = blockIdx.x, split = blockIdx.y, b = blockIdx.z, G = a.Hq / a.Hkv;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int seq = a.tok_seq[b], pos = a.tok_pos[b];
+  const bool ok = token_ok(a, seq, pos);                    // uniform; otherwise no token is seen
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (ok) {
+    const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
+    const int own = pos / PAGE, slot = pos % PAGE;
+    // the pages ahead of the own one: those of the sinks, then those of the window
+    const int least = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0, from = least / PAGE;
+    const int heads = a.sinks > 0 ? min((a.sinks - 1) / PAGE + 1, from) : 0;
+    const int n = heads + own - from, per = (n + a.splits - 1) / a.splits;
+    const int i0 = min(split * per, n), i1 = min(i0 + per, n);
+    const bool mine = split == a.splits - 1 && wave == (i1 - i0) % NW;       // the wave that has the own page
+    auto page_of = [&](int i) { return i < heads ? i : from + i - heads; };
+    const float* rc = a.rope_cos + (size_t)pos * (D / 2);
+    const float* rs = a.rope_sin + (size_t)pos * (D / 2);
+    f16x8 q[NKB];
+    if (col < G) load_rotated<D>(q, a.qkv + ((size_t)b * (a.Hq + 2 * a.Hkv) + kh * G + col) * D, rc, rs, g);
+    else
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) q[kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+
+    // the scores of a page become weights: st, by `scale`, of which a lane has tokens first .. first + 3; EDGE: some may not be seen
+    auto weights = [&](f32x4 st, float scale, int first, int end, f16x8& p, bool edge) {
+      float pm = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        st[e] *= scale;
+        if (edge && (first + e >= end || (first + e < least && first + e >= a.sinks))) st[e] = -INFINITY;
+        pm = fmaxf(pm, st[e]);
+      }
+      pm = groups_max(pm);
+      if (__any(pm > m)) {
+        const float mn = fmaxf(m, pm), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        l *= alpha;
+        m = mn;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db] *= alpha;
+      }
+      const float base = m == -INFINITY ? 0.f : m - TOP;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = __builtin_amdgcn_exp2f(st[e] - base);
+        l += w;
+        p[e] = (f16)w;
+        p[4 + e] = (f16)(w - (float)p[e]);
+      }
+    };
+
+    if (mine) {
+      int id = bt[own];
+      if (id < 0 || id >= a.n_pages) id = -1;
+      const bool there = Q8 || id >= 0;                     // uniform
+      f16* kp = Q8 ? a.tail_k + ((size_t)seq * a.Hkv + kh) * PAGE * D : (f16*)a.k + ((size_t)(there ? id : 0) * a.Hkv + kh) * PAGE * D;
+      f16* vp = Q8 ? a.tail_v + ((size_t)seq * a.Hkv + kh) * PAGE * D : (f16*)a.v + ((size_t)(there ? id : 0) * a.Hkv + kh) * PAGE * D;
+      if (there) {
+        f16x8 k[NKB], kn[NKB];
+        f16x4 v[NDB];
+        const f16* vn = a.qkv + ((size_t)b * (a.Hq + 2 * a.Hkv) + a.Hq + a.Hkv + kh) * D + col;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) k[kb] = ld8(kp + kb * 512 + lane * 8);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) v[db] = *reinterpret_cast<const f16x4*>(vp + (db * 16 + col) * PAGE + g * 4);
+        load_rotated<D>(kn, a.qkv + ((size_t)b * (a.Hq + 2 * a.Hkv) + a.Hq + kh) * D, rc, rs, g);
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+          if (col == slot) {
+            k[kb] = kn[kb];
+            st8(kp + kb * 512 + lane * 8, kn[kb]);
+          }
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const f16 x = vn[db * 16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (4 * g + e == slot) v[db][e] = x;
+          if (g == slot / 4) vp[(db * 16 + col) * PAGE + slot] = x;
+        }
+        if constexpr (Q8) {
+          if (slot == PAGE - 1 && id >= 0) store_codes<D>(a, id, kh, k, v);
+        }
+        f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) st = mfma_16x16x32(k[kb], q[kb], st);
+        const int first = own * PAGE + 4 * g;
+        f16x8 p;
+        weights(st, a.scale, first, pos + 1, p, true);
+        bool see[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) see[e] = first + e <= pos && (first + e >= least || first + e < a.sinks);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          f16x4 x;                                          // (slots behind the token hold anything)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = see[e] ? v[db][e] : (f16)0.f;
+          o[db] = mfma_16x16x32(f16x8{x[0], x[1], x[2], x[3], x[0], x[1], x[2], x[3]}, p, o[db]);
+        }
+      }
+    }
+
+    PageRegs<D, Q8> r[RING];
+    // 64 pages of the wave at a time, whose ids a lane each holds
+    for (int k0 = i0 + wave; k0 < i1; k0 += 64 * NW) {
+      const int i = k0 + lane * NW, count = min((i1 - k0 + NW - 1) / NW, 64);
+      int ids = i < i1 ? bt[page_of(i)] : -1;
+      if (ids >= a.n_pages) ids = -1;
+      auto load = [&](PageRegs<D, Q8>& r, int c) {
+        const int id = __builtin_amdgcn_readlane(ids, c < count ? c : count - 1);
+        r.page = c < count && id >= 0 ? page_of(k0 + c * NW) : -1;
+        const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh);
+        if constexpr (Q8) {
+          const uint8_t* kp = (const uint8_t*)a.k + at * (PAGE * D) + lane * 16;
+          const uint8_t* vp = (const uint8_t*)a.v + at * (PAGE * D) + lane * 16;
+#pragma unroll
+          for (int j = 0; j < NL; ++j) r.k[j] = *reinterpret_cast<const uint4*>(kp + j * 1024);
+#pragma unroll
+          for (int j = 0; j < NL; ++j) r.v[j] = *reinterpret_cast<const uint4*>(vp + j * 1024);
+          r.step = *reinterpret_cast<const f32x2*>(a.step + 2 * at);
+        } else {
+          const f16* kp = (const f16*)a.k + at * (PAGE * D) + lane * 8;
+          const f16* vp = (const f16*)a.v + at * (PAGE * D) + col * PAGE + g * 4;
+#pragma unroll
+          for (int j = 0; j < NL; ++j) r.k[j] = *reinterpret_cast<const uint4*>(kp + j * 512);
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            const uint2 lo = *reinterpret_cast<const uint2*>(vp + (2 * j) * 16 * PAGE), hi = *reinterpret_cast<const uint2*>(vp + (2 * j + 1) * 16 * PAGE);
+            r.v[j] = uint4{lo.x, lo.y, hi.x, hi.y};
+          }
+        }
+      };
+      auto work = [&](PageRegs<D, Q8>& r) {
+        if (r.page < 0) return;                             // uniform
+        f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (Q8) {
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            st = mfma_16x16x32(from_codes(r.k[j].x, r.k[j].y), q[2 * j], st);
+            st = mfma_16x16x32(from_codes(r.k[j].z, r.k[j].w), q[2 * j + 1], st);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            union { uint4 u; f16x8 h; } x = {r.k[j]};
+            st = mfma_16x16x32(x.h, q[j], st);
+          }
+        }
+        const int first = r.page * PAGE + 4 * g;
+        const bool edge = r.page * PAGE < least;            // uniform
+        f16x8 p;
+        weights(st, Q8 ? a.scale * r.step[0] : a.scale, first, 0x7fffffff, p, edge);
+        if constexpr (Q8) {
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            const uint32_t u[4] = {r.v[j].x, r.v[j].y, r.v[j].z, r.v[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f16x4 x = from_codes(u[i]);
+              const f32x4 t = mfma_16x16x32(f16x8{x[0], x[1], x[2], x[3], x[0], x[1], x[2], x[3]}, p, f32x4{0.f, 0.f, 0.f, 0.f});
+              o[4 * j + i] += t * r.step[1];
+            }
+          }
+        } else {
+          uint32_t keep[2] = {~0u, ~0u};                    // of a lane's four tokens (those that are not seen may be infinite)
+          if (edge) {
+            const int t0 = first, s = a.sinks;
+            const auto see = [&](int t) { return t >= least || t < s; };
+            keep[0] = (see(t0) ? 0xffffu : 0u) | (see(t0 + 1) ? 0xffff0000u : 0u);
+            keep[1] = (see(t0 + 2) ? 0xffffu : 0u) | (see(t0 + 3) ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            union { uint32_t u[4]; f16x8 h; } x = {{r.v[j].x & keep[0], r.v[j].y & keep[1], r.v[j].x & keep[0], r.v[j].y & keep[1]}},
+                                              y = {{r.v[j].z & keep[0], r.v[j].w & keep[1], r.v[j].z & keep[0], r.v[j].w & keep[1]}};
+            o[2 * j] = mfma_16x16x32(x.h, p, o[2 * j]);
+            o[2 * j + 1] = mfma_16x16x32(y.h, p, o[2 * j + 1]);
+          }
+        }
+      };
+#pragma unroll
+      for (int u = 0; u < RING; ++u) load(r[u], u);
+      for (int c = 0; c < count; c += RING) {
+#pragma unroll
+        for (int u = 0; u < RING; ++u) {
+          work(r[u]);
+          load(r[u], c + u + RING);
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 16, WAVE);
+  l += __shfl_xor(l, 32, WAVE);
+  if (col < G) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(&sacc[((size_t)wave * G + col) * D + db * 16 + 4 * g]) = o[db];
+    if (g == 0) {
+      sm[wave][col] = m;
+      sl[wave][col] = l;
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < G * D; e += NW * WAVE) {
+    const int qh = e / D, d = e % D, h = kh * G + qh;
+    float M = sm[0][qh];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, sm[w][qh]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][qh] - base);
+      L += sl[w][qh] * f;
+      x += sacc[((size_t)w * G + qh) * D + d] * f;
+    }
+    if (a.splits == 1) {
+      const size_t at = a.frag_tt ? frag_offset(b, h * D + d, a.frag_tt) : ((size_t)b * a.Hq + h) * D + d;
+      a.out[at] = (f16)(L == 0.f ? 0.f : x / L);            // no token: 0; a sum that is NaN stays so
+    } else {
+      const size_t at = ((size_t)b * a.Hq + h) * a.splits + split;
+      a.acc[at * D + d] = x;
+      if (d == 0) *reinterpret_cast<f32x2*>(a.ml + 2 * at) = f32x2{M, L};
+    }
+  }
+}
+
+// The shares of a row and head, joined by a wave
+template <int D>
+__global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
+  constexpr int PER = D / WAVE;
+  const int lane = threadIdx.x & 63, h = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
+  if (h >= a.Hq) return;
+  const size_t at = ((size_t)b * a.Hq + h) * a.splits;
+  float M = -INFINITY, L = 0.f, o[PER] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {                // four at a time, requested together
+    f32x2 ml[4];
+    float x[4][PER];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u;
+      ml[u] = s < a.splits ? *reinterpret_cast<const f32x2*>(a.ml + 2 * (at + s)) : f32x2{-INFINITY, 0.f};
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[u][e] = s < a.splits ? a.acc[(at + s) * D + lane * PER + e] : 0.f;
+    }
+    float m = M;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) m = fmaxf(m, ml[u][0]);
+    const float base = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(M - base);
+    M = m;
+    L *= f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float fu = __builtin_amdgcn_exp2f(ml[u][0] - base);
+      L += ml[u][1] * fu;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] += x[u][e] * fu;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int d = lane * PER + e;
+    const size_t oo = a.frag_tt ? frag_offset(b, h * D + d, a.frag_tt) : ((size_t)b * a.Hq + h) * D + d;
+    a.out[oo] = (f16)(L == 0.f ? 0.f : o[e] / L);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Prompts.  A workgroup has 64 NT consecutive tokens of a pass under one query head, a wave NT tiles of 16 of them; the tokens' runs (consecutive
+// positions of one sequence) are worked one behind the other, each over the pages that it sees, four at a time.  A wave brings one of the four from
+// the cache into LDS as fp16 operands while the workgroup multiplies the four before.
+//
+// Of a page's step 2^e f (1 <= f < 2), the power of two goes into the values' operand, relative to the largest so far, where it is exact, and f into the
+// weights, so that two pages with steps of their own fill one matrix instruction.
+// ---------------------------------------------------------------------------------------------
+constexpr int NO_EXP = -1000;                 // exponent of a step that is zero or NaN
+
+// Where a token of the pass lies: the row of position p of sequence seq, of which row t has position pos; -1: it is not in the pass
+__device__ __forceinline__ int row_of(const PageAttn& a, int t, int pos, int seq, int p) {
+  const long r = (long)t + p - pos;
+  return r >= 0 && r < a.T && p < a.max_pos && a.tok_seq[r] == seq && a.tok_pos[r] == p ? (int)r : -1;
+}
+
+// The operands of an unrounded page (tokens p0 .. p0 + 15 of seq, of which row t of the pass has position pos): from the pass's rows, and from the
+// tail what stands ahead of them.  Tokens that are in neither are zero.
+template <int D>
+__device__ __forceinline__ void load_own(const PageAttn& a, int seq, int kh, int t, int pos, f16x8 (&k)[D / 32], f16x4 (&v)[D / 16]) {
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, p0 = pos / PAGE * PAGE, HH = a.Hq + 2 * a.Hkv;
+  const int mine = row_of(a, t, pos, seq, p0 + col);        // of token col (lanes of all groups alike)
+  const size_t at = ((size_t)seq * a.Hkv + kh) * PAGE * D;
+  if (mine >= 0) {
+    const size_t p = (size_t)(p0 + col) * (D / 2);
+    load_rotated<D>(k, a.qkv + ((size_t)mine * HH + a.Hq + kh) * D, a.rope_cos + p, a.rope_sin + p, g);
+  } else {
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb) k[kb] = p0 + col < pos ? ld8(a.tail_k + at + kb * 512 + lane * 8) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = __shfl(mine, 4 * g + e, WAVE);
+    const f16* src = r >= 0 ? a.qkv + ((size_t)r * HH + a.Hq + a.Hkv + kh) * D + col : a.tail_v + at + (size_t)col * PAGE + 4 * g + e;
+    const int by = r >= 0 ? 16 : 16 * PAGE;
+    const bool there = r >= 0 || p0 + 4 * g + e < pos;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) v[db][e] = there ? src[db * by] : (f16)0.f;
+  }
+}
+
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // -126 <= e <= 127
+
+template <int D, bool Q8, int NT>
+__global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
+  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, NL = Q8 ? D / 64 : D / 32, QB = 64 * NT;
+  __shared__ __align__(16) f16 lk[2][4 * PE], lv[2][4 * PE];          // values: [pair of pages][db][lane][page of the pair][4 tokens]
+  __shared__ uint32_t odd[2][4];                                      // tokens of a page whose values are not all finite
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int h = blockIdx.x, G = a.Hq / a.Hkv, kh = h / G, HH = a.Hq + 2 * a.Hkv;
+  const int t0 = (gridDim.y - 1 - blockIdx.y) * QB, nt = min(QB, a.T - t0);
+  // where runs begin
+  unsigned long long begins[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int r = j * 64 + lane, t = t0 + r;
+    bool b = false;
+    if (r < nt) b = r == 0 || a.tok_seq[t] != a.tok_seq[t - 1] || a.tok_pos[t] != a.tok_pos[t - 1] + 1 || a.tok_pos[t] == 0;      // (0 behind -1, which is none)
+    begins[j] = __ballot(b);
+  }
+  f16x8 q[NT][NKB];
+  f32x4 o[NT][NDB];
+  float m[NT], l[NT];
+  int cpos[NT];                                                       // the column's position; -1: none
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int r = wave * 16 * NT + i * 16 + col, t = t0 + (r < nt ? r : 0);
+    const int pos = a.tok_pos[t];
+    cpos[i] = r < nt && token_ok(a, a.tok_seq[t], pos) ? pos : -1;
+    const f16* qp = a.qkv + ((size_t)t * HH + h) * D;
+    if (cpos[i] < 0) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) q[i][kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    } else if constexpr (Q8) {
+      load_rotated<D>(q[i], qp, a.rope_cos + (size_t)pos * (D / 2), a.rope_sin + (size_t)pos * (D / 2), g);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) q[i][kb] = ld8(qp + kb * 32 + g * 8);
+    }
+  }
+  int unit = NO_EXP;                                                  // o is in units of 2^unit
+
+  // scores of P pages (lane: tokens first[p] .. + 3) to weights, as two fp16 halves; lim, lo, sinks: what the column sees; fac: of a page's weights
+  auto weights = [&](int i, f32x4 (&st)[4], const float (&fac)[4], const int (&first)[4], int lim, int lo, bool edge, const uint32_t (&bad)[4], f16x8 (&hi)[2],
+                     f16x8 (&low)[2]) {
+    float pm = -INFINITY;
+    bool no[4][4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = first[p] + e;
+        no[p][e] = edge && (t >= lim || (t < lo && t >= a.sinks));
+        if (edge && (bad[p] >> (4 * g + e) & 1)) st[p][e] = NAN;
+        if (no[p][e]) st[p][e] = -INFINITY;
+        pm = fmaxf(pm, st[p][e]);
+      }
+    pm = groups_max(pm);
+    if (__any(pm > m[i])) {
+      const float mn = fmaxf(m[i], pm), alpha = __builtin_amdgcn_exp2f(m[i] - (mn == -INFINITY ? 0.f : mn));
+      l[i] *= alpha;
+      m[i] = mn;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[i][db] *= alpha;
+    }
+    const float base = m[i] == -INFINITY ? 0.f : m[i] - TOP;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float w = __builtin_amdgcn_exp2f(st[p][e] - base);
+        l[i] += w;
+        if constexpr (Q8) w = no[p][e] ? 0.f : w * fac[p];            // (a factor may be NaN)
+        const f16 x = (f16)w;
+        hi[p / 2][p % 2 * 4 + e] = x;
+        low[p / 2][p % 2 * 4 + e] = (f16)(w - (float)x);
+      }
+  };
+
+  for (int c = 0; c < nt;) {
+    int next = nt;                                                    // where the run ends
+#pragma unroll
+    for (int j = NT - 1; j >= 0; --j) {
+      const int from = c + 1 - 64 * j;
+      const unsigned long long rest = from >= 64 ? 0ull : from > 0 ? begins[j] >> from << from : begins[j];
+      if (rest) next = min(next, 64 * j + __builtin_ctzll(rest));
+    }
+    const int seq = __builtin_amdgcn_readfirstlane(a.tok_seq[t0 + c]), pc = __builtin_amdgcn_readfirstlane(a.tok_pos[t0 + c]);
+    const int c0 = c;
+    c = next;
+    if (!token_ok(a, seq, pc)) continue;
+    const int pe = min(pc + next - c0 - 1, min(a.max_pos, a.max_blocks * PAGE) - 1);
+    const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
+    // pages: those of the sinks, then those of the window
+    const int end = Q8 ? pe / PAGE : pe / PAGE + 1;
+    const int from = min(a.window > 0 && pc >= a.window ? (pc - a.window + 1) / PAGE : 0, end);
+    const int heads = a.sinks > 0 ? min((a.sinks - 1) / PAGE + 1, from) : 0;
+    const int n = heads + end - from;
+    auto page_of = [&](int i) { return i < heads ? i : from + i - heads; };
+    int lim[NT], lo[NT], least_lim[NT], most_lim[NT], least_lo[NT], most_lo[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int r = wave * 16 * NT + i * 16 + col;
+      const bool in = r >= c0 && r < next && cpos[i] >= 0;
+      lim[i] = !in ? 0 : Q8 ? cpos[i] / PAGE * PAGE : cpos[i] + 1;
+      lo[i] = in && a.window > 0 ? cpos[i] - a.window + 1 : 0;
+      int v[4] = {lim[i], lim[i], in ? lo[i] : 0x7fffffff, lo[i]};
+#pragma unroll
+      for (int s = 8; s > 0; s >>= 1) {
+        v[0] = min(v[0], __shfl_xor(v[0], s, WAVE));
+        v[1] = max(v[1], __shfl_xor(v[1], s, WAVE));
+        v[2] = min(v[2], __shfl_xor(v[2], s, WAVE));
+        v[3] = max(v[3], __shfl_xor(v[3], s, WAVE));
+      }
+      least_lim[i] = __builtin_amdgcn_readfirstlane(v[0]);
+      most_lim[i] = __builtin_amdgcn_readfirstlane(v[1]);
+      least_lo[i] = __builtin_amdgcn_readfirstlane(v[2]);
+      most_lo[i] = __builtin_amdgcn_readfirstlane(v[3]);
+    }
+    const int run_lim = Q8 ? pc / PAGE * PAGE : pc + 1, run_lo = a.window > 0 ? pe - a.window + 1 : 0;
+
+    // of the four pages on their way: a lane's id (of page lane % 4), this wave's operands; then what the block needs beside its operands
+    auto id_of = [&](int blk) {
+      const int i = 4 * blk + (lane & 3);
+      const int id = i < n ? bt[page_of(i)] : -1;
+      return id < a.n_pages ? id : -1;
+    };
+    uint4 rk[NL], rv[NL];
+    f32x2 rstep;
+    auto fetch = [&](int ids) {
+      const int id = __builtin_amdgcn_readlane(ids, wave);
+      const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh);
+      if constexpr (Q8) {
+        const uint8_t* kp = (const uint8_t*)a.k + at * PE + lane * 16;
+        const uint8_t* vp = (const uint8_t*)a.v + at * PE + lane * 16;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) rk[j] = *reinterpret_cast<const uint4*>(kp + j * 1024);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) rv[j] = *reinterpret_cast<const uint4*>(vp + j * 1024);
+        rstep = *reinterpret_cast<const f32x2*>(a.step + 2 * ((size_t)(ids < 0 ? 0 : ids) * a.Hkv + kh));
+      } else {
+        const f16* kp = (const f16*)a.k + at * PE + lane * 8;
+        const f16* vp = (const f16*)a.v + at * PE + col * PAGE + g * 4;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) rk[j] = *reinterpret_cast<const uint4*>(kp + j * 512);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          const uint2 x = *reinterpret_cast<const uint2*>(vp + (2 * j) * 16 * PAGE), y = *reinterpret_cast<const uint2*>(vp + (2 * j + 1) * 16 * PAGE);
+          rv[j] = uint4{x.x, x.y, y.x, y.y};
+        }
+      }
+    };
+    float sk[4], fac[4];                                              // of the block in LDS (uniform)
+    int there = 0, unit_next = unit;
+    auto stage = [&](int buf, int blk, int ids) {
+      there = (int)(__ballot(ids >= 0) & 15);
+      f16 by = (f16)1.f;
+      if constexpr (Q8) {
+        int ex[4];
+        float sv[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          sk[p] = a.scale * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rstep[0]), p));
+          sv[p] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rstep[1]), p));
+          const int e = (int)(__float_as_uint(sv[p]) >> 23 & 255);
+          ex[p] = (there >> p & 1) && e > 0 && e < 255 ? e - 127 : NO_EXP;
+          unit_next = max(unit_next, ex[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int k = ex[p] == NO_EXP ? 0 : max(ex[p] - unit_next, -24);       // (exact: codes have seven bits, fp16 numbers multiples of 2^-24)
+          fac[p] = ex[p] != NO_EXP ? sv[p] * power(-(unit_next + k)) : sv[p] == 0.f || !(there >> p & 1) ? 1.f : sv[p];
+          if (p == wave) by = (f16)power(k);
+        }
+      }
+      uint32_t bad = 0;
+      f16* kd = lk[buf] + wave * PE + lane * 8;
+      f16* vd = lv[buf] + ((wave >> 1) * NDB * 64 + lane) * 8 + (wave & 1) * 4;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          st8(kd + (2 * j) * 512, from_codes(rk[j].x, rk[j].y));
+          st8(kd + (2 * j + 1) * 512, from_codes(rk[j].z, rk[j].w));
+          const uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<f16x4*>(vd + (4 * j + i) * 512) = from_codes(u[i]) * f16x4{by, by, by, by};
+        }
+      } else {
+        const int first = 4 * blk + wave < n ? page_of(4 * blk + wave) * PAGE : 0;
+        // somebody may not see all of it: values that are not finite would reach those columns as well, by 0 * inf
+        const bool part = !(there >> wave & 1) || first + PAGE > run_lim || (first < run_lo && first + PAGE > a.sinks);        // uniform
+#pragma unroll
+        for (int j = 0; j < NL; ++j) *reinterpret_cast<uint4*>(kd + j * 512) = rk[j];
+        if (part) {
+          bool not_finite[4] = {};
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool x = (u[i] & 0x7c00u) == 0x7c00u, y = (u[i] & 0x7c000000u) == 0x7c000000u;
+              not_finite[2 * (i & 1)] |= x;
+              not_finite[2 * (i & 1) + 1] |= y;
+              u[i] &= (x ? 0u : 0xffffu) | (y ? 0u : 0xffff0000u);
+            }
+            rv[j] = uint4{u[0], u[1], u[2], u[3]};
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned long long b = __ballot(not_finite[e]);
+#pragma unroll
+            for (int gg = 0; gg < 4; ++gg)
+              if (b >> (16 * gg) & 0xffff) bad |= 1u << (4 * gg + e);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          *reinterpret_cast<uint2*>(vd + (2 * j) * 512) = uint2{rv[j].x, rv[j].y};
+          *reinterpret_cast<uint2*>(vd + (2 * j + 1) * 512) = uint2{rv[j].z, rv[j].w};
+        }
+        if (lane == 0) odd[buf][wave] = bad;
+      }
+    };
+
+    const int blocks = (n + 3) / 4;
+    if (blocks == 0) continue;                                        // uniform over the workgroup
+    int ids = id_of(0);
+    fetch(ids);
+    int ids_next = id_of(1);
+    __syncthreads();                                                  // (the run before may still be read)
+    stage(0, 0, ids);
+    __syncthreads();
+    for (int blk = 0; blk < blocks; ++blk) {
+      const int buf = blk & 1;
+      const int ids_then = id_of(blk + 2);
+      if (blk + 1 < blocks) fetch(ids_next);
+      if constexpr (Q8) {
+        if (unit_next != unit) {                                      // uniform
+          const float f = unit == NO_EXP ? 0.f : power(max(unit - unit_next, -126));
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[i][db] *= f;
+          unit = unit_next;
+        }
+      }
+      int first[4];
+      bool sees[NT], whole[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sees[i] = false, whole[i] = there == 15;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        first[p] = there >> p & 1 ? page_of(4 * blk + p) * PAGE : 0x3fffffff;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          sees[i] = sees[i] || (first[p] < most_lim[i] && (first[p] + PAGE > least_lo[i] || first[p] < a.sinks));
+          whole[i] = whole[i] && first[p] + PAGE <= least_lim[i] && (first[p] >= most_lo[i] || first[p] + PAGE <= a.sinks);
+        }
+        first[p] += 4 * g;
+      }
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) any = any || sees[i];
+      if (any) {                                                      // uniform over the wave
+        uint32_t bad[4] = {0, 0, 0, 0};
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) bad[p] = __builtin_amdgcn_readfirstlane(odd[buf][p]);
+          if (bad[0] | bad[1] | bad[2] | bad[3])
+#pragma unroll
+            for (int i = 0; i < NT; ++i) whole[i] = false;
+        }
+        f32x4 st[NT][4];
+        const f16* kl = lk[buf] + lane * 8;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i) st[i][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) {
+            const f16x8 k = ld8(kl + p * PE + kb * 512);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) st[i][p] = mfma_16x16x32(k, q[i][kb], st[i][p]);
+          }
+#pragma unroll
+          for (int i = 0; i < NT; ++i) st[i][p] *= Q8 ? sk[p] : a.scale;
+        }
+        f16x8 hi[NT][2], low[NT][2];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if (whole[i]) weights(i, st[i], fac, first, lim[i], lo[i], false, bad, hi[i], low[i]);
+          else weights(i, st[i], fac, first, lim[i], lo[i], true, bad, hi[i], low[i]);
+        }
+        const f16* vl = lv[buf] + lane * 8;
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair)
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            const f16x8 v = ld8(vl + (pair * NDB + db) * 512);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              o[i][db] = mfma_16x16x32(v, hi[i][pair], o[i][db]);
+              o[i][db] = mfma_16x16x32(v, low[i][pair], o[i][db]);
+            }
+          }
+      }
+      if (blk + 1 < blocks) stage(buf ^ 1, blk + 1, ids_next);
+      ids_next = ids_then;
+      __syncthreads();
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int r = wave * 16 * NT + i * 16 + col, t = t0 + (r < nt ? r : 0);
+    if constexpr (Q8) {
+      // the own pages, unrounded: those of the tile's columns one behind the other
+      const float f = unit == NO_EXP ? 1.f : power(unit);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[i][db] *= f;
+      const int seq = a.tok_seq[t], own = cpos[i] >= 0 ? cpos[i] / PAGE : -1;
+      unsigned todo = (unsigned)(__ballot(cpos[i] >= 0) & 0xffff);
+      while (todo) {
+        const int c = __builtin_ctz(todo);
+        const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(own, c), ps = __builtin_amdgcn_readlane(cpos[i], c);
+        const int row = __builtin_amdgcn_readlane(t, c);
+        const bool in = own == p && seq == s && t - row == cpos[i] - ps;        // (of the same run)
+        todo &= ~(unsigned)(__ballot(in) & 0xffff);
+        f16x8 k[NKB];
+        f16x4 v[NDB];
+        load_own<D>(a, s, kh, row, ps, k, v);
+        f32x4 st[4];
+        st[0] = st[1] = st[2] = st[3] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(k[kb], q[i][kb], st[0]);
+        st[0] *= a.scale;
+        uint32_t bad[4] = {0, 0, 0, 0};                               // tokens whose values are not finite: their scores are NaN where they are seen
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bool not_finite = false;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            const float x = (float)v[db][e];
+            const bool y = !(fabsf(x) <= 65504.f);
+            not_finite = not_finite || y;
+            if (y) v[db][e] = (f16)0.f;
+          }
+          const unsigned long long b = __ballot(not_finite);
+          if (b >> (16 * g) & 0xffff) bad[0] |= 1u << (4 * g + e);
+        }
+        const int none = 0x3fffffff;
+        const int first[4] = {p * PAGE + 4 * g, none, none, none};
+        const float one[4] = {1.f, 1.f, 1.f, 1.f};
+        f16x8 hi[2], low[2];
+        weights(i, st, one, first, in ? cpos[i] + 1 : 0, in && a.window > 0 ? cpos[i] - a.window + 1 : 0, true, bad, hi, low);
+        const f16x8 w = f16x8{hi[0][0], hi[0][1], hi[0][2], hi[0][3], low[0][0], low[0][1], low[0][2], low[0][3]};
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+          o[i][db] = mfma_16x16x32(f16x8{v[db][0], v[db][1], v[db][2], v[db][3], v[db][0], v[db][1], v[db][2], v[db][3]}, w, o[i][db]);
+      }
+    }
+    l[i] += __shfl_xor(l[i], 16, WAVE);
+    l[i] += __shfl_xor(l[i], 32, WAVE);
+    if (r >= nt) continue;
+    const float by = l[i] == 0.f ? 0.f : 1.f / l[i];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const int d = h * D + db * 16 + 4 * g;
+      f16x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = (f16)(l[i] == 0.f ? 0.f : o[i][db][e] * by);
+      *reinterpret_cast<f16x4*>(a.out + (a.frag_tt ? frag_offset(t, d, a.frag_tt) : (size_t)t * a.Hq * D + d)) = x;
+    }
+  }
+}
+
+// Pages that a pass completes, in 8 bits: a wave has 16 tokens of the pass and a kv head, and of them those that are the first of their page in the pass
+template <int D>
+__global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
+  const int lane = threadIdx.x & 63, kh = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = blockIdx.x * 16;
+  if (kh >= a.Hkv) return;
+  const int t = t0 + (lane & 15);
+  int seq = -1, pos = -1;
+  bool lead = false;
+  if (t < a.T) {
+    seq = a.tok_seq[t];
+    pos = a.tok_pos[t];
+    if (token_ok(a, seq, pos)) {
+      lead = t == 0 || pos % PAGE == 0 || a.tok_seq[t - 1] != seq || a.tok_pos[t - 1] != pos - 1;
+      lead = lead && row_of(a, t, pos, seq, pos / PAGE * PAGE + PAGE - 1) >= 0;
+    }
+  }
+  unsigned todo = (unsigned)(__ballot(lead) & 0xffff);
+  while (todo) {
+    const int c = __builtin_ctz(todo);
+    todo &= todo - 1;
+    const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(pos, c);
+    const int id = a.block_table[(size_t)s * a.max_blocks + p / PAGE];
+    if (id < 0 || id >= a.n_pages) continue;                          // uniform
+    f16x8 k[D / 32];
+    f16x4 v[D / 16];
+    load_own<D>(a, s, kh, t0 + c, p, k, v);
+    store_codes<D>(a, id, kh, k, v);
+  }
+}
+
+// The tokens of the pass that lie in their sequence's last page, into its tail: behind the launches that read what stands there
+template <int D>
+__global__ __launch_bounds__(4 * WAVE) void page_tail_kernel(PageAttn a) {
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, kh = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x * 16 + col;
+  if (kh >= a.Hkv || t >= a.T) return;
+  const int seq = a.tok_seq[t], pos = a.tok_pos[t];
+  if (!token_ok(a, seq, pos) || row_of(a, t, pos, seq, pos / PAGE * PAGE + PAGE) >= 0) return;
+  const f16* row = a.qkv + ((size_t)t * (a.Hq + 2 * a.Hkv) + a.Hq + kh) * D;
+  f16x8 k[D / 32];
+  load_rotated<D>(k, row, a.rope_cos + (size_t)pos * (D / 2), a.rope_sin + (size_t)pos * (D / 2), g);
+  const size_t at = ((size_t)seq * a.Hkv + kh) * PAGE * D;
+  const int slot = pos % PAGE;
+#pragma unroll
+  for (int kb = 0; kb < D / 32; ++kb) st8(a.tail_k + at + kb * 512 + (g * 16 + slot) * 8, k[kb]);
+  const f16* vr = row + (size_t)a.Hkv * D;
+#pragma unroll
+  for (int kb = 0; kb < D / 32; ++kb) {
+    const f16x8 v = ld8(vr + kb * 32 + g * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a.tail_v[at + (size_t)(kb * 32 + g * 8 + e) * PAGE + slot] = v[e];
+  }
+}
+
+// What pages of 8 bits stand for, as rows: a thread has eight dims of a token
+template <int D>
+__global__ __launch_bounds__(256) void page_values_kernel(f16* __restrict__ keys, f16* __restrict__ values, const uint8_t* __restrict__ k, const uint8_t* __restrict__ v,
+                                                          const float* __restrict__ step, const int32_t* __restrict__ ids, int Hkv, int n_pages) {
+  const int n = blockIdx.y, kh = blockIdx.x, id = ids[n];
+  if (id < 0 || id >= n_pages) return;
+  const size_t at = ((size_t)id * Hkv + kh), to = ((size_t)n * Hkv + kh) * PAGE * D;
+  const float sk = step[2 * at], sv = step[2 * at + 1];
+  for (int i = threadIdx.x; i < PAGE * D / 8; i += 256) {
+    const int token = i / (D / 8), d = i % (D / 8) * 8, j = d / 64;
+    const uint2 kc = *reinterpret_cast<const uint2*>(k + at * PAGE * D + j * 1024 + ((d % 32 / 8) * 16 + token) * 16 + (d % 64 / 32) * 8);
+    const f16x8 x = from_codes(kc.x, kc.y);
+    f16x8 a, b;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      a[e] = (f16)((float)x[e] * sk);
+      b[e] = (f16)((float)(int8_t)v[at * PAGE * D + j * 1024 + ((token / 4) * 16 + d % 16 + e) * 16 + (d % 64 / 16) * 4 + token % 4] * sv);
+    }
+    st8(keys + to + (size_t)token * D + d, a);
+    st8(values + to + (size_t)token * D + d, b);
+  }
+}
+
+int check(const char* who, const mlora_page_attn& p, bool rotates) {
+  if (int e = mlora_check_attn(who, p.Hq, p.Hkv, p.D, p.n_pages, p.n_seq, p.max_blocks)) return e;
+  MLORA_CHECK(p.out && p.qkv && p.k && p.v && p.block_table && p.tok_seq && p.tok_pos, MLORA_ERR_INVALID, "%s: null pointer", who);
+  MLORA_CHECK(!p.step || (p.tail_k && p.tail_v), MLORA_ERR_INVALID, "%s: pages of 8 bits without tails", who);
+  MLORA_CHECK(!rotates || (p.rope_cos && p.rope_sin), MLORA_ERR_INVALID, "%s: null pointer", who);
+  MLORA_CHECK(!rotates || (((uintptr_t)p.rope_cos | (uintptr_t)p.rope_sin) & 15) == 0, MLORA_ERR_INVALID, "%s: rotation tables not on 16 bytes", who);
+  MLORA_CHECK((((uintptr_t)p.out | (uintptr_t)p.qkv | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.tail_k | (uintptr_t)p.tail_v) & 15) == 0 && ((uintptr_t)p.step & 7) == 0,
+              MLORA_ERR_INVALID, "%s: tensors not on 16 bytes", who);
+  MLORA_CHECK(p.T >= 0 && p.max_pos > 0 && p.max_blocks <= 1 << 26, MLORA_ERR_INVALID, "%s: bad T=%d max_pos=%d max_blocks=%d", who, p.T, p.max_pos, p.max_blocks);
+  MLORA_CHECK(p.window >= 0 && p.sinks >= 0, MLORA_ERR_INVALID, "%s: a window of %d with %d sinks", who, p.window, p.sinks);
+  MLORA_CHECK(p.out_layout == MLORA_ROWMAJOR || p.out_layout == MLORA_FRAG, MLORA_ERR_INVALID, "%s: bad out_layout %d", who, p.out_layout);
+  return MLORA_OK;
+}
+
+PageAttn args_of(const mlora_page_attn& p) {
+  return PageAttn{(f16*)p.out, (const f16*)p.qkv, p.k, p.v, p.step, (f16*)p.tail_k, (f16*)p.tail_v, p.block_table, p.tok_seq, p.tok_pos, p.rope_cos, p.rope_sin,
+                  (float*)p.workspace, p.workspace ? (float*)p.workspace + (size_t)p.T * p.Hq * p.splits * p.D : nullptr, p.max_blocks, p.max_pos, p.T, p.Hq, p.Hkv, p.n_pages,
+                  p.n_seq, p.window, p.sinks, p.splits, p.out_layout == MLORA_FRAG ? mlora_frag_tiles(p.T) : 0, LOG2E / sqrtf((float)p.D)};
+}
+
+template <int D, bool Q8, int NW>
+int launch_decode(const PageAttn& a, hipStream_t s) {
+  const int G = a.Hq / a.Hkv;
+  const size_t lds = (size_t)NW * G * D * sizeof(float);
+  if constexpr (NW * 16 * D * 4 > 60 * 1024) {
+    static const hipError_t configured = hipFuncSetAttribute((const void*)page_decode_kernel<D, Q8, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, NW * 16 * D * 4);
+    if (configured != hipSuccess) return mlora_set_error(MLORA_ERR_LAUNCH, "page_attn_decode: cannot reserve LDS: %s", hipGetErrorString(configured));
+  }
+  hipLaunchKernelGGL((page_decode_kernel<D, Q8, NW>), dim3(a.Hkv, a.splits, a.T), dim3(NW * WAVE), lds, s, a);
+  return mlora_launch_status("page_attn_decode");
+}
+
+template <int D, bool Q8>
+int decode(const PageAttn& a, hipStream_t s) {
+  const long wgs = (long)a.T * a.Hkv * a.splits;
+  const int e = wgs > 2048 ? launch_decode<D, Q8, 4>(a, s) : launch_decode<D, Q8, 8>(a, s);
+  if (e || a.splits == 1) return e;
+  hipLaunchKernelGGL(page_join_kernel<D>, dim3(ceil_div(a.Hq, 4), a.T), dim3(4 * WAVE), 0, s, a);
+  return mlora_launch_status("page_attn_decode");
+}
+
+template <int D>
+int prefill(const PageAttn& a, hipStream_t s) {
+  const dim3 tiles(ceil_div(a.T, 16), ceil_div(a.Hkv, 4));
+  if (a.step) {
+    hipLaunchKernelGGL(page_store_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
+    if (int e = mlora_launch_status("page_attn_prefill")) return e;
+    hipLaunchKernelGGL((page_prefill_kernel<D, true, 2>), dim3(a.Hq, ceil_div(a.T, 128)), dim3(4 * WAVE), 0, s, a);
+    if (int e = mlora_launch_status("page_attn_prefill")) return e;
+    hipLaunchKernelGGL(page_tail_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((page_prefill_kernel<D, false, 2>), dim3(a.Hq, ceil_div(a.T, 128)), dim3(4 * WAVE), 0, s, a);
+  }
+  return mlora_launch_status("page_attn_prefill");
+}
+
+}  // namespace
+
+extern "C" int mlora_page_attn_splits(int T, int Hkv, int pages) {
+  if (T <= 0 || Hkv <= 0) return 1;
+  const long wgs = (long)T * Hkv;
+  long n = (512 + wgs - 1) / wgs;
+  n = n < pages / 16 ? n : pages / 16;
+  return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+}
+
+extern "C" size_t mlora_page_attn_workspace_bytes(int T, int Hq, int D, int splits) {
+  return T <= 0 || Hq <= 0 || D <= 0 || splits <= 1 ? 0 : (size_t)T * Hq * splits * (D + 2) * sizeof(float);
+}
+
+extern "C" int mlora_page_attn_decode(const mlora_page_attn* args, void* stream) {
+  MLORA_CHECK(args, MLORA_ERR_INVALID, "page_attn_decode: null pointer");
+  const mlora_page_attn& p = *args;
+  if (int e = check("page_attn_decode", p, true)) return e;
+  MLORA_CHECK(p.T <= 65535 && p.splits >= 1 && p.splits <= 64, MLORA_ERR_INVALID, "page_attn_decode: %d sequences in %d shares", p.T, p.splits);
+  MLORA_CHECK(p.Hq / p.Hkv <= 16, MLORA_ERR_UNSUPPORTED, "page_attn_decode: more than 16 query heads per kv head (%d)", p.Hq / p.Hkv);
+  if (p.T == 0) return MLORA_OK;
+  const size_t need = mlora_page_attn_workspace_bytes(p.T, p.Hq, p.D, p.splits);
+  MLORA_CHECK(need == 0 || (p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need), MLORA_ERR_WORKSPACE,
+              "page_attn_decode: workspace of %zu bytes, %zu needed", p.workspace_bytes, need);
+  const PageAttn a = args_of(p);
+  hipStream_t s = (hipStream_t)stream;
+  if (p.D == 128) return p.step ? decode<128, true>(a, s) : decode<128, false>(a, s);
+  return p.step ? decode<64, true>(a, s) : decode<64, false>(a, s);
+}
+
+extern "C" int mlora_page_attn_prefill(const mlora_page_attn* args, void* stream) {
+  MLORA_CHECK(args, MLORA_ERR_INVALID, "page_attn_prefill: null pointer");
+  const mlora_page_attn& p = *args;
+  if (int e = check("page_attn_prefill", p, p.step != nullptr)) return e;
+  MLORA_CHECK(p.T <= 1 << 22 && p.Hkv <= 4 * 65535, MLORA_ERR_UNSUPPORTED, "page_attn_prefill: %d tokens", p.T);
+  if (p.T == 0) return MLORA_OK;
+  const PageAttn a = args_of(p);
+  return p.D == 128 ? prefill<128>(a, (hipStream_t)stream) : prefill<64>(a, (hipStream_t)stream);
+}
+
+extern "C" int mlora_page_values(void* keys, void* values, const void* k, const void* v, const float* step, const int32_t* ids, int n, int Hkv, int D, int n_pages,
+                                 void* stream) {
+  MLORA_CHECK(D == 64 || D == 128, MLORA_ERR_UNSUPPORTED, "page_values: head_dim %d not in {64, 128}", D);
+  MLORA_CHECK(keys && values && k && v && step && (ids || n == 0), MLORA_ERR_INVALID, "page_values: null pointer");
+  MLORA_CHECK(n >= 0 && n <= 65535 && Hkv > 0 && n_pages > 0, MLORA_ERR_INVALID, "page_values: %d pages of %d under %d heads", n, n_pages, Hkv);
+  if (n == 0) return MLORA_OK;
+  const dim3 grid(Hkv, n);
+  if (D == 128) hipLaunchKernelGGL(page_values_kernel<128>, grid, dim3(256), 0, (hipStream_t)stream, (f16*)keys, (f16*)values, (const uint8_t*)k, (const uint8_t*)v, step, ids, Hkv, n_pages);
+  else hipLaunchKernelGGL(page_values_kernel<64>, grid, dim3(256), 0, (hipStream_t)stream, (f16*)keys, (f16*)values, (const uint8_t*)k, (const uint8_t*)v, step, ids, Hkv, n_pages);
+  return mlora_launch_status("page_values");
+}

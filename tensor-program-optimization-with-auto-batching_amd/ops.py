@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import struct
+import typing
 
 import torch
 
@@ -15,6 +16,8 @@ from . import _lib
 from ._lib import F16, F32, ROWMAJOR, FRAG, STORE, ACCUMULATE, GLU_SILU, GLU_CLIPPED, lib
 
 _BUCKET = struct.Struct("@PPiif4x")          # mlora_lora_bucket
+_PAGE_ATTN = struct.Struct("@13PN12i")       # mlora_page_attn
+_PAGE_POOL = struct.Struct("@Plii")          # mlora_page_pool
 _LIB_OF = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}
 
 
@@ -1157,3 +1160,231 @@ def paged_attn_prefill(qkv, k_cache, v_cache, block_table, tok_seq, tok_pos, Hq,
                                          _dev(tok_seq, torch.int32), _dev(tok_pos, torch.int32), T, Hq, Hkv, D,
                                          k_cache.shape[0], n_seq, _stream()))
     return out
+
+
+class QuantPages:
+    """A layer's pages of a paged cache in 8 bits, a step per page and head for keys and for values, with every sequence's last page unrounded (layouts and
+    rounding: mlora_page_attn in include/mlora.h).  k [n_pages, Hkv, D / 64, 4, 16, 2, 8] and v [n_pages, Hkv, D / 64, 4, 16, 4, 4] int8, step [n_pages, Hkv, 2] fp32,
+    tail_k [slots, Hkv, D / 32, 4, 16, 8] and tail_v [slots, Hkv, D, 16] fp16: a slot for every row of the block table.  The tensors are the caller's."""
+
+    def __init__(self, k, v, step, tail_k, tail_v):
+        if k.dim() != 7 or tail_v.dim() != 4:
+            raise ValueError(f"QuantPages: k{tuple(k.shape)} tail_v{tuple(tail_v.shape)}")
+        self.n_pages, self.Hkv, self.D, self.slots = k.shape[0], k.shape[1], 64 * k.shape[2], tail_v.shape[0]
+        n, H, J, S = self.n_pages, self.Hkv, k.shape[2], self.slots
+        given = {"k": (k, torch.int8, (n, H, J, 4, 16, 2, 8)), "v": (v, torch.int8, (n, H, J, 4, 16, 4, 4)), "step": (step, torch.float32, (n, H, 2)),
+                 "tail_k": (tail_k, torch.float16, (S, H, 2 * J, 4, 16, 8)), "tail_v": (tail_v, torch.float16, (S, H, 64 * J, 16))}
+        self.device = k.device
+        for name, (t, dt, shape) in given.items():
+            if t.dtype is not dt:
+                raise TypeError(f"QuantPages: {name} must be {dt}, got {t.dtype}")
+            if t.shape != shape or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"QuantPages: {name}{tuple(t.shape)} on {t.device}, expected {shape} on {self.device}, contiguous")
+            setattr(self, name, t)
+
+    @classmethod
+    def empty(cls, n_pages, slots, Hkv, D, device):
+        """Pages that hold nothing yet."""
+        if D % 64:
+            raise ValueError(f"QuantPages: head_dim {D} is not a multiple of 64")
+        z = lambda shape, dt: torch.zeros(shape, dtype=dt, device=device)                                          # noqa: E731
+        return cls(z((n_pages, Hkv, D // 64, 4, 16, 2, 8), torch.int8), z((n_pages, Hkv, D // 64, 4, 16, 4, 4), torch.int8), z((n_pages, Hkv, 2), torch.float32),
+                   z((slots, Hkv, D // 32, 4, 16, 8), torch.float16), z((slots, Hkv, D, 16), torch.float16))
+
+    def values(self, ids):
+        """(keys, values) [n, Hkv, 16, D] fp16: what pages ids [n] int32 stand for (an id that is no page leaves its rows as they come)."""
+        dev = _here(self.device, "QuantPages.values")
+        if ids.dim() != 1 or ids.device != dev:
+            raise ValueError(f"QuantPages.values: ids{tuple(ids.shape)} on {ids.device}")
+        n, p = ids.shape[0], _dev(ids, torch.int32, "ids")
+        shape, stride = (n, self.Hkv, 16, self.D), (self.Hkv * 16 * self.D, 16 * self.D, self.D, 1)
+        keys, values = (_empty_strided_cuda(shape, stride, torch.float16) for _ in range(2))
+        for i in range(0, n, 65535):                                     # (a launch's)
+            m = min(n - i, 65535)
+            check(lib().mlora_page_values(keys[i:].data_ptr(), values[i:].data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.step.data_ptr(), p + 4 * i, m, self.Hkv,
+                                          self.D, self.n_pages, _stream()))
+        return keys, values
+
+
+def _window(who, window, sinks):
+    if window is None and not sinks:
+        return 0, 0
+    if window is None or not 1 <= window <= 0x7fffffff or not 0 <= sinks <= 0x7fffffff:
+        raise ValueError(f"{who}: a window of {window} tokens with {sinks} sinks")
+    return int(window), int(sinks)
+
+
+_NO_ROPE = (None, None)
+
+
+def _page_attn(who, fn, qkv, k, v, quant, block_table, tok_seq, tok_pos, rope, Hq, Hkv, D, window, sinks, out, frag, longest):
+    """The call behind attention over pages that k and v name; longest < 0: a prompt."""
+    T, (n_seq, max_blocks), dev = qkv.shape[0], block_table.shape, _here(qkv.device, who)
+    window, sinks = _window(who, window, sinks)
+    n_pages = k.shape[0]
+    if qkv.numel() != T * (Hq + 2 * Hkv) * D or tok_seq.shape != (T,) or tok_pos.shape != (T,):
+        raise ValueError(f"{who}: qkv{tuple(qkv.shape)} for {T} x {Hq + 2 * Hkv} x {D}, rows{tuple(tok_seq.shape)} positions{tuple(tok_pos.shape)}")
+    cos, sin = rope
+    f16, i32, max_pos = torch.float16, torch.int32, 0x7fffffff
+    tensors = [(qkv, f16, "qkv"), (block_table, i32, "block_table"), (tok_seq, i32, "rows"), (tok_pos, i32, "positions")]
+    if cos is not None:
+        max_pos = cos.shape[0]
+        if cos.shape != (max_pos, D // 2) or sin.shape != cos.shape:
+            raise ValueError(f"{who}: rotation tables {tuple(cos.shape)} and {tuple(sin.shape)} for head_dim {D}")
+        tensors += [(cos, torch.float32, "rope_cos"), (sin, torch.float32, "rope_sin")]
+    if quant is not None:
+        if (quant.Hkv, quant.D) != (Hkv, D) or quant.slots < n_seq or quant.device != dev:
+            raise ValueError(f"{who}: pages of {quant.Hkv} heads of {quant.D} with {quant.slots} slots on {quant.device} for {Hkv} of {D}, {n_seq} rows of the table, on {dev}")
+        step, tail_k, tail_v = quant.step.data_ptr(), quant.tail_k.data_ptr(), quant.tail_v.data_ptr()
+    else:
+        if D % 32 or k.shape != (n_pages, Hkv, D // 32, 4, 16, 8) or v.shape != (n_pages, Hkv, D, 16):
+            raise ValueError(f"{who}: k{tuple(k.shape)} v{tuple(v.shape)} for {Hkv} heads of {D}")
+        tensors += [(k, f16, "k_cache"), (v, f16, "v_cache")]
+        step = tail_k = tail_v = 0
+    for t, dt, name in tensors:
+        if t.dtype is not dt or t.device != dev or not t.is_contiguous():
+            _dev(t, dt, name)                                            # (says which)
+            raise ValueError(f"{who}: {name} on {t.device}, others on {dev}")
+    if out is None and not frag:
+        out, lay = _empty_strided_cuda((T, Hq * D), (Hq * D, 1), f16), ROWMAJOR
+        optr = out.data_ptr()
+    else:
+        if out is not None and (tuple(out.shape) != (T, Hq * D) or isinstance(out, FragActivation) != frag or out.device != dev):
+            raise ValueError(f"{who}: out{tuple(out.shape)} on {out.device}")
+        out, optr, lay = _out_arg(out, T, Hq * D, frag, dev)
+    if T == 0:
+        return out
+    splits, ws, nb = 1, 0, 0
+    if longest >= 0:
+        pages = max_blocks if longest == 0 else min(-(-longest // 16), max_blocks)
+        if window:
+            pages = min(pages, (window + 30) // 16 + (sinks + 15) // 16)
+        splits = _size(f16, "mlora_page_attn_splits", T, Hkv, pages)
+        if splits > 1:
+            nb = _size(f16, "mlora_page_attn_workspace_bytes", T, Hq, D, splits)
+            w = _empty_strided_cuda((nb // 4,), (1,), torch.float32)
+            ws = w.data_ptr()
+    args = _PAGE_ATTN.pack(optr, qkv.data_ptr(), k.data_ptr(), v.data_ptr(), step, tail_k, tail_v, block_table.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(),
+                           0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), ws, nb, lay, max_blocks, max_pos, T, Hq, Hkv, D, n_pages, n_seq,
+                           window, sinks, splits)
+    code = getattr(lib(), fn)(args, _stream())
+    if code:
+        check(code)
+    return out
+
+
+def rope_attn_decode_q8(qkv, pages: QuantPages, block_table, seq_ids, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, longest=None, out=None, frag=False):
+    """One token of each of T different sequences on pages of 8 bits: q and k are rotated, the token's k and v stored (its page rounded to 8 bits, where it completes it),
+    and the token attends to its own page unrounded and to those ahead of it.  qkv is left as it is.  window: only the last so many tokens are seen, the
+    token itself among them, and the first `sinks`.  longest: most tokens of a row, its new one among them; it chooses how the work is cut (None: as many as the table holds)."""
+    return _page_attn("rope_attn_decode_q8", "mlora_page_attn_decode", qkv, pages.k, pages.v, pages, block_table, seq_ids, tok_pos, (rope_cos, rope_sin), Hq, Hkv, D, window,
+                      sinks, out, frag, longest or 0)
+
+
+def rope_attn_prefill_q8(qkv, pages: QuantPages, block_table, tok_seq, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, out=None, frag=False):
+    """`rope_attn_decode_q8` for the tokens of a pass, those of a sequence consecutive with increasing positions: the same results however a prompt is cut into passes, up to
+    the order of sums."""
+    return _page_attn("rope_attn_prefill_q8", "mlora_page_attn_prefill", qkv, pages.k, pages.v, pages, block_table, tok_seq, tok_pos, (rope_cos, rope_sin), Hq, Hkv, D, window,
+                      sinks, out, frag, -1)
+
+
+def rope_attn_decode_window(qkv, k_cache, v_cache, block_table, seq_ids, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, longest=None, out=None, frag=False):
+    """`rope_attn_decode` under a sliding window with sinks, and with long contexts shared out over the device (arguments as for `rope_attn_decode_q8`)."""
+    return _page_attn("rope_attn_decode_window", "mlora_page_attn_decode", qkv, k_cache, v_cache, None, block_table, seq_ids, tok_pos, (rope_cos, rope_sin), Hq, Hkv, D, window,
+                      sinks, out, frag, longest or 0)
+
+
+def paged_attn_prefill_window(qkv, k_cache, v_cache, block_table, tok_seq, tok_pos, Hq, Hkv, D, window=None, sinks=0, out=None, frag=False):
+    """`paged_attn_prefill` under a sliding window with sinks: behind `rope_kv_append` of the same tokens."""
+    return _page_attn("paged_attn_prefill_window", "mlora_page_attn_prefill", qkv, k_cache, v_cache, None, block_table, tok_seq, tok_pos, _NO_ROPE, Hq, Hkv, D, window, sinks,
+                      out, frag, -1)
+
+
+def copy_pages(pools, src, dst):
+    """Rows src [n] int32 of pools [layers, rows, ...] (contiguous tensors of any type, up to 8) go to rows dst [n], in every layer, in one launch.  A row that is written is in
+    no other pair; indices that are no row copy nothing."""
+    pools = list(pools)
+    if not 1 <= len(pools) <= 8 or any(p.dim() < 2 for p in pools):
+        raise ValueError(f"copy_pages: {[tuple(p.shape) for p in pools]}: one to eight pools of [layers, rows, ...]")
+    dev = _here(pools[0].device, "copy_pages")
+    if src.dim() != 1 or src.shape != dst.shape or src.device != dev or dst.device != dev:
+        raise ValueError(f"copy_pages: src{tuple(src.shape)} on {src.device}, dst{tuple(dst.shape)} on {dst.device}, pools on {dev}")
+    n, ps, pd, args = src.shape[0], _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst"), b""
+    for p in pools:
+        if p.device != dev:
+            raise ValueError(f"copy_pages: a pool on {p.device}, others on {dev}")
+        at, (layers, rows), size = _dev(p, None, "pool"), p.shape[:2], p.element_size()
+        if not p.numel():
+            raise ValueError(f"copy_pages: a pool{tuple(p.shape)} without elements")
+        args += _PAGE_POOL.pack(at, p.stride(1) * size if rows > 1 else p.numel() // layers * size, layers, rows)
+    if n:
+        L = _lib.loaded()
+        code = L.mlora_copy_pages(args, len(pools), ps, pd, n, _stream())
+        if code:
+            raise _lib.MloraError(code, L.mlora_last_error().decode())
+
+
+def beam_select(logits, scores, ended=None, eos=None, k=None):
+    """The k (None: as many as beams) best continuations of R requests of W beams each: of beam b by token v with value scores[b] + logits[b, v] - logsumexp(logits[b]).
+    logits [R * W, V] fp32 (any row stride), scores [R, W] fp32 (-inf: no beam there).  ended [R, W] int32: such a beam goes on with `eos` alone, at its score.
+    -> scores [R, k] fp32, tokens [R, k], parents [R, k] int32 (the beam within its request), the best first, of equal values the lower beam and token;
+    -inf, -1, -1 where candidates run out."""
+    (N, V), (R, W) = logits.shape, scores.shape
+    dev = _here(logits.device, "beam_select")
+    k = W if k is None else k
+    ld, inner = logits.stride()
+    if logits.dtype is not torch.float32 or (inner != 1 and V > 1) or (ld < V and N > 1):
+        raise ValueError("beam_select: logits must be fp32 rows with unit inner stride")
+    if N != R * W or scores.device != dev or ended is not None and (ended.shape != (R, W) or ended.device != dev or eos is None):
+        raise ValueError(f"beam_select: logits{tuple(logits.shape)} scores{tuple(scores.shape)} ended{None if ended is None else tuple(ended.shape)} eos={eos}")
+    if ended is not None and not 0 <= eos < V:
+        raise ValueError(f"beam_select: eos={eos} of {V} tokens")
+    p_scores, p_ended = _dev(scores, torch.float32, "scores"), None if ended is None else _dev(ended, torch.int32, "ended")
+    best = _empty_strided_cuda((R, k), (k, 1), torch.float32)
+    tokens, parents = _empty_strided_cuda((R, k), (k, 1), torch.int32), _empty_strided_cuda((R, k), (k, 1), torch.int32)
+    if R == 0:
+        return best, tokens, parents
+    L = _lib.loaded()
+    nb = _beam_bytes(R, W, V, k)
+    ws = _empty_strided_cuda((nb // 8,), (1,), torch.int64)
+    code = L.mlora_beam_select(best.data_ptr(), tokens.data_ptr(), parents.data_ptr(), logits.data_ptr(), ld if N > 1 else max(V, ld), p_scores, p_ended,
+                               -1 if eos is None else eos, R, W, V, k, ws.data_ptr(), nb, _stream())
+    if code:
+        raise _lib.MloraError(code, L.mlora_last_error().decode())
+    return best, tokens, parents
+
+
+@functools.lru_cache(maxsize=256)
+def _beam_bytes(R, W, V, k):
+    return _lib.loaded().mlora_beam_select_workspace_bytes(R, W, V, k)
+
+
+class BeamMoves(typing.NamedTuple):
+    """What is to be copied behind a reordering, [R * W] int32 each, -1 for nothing: the contents of slots, and of last pages (for `copy_pages`)."""
+    src_slot: torch.Tensor
+    dst_slot: torch.Tensor
+    src_page: torch.Tensor
+    dst_page: torch.Tensor
+
+
+def beam_reorder(parents, slots, block_table, tok_pos):
+    """Where beams go on whose parents [R, W] int32 `beam_select` has chosen: slots [R * W] int32, the rows of block_table that the beams have, become those returned: a
+    parent's first child keeps its slot, further children take those of beams without any, whose rows of the table are changed to the parent's pages up to
+    that of the token appended last (tok_pos [R * W] int32).  -> (slots, BeamMoves): the last pages, and what else a slot holds, are to be copied by the moves."""
+    dev = _here(parents.device, "beam_reorder")
+    if parents.dim() != 2 or block_table.dim() != 2 or slots.shape != (parents.numel(),) or tok_pos.shape != slots.shape:
+        raise ValueError(f"beam_reorder: parents{tuple(parents.shape)} slots{tuple(slots.shape)} table{tuple(block_table.shape)} positions{tuple(tok_pos.shape)}")
+    ptrs = []
+    for t, name in ((parents, "parents"), (slots, "slots"), (block_table, "block_table"), (tok_pos, "tok_pos")):
+        if t.device != dev:
+            raise ValueError(f"beam_reorder: {name} on {t.device}, others on {dev}")
+        ptrs.append(_dev(t, torch.int32, name))
+    R, W = parents.shape
+    N = R * W
+    new = _empty_strided_cuda((5, N), (N, 1), torch.int32)
+    if N:
+        at, L = new.data_ptr(), _lib.loaded()
+        code = L.mlora_beam_reorder(at, at + 4 * N, at + 8 * N, at + 12 * N, at + 16 * N, *ptrs, R, W, *block_table.shape, _stream())
+        if code:
+            raise _lib.MloraError(code, L.mlora_last_error().decode())
+    return new[0], BeamMoves(new[1], new[2], new[3], new[4])
