@@ -437,10 +437,11 @@ int mlora_paged_attn_decode_shared(void* out, int out_layout, const void* qkv, c
  * range sees nothing (the result is 0) and is not stored.
  *
  * mlora_page_attn_decode: T single tokens of different sequences: rotates q and k (qkv stays as it is), puts the token's k and v in its place - completing its page, where
- * it is the last -, attends.  The work of a row is cut into `splits` shares (mlora_page_attn_splits names a good number for rows of up to `pages` visible pages);
- * with more than one: workspace of mlora_page_attn_workspace_bytes, 16-byte aligned, and a second launch.  Hq / Hkv <= 16.
+ * it is the last -, attends.  Hq / Hkv <= 16.
  * mlora_page_attn_prefill: T tokens of a pass, those of a sequence consecutive with increasing positions.  Pages of 8 bits: rotates, stores and attends, as above
- * (three launches).  fp16 pages: as mlora_paged_attn_prefill, on rotated queries and stored keys (rope_cos, rope_sin unused). */
+ * (three launches).  fp16 pages: as mlora_paged_attn_prefill, on rotated queries and stored keys (rope_cos, rope_sin unused).  Hq / Hkv <= 64.
+ * The pages that a token sees are cut into `splits` shares, 1 .. 64 (mlora_page_attn_splits names a good number, of tokens that see up to `pages` pages); with more than
+ * one: workspace of mlora_page_attn_workspace_bytes, 16-byte aligned, and one launch more. */
 typedef struct {
   void* out;
   const void* qkv;
@@ -453,7 +454,7 @@ typedef struct {
   size_t workspace_bytes;
   int out_layout, max_blocks, max_pos, T, Hq, Hkv, D, n_pages, n_seq, window, sinks, splits;
 } mlora_page_attn;
-int mlora_page_attn_splits(int T, int Hkv, int pages);
+int mlora_page_attn_splits(int prompt, int T, int Hq, int Hkv, int pages);
 size_t mlora_page_attn_workspace_bytes(int T, int Hq, int D, int splits);
 int mlora_page_attn_decode(const mlora_page_attn* host_args, void* stream);
 int mlora_page_attn_prefill(const mlora_page_attn* host_args, void* stream);

@@ -92,7 +92,7 @@ SIGNATURES = {
     "mlora_argmax": (_i, [_p, _p, _i, _i, _p]),
     "mlora_rope_kv_append": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p]),
     "mlora_paged_attn_decode": (_i, [_p, _i, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
-    "mlora_page_attn_splits": (_i, [_i, _i, _i]),
+    "mlora_page_attn_splits": (_i, [_i, _i, _i, _i, _i]),
     "mlora_page_attn_workspace_bytes": (_z, [_i, _i, _i, _i]),
     "mlora_page_attn_decode": (_i, [_p, _p]),
     "mlora_page_attn_prefill": (_i, [_p, _p]),

@@ -64,41 +64,58 @@ __device__ __forceinline__ f16x4 from_codes(uint32_t a) {
   return x.h - f16x4{c, c, c, c};
 }
 
-// A head row of a token as the lane (group g) of an operand holds it - dims 32 kb + 8 g .. + 7 -, rotated.  Separately rounded products, as in
-// attention.hip: the keys are those of the fp16 cache bit for bit.  (Both elements of a pair are the lane's own.)
+// Eight pairs (x, y) of a head row, rotated.  Separately rounded products, as in attention.hip: the keys are those of the fp16 cache bit for bit.
+__device__ __forceinline__ void rotate8(f16x8& x, f16x8& y, const float* __restrict__ c, const float* __restrict__ s) {
+  const f32x4 c0 = *reinterpret_cast<const f32x4*>(c), c1 = *reinterpret_cast<const f32x4*>(c + 4);
+  const f32x4 s0 = *reinterpret_cast<const f32x4*>(s), s1 = *reinterpret_cast<const f32x4*>(s + 4);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float cc = e < 4 ? c0[e & 3] : c1[e & 3], ss = e < 4 ? s0[e & 3] : s1[e & 3], a = (float)x[e], b = (float)y[e];
+    float r1, r2;
+    {
+#pragma clang fp contract(off)
+      r1 = a * cc - b * ss;
+      r2 = b * cc + a * ss;
+    }
+    asm volatile("" : "+v"(r1), "+v"(r2));                 // the fp32 result exists before the conversion
+    x[e] = (f16)r1;
+    y[e] = (f16)r2;
+  }
+}
+
+// A head row of a token as the lane (group g) of an operand holds it - dims 32 kb + 8 g .. + 7 -, rotated: both elements of a pair are the lane's own
 template <int D>
 __device__ __forceinline__ void load_rotated(f16x8 (&x)[D / 32], const f16* __restrict__ row, const float* __restrict__ c, const float* __restrict__ s, int g) {
   constexpr int H = D / 64;
 #pragma unroll
   for (int kb = 0; kb < D / 32; ++kb) x[kb] = ld8(row + kb * 32 + g * 8);
 #pragma unroll
-  for (int kb = 0; kb < H; ++kb) {
-    const float* cp = c + kb * 32 + g * 8;
-    const float* sp = s + kb * 32 + g * 8;
-    const f32x4 c0 = *reinterpret_cast<const f32x4*>(cp), c1 = *reinterpret_cast<const f32x4*>(cp + 4);
-    const f32x4 s0 = *reinterpret_cast<const f32x4*>(sp), s1 = *reinterpret_cast<const f32x4*>(sp + 4);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float cc = e < 4 ? c0[e & 3] : c1[e & 3], ss = e < 4 ? s0[e & 3] : s1[e & 3], a = (float)x[kb][e], b = (float)x[kb + H][e];
-      float r1, r2;
-      {
-#pragma clang fp contract(off)
-        r1 = a * cc - b * ss;
-        r2 = b * cc + a * ss;
-      }
-      asm volatile("" : "+v"(r1), "+v"(r2));               // the fp32 result exists before the conversion
-      x[kb][e] = (f16)r1;
-      x[kb + H][e] = (f16)r2;
-    }
-  }
+  for (int kb = 0; kb < H; ++kb) rotate8(x[kb], x[kb + H], c + kb * 32 + g * 8, s + kb * 32 + g * 8);
 }
 
 __device__ __forceinline__ bool token_ok(const PageAttn& a, int seq, int pos) {
   return seq >= 0 && seq < a.n_seq && pos >= 0 && pos < a.max_pos && pos / PAGE < a.max_blocks;
 }
 
-__device__ __forceinline__ int8_t code_of(float x, float most) {
-  return (int8_t)(int)rintf(127.f * x / most);
+// How a page's keys or values are rounded, of which a wave holds all
+struct Rounding {
+  float most, step;                                        // infinite: codes 0
+  __device__ __forceinline__ int8_t code(float x) const { return (int8_t)(int)rintf(127.f * (most == INFINITY ? 0.f : x) / most); }
+};
+template <class T, int N>
+__device__ __forceinline__ Rounding rounding_of(const T (&x)[N]) {
+  float most = 0.f, odd = 0.f;                             // odd: x - x, which is zero but for infinities and NaN
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < (int)(sizeof(T) / 2); ++e) {
+      const float y = (float)x[i][e];
+      most = fmaxf(most, fabsf(y));
+      odd += y - y;
+    }
+  most = wave_max(most);
+  const bool bad = __any(odd != 0.f);
+  return Rounding{most > 0.f && !bad ? most : INFINITY, bad ? NAN : most / 127.f};
 }
 
 // A whole page of a head from a wave's operands - keys: lane (g, token) dims 32 kb + 8 g ..; values: lane (g, col) tokens 4 g .. of dims 16 db + col -
@@ -106,27 +123,7 @@ __device__ __forceinline__ int8_t code_of(float x, float most) {
 template <int D>
 __device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh, const f16x8 (&k)[D / 32], const f16x4 (&v)[D / 16]) {
   const int lane = threadIdx.x & 63;
-  float mk = 0.f, mv = 0.f, odd_k = 0.f, odd_v = 0.f;       // odd: x - x, which is zero but for infinities and NaN
-#pragma unroll
-  for (int kb = 0; kb < D / 32; ++kb)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = (float)k[kb][e];
-      mk = fmaxf(mk, fabsf(x));
-      odd_k += x - x;
-    }
-#pragma unroll
-  for (int db = 0; db < D / 16; ++db)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = (float)v[db][e];
-      mv = fmaxf(mv, fabsf(x));
-      odd_v += x - x;
-    }
-  mk = wave_max(mk);
-  mv = wave_max(mv);
-  const bool bad_k = __any(odd_k != 0.f), bad_v = __any(odd_v != 0.f);
-  const float dk = mk > 0.f && !bad_k ? mk : INFINITY, dv = mv > 0.f && !bad_v ? mv : INFINITY;      // (x / inf: codes 0)
+  const Rounding rk = rounding_of(k), rv = rounding_of(v);
   uint8_t* kp = (uint8_t*)a.k + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 16;
   uint8_t* vp = (uint8_t*)a.v + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 16;
 #pragma unroll
@@ -134,14 +131,13 @@ __device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh,
     union { int8_t b[16]; uint4 u; } x, y;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      x.b[e] = code_of(bad_k ? 0.f : (float)k[2 * j + e / 8][e % 8], dk);
-      y.b[e] = code_of(bad_v ? 0.f : (float)v[4 * j + e / 4][e % 4], dv);
+      x.b[e] = rk.code((float)k[2 * j + e / 8][e % 8]);
+      y.b[e] = rv.code((float)v[4 * j + e / 4][e % 4]);
     }
     *reinterpret_cast<uint4*>(kp + j * 1024) = x.u;
     *reinterpret_cast<uint4*>(vp + j * 1024) = y.u;
   }
-  if (lane == 0)
-    *reinterpret_cast<f32x2*>(a.step + 2 * ((size_t)page * a.Hkv + kh)) = f32x2{bad_k ? NAN : mk / 127.f, bad_v ? NAN : mv / 127.f};
+  if (lane == 0) *reinterpret_cast<f32x2*>(a.step + 2 * ((size_t)page * a.Hkv + kh)) = f32x2{rk.step, rv.step};
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -447,45 +443,113 @@ __device__ __forceinline__ int row_of(const PageAttn& a, int t, int pos, int seq
   return r >= 0 && r < a.T && p < a.max_pos && a.tok_seq[r] == seq && a.tok_pos[r] == p ? (int)r : -1;
 }
 
-// The operands of an unrounded page (tokens p0 .. p0 + 15 of seq, of which row t of the pass has position pos): from the pass's rows, and from the
-// tail what stands ahead of them.  Tokens that are in neither are zero.
+// The rows of an unrounded page (tokens p0 .. p0 + 15 of seq, of which row t of the pass has position pos), lane (g, token) with dims 32 kb + 8 g .. + 7 of
+// its token: from the pass's rows, and from the tail what stands ahead of them.  Tokens that are in neither are zero.
 template <int D>
-__device__ __forceinline__ void load_own(const PageAttn& a, int seq, int kh, int t, int pos, f16x8 (&k)[D / 32], f16x4 (&v)[D / 16]) {
+__device__ __forceinline__ void load_own(const PageAttn& a, int seq, int kh, int t, int pos, f16x8 (&k)[D / 32], f16x8 (&v)[D / 32]) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, p0 = pos / PAGE * PAGE, HH = a.Hq + 2 * a.Hkv;
-  const int mine = row_of(a, t, pos, seq, p0 + col);        // of token col (lanes of all groups alike)
+  const int mine = row_of(a, t, pos, seq, p0 + col);
   const size_t at = ((size_t)seq * a.Hkv + kh) * PAGE * D;
   if (mine >= 0) {
     const size_t p = (size_t)(p0 + col) * (D / 2);
-    load_rotated<D>(k, a.qkv + ((size_t)mine * HH + a.Hq + kh) * D, a.rope_cos + p, a.rope_sin + p, g);
+    const f16* row = a.qkv + ((size_t)mine * HH + a.Hq + kh) * D;
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb) v[kb] = ld8(row + (size_t)a.Hkv * D + kb * 32 + g * 8);
+    load_rotated<D>(k, row, a.rope_cos + p, a.rope_sin + p, g);
+  } else if (p0 + col < pos) {
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb) {
+      k[kb] = ld8(a.tail_k + at + kb * 512 + lane * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[kb][e] = a.tail_v[at + (size_t)(kb * 32 + g * 8 + e) * PAGE + col];
+    }
   } else {
 #pragma unroll
-    for (int kb = 0; kb < D / 32; ++kb) k[kb] = p0 + col < pos ? ld8(a.tail_k + at + kb * 512 + lane * 8) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int r = __shfl(mine, 4 * g + e, WAVE);
-    const f16* src = r >= 0 ? a.qkv + ((size_t)r * HH + a.Hq + a.Hkv + kh) * D + col : a.tail_v + at + (size_t)col * PAGE + 4 * g + e;
-    const int by = r >= 0 ? 16 : 16 * PAGE;
-    const bool there = r >= 0 || p0 + 4 * g + e < pos;
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) v[db][e] = there ? src[db * by] : (f16)0.f;
+    for (int kb = 0; kb < D / 32; ++kb) k[kb] = v[kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
 
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // -126 <= e <= 127
 
-template <int D, bool Q8, int NT>
-__global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
-  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, NL = Q8 ? D / 64 : D / 32, QB = 64 * NT;
-  __shared__ __align__(16) f16 lk[2][4 * PE], lv[2][4 * PE];          // values: [pair of pages][db][lane][page of the pair][4 tokens]
-  __shared__ uint32_t odd[2][4];                                      // tokens of a page whose values are not all finite
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x, G = a.Hq / a.Hkv, kh = h / G, HH = a.Hq + 2 * a.Hkv;
-  const int t0 = (gridDim.y - 1 - blockIdx.y) * QB, nt = min(QB, a.T - t0);
-  // where runs begin
-  unsigned long long begins[NT];
+// What a tile's column does not see of P pages, which begin with tokens first[p]: those from lim on, and those ahead of lo but for the sinks.  Of what it sees,
+// the tokens of `bad` (a bit for each of a page's) are NaN.
+template <int P>
+__device__ __forceinline__ void tile_mask(f32x4 (&st)[P], const int (&first)[P], int lim, int lo, int sinks, const uint32_t (&bad)[P]) {
+  int g = (threadIdx.x & 63) >> 4;
+  asm volatile("" : "+v"(g), "+v"(lim), "+v"(lo));         // (or its comparisons are made ahead of the branch that seldom leads here)
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = first[p] + 4 * g + e;
+      if (bad[p] >> (4 * g + e) & 1) st[p][e] = NAN;
+      if (t >= lim || (t < lo && t >= sinks)) st[p][e] = -INFINITY;
+    }
+}
+
+// w - h, of an fp16 number in the lower or upper half of a register (the compiler converts it first)
+template <int HALF>
+__device__ __forceinline__ float rest_of(float w, f16x2 h) {
+  union { f16x2 h; uint32_t u; } x = {h};
+  float r;
+  if constexpr (HALF) asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(x.u), "v"(w));
+  else asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(x.u), "v"(w));
+  return r;
+}
+
+// Scores of P pages under a tile's column, in units by[p] > 0, become weights, as pairs of fp16 halves, and the column's maximum and sum go on.  A page's weights
+// come times 2^up[p] = 1 / share[p].
+template <int D, int P, bool UP>
+__device__ __forceinline__ void tile_weights(const f32x4 (&st)[P], const float (&by)[P], const float (&up)[P], const float (&share)[P], float& m, float& l, f32x4 (&o)[D / 16],
+                                             f16x2 (&hi)[2 * P], f16x2 (&low)[2 * P]) {
+  float pm = -INFINITY;
+#pragma unroll
+  for (int p = 0; p < P; ++p) pm = fmaxf(pm, fmaxf(fmaxf(st[p][0], st[p][1]), fmaxf(st[p][2], st[p][3])) * by[p]);
+  pm = groups_max(pm);
+  if (__any(pm > m)) {
+    const float mn = fmaxf(m, pm), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= alpha;
+    m = mn;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) o[db] *= alpha;
+  }
+  const float base = m == -INFINITY ? 0.f : m - TOP;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const float b = UP ? up[p] - base : -base;
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[p][e], by[p], b));
+    const float sum = (w[0] + w[1]) + (w[2] + w[3]);
+    l = UP ? __builtin_fmaf(sum, share[p], l) : l + sum;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f16x2 h = __builtin_convertvector((f32x2{w[2 * i], w[2 * i + 1]}), f16x2);
+      hi[2 * p + i] = h;
+      low[2 * p + i] = __builtin_convertvector((f32x2{rest_of<0>(w[2 * i], h), rest_of<1>(w[2 * i + 1], h)}), f16x2);
+    }
+  }
+}
+
+__device__ __forceinline__ f16x8 join(f16x2 a, f16x2 b, f16x2 c, f16x2 d) { return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
+
+template <int D, bool Q8, int NT, int NW>
+__global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel(PageAttn a) {
+  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, QB = 16 * NT * NW, KLD = QB + 1, VLD = QB + 2;
+  constexpr int NL = Q8 ? D / 64 : D / 32, NU = (8 * NL + NW - 1) / NW;        // KiB of a page's keys or values; pieces of 1 KiB that a wave brings of four pages
+  // two buffers of four pages: keys [page][kb][lane][8]; values of 8-bit pages [pair of pages][db][lane][page of the pair][4 tokens], of fp16 pages
+  // [pair][32 dims][page][half of the tokens][dim][8].  Before that, of pages of 8 bits, the tokens' own keys [kb][g][token][8] and values [d][token]
+  constexpr int RING = 16 * PE, OWN = Q8 ? 4 * NKB * KLD * 8 + D * VLD : 0;
+  __shared__ __align__(16) f16 lds[RING > OWN ? RING : OWN];
+  __shared__ uint32_t odd[2][4 * NL];                                 // tokens of a page whose values are not all finite, by piece
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int kh = blockIdx.x, split = blockIdx.z, G = a.Hq / a.Hkv, HH = a.Hq + 2 * a.Hkv;
+  const int TB = QB / G, t0 = (gridDim.y - 1 - blockIdx.y) * TB, nt = min(TB, a.T - t0);       // tokens; a row of a tile is one of them under one of the kv head's heads
+  // where runs begin
+  constexpr int NB = QB / 64;
+  unsigned long long begins[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
     const int r = j * 64 + lane, t = t0 + r;
     bool b = false;
     if (r < nt) b = r == 0 || a.tok_seq[t] != a.tok_seq[t - 1] || a.tok_pos[t] != a.tok_pos[t - 1] + 1 || a.tok_pos[t] == 0;      // (0 behind -1, which is none)
@@ -494,17 +558,18 @@ __global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
   f16x8 q[NT][NKB];
   f32x4 o[NT][NDB];
   float m[NT], l[NT];
-  int cpos[NT];                                                       // the column's position; -1: none
+  int ctok[NT], cpos[NT];                                             // the column's token, nt: none, and its position, -1: none
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int r = wave * 16 * NT + i * 16 + col, t = t0 + (r < nt ? r : 0);
-    const int pos = a.tok_pos[t];
-    cpos[i] = r < nt && token_ok(a, a.tok_seq[t], pos) ? pos : -1;
-    const f16* qp = a.qkv + ((size_t)t * HH + h) * D;
+    const int r = wave * 16 * NT + i * 16 + col;
+    ctok[i] = min(r / G, nt);
+    const int t = t0 + (ctok[i] < nt ? ctok[i] : 0), pos = a.tok_pos[t];
+    cpos[i] = ctok[i] < nt && token_ok(a, a.tok_seq[t], pos) ? pos : -1;
+    const f16* qp = a.qkv + ((size_t)t * HH + kh * G + r % G) * D;
     if (cpos[i] < 0) {
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) q[i][kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -515,49 +580,102 @@ __global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
       for (int kb = 0; kb < NKB; ++kb) q[i][kb] = ld8(qp + kb * 32 + g * 8);
     }
   }
-  int unit = NO_EXP;                                                  // o is in units of 2^unit
 
-  // scores of P pages (lane: tokens first[p] .. + 3) to weights, as two fp16 halves; lim, lo, sinks: what the column sees; fac: of a page's weights
-  auto weights = [&](int i, f32x4 (&st)[4], const float (&fac)[4], const int (&first)[4], int lim, int lo, bool edge, const uint32_t (&bad)[4], f16x8 (&hi)[2],
-                     f16x8 (&low)[2]) {
-    float pm = -INFINITY;
-    bool no[4][4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = first[p] + e;
-        no[p][e] = edge && (t >= lim || (t < lo && t >= a.sinks));
-        if (edge && (bad[p] >> (4 * g + e) & 1)) st[p][e] = NAN;
-        if (no[p][e]) st[p][e] = -INFINITY;
-        pm = fmaxf(pm, st[p][e]);
-      }
-    pm = groups_max(pm);
-    if (__any(pm > m[i])) {
-      const float mn = fmaxf(m[i], pm), alpha = __builtin_amdgcn_exp2f(m[i] - (mn == -INFINITY ? 0.f : mn));
-      l[i] *= alpha;
-      m[i] = mn;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) o[i][db] *= alpha;
+  if (Q8 && split == 0) {
+    // The own pages, unrounded: the tokens' keys and values by way of LDS
+    f16* ok = lds;
+    f16* ov = lds + 4 * NKB * KLD * 8;
+    for (int i = threadIdx.x; i < nt * (D / 16); i += NW * WAVE) {     // 8 pairs of a key
+      const int r = i / (D / 16), c = i % (D / 16), gg = c & 3, kb = c >> 2, t = t0 + r;
+      const int pos = a.tok_pos[t];
+      if (!token_ok(a, a.tok_seq[t], pos)) continue;
+      const f16* row = a.qkv + ((size_t)t * HH + a.Hq + kh) * D + kb * 32 + gg * 8;
+      const size_t at = (size_t)pos * (D / 2) + kb * 32 + gg * 8;
+      f16x8 x = ld8(row), y = ld8(row + D / 2);
+      rotate8(x, y, a.rope_cos + at, a.rope_sin + at);
+      st8(ok + ((kb * 4 + gg) * KLD + r) * 8, x);
+      st8(ok + (((kb + NKB / 2) * 4 + gg) * KLD + r) * 8, y);
     }
-    const float base = m[i] == -INFINITY ? 0.f : m[i] - TOP;
+    for (int i = threadIdx.x; i < nt * (D / 8); i += NW * WAVE) {      // 8 dims of a value
+      const int r = i / (D / 8), c = i % (D / 8);
+      const f16x8 x = ld8(a.qkv + ((size_t)(t0 + r) * HH + a.Hq + a.Hkv + kh) * D + c * 8);
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
+      for (int e = 0; e < 8; ++e) ov[(c * 8 + e) * VLD + r] = x[e];
+    }
+    __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float w = __builtin_amdgcn_exp2f(st[p][e] - base);
-        l[i] += w;
-        if constexpr (Q8) w = no[p][e] ? 0.f : w * fac[p];            // (a factor may be NaN)
-        const f16 x = (f16)w;
-        hi[p / 2][p % 2 * 4 + e] = x;
-        low[p / 2][p % 2 * 4 + e] = (f16)(w - (float)x);
+    for (int i = 0; i < NT; ++i) {
+      const int t = t0 + (ctok[i] < nt ? ctok[i] : 0);
+      const int seq = a.tok_seq[t], own = cpos[i] >= 0 ? cpos[i] / PAGE : -1;
+      unsigned todo = (unsigned)(__ballot(cpos[i] >= 0) & 0xffff);
+      while (todo) {                                                  // the pages of a tile's columns one behind the other
+        const int c = __builtin_ctz(todo);
+        const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(own, c), ps = __builtin_amdgcn_readlane(cpos[i], c);
+        const int row = __builtin_amdgcn_readlane(t, c), r0 = row - t0 - (ps - p * PAGE);       // where the page would begin among the workgroup's tokens
+        const bool in = own == p && seq == s && t - row == cpos[i] - ps;        // (of the same run)
+        todo &= ~(unsigned)(__ballot(in) & 0xffff);
+        f32x4 st[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+        f16x4 v[NDB];
+        if (r0 >= 0 && a.tok_seq[t0 + r0] == s && a.tok_pos[t0 + r0] == p * PAGE) {       // uniform
+          const int rk = min(r0 + col, QB - 1);
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(ld8(ok + ((kb * 4 + g) * KLD + rk) * 8), q[i][kb], st[0]);
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[db][e] = ov[(db * 16 + col) * VLD + min(r0 + 4 * g + e, QB - 1)];
+        } else {                                                      // tokens ahead of the workgroup's, of the pass or of the tail
+          f16x8 k[NKB], vr[NKB];
+          load_own<D>(a, s, kh, row, ps, k, vr);
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(k[kb], q[i][kb], st[0]);
+          // rows to columns: the lane of (dim 16 db + col, token 4 g + e) asks lane (dim % 32 / 8, token)
+#pragma unroll
+          for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int from = (((db & 1) * 2 + (col >> 3)) << 4) + 4 * g + e;
+              union { f16x8 h; uint32_t u[4]; } x = {vr[db >> 1]};
+              uint32_t y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[j] = __shfl(x.u[j], from, WAVE);
+              const uint32_t w = col & 4 ? (col & 2 ? y[3] : y[2]) : (col & 2 ? y[1] : y[0]);
+              union { uint16_t u; f16 h; } z = {(uint16_t)(col & 1 ? w >> 16 : w)};
+              v[db][e] = z.h;
+            }
+        }
+        uint32_t bad[1] = {0};                                        // tokens whose values are not finite: their scores are NaN where they are seen
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bool not_finite = false;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            const bool y = !(fabsf((float)v[db][e]) <= 65504.f);
+            not_finite = not_finite || y;
+            if (y) v[db][e] = (f16)0.f;
+          }
+          const unsigned long long b = __ballot(not_finite);
+          if (b >> (16 * g) & 0xffff) bad[0] |= 1u << (4 * g + e);
+        }
+        const float by[1] = {a.scale}, one[1] = {1.f};
+        const int first[1] = {p * PAGE};
+        f16x2 hi[2], low[2];
+        tile_mask<1>(st, first, in ? cpos[i] + 1 : 0, in && a.window > 0 ? cpos[i] - a.window + 1 : 0, a.sinks, bad);
+        tile_weights<D, 1, false>(st, by, one, one, m[i], l[i], o[i], hi, low);
+        const f16x8 w = join(hi[0], hi[1], low[0], low[1]);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+          o[i][db] = mfma_16x16x32(f16x8{v[db][0], v[db][1], v[db][2], v[db][3], v[db][0], v[db][1], v[db][2], v[db][3]}, w, o[i][db]);
       }
-  };
+    }
+    __syncthreads();                                                  // (the ring begins)
+  }
+  int unit = 0;                                                       // o is in units of 2^unit
 
   for (int c = 0; c < nt;) {
     int next = nt;                                                    // where the run ends
 #pragma unroll
-    for (int j = NT - 1; j >= 0; --j) {
+    for (int j = NB - 1; j >= 0; --j) {
       const int from = c + 1 - 64 * j;
       const unsigned long long rest = from >= 64 ? 0ull : from > 0 ? begins[j] >> from << from : begins[j];
       if (rest) next = min(next, 64 * j + __builtin_ctzll(rest));
@@ -568,17 +686,18 @@ __global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
     if (!token_ok(a, seq, pc)) continue;
     const int pe = min(pc + next - c0 - 1, min(a.max_pos, a.max_blocks * PAGE) - 1);
     const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
-    // pages: those of the sinks, then those of the window
+    // blocks of four pages: those of the sinks, then those of the window
     const int end = Q8 ? pe / PAGE : pe / PAGE + 1;
     const int from = min(a.window > 0 && pc >= a.window ? (pc - a.window + 1) / PAGE : 0, end);
     const int heads = a.sinks > 0 ? min((a.sinks - 1) / PAGE + 1, from) : 0;
-    const int n = heads + end - from;
-    auto page_of = [&](int i) { return i < heads ? i : from + i - heads; };
+    const int head_blocks = (heads + 3) / 4, blocks = head_blocks + (end - from + 3) / 4;
+    const int blk0 = (int)((long)blocks * split / a.splits), blk1 = (int)((long)blocks * (split + 1) / a.splits);
+    auto begin_of = [&](int blk) { return blk < head_blocks ? 4 * blk : from + 4 * (blk - head_blocks); };       // a block's first page
+    auto end_of = [&](int blk) { return blk < head_blocks ? heads : end; };                                         // and where its pages end, at most four on
     int lim[NT], lo[NT], least_lim[NT], most_lim[NT], least_lo[NT], most_lo[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int r = wave * 16 * NT + i * 16 + col;
-      const bool in = r >= c0 && r < next && cpos[i] >= 0;
+      const bool in = ctok[i] >= c0 && ctok[i] < next && cpos[i] >= 0;
       lim[i] = !in ? 0 : Q8 ? cpos[i] / PAGE * PAGE : cpos[i] + 1;
       lo[i] = in && a.window > 0 ? cpos[i] - a.window + 1 : 0;
       int v[4] = {lim[i], lim[i], in ? lo[i] : 0x7fffffff, lo[i]};
@@ -598,122 +717,110 @@ __global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
 
     // of the four pages on their way: a lane's id (of page lane % 4), this wave's operands; then what the block needs beside its operands
     auto id_of = [&](int blk) {
-      const int i = 4 * blk + (lane & 3);
-      const int id = i < n ? bt[page_of(i)] : -1;
+      const int i = begin_of(blk) + (lane & 3);
+      const int id = blk < blk1 && i < end_of(blk) ? bt[i] : -1;
       return id < a.n_pages ? id : -1;
     };
-    uint4 rk[NL], rv[NL];
+    // (piece u of a block: page u / (2 NL), its keys, then its values)
+    uint4 piece[Q8 ? NU : 1];
     f32x2 rstep;
-    auto fetch = [&](int ids) {
-      const int id = __builtin_amdgcn_readlane(ids, wave);
-      const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh);
-      if constexpr (Q8) {
-        const uint8_t* kp = (const uint8_t*)a.k + at * PE + lane * 16;
-        const uint8_t* vp = (const uint8_t*)a.v + at * PE + lane * 16;
+    auto fetch = [&](int buf, int ids) {
 #pragma unroll
-        for (int j = 0; j < NL; ++j) rk[j] = *reinterpret_cast<const uint4*>(kp + j * 1024);
-#pragma unroll
-        for (int j = 0; j < NL; ++j) rv[j] = *reinterpret_cast<const uint4*>(vp + j * 1024);
-        rstep = *reinterpret_cast<const f32x2*>(a.step + 2 * ((size_t)(ids < 0 ? 0 : ids) * a.Hkv + kh));
-      } else {
-        const f16* kp = (const f16*)a.k + at * PE + lane * 8;
-        const f16* vp = (const f16*)a.v + at * PE + col * PAGE + g * 4;
-#pragma unroll
-        for (int j = 0; j < NL; ++j) rk[j] = *reinterpret_cast<const uint4*>(kp + j * 512);
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const uint2 x = *reinterpret_cast<const uint2*>(vp + (2 * j) * 16 * PAGE), y = *reinterpret_cast<const uint2*>(vp + (2 * j + 1) * 16 * PAGE);
-          rv[j] = uint4{x.x, x.y, y.x, y.y};
+      for (int i = 0; i < NU; ++i) {
+        const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
+        const bool values = u / NL & 1;
+        if (8 * NL % NW != 0 && u >= 8 * NL) break;
+        const int id = __builtin_amdgcn_readlane(ids, p);
+        const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh) * PE;
+        if constexpr (Q8) {
+          piece[i] = *reinterpret_cast<const uint4*>((const uint8_t*)(values ? a.v : a.k) + at + j * 1024 + lane * 16);
+        } else {                                                      // straight into the ring
+          const f16* from = values ? (const f16*)a.v + at + j * 512 + (lane & 31) * PAGE + (lane >> 5) * 8 : (const f16*)a.k + at + j * 512 + lane * 8;
+          f16* to = lds + buf * 4 * PE + (values ? 8 * PE + (p >> 1) * 2 * PE + (p & 1) * 512 + j * 1024 : p * PE + j * 512);
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
         }
       }
+      if constexpr (Q8) rstep = *reinterpret_cast<const f32x2*>(a.step + 2 * ((size_t)(ids < 0 ? 0 : ids) * a.Hkv + kh));
     };
-    float sk[4], fac[4];                                              // of the block in LDS (uniform)
+    float by[4] = {a.scale, a.scale, a.scale, a.scale}, up[4] = {0.f, 0.f, 0.f, 0.f}, share[4] = {1.f, 1.f, 1.f, 1.f};       // of the block in LDS (uniform)
     int there = 0, unit_next = unit;
+    uint32_t nans = 0;                                                // pages of 8 bits that are NaN
     auto stage = [&](int buf, int blk, int ids) {
       there = (int)(__ballot(ids >= 0) & 15);
-      f16 by = (f16)1.f;
       if constexpr (Q8) {
-        int ex[4];
-        float sv[4];
+        // a lane for page lane % 4
+        const int ek = (int)(__float_as_uint(rstep[0]) >> 23 & 255), ev = (int)(__float_as_uint(rstep[1]) >> 23 & 255);
+        nans = (uint32_t)(__ballot(ids >= 0 && (ek == 255 || ev == 255)) & 15);
+        const int ex = ids >= 0 && ev > 0 && ev < 255 ? ev - 127 : NO_EXP;
+        int most = max(ex, __builtin_amdgcn_update_dpp(0, ex, 0xb1, 0xf, 0xf, false));       // over the four: lanes 1 0 3 2, then 2 3 0 1
+        most = max(most, __builtin_amdgcn_update_dpp(0, most, 0x4e, 0xf, 0xf, false));
+        unit_next = max(unit_next, __builtin_amdgcn_readfirstlane(most));
+        const int k = ex == NO_EXP ? 0 : max(ex - unit_next, -24);    // (exact: codes have seven bits, fp16 numbers multiples of 2^-24)
+        const float f = ex == NO_EXP ? 1.f : rstep[1] * power(-(unit_next + k));
+        const float lane_by = ek == 255 ? 1.f : fmaxf(a.scale * rstep[0], 0x1p-126f);        // (a page of zeros: scores of zero, and -inf stays what it is)
+        const float lane_up = __builtin_amdgcn_logf(f), lane_share = 1.f / f;
+        const float mult = ex == NO_EXP ? 0.f : power(k);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          sk[p] = a.scale * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rstep[0]), p));
-          sv[p] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rstep[1]), p));
-          const int e = (int)(__float_as_uint(sv[p]) >> 23 & 255);
-          ex[p] = (there >> p & 1) && e > 0 && e < 255 ? e - 127 : NO_EXP;
-          unit_next = max(unit_next, ex[p]);
+          by[p] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_by), p));
+          up[p] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_up), p));
+          share[p] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_share), p));
         }
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int k = ex[p] == NO_EXP ? 0 : max(ex[p] - unit_next, -24);       // (exact: codes have seven bits, fp16 numbers multiples of 2^-24)
-          fac[p] = ex[p] != NO_EXP ? sv[p] * power(-(unit_next + k)) : sv[p] == 0.f || !(there >> p & 1) ? 1.f : sv[p];
-          if (p == wave) by = (f16)power(k);
-        }
-      }
-      uint32_t bad = 0;
-      f16* kd = lk[buf] + wave * PE + lane * 8;
-      f16* vd = lv[buf] + ((wave >> 1) * NDB * 64 + lane) * 8 + (wave & 1) * 4;
-      if constexpr (Q8) {
+        for (int i = 0; i < NU; ++i) {
+          const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
+          if (8 * NL % NW != 0 && u >= 8 * NL) break;
+          if (u / NL & 1) {                                           // uniform
+            const f16 x = (f16)__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mult), p));
+            f16* to = lds + 8 * PE + buf * 4 * PE + ((p >> 1) * NDB * 64 + lane) * 8 + (p & 1) * 4 + 4 * j * 512;
+            const uint32_t y[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          st8(kd + (2 * j) * 512, from_codes(rk[j].x, rk[j].y));
-          st8(kd + (2 * j + 1) * 512, from_codes(rk[j].z, rk[j].w));
-          const uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<f16x4*>(vd + (4 * j + i) * 512) = from_codes(u[i]) * f16x4{by, by, by, by};
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<f16x4*>(to + e * 512) = from_codes(y[e]) * f16x4{x, x, x, x};
+          } else {
+            f16* to = lds + buf * 4 * PE + p * PE + 2 * j * 512 + lane * 8;
+            st8(to, from_codes(piece[i].x, piece[i].y));
+            st8(to + 512, from_codes(piece[i].z, piece[i].w));
+          }
         }
       } else {
-        const int first = 4 * blk + wave < n ? page_of(4 * blk + wave) * PAGE : 0;
-        // somebody may not see all of it: values that are not finite would reach those columns as well, by 0 * inf
-        const bool part = !(there >> wave & 1) || first + PAGE > run_lim || (first < run_lo && first + PAGE > a.sinks);        // uniform
+        // Where somebody may not see all of a page, values that are not finite would reach those columns as well, by 0 * inf: the wave looks at what it has brought
 #pragma unroll
-        for (int j = 0; j < NL; ++j) *reinterpret_cast<uint4*>(kd + j * 512) = rk[j];
-        if (part) {
-          bool not_finite[4] = {};
+        for (int i = 0; i < NU; ++i) {
+          const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
+          if ((8 * NL % NW != 0 && u >= 8 * NL) || !(u / NL & 1)) continue;
+          uint32_t bad = 0;
+          const int first = (begin_of(blk) + p) * PAGE;
+          if (!(there >> p & 1) || first + PAGE > run_lim || (first < run_lo && first + PAGE > a.sinks)) {        // uniform
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            f16* at = lds + 8 * PE + buf * 4 * PE + (p >> 1) * 2 * PE + (p & 1) * 512 + j * 1024 + lane * 8;
+            f16x8 x = ld8(at);
 #pragma unroll
-          for (int j = 0; j < NL; ++j) {
-            uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool x = (u[i] & 0x7c00u) == 0x7c00u, y = (u[i] & 0x7c000000u) == 0x7c000000u;
-              not_finite[2 * (i & 1)] |= x;
-              not_finite[2 * (i & 1) + 1] |= y;
-              u[i] &= (x ? 0u : 0xffffu) | (y ? 0u : 0xffff0000u);
+            for (int e = 0; e < 8; ++e) {                             // tokens 8 (lane / 32) + e
+              const bool not_finite = !(fabsf((float)x[e]) <= 65504.f);
+              if (not_finite) x[e] = (f16)0.f;
+              const unsigned long long b = __ballot(not_finite);
+              bad |= (uint32_t)((b & 0xffffffffull) != 0) << e | (uint32_t)(b >> 32 != 0) << (8 + e);
             }
-            rv[j] = uint4{u[0], u[1], u[2], u[3]};
+            st8(at, x);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned long long b = __ballot(not_finite[e]);
-#pragma unroll
-            for (int gg = 0; gg < 4; ++gg)
-              if (b >> (16 * gg) & 0xffff) bad |= 1u << (4 * gg + e);
-          }
+          if (lane == 0) odd[buf][p * NL + j] = bad;
         }
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          *reinterpret_cast<uint2*>(vd + (2 * j) * 512) = uint2{rv[j].x, rv[j].y};
-          *reinterpret_cast<uint2*>(vd + (2 * j + 1) * 512) = uint2{rv[j].z, rv[j].w};
-        }
-        if (lane == 0) odd[buf][wave] = bad;
       }
     };
 
-    const int blocks = (n + 3) / 4;
-    if (blocks == 0) continue;                                        // uniform over the workgroup
-    int ids = id_of(0);
-    fetch(ids);
-    int ids_next = id_of(1);
-    __syncthreads();                                                  // (the run before may still be read)
-    stage(0, 0, ids);
+    if (blk0 == blk1) continue;                                        // uniform over the workgroup
+    int ids = id_of(blk0);
+    fetch(0, ids);
+    int ids_next = id_of(blk0 + 1);
+    stage(0, blk0, ids);                                                 // (everybody is done with the ring: a barrier ends every block)
     __syncthreads();
-    for (int blk = 0; blk < blocks; ++blk) {
-      const int buf = blk & 1;
+    for (int blk = blk0; blk < blk1; ++blk) {
+      const int buf = (blk - blk0) & 1;
       const int ids_then = id_of(blk + 2);
-      if (blk + 1 < blocks) fetch(ids_next);
+      if (blk + 1 < blk1) fetch(buf ^ 1, ids_next);
       if constexpr (Q8) {
         if (unit_next != unit) {                                      // uniform
-          const float f = unit == NO_EXP ? 0.f : power(max(unit - unit_next, -126));
+          const float f = power(max(unit - unit_next, -126));
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -721,142 +828,126 @@ __global__ __launch_bounds__(4 * WAVE, 2) void page_prefill_kernel(PageAttn a) {
           unit = unit_next;
         }
       }
-      int first[4];
+      const int first0 = begin_of(blk) * PAGE;
       bool sees[NT], whole[NT];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) sees[i] = false, whole[i] = there == 15;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        first[p] = there >> p & 1 ? page_of(4 * blk + p) * PAGE : 0x3fffffff;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          sees[i] = sees[i] || (first[p] < most_lim[i] && (first[p] + PAGE > least_lo[i] || first[p] < a.sinks));
-          whole[i] = whole[i] && first[p] + PAGE <= least_lim[i] && (first[p] >= most_lo[i] || first[p] + PAGE <= a.sinks);
-        }
-        first[p] += 4 * g;
+      for (int i = 0; i < NT; ++i) {
+        sees[i] = first0 < most_lim[i] && (first0 + 4 * PAGE > least_lo[i] || first0 < a.sinks);
+        whole[i] = there == 15 && first0 + 4 * PAGE <= least_lim[i] && (first0 >= most_lo[i] || first0 + 4 * PAGE <= a.sinks);
       }
       bool any = false;
 #pragma unroll
       for (int i = 0; i < NT; ++i) any = any || sees[i];
       if (any) {                                                      // uniform over the wave
-        uint32_t bad[4] = {0, 0, 0, 0};
-        if constexpr (!Q8) {
-#pragma unroll
-          for (int p = 0; p < 4; ++p) bad[p] = __builtin_amdgcn_readfirstlane(odd[buf][p]);
-          if (bad[0] | bad[1] | bad[2] | bad[3])
-#pragma unroll
-            for (int i = 0; i < NT; ++i) whole[i] = false;
-        }
-        f32x4 st[NT][4];
-        const f16* kl = lk[buf] + lane * 8;
+        uint32_t bad[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
+          bad[p] = Q8 && (nans >> p & 1) ? 0xffffu : 0u;
+          if constexpr (!Q8) {
+            uint32_t x = 0;
+#pragma unroll
+            for (int j = 0; j < NL; ++j) x |= odd[buf][p * NL + j];
+            bad[p] = __builtin_amdgcn_readfirstlane(x);
+          }
+        }
+        if (bad[0] | bad[1] | bad[2] | bad[3])
+#pragma unroll
+          for (int i = 0; i < NT; ++i) whole[i] = false;
+        f32x4 st[NT][4];
+        const f16* kl = lds + buf * 4 * PE + lane * 8;
+        constexpr int KR = NT == 1 ? 1 : 2;
+        f16x8 k[KR][NKB];                                             // a page's keys while those of the one before are multiplied
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) k[0][kb] = ld8(kl + kb * 512);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          if (KR == 2 ? p < 3 : p > 0)
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb) k[KR == 2 ? (p + 1) & 1 : 0][kb] = ld8(kl + (KR == 2 ? p + 1 : p) * PE + kb * 512);
 #pragma unroll
           for (int i = 0; i < NT; ++i) st[i][p] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kb = 0; kb < NKB; ++kb) {
-            const f16x8 k = ld8(kl + p * PE + kb * 512);
+          for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) st[i][p] = mfma_16x16x32(k, q[i][kb], st[i][p]);
-          }
-#pragma unroll
-          for (int i = 0; i < NT; ++i) st[i][p] *= Q8 ? sk[p] : a.scale;
+            for (int i = 0; i < NT; ++i) st[i][p] = mfma_16x16x32(k[p % KR][kb], q[i][kb], st[i][p]);
         }
-        f16x8 hi[NT][2], low[NT][2];
+        f16x2 hi[NT][8], low[NT][8];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if (whole[i]) weights(i, st[i], fac, first, lim[i], lo[i], false, bad, hi[i], low[i]);
-          else weights(i, st[i], fac, first, lim[i], lo[i], true, bad, hi[i], low[i]);
-        }
-        const f16* vl = lv[buf] + lane * 8;
+          if (!whole[i]) {                                            // uniform
+            int first[4];
 #pragma unroll
-        for (int pair = 0; pair < 2; ++pair)
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) {
-            const f16x8 v = ld8(vl + (pair * NDB + db) * 512);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              o[i][db] = mfma_16x16x32(v, hi[i][pair], o[i][db]);
-              o[i][db] = mfma_16x16x32(v, low[i][pair], o[i][db]);
-            }
+            for (int p = 0; p < 4; ++p) first[p] = there >> p & 1 ? first0 + p * PAGE : 0x3fffffff;
+            tile_mask<4>(st[i], first, lim[i], lo[i], a.sinks, bad);
           }
+          tile_weights<D, 4, Q8>(st[i], by, up, share, m[i], l[i], o[i], hi[i], low[i]);
+        }
+        const f16* vl = lds + 8 * PE + buf * 4 * PE + (Q8 ? lane * 8 : (g >> 1) * 256 + col * 8 + (g & 1) * 4);
+        auto values = [&](int j) {                                    // of pair j / NDB, dims 16 (j % NDB) ..
+          const int pair = j / NDB, db = j % NDB;
+          if constexpr (Q8) return ld8(vl + (pair * NDB + db) * 512);
+          const f16* p = vl + pair * 2 * PE + (db >> 1) * 1024 + (db & 1) * 128;
+          const f16x4 x = *reinterpret_cast<const f16x4*>(p), y = *reinterpret_cast<const f16x4*>(p + 512);
+          return f16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        };
+        constexpr int AHEAD = NT == 1 ? 2 : 4;
+        f16x8 v[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) v[j] = values(j);
+#pragma unroll
+        for (int j = 0; j < 2 * NDB; ++j) {
+          const int pair = j / NDB, db = j % NDB;
+          const f16x8 x = v[j % AHEAD];
+          if (j + AHEAD < 2 * NDB) v[j % AHEAD] = values(j + AHEAD);
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            o[i][db] = mfma_16x16x32(x, join(hi[i][4 * pair], hi[i][4 * pair + 1], hi[i][4 * pair + 2], hi[i][4 * pair + 3]), o[i][db]);
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            o[i][db] = mfma_16x16x32(x, join(low[i][4 * pair], low[i][4 * pair + 1], low[i][4 * pair + 2], low[i][4 * pair + 3]), o[i][db]);
+        }
       }
-      if (blk + 1 < blocks) stage(buf ^ 1, blk + 1, ids_next);
+      if (blk + 1 < blk1) stage(buf ^ 1, blk + 1, ids_next);
       ids_next = ids_then;
       __syncthreads();
     }
   }
 
+  const float scale_up = power(unit);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    const int r = wave * 16 * NT + i * 16 + col, t = t0 + (r < nt ? r : 0);
-    if constexpr (Q8) {
-      // the own pages, unrounded: those of the tile's columns one behind the other
-      const float f = unit == NO_EXP ? 1.f : power(unit);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) o[i][db] *= f;
-      const int seq = a.tok_seq[t], own = cpos[i] >= 0 ? cpos[i] / PAGE : -1;
-      unsigned todo = (unsigned)(__ballot(cpos[i] >= 0) & 0xffff);
-      while (todo) {
-        const int c = __builtin_ctz(todo);
-        const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(own, c), ps = __builtin_amdgcn_readlane(cpos[i], c);
-        const int row = __builtin_amdgcn_readlane(t, c);
-        const bool in = own == p && seq == s && t - row == cpos[i] - ps;        // (of the same run)
-        todo &= ~(unsigned)(__ballot(in) & 0xffff);
-        f16x8 k[NKB];
-        f16x4 v[NDB];
-        load_own<D>(a, s, kh, row, ps, k, v);
-        f32x4 st[4];
-        st[0] = st[1] = st[2] = st[3] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(k[kb], q[i][kb], st[0]);
-        st[0] *= a.scale;
-        uint32_t bad[4] = {0, 0, 0, 0};                               // tokens whose values are not finite: their scores are NaN where they are seen
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          bool not_finite = false;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) {
-            const float x = (float)v[db][e];
-            const bool y = !(fabsf(x) <= 65504.f);
-            not_finite = not_finite || y;
-            if (y) v[db][e] = (f16)0.f;
-          }
-          const unsigned long long b = __ballot(not_finite);
-          if (b >> (16 * g) & 0xffff) bad[0] |= 1u << (4 * g + e);
-        }
-        const int none = 0x3fffffff;
-        const int first[4] = {p * PAGE + 4 * g, none, none, none};
-        const float one[4] = {1.f, 1.f, 1.f, 1.f};
-        f16x8 hi[2], low[2];
-        weights(i, st, one, first, in ? cpos[i] + 1 : 0, in && a.window > 0 ? cpos[i] - a.window + 1 : 0, true, bad, hi, low);
-        const f16x8 w = f16x8{hi[0][0], hi[0][1], hi[0][2], hi[0][3], low[0][0], low[0][1], low[0][2], low[0][3]};
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-          o[i][db] = mfma_16x16x32(f16x8{v[db][0], v[db][1], v[db][2], v[db][3], v[db][0], v[db][1], v[db][2], v[db][3]}, w, o[i][db]);
-      }
-    }
+    const int t = t0 + ctok[i], h = kh * G + (wave * 16 * NT + i * 16 + col) % G;
     l[i] += __shfl_xor(l[i], 16, WAVE);
     l[i] += __shfl_xor(l[i], 32, WAVE);
-    if (r >= nt) continue;
-    const float by = l[i] == 0.f ? 0.f : 1.f / l[i];
+    if (ctok[i] >= nt) continue;
+    if (a.splits > 1) {
+      const size_t at = ((size_t)t * a.Hq + h) * a.splits + split;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(a.acc + at * D + db * 16 + 4 * g) = o[i][db] * scale_up;
+      if (g == 0) *reinterpret_cast<f32x2*>(a.ml + 2 * at) = f32x2{m[i], l[i]};
+      continue;
+    }
+    const float f = l[i] == 0.f ? 0.f : scale_up / l[i];
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const int d = h * D + db * 16 + 4 * g;
       f16x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (f16)(l[i] == 0.f ? 0.f : o[i][db][e] * by);
+      for (int e = 0; e < 4; ++e) x[e] = (f16)(l[i] == 0.f ? 0.f : o[i][db][e] * f);
       *reinterpret_cast<f16x4*>(a.out + (a.frag_tt ? frag_offset(t, d, a.frag_tt) : (size_t)t * a.Hq * D + d)) = x;
     }
   }
 }
 
-// Pages that a pass completes, in 8 bits: a wave has 16 tokens of the pass and a kv head, and of them those that are the first of their page in the pass
+// Pages that a pass completes, in 8 bits: a wave has 16 tokens of the pass and a kv head, and of them those that are the first of their page in the pass.  Values
+// are turned over as codes, by way of LDS.
 template <int D>
 __global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
-  const int lane = threadIdx.x & 63, kh = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = blockIdx.x * 16;
+  constexpr int LD = 20;                                              // bytes of a dim's tokens in LDS, apart for the banks
+  __shared__ __align__(16) uint8_t turn[4][D * LD];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, kh = blockIdx.y * 4 + wave, t0 = blockIdx.x * 16;
   if (kh >= a.Hkv) return;
-  const int t = t0 + (lane & 15);
+  const int t = t0 + col;
   int seq = -1, pos = -1;
   bool lead = false;
   if (t < a.T) {
@@ -874,10 +965,33 @@ __global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
     const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(pos, c);
     const int id = a.block_table[(size_t)s * a.max_blocks + p / PAGE];
     if (id < 0 || id >= a.n_pages) continue;                          // uniform
-    f16x8 k[D / 32];
-    f16x4 v[D / 16];
+    f16x8 k[D / 32], v[D / 32];
     load_own<D>(a, s, kh, t0 + c, p, k, v);
-    store_codes<D>(a, id, kh, k, v);
+    const Rounding rk = rounding_of(k), rv = rounding_of(v);
+    uint8_t* kp = (uint8_t*)a.k + ((size_t)id * a.Hkv + kh) * PAGE * D + lane * 16;
+    uint8_t* vp = (uint8_t*)a.v + ((size_t)id * a.Hkv + kh) * PAGE * D + lane * 16;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      union { int8_t b[16]; uint4 u; } x;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        x.b[e] = rk.code((float)k[2 * j + e / 8][e % 8]);
+        turn[wave][(64 * j + 32 * (e / 8) + 8 * g + e % 8) * LD + col] = (uint8_t)rv.code((float)v[2 * j + e / 8][e % 8]);
+      }
+      *reinterpret_cast<uint4*>(kp + j * 1024) = x.u;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      uint32_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint32_t*>(&turn[wave][(64 * j + 16 * i + col) * LD + 4 * g]);
+      *reinterpret_cast<uint4*>(vp + j * 1024) = uint4{y[0], y[1], y[2], y[3]};
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane == 0) *reinterpret_cast<f32x2*>(a.step + 2 * ((size_t)id * a.Hkv + kh)) = f32x2{rk.step, rv.step};
   }
 }
 
@@ -939,6 +1053,10 @@ int check(const char* who, const mlora_page_attn& p, bool rotates) {
   MLORA_CHECK(p.T >= 0 && p.max_pos > 0 && p.max_blocks <= 1 << 26, MLORA_ERR_INVALID, "%s: bad T=%d max_pos=%d max_blocks=%d", who, p.T, p.max_pos, p.max_blocks);
   MLORA_CHECK(p.window >= 0 && p.sinks >= 0, MLORA_ERR_INVALID, "%s: a window of %d with %d sinks", who, p.window, p.sinks);
   MLORA_CHECK(p.out_layout == MLORA_ROWMAJOR || p.out_layout == MLORA_FRAG, MLORA_ERR_INVALID, "%s: bad out_layout %d", who, p.out_layout);
+  MLORA_CHECK(p.splits >= 1 && p.splits <= 64 && (p.splits == 1 || p.T <= 65535), MLORA_ERR_INVALID, "%s: %d tokens in %d shares", who, p.T, p.splits);
+  const size_t need = mlora_page_attn_workspace_bytes(p.T, p.Hq, p.D, p.splits);
+  MLORA_CHECK(need == 0 || (p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need), MLORA_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes, %zu needed", who, p.workspace_bytes, need);
   return MLORA_OK;
 }
 
@@ -969,25 +1087,43 @@ int decode(const PageAttn& a, hipStream_t s) {
   return mlora_launch_status("page_attn_decode");
 }
 
+// Eight waves of one tile: four waves on a SIMD.  (Us, so / four waves of two tiles, whose registers leave two: 8 prompts of 456 115 / 128, 777 tokens behind 3500
+// 136 / 165, 4096 tokens under a window of 1024 in fp16 185 / 179)
+constexpr int PREFILL_TILES = 1, PREFILL_WAVES = 8, PREFILL_ROWS = 16 * PREFILL_TILES * PREFILL_WAVES;
+
+template <int D, bool Q8>
+int launch_prefill(const PageAttn& a, hipStream_t s) {
+  const int G = a.Hq / a.Hkv;
+  hipLaunchKernelGGL((page_prefill_kernel<D, Q8, PREFILL_TILES, PREFILL_WAVES>), dim3(a.Hkv, ceil_div(a.T, PREFILL_ROWS / G), a.splits), dim3(PREFILL_WAVES * WAVE), 0, s, a);
+  if (int e = mlora_launch_status("page_attn_prefill")) return e;
+  if (a.splits == 1) return MLORA_OK;
+  hipLaunchKernelGGL(page_join_kernel<D>, dim3(ceil_div(a.Hq, 4), a.T), dim3(4 * WAVE), 0, s, a);
+  return mlora_launch_status("page_attn_prefill");
+}
+
 template <int D>
 int prefill(const PageAttn& a, hipStream_t s) {
+  if (!a.step) return launch_prefill<D, false>(a, s);
   const dim3 tiles(ceil_div(a.T, 16), ceil_div(a.Hkv, 4));
-  if (a.step) {
-    hipLaunchKernelGGL(page_store_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
-    if (int e = mlora_launch_status("page_attn_prefill")) return e;
-    hipLaunchKernelGGL((page_prefill_kernel<D, true, 2>), dim3(a.Hq, ceil_div(a.T, 128)), dim3(4 * WAVE), 0, s, a);
-    if (int e = mlora_launch_status("page_attn_prefill")) return e;
-    hipLaunchKernelGGL(page_tail_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((page_prefill_kernel<D, false, 2>), dim3(a.Hq, ceil_div(a.T, 128)), dim3(4 * WAVE), 0, s, a);
-  }
+  hipLaunchKernelGGL(page_store_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
+  if (int e = mlora_launch_status("page_attn_prefill")) return e;
+  if (int e = launch_prefill<D, true>(a, s)) return e;
+  hipLaunchKernelGGL(page_tail_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
   return mlora_launch_status("page_attn_prefill");
 }
 
 }  // namespace
 
-extern "C" int mlora_page_attn_splits(int T, int Hkv, int pages) {
-  if (T <= 0 || Hkv <= 0) return 1;
+extern "C" int mlora_page_attn_splits(int prompt, int T, int Hq, int Hkv, int pages) {
+  if (T <= 0 || Hkv <= 0 || Hq < Hkv || T > 65535) return 1;
+  const int G = Hq / Hkv;
+  if (prompt) {
+    if (G > PREFILL_ROWS) return 1;
+    const long wgs = (long)Hkv * ceil_div(T, PREFILL_ROWS / G);
+    long n = 512 / wgs;
+    n = n < pages / 32 ? n : pages / 32;
+    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  }
   const long wgs = (long)T * Hkv;
   long n = (512 + wgs - 1) / wgs;
   n = n < pages / 16 ? n : pages / 16;
@@ -1002,12 +1138,9 @@ extern "C" int mlora_page_attn_decode(const mlora_page_attn* args, void* stream)
   MLORA_CHECK(args, MLORA_ERR_INVALID, "page_attn_decode: null pointer");
   const mlora_page_attn& p = *args;
   if (int e = check("page_attn_decode", p, true)) return e;
-  MLORA_CHECK(p.T <= 65535 && p.splits >= 1 && p.splits <= 64, MLORA_ERR_INVALID, "page_attn_decode: %d sequences in %d shares", p.T, p.splits);
+  MLORA_CHECK(p.T <= 65535, MLORA_ERR_INVALID, "page_attn_decode: %d sequences", p.T);
   MLORA_CHECK(p.Hq / p.Hkv <= 16, MLORA_ERR_UNSUPPORTED, "page_attn_decode: more than 16 query heads per kv head (%d)", p.Hq / p.Hkv);
   if (p.T == 0) return MLORA_OK;
-  const size_t need = mlora_page_attn_workspace_bytes(p.T, p.Hq, p.D, p.splits);
-  MLORA_CHECK(need == 0 || (p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need), MLORA_ERR_WORKSPACE,
-              "page_attn_decode: workspace of %zu bytes, %zu needed", p.workspace_bytes, need);
   const PageAttn a = args_of(p);
   hipStream_t s = (hipStream_t)stream;
   if (p.D == 128) return p.step ? decode<128, true>(a, s) : decode<128, false>(a, s);
@@ -1018,7 +1151,8 @@ extern "C" int mlora_page_attn_prefill(const mlora_page_attn* args, void* stream
   MLORA_CHECK(args, MLORA_ERR_INVALID, "page_attn_prefill: null pointer");
   const mlora_page_attn& p = *args;
   if (int e = check("page_attn_prefill", p, p.step != nullptr)) return e;
-  MLORA_CHECK(p.T <= 1 << 22 && p.Hkv <= 4 * 65535, MLORA_ERR_UNSUPPORTED, "page_attn_prefill: %d tokens", p.T);
+  MLORA_CHECK(p.Hq / p.Hkv <= 64, MLORA_ERR_UNSUPPORTED, "page_attn_prefill: more than 64 query heads per kv head (%d)", p.Hq / p.Hkv);
+  MLORA_CHECK(ceil_div(p.T, PREFILL_ROWS / (p.Hq / p.Hkv)) <= 65535 && p.Hkv <= 65535, MLORA_ERR_UNSUPPORTED, "page_attn_prefill: %d tokens under %d heads", p.T, p.Hq);
   if (p.T == 0) return MLORA_OK;
   const PageAttn a = args_of(p);
   return p.D == 128 ? prefill<128>(a, (hipStream_t)stream) : prefill<64>(a, (hipStream_t)stream);

@@ -1218,7 +1218,7 @@ _NO_ROPE = (None, None)
 
 
 def _page_attn(who, fn, qkv, k, v, quant, block_table, tok_seq, tok_pos, rope, Hq, Hkv, D, window, sinks, out, frag, longest):
-    """The call behind attention over pages that k and v name; longest < 0: a prompt."""
+    """The call behind attention over pages that k and v name."""
     T, (n_seq, max_blocks), dev = qkv.shape[0], block_table.shape, _here(qkv.device, who)
     window, sinks = _window(who, window, sinks)
     n_pages = k.shape[0]
@@ -1254,16 +1254,14 @@ def _page_attn(who, fn, qkv, k, v, quant, block_table, tok_seq, tok_pos, rope, H
         out, optr, lay = _out_arg(out, T, Hq * D, frag, dev)
     if T == 0:
         return out
-    splits, ws, nb = 1, 0, 0
-    if longest >= 0:
-        pages = max_blocks if longest == 0 else min(-(-longest // 16), max_blocks)
-        if window:
-            pages = min(pages, (window + 30) // 16 + (sinks + 15) // 16)
-        splits = _size(f16, "mlora_page_attn_splits", T, Hkv, pages)
-        if splits > 1:
-            nb = _size(f16, "mlora_page_attn_workspace_bytes", T, Hq, D, splits)
-            w = _empty_strided_cuda((nb // 4,), (1,), torch.float32)
-            ws = w.data_ptr()
+    pages, ws, nb, prompt = max_blocks if longest is None else min(-(-longest // 16), max_blocks), 0, 0, int(fn == "mlora_page_attn_prefill")
+    if window:
+        pages = min(pages, (window + (T if prompt else 0) + 30) // 16 + (sinks + 15) // 16)
+    splits = _size(f16, "mlora_page_attn_splits", prompt, T, Hq, Hkv, pages)
+    if splits > 1:
+        nb = _size(f16, "mlora_page_attn_workspace_bytes", T, Hq, D, splits)
+        w = _empty_strided_cuda((nb // 4,), (1,), torch.float32)
+        ws = w.data_ptr()
     args = _PAGE_ATTN.pack(optr, qkv.data_ptr(), k.data_ptr(), v.data_ptr(), step, tail_k, tail_v, block_table.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(),
                            0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), ws, nb, lay, max_blocks, max_pos, T, Hq, Hkv, D, n_pages, n_seq,
                            window, sinks, splits)
@@ -1276,28 +1274,28 @@ def _page_attn(who, fn, qkv, k, v, quant, block_table, tok_seq, tok_pos, rope, H
 def rope_attn_decode_q8(qkv, pages: QuantPages, block_table, seq_ids, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, longest=None, out=None, frag=False):
     """One token of each of T different sequences on pages of 8 bits: q and k are rotated, the token's k and v stored (its page rounded to 8 bits, where it completes it),
     and the token attends to its own page unrounded and to those ahead of it.  qkv is left as it is.  window: only the last so many tokens are seen, the
-    token itself among them, and the first `sinks`.  longest: most tokens of a row, its new one among them; it chooses how the work is cut (None: as many as the table holds)."""
+    token itself among them, and the first `sinks`.  longest: most tokens of a row, its new ones among them; it chooses how the work is cut (None: as many as the table holds)."""
     return _page_attn("rope_attn_decode_q8", "mlora_page_attn_decode", qkv, pages.k, pages.v, pages, block_table, seq_ids, tok_pos, (rope_cos, rope_sin), Hq, Hkv, D, window,
-                      sinks, out, frag, longest or 0)
+                      sinks, out, frag, longest)
 
 
-def rope_attn_prefill_q8(qkv, pages: QuantPages, block_table, tok_seq, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, out=None, frag=False):
+def rope_attn_prefill_q8(qkv, pages: QuantPages, block_table, tok_seq, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, longest=None, out=None, frag=False):
     """`rope_attn_decode_q8` for the tokens of a pass, those of a sequence consecutive with increasing positions: the same results however a prompt is cut into passes, up to
     the order of sums."""
     return _page_attn("rope_attn_prefill_q8", "mlora_page_attn_prefill", qkv, pages.k, pages.v, pages, block_table, tok_seq, tok_pos, (rope_cos, rope_sin), Hq, Hkv, D, window,
-                      sinks, out, frag, -1)
+                      sinks, out, frag, longest)
 
 
 def rope_attn_decode_window(qkv, k_cache, v_cache, block_table, seq_ids, tok_pos, rope_cos, rope_sin, Hq, Hkv, D, window=None, sinks=0, longest=None, out=None, frag=False):
     """`rope_attn_decode` under a sliding window with sinks, and with long contexts shared out over the device (arguments as for `rope_attn_decode_q8`)."""
     return _page_attn("rope_attn_decode_window", "mlora_page_attn_decode", qkv, k_cache, v_cache, None, block_table, seq_ids, tok_pos, (rope_cos, rope_sin), Hq, Hkv, D, window,
-                      sinks, out, frag, longest or 0)
+                      sinks, out, frag, longest)
 
 
-def paged_attn_prefill_window(qkv, k_cache, v_cache, block_table, tok_seq, tok_pos, Hq, Hkv, D, window=None, sinks=0, out=None, frag=False):
+def paged_attn_prefill_window(qkv, k_cache, v_cache, block_table, tok_seq, tok_pos, Hq, Hkv, D, window=None, sinks=0, longest=None, out=None, frag=False):
     """`paged_attn_prefill` under a sliding window with sinks: behind `rope_kv_append` of the same tokens."""
     return _page_attn("paged_attn_prefill_window", "mlora_page_attn_prefill", qkv, k_cache, v_cache, None, block_table, tok_seq, tok_pos, _NO_ROPE, Hq, Hkv, D, window, sinks,
-                      out, frag, -1)
+                      out, frag, longest)
 
 
 def copy_pages(pools, src, dst):

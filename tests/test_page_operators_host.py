@@ -26,13 +26,17 @@ def test_page_attention_refusals():
         assert call(D=96) == -2 and call(Hq=9, Hkv=2) == -1 and call(window=-1) == -1 and call(sinks=-1) == -1 and call(lay=5) == -1
         assert call(T=0) == 0
     assert _attn(lib, "mlora_page_attn_decode", Hq=34, Hkv=2) == -2 and _attn(lib, "mlora_page_attn_decode", T=70000) == -1
-    assert _attn(lib, "mlora_page_attn_decode", splits=0) == -1 and _attn(lib, "mlora_page_attn_decode", splits=65) == -1
     need = lib.mlora_page_attn_workspace_bytes(2, 8, 128, 3)
     assert need == 2 * 8 * 3 * 130 * 4 and lib.mlora_page_attn_workspace_bytes(2, 8, 128, 1) == 0 and lib.mlora_page_attn_workspace_bytes(0, 8, 128, 3) == 0
-    for ws, nb in ((0, need), (16, need - 1), (24, need)):
-        assert _attn(lib, "mlora_page_attn_decode", splits=3, ws=ws, nb=nb) == -3
-    assert _attn(lib, "mlora_page_attn_prefill", step=0, cos=0, sin=0, T=0) == 0 and _attn(lib, "mlora_page_attn_prefill", T=(1 << 22) + 1) == -2
-    assert lib.mlora_page_attn_splits(0, 8, 100) == 1 and lib.mlora_page_attn_splits(1, 8, 1) == 1 and 1 < lib.mlora_page_attn_splits(1, 8, 1 << 20) <= 64
+    for fn in ("mlora_page_attn_decode", "mlora_page_attn_prefill"):
+        assert _attn(lib, fn, splits=0) == -1 and _attn(lib, fn, splits=65) == -1 and _attn(lib, fn, T=70000, splits=2, ws=16, nb=1 << 40) == -1
+        for ws, nb in ((0, need), (16, need - 1), (24, need)):
+            assert _attn(lib, fn, splits=3, ws=ws, nb=nb) == -3
+    assert _attn(lib, "mlora_page_attn_prefill", step=0, cos=0, sin=0, T=0) == 0 and _attn(lib, "mlora_page_attn_prefill", T=1 << 24) == -2
+    assert _attn(lib, "mlora_page_attn_prefill", Hq=130, Hkv=2) == -2
+    for prompt in (0, 1):
+        splits = lambda *a: lib.mlora_page_attn_splits(prompt, *a)                                                 # noqa: E731
+        assert splits(0, 8, 8, 100) == 1 and splits(1, 8, 8, 1) == 1 and 1 < splits(1, 8, 8, 1 << 20) <= 64 and splits(70000, 8, 8, 1 << 20) == 1 and splits(4, 8, 0, 9) == 1
     assert lib.mlora_page_values(16, 16, 16, 16, 16, 16, 1, 8, 96, 4, None) == -2 and lib.mlora_page_values(16, 16, 16, 16, None, 16, 1, 8, 64, 4, None) == -1
     assert lib.mlora_page_values(16, 16, 16, 16, 16, None, 1, 8, 64, 4, None) == -1 and lib.mlora_page_values(16, 16, 16, 16, 16, 16, 65536, 8, 64, 4, None) == -1
     assert lib.mlora_page_values(16, 16, 16, 16, 16, None, 0, 8, 64, 4, None) == 0
