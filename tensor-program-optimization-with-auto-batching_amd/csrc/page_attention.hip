@@ -100,7 +100,7 @@ __device__ __forceinline__ bool token_ok(const PageAttn& a, int seq, int pos) {
 // How a page's keys or values are rounded, of which a wave holds all
 struct Rounding {
   float most, step;                                        // infinite: codes 0
-  __device__ __forceinline__ int8_t code(float x) const { return (int8_t)(int)rintf(127.f * (most == INFINITY ? 0.f : x) / most); }
+  __device__ __forceinline__ uint32_t code(float x) const { return (uint32_t)((int)rintf(127.f * (most == INFINITY ? 0.f : x) / most) & 255); }
 };
 template <class T, int N>
 __device__ __forceinline__ Rounding rounding_of(const T (&x)[N]) {
@@ -128,14 +128,14 @@ __device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh,
   uint8_t* vp = (uint8_t*)a.v + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 16;
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) {
-    union { int8_t b[16]; uint4 u; } x, y;
+    uint32_t x[4] = {}, y[4] = {};
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      x.b[e] = rk.code((float)k[2 * j + e / 8][e % 8]);
-      y.b[e] = rv.code((float)v[4 * j + e / 4][e % 4]);
+      x[e / 4] |= rk.code((float)k[2 * j + e / 8][e % 8]) << (8 * (e % 4));
+      y[e / 4] |= rv.code((float)v[4 * j + e / 4][e % 4]) << (8 * (e % 4));
     }
-    *reinterpret_cast<uint4*>(kp + j * 1024) = x.u;
-    *reinterpret_cast<uint4*>(vp + j * 1024) = y.u;
+    *reinterpret_cast<uint4*>(kp + j * 1024) = uint4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<uint4*>(vp + j * 1024) = uint4{y[0], y[1], y[2], y[3]};
   }
   if (lane == 0) *reinterpret_cast<f32x2*>(a.step + 2 * ((size_t)page * a.Hkv + kh)) = f32x2{rk.step, rv.step};
 }
@@ -443,48 +443,60 @@ __device__ __forceinline__ int row_of(const PageAttn& a, int t, int pos, int seq
   return r >= 0 && r < a.T && p < a.max_pos && a.tok_seq[r] == seq && a.tok_pos[r] == p ? (int)r : -1;
 }
 
-// The rows of an unrounded page (tokens p0 .. p0 + 15 of seq, of which row t of the pass has position pos), lane (g, token) with dims 32 kb + 8 g .. + 7 of
-// its token: from the pass's rows, and from the tail what stands ahead of them.  Tokens that are in neither are zero.
+// The rows of an unrounded page (tokens p0 .. p0 + 15 of seq, of which the pass has position pos), keys or values, lane (g, token) with dims 32 kb + 8 g .. + 7 of its token:
+// from the pass's row `mine` of the token, and from the tail what stands ahead of those.  Tokens that are in neither are zero.
 template <int D>
-__device__ __forceinline__ void load_own(const PageAttn& a, int seq, int kh, int t, int pos, f16x8 (&k)[D / 32], f16x8 (&v)[D / 32]) {
+__device__ __forceinline__ void load_own(const PageAttn& a, int seq, int kh, int mine, int pos, bool values, f16x8 (&x)[D / 32]) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, p0 = pos / PAGE * PAGE, HH = a.Hq + 2 * a.Hkv;
-  const int mine = row_of(a, t, pos, seq, p0 + col);
-  const size_t at = ((size_t)seq * a.Hkv + kh) * PAGE * D;
+  const size_t at = ((size_t)seq * a.Hkv + kh) * PAGE * D, p = (size_t)(p0 + col) * (D / 2);
+  const f16* row = a.qkv + ((size_t)(mine < 0 ? 0 : mine) * HH + a.Hq + (values ? a.Hkv : 0) + kh) * D;
   if (mine >= 0) {
-    const size_t p = (size_t)(p0 + col) * (D / 2);
-    const f16* row = a.qkv + ((size_t)mine * HH + a.Hq + kh) * D;
 #pragma unroll
-    for (int kb = 0; kb < D / 32; ++kb) v[kb] = ld8(row + (size_t)a.Hkv * D + kb * 32 + g * 8);
-    load_rotated<D>(k, row, a.rope_cos + p, a.rope_sin + p, g);
+    for (int kb = 0; kb < D / 32; ++kb) x[kb] = ld8(row + kb * 32 + g * 8);
+    if (!values)
+#pragma unroll
+      for (int kb = 0; kb < D / 64; ++kb) rotate8(x[kb], x[kb + D / 64], a.rope_cos + p + kb * 32 + g * 8, a.rope_sin + p + kb * 32 + g * 8);
   } else if (p0 + col < pos) {
 #pragma unroll
     for (int kb = 0; kb < D / 32; ++kb) {
-      k[kb] = ld8(a.tail_k + at + kb * 512 + lane * 8);
+      if (!values) x[kb] = ld8(a.tail_k + at + kb * 512 + lane * 8);
+      else
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[kb][e] = a.tail_v[at + (size_t)(kb * 32 + g * 8 + e) * PAGE + col];
+        for (int e = 0; e < 8; ++e) x[kb][e] = a.tail_v[at + (size_t)(kb * 32 + g * 8 + e) * PAGE + col];
     }
   } else {
 #pragma unroll
-    for (int kb = 0; kb < D / 32; ++kb) k[kb] = v[kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    for (int kb = 0; kb < D / 32; ++kb) x[kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
 
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // -126 <= e <= 127
 
-// What a tile's column does not see of P pages, which begin with tokens first[p]: those from lim on, and those ahead of lo but for the sinks.  Of what it sees,
-// the tokens of `bad` (a bit for each of a page's) are NaN.
+// What a tile's column does not see, of P times four tokens that begin with first[p]: those from lim on, and those ahead of lo (0 <= lo, or 0 where nothing is
+// seen) but for the sinks, if there are any.  Of what it sees, the tokens of `bad` (a bit for each of the four) are NaN.
 template <int P>
-__device__ __forceinline__ void tile_mask(f32x4 (&st)[P], const int (&first)[P], int lim, int lo, int sinks, const uint32_t (&bad)[P]) {
-  int g = (threadIdx.x & 63) >> 4;
-  asm volatile("" : "+v"(g), "+v"(lim), "+v"(lo));         // (or its comparisons are made ahead of the branch that seldom leads here)
+__device__ __forceinline__ void tile_mask(f32x4 (&st)[P], const int (&first)[P], int lim, int lo, int sinks, const uint32_t (&bad)[P], bool any_bad) {
+  if (any_bad) {                                           // uniform, seldom
 #pragma unroll
-  for (int p = 0; p < P; ++p)
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int t = first[p] + 4 * g + e;
-      if (bad[p] >> (4 * g + e) & 1) st[p][e] = NAN;
-      if (t >= lim || (t < lo && t >= sinks)) st[p][e] = -INFINITY;
-    }
+      for (int e = 0; e < 4; ++e)
+        if (bad[p] >> e & 1) st[p][e] = NAN;
+  }
+  const uint32_t reach = (uint32_t)max(lim - lo, 0), few = (uint32_t)min(sinks, lim);
+  if (sinks > 0) {                                         // uniform
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((uint32_t)(first[p] + e - lo) >= reach && (uint32_t)(first[p] + e) >= few) st[p][e] = -INFINITY;
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((uint32_t)(first[p] + e - lo) >= reach) st[p][e] = -INFINITY;
+  }
 }
 
 // w - h, of an fp16 number in the lower or upper half of a register (the compiler converts it first)
@@ -535,11 +547,11 @@ __device__ __forceinline__ f16x8 join(f16x2 a, f16x2 b, f16x2 c, f16x2 d) { retu
 
 template <int D, bool Q8, int NT, int NW>
 __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel(PageAttn a) {
-  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, QB = 16 * NT * NW, KLD = QB + 1, VLD = QB + 2;
+  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, QB = 16 * NT * NW, KLD = QB + 1, VLD = D + 8;
   constexpr int NL = Q8 ? D / 64 : D / 32, NU = (8 * NL + NW - 1) / NW;        // KiB of a page's keys or values; pieces of 1 KiB that a wave brings of four pages
   // two buffers of four pages: keys [page][kb][lane][8]; values of 8-bit pages [pair of pages][db][lane][page of the pair][4 tokens], of fp16 pages
-  // [pair][32 dims][page][half of the tokens][dim][8].  Before that, of pages of 8 bits, the tokens' own keys [kb][g][token][8] and values [d][token]
-  constexpr int RING = 16 * PE, OWN = Q8 ? 4 * NKB * KLD * 8 + D * VLD : 0;
+  // [pair][32 dims][page][half of the tokens][dim][8].  Before that, of pages of 8 bits, the tokens' own keys [kb][g][token][8] and values [token][d]
+  constexpr int RING = 16 * PE, OWN = Q8 ? 4 * NKB * KLD * 8 + QB * VLD : 0;
   __shared__ __align__(16) f16 lds[RING > OWN ? RING : OWN];
   __shared__ uint32_t odd[2][4 * NL];                                 // tokens of a page whose values are not all finite, by piece
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
@@ -598,9 +610,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     }
     for (int i = threadIdx.x; i < nt * (D / 8); i += NW * WAVE) {      // 8 dims of a value
       const int r = i / (D / 8), c = i % (D / 8);
-      const f16x8 x = ld8(a.qkv + ((size_t)(t0 + r) * HH + a.Hq + a.Hkv + kh) * D + c * 8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ov[(c * 8 + e) * VLD + r] = x[e];
+      st8(ov + r * VLD + c * 8, ld8(a.qkv + ((size_t)(t0 + r) * HH + a.Hq + a.Hkv + kh) * D + c * 8));
     }
     __syncthreads();
 #pragma unroll
@@ -623,12 +633,14 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
           for (int db = 0; db < NDB; ++db)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[db][e] = ov[(db * 16 + col) * VLD + min(r0 + 4 * g + e, QB - 1)];
+            for (int e = 0; e < 4; ++e) v[db][e] = ov[min(r0 + 4 * g + e, QB - 1) * VLD + db * 16 + col];
         } else {                                                      // tokens ahead of the workgroup's, of the pass or of the tail
-          f16x8 k[NKB], vr[NKB];
-          load_own<D>(a, s, kh, row, ps, k, vr);
+          f16x8 vr[NKB];
+          const int mine = row_of(a, row, ps, s, p * PAGE + col);
+          load_own<D>(a, s, kh, mine, ps, false, vr);
 #pragma unroll
-          for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(k[kb], q[i][kb], st[0]);
+          for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(vr[kb], q[i][kb], st[0]);
+          load_own<D>(a, s, kh, mine, ps, true, vr);
           // rows to columns: the lane of (dim 16 db + col, token 4 g + e) asks lane (dim % 32 / 8, token)
 #pragma unroll
           for (int db = 0; db < NDB; ++db)
@@ -655,12 +667,12 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
             if (y) v[db][e] = (f16)0.f;
           }
           const unsigned long long b = __ballot(not_finite);
-          if (b >> (16 * g) & 0xffff) bad[0] |= 1u << (4 * g + e);
+          if (b >> (16 * g) & 0xffff) bad[0] |= 1u << e;
         }
         const float by[1] = {a.scale}, one[1] = {1.f};
-        const int first[1] = {p * PAGE};
+        const int first[1] = {p * PAGE + 4 * g};
         f16x2 hi[2], low[2];
-        tile_mask<1>(st, first, in ? cpos[i] + 1 : 0, in && a.window > 0 ? cpos[i] - a.window + 1 : 0, a.sinks, bad);
+        tile_mask<1>(st, first, in ? cpos[i] + 1 : 0, in && a.window > 0 ? max(cpos[i] - a.window + 1, 0) : 0, a.sinks, bad, __any(bad[0]));
         tile_weights<D, 1, false>(st, by, one, one, m[i], l[i], o[i], hi, low);
         const f16x8 w = join(hi[0], hi[1], low[0], low[1]);
 #pragma unroll
@@ -699,7 +711,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     for (int i = 0; i < NT; ++i) {
       const bool in = ctok[i] >= c0 && ctok[i] < next && cpos[i] >= 0;
       lim[i] = !in ? 0 : Q8 ? cpos[i] / PAGE * PAGE : cpos[i] + 1;
-      lo[i] = in && a.window > 0 ? cpos[i] - a.window + 1 : 0;
+      lo[i] = in && a.window > 0 ? max(cpos[i] - a.window + 1, 0) : 0;
       int v[4] = {lim[i], lim[i], in ? lo[i] : 0x7fffffff, lo[i]};
 #pragma unroll
       for (int s = 8; s > 0; s >>= 1) {
@@ -758,7 +770,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
         const int k = ex == NO_EXP ? 0 : max(ex - unit_next, -24);    // (exact: codes have seven bits, fp16 numbers multiples of 2^-24)
         const float f = ex == NO_EXP ? 1.f : rstep[1] * power(-(unit_next + k));
         const float lane_by = ek == 255 ? 1.f : fmaxf(a.scale * rstep[0], 0x1p-126f);        // (a page of zeros: scores of zero, and -inf stays what it is)
-        const float lane_up = __builtin_amdgcn_logf(f), lane_share = 1.f / f;
+        const float lane_up = __builtin_amdgcn_logf(f), lane_share = __builtin_amdgcn_rcpf(f);
         const float mult = ex == NO_EXP ? 0.f : power(k);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -839,7 +851,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
       for (int i = 0; i < NT; ++i) any = any || sees[i];
       if (any) {                                                      // uniform over the wave
-        uint32_t bad[4];
+        uint32_t bad[4];                                              // of the pages
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           bad[p] = Q8 && (nans >> p & 1) ? 0xffffu : 0u;
@@ -853,17 +865,20 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
         if (bad[0] | bad[1] | bad[2] | bad[3])
 #pragma unroll
           for (int i = 0; i < NT; ++i) whole[i] = false;
+        // Four products of scores.  8 bits: of a page each; a lane has tokens 4 g .. + 3, as its values lie.  fp16: two of a pair of pages, so that over both a lane has the
+        // eight tokens that are 16 bytes of the values as they come, half g % 2 of page g / 2
         f32x4 st[NT][4];
-        const f16* kl = lds + buf * 4 * PE + lane * 8;
+        const f16* kl = lds + buf * 4 * PE + (Q8 ? lane * 8 : (col >> 3) * PE + (g * 16 + (col >> 2 & 1) * 8 + (col & 3)) * 8);
+        auto keys = [&](int p, int kb) { return ld8(kl + (Q8 ? p * PE : (p >> 1) * 2 * PE + (p & 1) * 32) + kb * 512); };
         constexpr int KR = NT == 1 ? 1 : 2;
         f16x8 k[KR][NKB];                                             // a page's keys while those of the one before are multiplied
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) k[0][kb] = ld8(kl + kb * 512);
+        for (int kb = 0; kb < NKB; ++kb) k[0][kb] = keys(0, kb);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           if (KR == 2 ? p < 3 : p > 0)
 #pragma unroll
-            for (int kb = 0; kb < NKB; ++kb) k[KR == 2 ? (p + 1) & 1 : 0][kb] = ld8(kl + (KR == 2 ? p + 1 : p) * PE + kb * 512);
+            for (int kb = 0; kb < NKB; ++kb) k[KR == 2 ? (p + 1) & 1 : 0][kb] = keys(KR == 2 ? p + 1 : p, kb);
 #pragma unroll
           for (int i = 0; i < NT; ++i) st[i][p] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -875,20 +890,23 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           if (!whole[i]) {                                            // uniform
-            int first[4];
+            int first[4], gm = g, lim_ = lim[i], lo_ = lo[i];
+            asm volatile("" : "+v"(gm), "+v"(lim_), "+v"(lo_));       // (or the comparisons are made ahead of the branch that seldom leads here)
+            uint32_t four[4];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) first[p] = there >> p & 1 ? first0 + p * PAGE : 0x3fffffff;
-            tile_mask<4>(st[i], first, lim[i], lo[i], a.sinks, bad);
+            for (int p = 0; p < 4; ++p) {
+              const int page = Q8 ? p : (p & 2) + (gm >> 1), in = Q8 ? 4 * gm : 8 * (gm & 1) + 4 * (p & 1);
+              first[p] = there >> page & 1 ? first0 + page * PAGE + in : 0x3fffffff;
+              four[p] = (Q8 ? bad[p] : gm >> 1 ? bad[p | 1] : bad[p & 2]) >> in & 15;
+            }
+            tile_mask<4>(st[i], first, lim_, lo_, first0 < a.sinks ? a.sinks : 0, four, (bad[0] | bad[1] | bad[2] | bad[3]) != 0);
           }
           tile_weights<D, 4, Q8>(st[i], by, up, share, m[i], l[i], o[i], hi[i], low[i]);
         }
-        const f16* vl = lds + 8 * PE + buf * 4 * PE + (Q8 ? lane * 8 : (g >> 1) * 256 + col * 8 + (g & 1) * 4);
+        const f16* vl = lds + 8 * PE + buf * 4 * PE + (Q8 ? lane * 8 : (g >> 1) * 512 + (g & 1) * 256 + col * 8);
         auto values = [&](int j) {                                    // of pair j / NDB, dims 16 (j % NDB) ..
           const int pair = j / NDB, db = j % NDB;
-          if constexpr (Q8) return ld8(vl + (pair * NDB + db) * 512);
-          const f16* p = vl + pair * 2 * PE + (db >> 1) * 1024 + (db & 1) * 128;
-          const f16x4 x = *reinterpret_cast<const f16x4*>(p), y = *reinterpret_cast<const f16x4*>(p + 512);
-          return f16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+          return ld8(vl + (Q8 ? (pair * NDB + db) * 512 : pair * 2 * PE + (db >> 1) * 1024 + (db & 1) * 128));
         };
         constexpr int AHEAD = NT == 1 ? 2 : 4;
         f16x8 v[AHEAD];
@@ -939,59 +957,94 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
   }
 }
 
-// Pages that a pass completes, in 8 bits: a wave has 16 tokens of the pass and a kv head, and of them those that are the first of their page in the pass.  Values
-// are turned over as codes, by way of LDS.
+// Pages that a pass completes, in 8 bits: a wave has the keys or the values of 16 tokens of the pass under a kv head, and of the tokens those that are the first of their page
+// in the pass.  D / 16 lanes take a token's row, so that a load's lines are whole; the codes go by way of LDS into their order.
 template <int D>
 __global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
-  constexpr int LD = 20;                                              // bytes of a dim's tokens in LDS, apart for the banks
+  constexpr int LD = 20, NCH = D / 16, PER = WAVE / NCH, NP = 16 / PER;       // bytes of a dim's tokens in LDS, apart for the banks; lanes of a row; rows of a load; loads
   __shared__ __align__(16) uint8_t turn[4][D * LD];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, kh = blockIdx.y * 4 + wave, t0 = blockIdx.x * 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, kh = blockIdx.y * 2 + (wave >> 1), t0 = blockIdx.x * 16;
+  const int ch = lane % NCH, HH = a.Hq + 2 * a.Hkv;
+  const bool values = wave & 1;                                       // uniform
   if (kh >= a.Hkv) return;
-  const int t = t0 + col;
+  // a lane knows token t0 - 16 + lane: all that the pages of the wave's tokens can reach
+  const int t = t0 - 16 + lane;
   int seq = -1, pos = -1;
-  bool lead = false;
-  if (t < a.T) {
+  if (t >= 0 && t < a.T) {
     seq = a.tok_seq[t];
     pos = a.tok_pos[t];
-    if (token_ok(a, seq, pos)) {
-      lead = t == 0 || pos % PAGE == 0 || a.tok_seq[t - 1] != seq || a.tok_pos[t - 1] != pos - 1;
-      lead = lead && row_of(a, t, pos, seq, pos / PAGE * PAGE + PAGE - 1) >= 0;
-    }
+    if (!token_ok(a, seq, pos)) seq = -1;
   }
-  unsigned todo = (unsigned)(__ballot(lead) & 0xffff);
+  const int before_seq = __shfl(seq, lane - 1, WAVE), before_pos = __shfl(pos, lane - 1, WAVE);
+  const int last = (lane + PAGE - 1 - pos % PAGE) & 63, last_seq = __shfl(seq, last, WAVE), last_pos = __shfl(pos, last, WAVE);      // of its page's last token
+  bool lead = lane >= 16 && lane < 32 && seq >= 0 && (pos % PAGE == 0 || before_seq != seq || before_pos != pos - 1);
+  lead = lead && last_seq == seq && last_pos == pos / PAGE * PAGE + PAGE - 1;
+  int page = -1;
+  if (lead) page = a.block_table[(size_t)seq * a.max_blocks + pos / PAGE];
+  unsigned todo = (unsigned)__ballot(lead);
   while (todo) {
     const int c = __builtin_ctz(todo);
     todo &= todo - 1;
-    const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(pos, c);
-    const int id = a.block_table[(size_t)s * a.max_blocks + p / PAGE];
-    if (id < 0 || id >= a.n_pages) continue;                          // uniform
-    f16x8 k[D / 32], v[D / 32];
-    load_own<D>(a, s, kh, t0 + c, p, k, v);
-    const Rounding rk = rounding_of(k), rv = rounding_of(v);
-    uint8_t* kp = (uint8_t*)a.k + ((size_t)id * a.Hkv + kh) * PAGE * D + lane * 16;
-    uint8_t* vp = (uint8_t*)a.v + ((size_t)id * a.Hkv + kh) * PAGE * D + lane * 16;
+    const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(pos, c), p0 = p / PAGE * PAGE;
+    f16x8 x[2 * NP];                                                  // dims 8 ch .. + 7 of a token, then those half a row on
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      union { int8_t b[16]; uint4 u; } x;
+    for (int i = 0; i < NP; ++i) {
+      const int token = lane / NCH + PER * i, from = c + token - (p - p0);                  // the lane that knows the token
+      const int from_seq = __shfl(seq, from, WAVE), from_pos = __shfl(pos, from, WAVE);
+      if (from_seq == s && from_pos == p0 + token) {
+        const f16* row = a.qkv + ((size_t)(t0 - 16 + from) * HH + a.Hq + (values ? a.Hkv : 0) + kh) * D + ch * 8;
+        x[2 * i] = ld8(row);
+        x[2 * i + 1] = ld8(row + D / 2);
+        if (!values) {
+          const size_t at = (size_t)(p0 + token) * (D / 2) + ch * 8;
+          rotate8(x[2 * i], x[2 * i + 1], a.rope_cos + at, a.rope_sin + at);
+        }
+      } else {                                                        // (a page that the pass completes has its other tokens in the tail)
+        const size_t at = ((size_t)s * a.Hkv + kh) * PAGE * D;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x.b[e] = rk.code((float)k[2 * j + e / 8][e % 8]);
-        turn[wave][(64 * j + 32 * (e / 8) + 8 * g + e % 8) * LD + col] = (uint8_t)rv.code((float)v[2 * j + e / 8][e % 8]);
+        for (int h = 0; h < 2; ++h) {
+          const int k8 = ch + h * NCH;                                // dims 8 k8 ..
+          if (!values) x[2 * i + h] = ld8(a.tail_k + at + ((size_t)k8 * 16 + token) * 8);
+          else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[2 * i + h][e] = a.tail_v[at + (size_t)(k8 * 8 + e) * PAGE + token];
+        }
       }
-      *reinterpret_cast<uint4*>(kp + j * 1024) = x.u;
+    }
+    const int id = __builtin_amdgcn_readlane(page, c);
+    if (id < 0 || id >= a.n_pages) continue;                          // uniform
+    const Rounding r = rounding_of(x);
+    uint8_t* at = turn[wave];
+#pragma unroll
+    for (int i = 0; i < 2 * NP; ++i) {
+      const int token = lane / NCH + PER * (i / 2), k8 = ch + (i % 2) * NCH;
+      uint32_t y[2] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e / 4] |= r.code((float)x[i][e]) << (8 * (e % 4));
+      if (!values) *reinterpret_cast<uint2*>(at + (((k8 / 8) * 4 + k8 % 4) * 16 + token) * 16 + (k8 / 4 % 2) * 8) = uint2{y[0], y[1]};
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) at[(k8 * 8 + e) * LD + token] = (uint8_t)(y[e / 4] >> (8 * (e % 4)));
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    uint8_t* to = (uint8_t*)(values ? a.v : a.k) + ((size_t)id * a.Hkv + kh) * PAGE * D + lane * 16;
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
-      uint32_t y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint32_t*>(&turn[wave][(64 * j + 16 * i + col) * LD + 4 * g]);
-      *reinterpret_cast<uint4*>(vp + j * 1024) = uint4{y[0], y[1], y[2], y[3]};
+      uint4 y;
+      if (!values) y = *reinterpret_cast<const uint4*>(at + j * 1024 + lane * 16);
+      else {
+        const uint8_t* from = at + (64 * j + col) * LD + 4 * g;
+        y = uint4{*reinterpret_cast<const uint32_t*>(from), *reinterpret_cast<const uint32_t*>(from + 16 * LD), *reinterpret_cast<const uint32_t*>(from + 32 * LD),
+                  *reinterpret_cast<const uint32_t*>(from + 48 * LD)};
+      }
+      *reinterpret_cast<uint4*>(to + j * 1024) = y;
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (lane == 0) *reinterpret_cast<f32x2*>(a.step + 2 * ((size_t)id * a.Hkv + kh)) = f32x2{rk.step, rv.step};
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (lane == 0) a.step[2 * ((size_t)id * a.Hkv + kh) + values] = r.step;
   }
 }
 
@@ -1105,7 +1158,7 @@ template <int D>
 int prefill(const PageAttn& a, hipStream_t s) {
   if (!a.step) return launch_prefill<D, false>(a, s);
   const dim3 tiles(ceil_div(a.T, 16), ceil_div(a.Hkv, 4));
-  hipLaunchKernelGGL(page_store_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);
+  hipLaunchKernelGGL(page_store_kernel<D>, dim3(ceil_div(a.T, 16), ceil_div(a.Hkv, 2)), dim3(4 * WAVE), 0, s, a);
   if (int e = mlora_launch_status("page_attn_prefill")) return e;
   if (int e = launch_prefill<D, true>(a, s)) return e;
   hipLaunchKernelGGL(page_tail_kernel<D>, tiles, dim3(4 * WAVE), 0, s, a);

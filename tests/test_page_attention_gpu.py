@@ -285,3 +285,25 @@ def test_refusals(ops):
             ops.QuantPages(*bad)
     with pytest.raises(ValueError):
         ops.QuantPages.empty(4, 2, 2, 96, book.dev)
+
+
+def test_quotients_half_way_between_two_codes(ops):
+    """Pages of small whole numbers, whose 127 x / a are often exactly half-way: ties go to the even code, also beside a page of zeros and one with an infinity."""
+    g = torch.Generator().manual_seed(11)
+    for most in (254, 2, 127, 508, 1016, 6, 40, 2032):
+        book = Book([0], 4, 2, 64, True, seed=most, room=70)
+        y = torch.randint(-most, most + 1, (64, 8, 64), generator=g).to(book.dev).half()
+        y[:, 6:, 0] = most
+        y[5, 7, 3], y[20, 7, 9] = 0, most / 2
+        y[32:48, 6] = 0
+        x, seqs, poss, q = book.take(y, [0], [64], [0] * 64, list(range(64)))
+        book.cos.fill_(1), book.sin.fill_(0)               # keys as they come
+        book.k[0] = x[:, 4:6].clone()
+        prompt(ops, book, x, seqs, poss)
+        book.same_pages(0)
+        one = Book([0], 4, 2, 64, True, seed=most, room=70)
+        one.cos.fill_(1), one.sin.fill_(0)
+        for t in range(64):
+            step(ops, one, x[t:t + 1], seqs[t:t + 1], poss[t:t + 1])
+        one.k, one.v, one.lens = book.k, book.v, book.lens
+        one.same_pages(0)
