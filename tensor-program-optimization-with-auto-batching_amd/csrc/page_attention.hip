@@ -214,8 +214,8 @@ __global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
       int id = bt[own];
       if (id < 0 || id >= a.n_pages) id = -1;
       const bool there = Q8 || id >= 0;                     // uniform
-      f16* kp = Q8 ? a.tail_k + ((size_t)seq * a.Hkv + kh) * PAGE * D : (f16*)a.k + ((size_t)(there ? id : 0) * a.Hkv + kh) * PAGE * D;
-      f16* vp = Q8 ? a.tail_v + ((size_t)seq * a.Hkv + kh) * PAGE * D : (f16*)a.v + ((size_t)(there ? id : 0) * a.Hkv + kh) * PAGE * D;
+      const f16* kp = Q8 ? a.tail_k + ((size_t)seq * a.Hkv + kh) * PAGE * D : (const f16*)a.k + ((size_t)(there ? id : 0) * a.Hkv + kh) * PAGE * D;
+      const f16* vp = Q8 ? a.tail_v + ((size_t)seq * a.Hkv + kh) * PAGE * D : (const f16*)a.v + ((size_t)(there ? id : 0) * a.Hkv + kh) * PAGE * D;
       if (there) {
         f16x8 k[NKB], kn[NKB];
         f16x4 v[NDB];
@@ -227,17 +227,13 @@ __global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
         load_rotated<D>(kn, a.qkv + ((size_t)b * (a.Hq + 2 * a.Hkv) + a.Hq + kh) * D, rc, rs, g);
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
-          if (col == slot) {
-            k[kb] = kn[kb];
-            st8(kp + kb * 512 + lane * 8, kn[kb]);
-          }
+          if (col == slot) k[kb] = kn[kb];
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
           const f16 x = vn[db * 16];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (4 * g + e == slot) v[db][e] = x;
-          if (g == slot / 4) vp[(db * 16 + col) * PAGE + slot] = x;
         }
         if constexpr (Q8) {
           if (slot == PAGE - 1 && id >= 0) store_codes<D>(a, id, kh, k, v);
@@ -347,6 +343,24 @@ __global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
           work(r[u]);
           load(r[u], c + u + RING);
         }
+      }
+    }
+    // The token is appended last, by stores that go past the caches: a wave's loads are waited for behind its stores, and 256 rows of 1080 tokens under
+    // 32 / 8 heads take 125 us so, 131 with the stores ahead of the pages (114 with none: they touch 48 lines of a page for a token's two).
+    if (mine) {
+      const int id = bt[own];
+      if (Q8 || (id >= 0 && id < a.n_pages)) {
+        const size_t at = ((size_t)(Q8 ? seq : id) * a.Hkv + kh) * PAGE * D;
+        f16* kp = Q8 ? a.tail_k + at : (f16*)a.k + at;
+        f16* vp = Q8 ? a.tail_v + at : (f16*)a.v + at;
+        const f16* row = a.qkv + ((size_t)b * (a.Hq + 2 * a.Hkv) + a.Hq + kh) * D;
+        f16x8 k[NKB];
+        load_rotated<D>(k, row, rc, rs, g);
+        if (col == slot)
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) __builtin_nontemporal_store(k[kb], reinterpret_cast<f16x8*>(kp + kb * 512 + lane * 8));
+#pragma unroll
+        for (int d = lane; d < D; d += WAVE) __builtin_nontemporal_store(row[a.Hkv * D + d], vp + d * PAGE + slot);
       }
     }
   }
