@@ -38,19 +38,20 @@ struct Best {
   int v;
 };
 
-// (z, v) takes its place; those that are equal to it and there already have lower columns
+// (z, v) takes its place behind those that are greater, or equal and of lower columns
 __device__ __forceinline__ void insert(Best& b, int k, float z, int v) {
   const int lane = threadIdx.x & 63;
-  const int at = __popcll(__ballot(lane < k && b.z >= z));
-  const float uz = __shfl_up(b.z, 1, WAVE);
-  const int uv = __shfl_up(b.v, 1, WAVE);
+  const int at = __popcll(__ballot(lane < k && (b.z > z || (b.z == z && b.v < v))));
+  const float uz = __uint_as_float(dpp<0x138>(__float_as_uint(b.z)));           // the lane's before
+  const int uv = (int)dpp<0x138>((uint32_t)b.v);
   if (lane == at) b = Best{z, v};
   else if (lane > at) b = Best{uz, uv};
 }
 
 __device__ __forceinline__ float last(const Best& b, int k) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(b.z), k - 1)); }
 
-// Wave (part, row): the row's tiles part * per .. of 1024 columns
+// Wave (part, row): the row's tiles part * per .. of 1024 columns, of which it has one in registers and the next on its way.  64 requests of 8 beams over
+// 128256 columns take 50 us, 5.3 TB/s: the rate of the memory.  4 beams over 32000: 5 us, most of it the launch and one read's latency.
 __global__ __launch_bounds__(4 * WAVE) void beam_scan_kernel(Best* __restrict__ best, f32x2* __restrict__ sums, const float* __restrict__ logits, long ld,
                                                              const float* __restrict__ scores, const int32_t* __restrict__ ended, int V, int k, int parts, int per) {
   constexpr int E = TILE / (4 * WAVE);
@@ -63,13 +64,18 @@ __global__ __launch_bounds__(4 * WAVE) void beam_scan_kernel(Best* __restrict__ 
   float m = -INFINITY, s = 0.f;
   f32x4 z[E], nz[E];
   auto load = [&](f32x4 (&z)[E], int tile) {
+    const int c0 = tile * TILE - lead;
+    if (c0 >= 0 && c0 + TILE <= V) {                                            // uniform
 #pragma unroll
-    for (int u = 0; u < E; ++u) {
-      const int c = tile * TILE - lead + (u * WAVE + lane) * 4;
-      if (c >= 0 && c + 3 < V) z[u] = *reinterpret_cast<const f32x4*>(zr + c);
-      else
+      for (int u = 0; u < E; ++u) z[u] = *reinterpret_cast<const f32x4*>(zr + c0 + (u * WAVE + lane) * 4);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[u][e] = c + e >= 0 && c + e < V ? zr[c + e] : -INFINITY;
+      for (int u = 0; u < E; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = c0 + (u * WAVE + lane) * 4 + e;
+          z[u][e] = c >= 0 && c < V ? zr[c] : -INFINITY;
+        }
     }
   };
   const int from = part * per, tiles = (V + lead + TILE - 1) / TILE, to = min(from + per, tiles);
@@ -90,25 +96,30 @@ __global__ __launch_bounds__(4 * WAVE) void beam_scan_kernel(Best* __restrict__ 
     for (int u = 0; u < E; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((z[u][e] - base) * LOG2E);       // (the difference is exact where it counts)
-    // what beats the last of the best goes in, the greatest first
-    float least = last(b, k);
-    while (__any(top > least)) {
-      const float w = all_max(top);
-      int v = 0x7fffffff;                                                       // the lane's lowest column with it
-#pragma unroll
-      for (int u = E - 1; u >= 0; --u)
-#pragma unroll
-        for (int e = 3; e >= 0; --e) v = z[u][e] == w ? tile * TILE - lead + (u * WAVE + lane) * 4 + e : v;
-      v = (int)all_min((uint32_t)v);
-      insert(b, k, w, v);
-      least = last(b, k);
-      top = -INFINITY;
+    // What beats the last of the best goes in.  When more than k lanes have such a logit, the k-th of the lanes' greatest is a bound that no less one passes,
+    // found by taking the greatest away k - 1 times: the columns are looked through once (50 us, above; 72 where they are for each logit that is taken).
+    const float least = last(b, k);
+    if (__any(top > least)) {
+      float bound = least;
+      if (__popcll(__ballot(top > least)) > k) {
+        float t = top;
+        for (int i = 1; i < k; ++i) {
+          const unsigned long long first = __ballot(t == all_max(t));
+          if (lane == __builtin_ctzll(first)) t = -INFINITY;
+        }
+        bound = all_max(t);                                                     // > least, and taken itself
+      }
 #pragma unroll
       for (int u = 0; u < E; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (tile * TILE - lead + (u * WAVE + lane) * 4 + e == v) z[u][e] = -INFINITY;
-          top = fmaxf(top, z[u][e]);
+          unsigned long long in = __ballot(z[u][e] > least && z[u][e] >= bound);
+          while (in) {                                                          // uniform
+            const int l = __builtin_ctzll(in);
+            in &= in - 1;
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(z[u][e]), l));
+            insert(b, k, w, tile * TILE - lead + (u * WAVE + l) * 4 + e);       // (one that is behind all of them falls off the end)
+          }
         }
     }
 #pragma unroll
@@ -121,93 +132,83 @@ __global__ __launch_bounds__(4 * WAVE) void beam_scan_kernel(Best* __restrict__ 
   if (lane == 0) sums[at] = f32x2{M, s};
 }
 
-// A request: every beam's parts merged by a wave, then the beams by one
-__global__ __launch_bounds__(4 * WAVE) void beam_join_kernel(float* __restrict__ out_scores, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
-                                                             const Best* __restrict__ best, const f32x2* __restrict__ sums, const float* __restrict__ scores,
-                                                             const int32_t* __restrict__ ended, int eos, int W, int k, int parts) {
+// A request, of which a wave each merges a beam's parts.  A candidate's place is then the number of those ahead of it: in its own beam, which is looked through,
+// and in the others, whose values fall, by halving.  9 us for 64 requests of 8 beams, 6 for one of 4 (17 and 9 with four waves a request that take out the
+// greatest k times): bound by steps that wait for one another, most of them the merge's.
+__global__ __launch_bounds__(MAX_BEAMS* WAVE) void beam_join_kernel(float* __restrict__ out_scores, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
+                                                                    const Best* __restrict__ best, const f32x2* __restrict__ sums, const float* __restrict__ scores,
+                                                                    const int32_t* __restrict__ ended, int eos, int W, int k, int parts) {
   __shared__ double value[MAX_BEAMS * MAX_BEST];
   __shared__ int column[MAX_BEAMS * MAX_BEST];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x;
-  for (int w = wave; w < W; w += 4) {
-    const int row = r * W + w;
-    const float score = scores[row];
-    Best b = {-INFINITY, 0x7fffffff};
-    double val = -INFINITY;
-    if (!(score > -INFINITY)) {
-    } else if (ended && ended[row]) {
-      if (lane == 0) b.v = eos, val = score;
-    } else {
-      float M = -INFINITY;
-      for (int i = lane; i < parts; i += WAVE) M = fmaxf(M, sums[(size_t)row * parts + i][0]);
-      M = all_max(M);
-      double s = 0;
-      for (int i = lane; i < parts; i += WAVE) {
-        const f32x2 x = sums[(size_t)row * parts + i];
-        s += x[0] == -INFINITY && x[1] == 0.f ? 0. : (double)x[1] * exp2(((double)x[0] - M) * 1.4426950408889634);
-      }
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = blockIdx.x, row = r * W + w;
+  const int n = parts * k;
+  const float score = scores[row];
+  const bool over = ended && ended[row];
+  // (requested together; of a row that the first launch passed over they hold anything, and are not looked at)
+  const f32x2 none = {-INFINITY, 0.f}, first = lane < parts ? sums[(size_t)row * parts + lane] : none;
+  Best c = lane < n ? best[(size_t)row * n + lane] : Best{-INFINITY, 0x7fffffff};
+  Best b = {-INFINITY, 0x7fffffff};
+  double val = -INFINITY;
+  if (!(score > -INFINITY)) {                                                   // uniform
+  } else if (over) {
+    if (lane == 0) b.v = eos, val = score;
+  } else {
+    float M = first[0];
+    for (int i = lane + WAVE; i < parts; i += WAVE) M = fmaxf(M, sums[(size_t)row * parts + i][0]);
+    M = all_max(M);
+    double s = 0;
+    for (int i = lane; i < parts; i += WAVE) {
+      const f32x2 x = i == lane ? first : sums[(size_t)row * parts + i];
+      s += x[0] == -INFINITY && x[1] == 0.f ? 0. : (double)x[1] * exp2(((double)x[0] - M) * 1.4426950408889634);
+    }
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, WAVE);
-      const double lse = M + log(s);
-      const int n = parts * k;
-      for (int i0 = 0; i0 < n; i0 += WAVE) {                                    // (parts are in the order of their columns)
-        Best c = i0 + lane < n ? best[(size_t)row * n + i0 + lane] : Best{-INFINITY, 0x7fffffff};
-        float least = last(b, k);
-        while (__any(c.z > least)) {
-          const float z = all_max(c.z);
-          const int v = (int)all_min(c.z == z ? (uint32_t)c.v : 0x7fffffffu);
-          insert(b, k, z, v);
-          least = last(b, k);
-          if (c.v == v) c.z = -INFINITY;
-        }
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, WAVE);
+    const double lse = M + log(s);
+    for (int i0 = 0; i0 < n; i0 += WAVE) {
+      if (i0 > 0) c = i0 + lane < n ? best[(size_t)row * n + i0 + lane] : Best{-INFINITY, 0x7fffffff};
+      while (__any(c.z > last(b, k))) {                                         // (parts are in the order of their columns)
+        const float z = all_max(c.z);
+        const int v = (int)all_min(c.z == z ? (uint32_t)c.v : 0x7fffffffu);
+        insert(b, k, z, v);
+        if (c.v == v) c.z = -INFINITY;
       }
-      if (b.z > -INFINITY) val = (double)score + ((double)b.z - lse);
     }
-    if (lane < k) {
-      value[w * k + lane] = val;
-      column[w * k + lane] = b.v;
-    }
+    if (b.z > -INFINITY) val = (double)score + ((double)b.z - lse);
+    if (!(val > -INFINITY)) val = -INFINITY;                                    // NaN is no candidate
+  }
+  if (lane < k) {
+    value[w * k + lane] = val;
+    column[w * k + lane] = b.v;
   }
   __syncthreads();
-  if (wave > 0) return;
-  constexpr int PER = MAX_BEAMS * MAX_BEST / WAVE;
-  double x[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) x[j] = j * WAVE + lane < W * k ? value[j * WAVE + lane] : -INFINITY;
-  for (int i = 0; i < k; ++i) {
-    double top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) top = x[j] > top ? x[j] : top;                // (NaN is no candidate)
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const double y = __shfl_xor(top, o, WAVE);
-      top = y > top ? y : top;
-    }
-    // entries lie by beam, those of a beam by logit and column: the first of equal ones has the lowest b V + v
-    // unless rounding made the values of different logits equal, so columns are compared
-    unsigned long long id = ~0ull;                                              // beam, column, entry
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int e = j * WAVE + lane;
-      if (top > -INFINITY && x[j] == top) {
-        const unsigned long long y = (unsigned long long)(e / k) << 48 | (unsigned long long)(uint32_t)column[e] << 16 | (unsigned)e;
-        id = y < id ? y : id;
+  int place = 0;
+  for (int o = 0; o < W; ++o) {
+    if (o == w) {
+      for (int i = 0; i < k; ++i) {
+        const double x = value[w * k + i];
+        place += x > val || (x == val && column[w * k + i] < b.v);
       }
-    }
+    } else {                                                                    // equal ones of an earlier beam are ahead
+      int n = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const unsigned long long y = __shfl_xor(id, o, WAVE);
-      id = y < id ? y : id;
+      for (int step = MAX_BEST; step > 0; step >>= 1)
+        if (n + step <= k) {
+          const double x = value[o * k + n + step - 1];
+          if (x > val || (x == val && o < w)) n += step;
+        }
+      place += n;
     }
-    const bool none = id == ~0ull;
-    const int e = (int)(id & 0xffff);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (!none && j * WAVE + lane == e) x[j] = -INFINITY;
-    if (lane == 0) {
-      out_scores[(size_t)r * k + i] = none ? -INFINITY : (float)top;
-      tokens[(size_t)r * k + i] = none ? -1 : column[e];
-      parents[(size_t)r * k + i] = none ? -1 : e / k;
-    }
+  }
+  const bool in = lane < k && val > -INFINITY;
+  if (in && place < k) {
+    out_scores[(size_t)r * k + place] = (float)val;
+    tokens[(size_t)r * k + place] = b.v;
+    parents[(size_t)r * k + place] = w;
+  }
+  const int all = __syncthreads_count(in);                                      // fewer than k candidates: none behind them
+  if (w == 0 && lane >= all && lane < k) {
+    out_scores[(size_t)r * k + lane] = -INFINITY;
+    tokens[(size_t)r * k + lane] = parents[(size_t)r * k + lane] = -1;
   }
 }
 
@@ -257,26 +258,30 @@ __global__ __launch_bounds__(WAVE) void beam_reorder_kernel(int32_t* __restrict_
   }
 }
 
-// Rows copied within pools [layers][n][bytes]: a workgroup has a piece of a row
-constexpr int MAX_POOLS = 8, PIECE = 8192;
+// Rows copied within pools [layers][n][bytes]: a workgroup has a piece of a row, each thread 64 bytes of it on their way at once.  600 pages of 32 KiB in two
+// pools of 16 layers, 1.26 GB read and written: 260 us, 4.8 TB/s, near the 5.2 of one large copy.  A step of 16 requests of 4 beams, in 32 layers: 19 us.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr int MAX_POOLS = 8, PIECE = 16384;
+struct Pool {
+  uint8_t* p;
+  size_t layer;                // bytes of a layer
+  int bytes, pieces, rows;     // of a row; pieces of a row; rows
+  int begin;                   // the first unit
+};
 struct Pools {
-  uint8_t* p[MAX_POOLS];
-  size_t layer[MAX_POOLS];     // bytes of a layer
-  int bytes[MAX_POOLS], pieces[MAX_POOLS], rows[MAX_POOLS], begin[MAX_POOLS + 1];       // of a row; pieces of a row; rows; the first unit
-  int n;
+  Pool at[MAX_POOLS];
 };
 
 template <class T>
 __device__ __forceinline__ void copy_piece(uint8_t* __restrict__ to, const uint8_t* __restrict__ from, int bytes) {
-  constexpr int U = PIECE / 256 / sizeof(T) < 4 ? PIECE / 256 / sizeof(T) : 4;
   const int n = bytes / (int)sizeof(T);
-  for (int i0 = threadIdx.x; i0 < n; i0 += 256 * U) {
-    T x[U];
+  for (int i0 = threadIdx.x; i0 < n; i0 += 256 * 4) {
+    T x[4];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < 4; ++u)
       if (i0 + u * 256 < n) x[u] = reinterpret_cast<const T*>(from)[i0 + u * 256];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < 4; ++u)
       if (i0 + u * 256 < n) reinterpret_cast<T*>(to)[i0 + u * 256] = x[u];
   }
 }
@@ -284,17 +289,18 @@ __device__ __forceinline__ void copy_piece(uint8_t* __restrict__ to, const uint8
 __global__ __launch_bounds__(256) void copy_pages_kernel(Pools a, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int pairs) {
   const int unit = blockIdx.x;
   int i = 0;
-  while (i + 1 < a.n && unit >= a.begin[i + 1]) ++i;
-  const int u = unit - a.begin[i], layer = u / a.pieces[i], piece = u % a.pieces[i];
-  const int off = piece * PIECE, bytes = min(PIECE, a.bytes[i] - off);
-  uint8_t* base = a.p[i] + a.layer[i] * layer + off;
+#pragma unroll
+  for (int k = 1; k < MAX_POOLS; ++k) i += unit >= a.at[k].begin;
+  const Pool p = a.at[i];                                                       // uniform: read from the arguments
+  const int u = unit - p.begin, layer = u / p.pieces, off = (u - layer * p.pieces) * PIECE, bytes = min(PIECE, p.bytes - off);
+  uint8_t* base = p.p + p.layer * layer + off;
   for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
     const int s = src[pair], d = dst[pair];
-    if (s < 0 || s >= a.rows[i] || d < 0 || d >= a.rows[i] || s == d) continue;         // uniform
-    uint8_t* to = base + (size_t)d * a.bytes[i];
-    const uint8_t* from = base + (size_t)s * a.bytes[i];
+    if (s < 0 || s >= p.rows || d < 0 || d >= p.rows || s == d) continue;               // uniform
+    uint8_t* to = base + (size_t)d * p.bytes;
+    const uint8_t* from = base + (size_t)s * p.bytes;
     const size_t all = (uintptr_t)to | (uintptr_t)from | (size_t)bytes;                 // uniform
-    if ((all & 15) == 0) copy_piece<uint4>(to, from, bytes);
+    if ((all & 15) == 0) copy_piece<u32x4>(to, from, bytes);
     else if ((all & 3) == 0) copy_piece<uint32_t>(to, from, bytes);
     else copy_piece<uint8_t>(to, from, bytes);
   }
@@ -337,7 +343,7 @@ extern "C" int mlora_beam_select(float* out_scores, int32_t* tokens, int32_t* pa
   hipStream_t s = (hipStream_t)stream;
   hipLaunchKernelGGL(beam_scan_kernel, dim3(ceil_div(cut.parts, 4), R * W), dim3(4 * WAVE), 0, s, best, sums, logits, ld, scores, ended, V, k, cut.parts, cut.per);
   if (int e = mlora_launch_status("beam_select")) return e;
-  hipLaunchKernelGGL(beam_join_kernel, dim3(R), dim3(4 * WAVE), 0, s, out_scores, tokens, parents, (const Best*)best, (const f32x2*)sums, scores, ended, eos, W, k, cut.parts);
+  hipLaunchKernelGGL(beam_join_kernel, dim3(R), dim3(W * WAVE), 0, s, out_scores, tokens, parents, (const Best*)best, (const f32x2*)sums, scores, ended, eos, W, k, cut.parts);
   return mlora_launch_status("beam_select");
 }
 
@@ -356,22 +362,17 @@ extern "C" int mlora_copy_pages(const mlora_page_pool* pools, int n_pools, const
   MLORA_CHECK(pools && (n == 0 || (src && dst)), MLORA_ERR_INVALID, "copy_pages: null pointer");
   MLORA_CHECK(n_pools >= 1 && n_pools <= MAX_POOLS && n >= 0, MLORA_ERR_INVALID, "copy_pages: %d rows of %d pools, at most %d", n, n_pools, MAX_POOLS);
   Pools a = {};
-  a.n = n_pools;
   long units = 0;
   for (int i = 0; i < n_pools; ++i) {
     const mlora_page_pool& p = pools[i];
     MLORA_CHECK(p.data && p.layers > 0 && p.rows > 0 && p.row_bytes > 0 && p.row_bytes <= 1l << 30, MLORA_ERR_INVALID, "copy_pages: pool %d of %d x %d rows of %ld bytes", i,
                 p.layers, p.rows, p.row_bytes);
-    a.p[i] = (uint8_t*)p.data;
-    a.bytes[i] = (int)p.row_bytes;
-    a.rows[i] = p.rows;
-    a.layer[i] = (size_t)p.rows * p.row_bytes;
-    a.pieces[i] = (int)((p.row_bytes + PIECE - 1) / PIECE);
-    a.begin[i] = (int)units;
-    units += (long)p.layers * a.pieces[i];
-    MLORA_CHECK(units <= 1 << 30, MLORA_ERR_UNSUPPORTED, "copy_pages: too many pieces");
+    const int pieces = (int)((p.row_bytes + PIECE - 1) / PIECE);
+    a.at[i] = Pool{(uint8_t*)p.data, (size_t)p.rows * p.row_bytes, (int)p.row_bytes, pieces, p.rows, (int)units};
+    units += (long)p.layers * pieces;
+    MLORA_CHECK(units < 1 << 30, MLORA_ERR_UNSUPPORTED, "copy_pages: too many pieces");
   }
-  a.begin[n_pools] = (int)units;
+  for (int i = n_pools; i < MAX_POOLS; ++i) a.at[i].begin = 0x7fffffff;
   if (n == 0) return MLORA_OK;
   hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)units, n < 65535 ? n : 65535), dim3(256), 0, (hipStream_t)stream, a, src, dst, n);
   return mlora_launch_status("copy_pages");
