@@ -11,13 +11,20 @@ import numpy as np
 import torch
 
 from . import ops
+from .kv_cache import PAGE
 from .llama import share_of
+
+
+def step_form(kv):
+    """(plan, cut): what the launches of a step on a cache depend on beside their batch."""
+    return getattr(kv, "plan", None), getattr(kv, "cut", None)
 
 
 class DecodeSession:
     """Fixed-batch greedy decode through the per-operator path (any mix of adapter types and ranks).  With
     use_graph the launch sequence of a step is captured once - after one eager step, which also sizes the model's
-    scratch buffers outside the graph's memory pool, and again when the cache's plan over shared prefixes changes - and replayed,
+    scratch buffers outside the graph's memory pool, and again when the cache's plan over shared prefixes changes, or the length that
+    its attention's work is cut for - and replayed,
     so the interpreter is out of the loop; the kernels and their order are those of the eager step, hence the same tokens bit for bit."""
 
     def __init__(self, model, kv, seq_ids, tok_adapter, first_tokens, use_graph=False, longest_first=False, rules=None):
@@ -52,7 +59,7 @@ class DecodeSession:
         self.pos = i32([kv.lens[s] for s in self.seq_ids])
         self.ctx = self.pos + 1
         self.use_graph = use_graph
-        self.graph = self._plan = None
+        self.graph = self._plan = self._cut = None
         self._eager_steps = 0
         self.history = []
 
@@ -73,12 +80,12 @@ class DecodeSession:
             self.rules.take()
         kv.begin_forward(self.seq_ids, [1] * len(self.seq_ids), device_meta=(self.rows, self.pos, self.ctx))
         if self.use_graph and self._eager_steps >= 1:
-            plan = getattr(kv, "plan", None)
-            if self.graph is None or plan is not self._plan:     # (a plan that its rows have outgrown is replaced)
+            plan, cut = step_form(kv)
+            if self.graph is None or plan is not self._plan or cut != self._cut:     # (a plan that its rows have outgrown is replaced)
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g):         # behind a wait for the device; records, does not run
                     self._enqueue()
-                self.graph, self._plan = g, plan  # what the recorded launches read
+                self.graph, self._plan, self._cut = g, plan, cut  # what the recorded launches read
             self.graph.replay()
         else:
             self._enqueue()
@@ -88,6 +95,113 @@ class DecodeSession:
         if keep_history:
             self.history.append(out.clone() if self._inv is None else out)
         return out
+
+
+class BeamSession:
+    """Beam search over a batch of prefilled sequences: the `beams` best continuations of each by the sum of their tokens' log-probabilities, kept on
+    the device.  A step is the model's forward for every beam, ops.beam_select, and PagedKVCache.reorder: the beams go on in one another's rows of the block
+    table, so that what they share is held and, where that pays, read once.  The host reads the rows back when pages are needed, every 16 steps.
+    A beam that has chosen `eos` goes on as it is.  use_graph, longest contexts and adapters as in DecodeSession."""
+
+    def __init__(self, model, kv, seq_ids, tok_adapter, logits, beams, eos=None, steps=None, use_graph=False):
+        """seq_ids: sequences already prefilled in `kv`, which need `beams` rows of it each; tok_adapter: {tid: ids per sequence}; logits [R, V] fp32: of the sequences' last
+        tokens, by which the first tokens are chosen here; steps: most steps that will follow (None: any number), for which pages are looked for ahead."""
+        if not model.cache_forms:
+            raise ValueError(f"BeamSession: {type(model).__name__} has no caches that beams share")
+        R, W = len(seq_ids), int(beams)
+        if not 1 <= W <= 16 or logits.shape[0] != R:
+            raise ValueError(f"BeamSession: {W} beams (1 to 16) of {R} sequences, logits of {logits.shape[0]}")
+        self.model, self.kv, self.R, self.W, self.eos, self.left = model, kv, R, W, eos, steps
+        dev = model.device
+        i32 = lambda a: (a if isinstance(a, torch.Tensor) else torch.as_tensor(np.asarray(a, dtype=np.int32))).to(dev, torch.int32)      # noqa: E731
+        self.seq_ids = []
+        for sid in seq_ids:
+            forks = [("beam", sid, w) for w in range(1, W)]
+            kv.fork(forks, sid)
+            self.seq_ids += [sid, *forks]
+        self.tok_adapter = {tid: i32(ids).repeat_interleave(W) for tid, ids in tok_adapter.items()}
+        if len(self.tok_adapter) > 1:
+            self.tok_adapter = model._merge_types(self.tok_adapter)
+        self.slots = i32([kv.slot[s] for s in self.seq_ids])
+        self.pos = i32([kv.lens[s] for s in self.seq_ids])
+        self.ctx = self.pos + 1
+        # of the step before: scores (fp32), tokens, parents (-1: no beam), by request and beam, the best first
+        self.state = torch.empty((3, R, W), dtype=torch.int32, device=dev)
+        self.scores, self.chosen, self.parents = self.state[0].view(torch.float32), self.state[1], self.state[2]
+        self.ended = None if eos is None else torch.zeros((R, W), dtype=torch.int32, device=dev)
+        self.tokens = torch.empty(R * W, dtype=torch.int32, device=dev)
+        self._take(*ops.beam_select(logits, torch.zeros((R, 1), dtype=torch.float32, device=dev), k=W))
+        self.history = [self.state.clone()]
+        self.use_graph, self._eager_steps = use_graph, 0
+        self.graph = self._plan = self._cut = None
+
+    def _take(self, scores, tokens, parents):
+        if self.ended is not None:
+            self.ended.copy_(self.ended.gather(1, parents.clamp(min=0).long()) | (tokens == self.eos))
+        self.scores.copy_(scores)
+        self.chosen.copy_(tokens)
+        self.parents.copy_(parents)
+        self.tokens.copy_(tokens.clamp(min=0).view(-1))
+
+    def _enqueue(self):
+        m = self.model
+        logits = m.forward(m.embed(self.tokens), self.kv, self.tok_adapter)
+        self._take(*ops.beam_select(logits, self.scores, ended=self.ended, eos=self.eos))
+        self.kv.reorder(self.seq_ids, self.parents, self.slots, self.ctx)
+        self.pos.add_(1)
+        self.ctx.add_(1)
+
+    def step(self):
+        """One step of every beam; returns (scores, tokens, parents) [R, W] on the device, which the next step overwrites."""
+        kv = self.kv
+        if any(kv.lacks_page(s) for s in self.seq_ids[::self.W]):
+            kv.reserve(self.seq_ids, PAGE if self.left is None else max(1, min(PAGE, self.left)))
+        kv.begin_forward(self.seq_ids, [1] * len(self.seq_ids), device_meta=(self.slots, self.pos, self.ctx))
+        if self.use_graph and self._eager_steps >= 1:
+            plan, cut = step_form(kv)
+            if self.graph is None or plan is not self._plan or cut != self._cut:
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    self._enqueue()
+                self.graph, self._plan, self._cut = g, plan, cut
+            self.graph.replay()
+        else:
+            self._enqueue()
+            self._eager_steps += 1
+        kv.end_forward()
+        kv.adrift(self.seq_ids, self.slots)
+        self.history.append(self.state.clone())
+        if self.left is not None:
+            self.left -= 1
+        return self.scores, self.chosen, self.parents
+
+    def done(self) -> bool:
+        """Whether every request's best beam has ended: scores only fall, so none overtakes it.  Waits for the device."""
+        return self.ended is not None and bool(self.ended[:, 0].all())
+
+    def answers(self):
+        """Per request its beams so far as (score, tokens), the best first, up to `eos`.  Waits for the device."""
+        h = torch.stack(self.history).cpu().numpy()
+        scores, out = h[-1, 0].view(np.float32), []
+        at, alive = np.broadcast_to(np.arange(self.W), (self.R, self.W)), h[-1, 1] >= 0
+        rows = np.arange(self.R)[:, None]
+        tokens = np.empty((len(h), self.R, self.W), np.int32)
+        for i in reversed(range(len(h))):
+            tokens[i] = h[i, 1][rows, at]
+            at = np.maximum(h[i, 2][rows, at], 0)
+        for r in range(self.R):
+            beams = []
+            for w in np.flatnonzero(alive[r]):
+                t = tokens[:, r, w].tolist()
+                beams.append((float(scores[r, w]), t[:t.index(self.eos) + 1] if self.eos in t else t))
+            out.append(beams)
+        return out
+
+    def close(self):
+        """Gives back the rows and pages of all beams but each request's first, which goes on under its sequence's id (at whatever beam it is)."""
+        for s in self.seq_ids:
+            if isinstance(s, tuple) and s[0] == "beam":
+                self.kv.free_sequence(s)
 
 
 class NativeDecodeSession:
@@ -105,6 +219,8 @@ class NativeDecodeSession:
         from . import _lib
         if not model.native_step:
             raise ValueError("NativeDecodeSession: the model has no C decode step")
+        if not kv.plain:
+            raise ValueError("NativeDecodeSession: the C decode step reads fp16 caches without a window")
         self.model, self.kv = model, kv
         self.seq_ids = list(seq_ids)
         s = model.shape

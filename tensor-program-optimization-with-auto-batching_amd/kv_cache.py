@@ -9,9 +9,10 @@ scale 1, no sliding window).  Keys are stored already rotated, which is equivale
 read time and saves the per-step re-rotation of the whole context.
 
 A finished sequence gives its pages and its slot back with free_sequence(sid).  A sequence may begin with the whole pages of another
-(share_prefix): they then have several owners and go back with the last of them.
+(share_prefix): they then have several owners and go back with the last of them.  Sequences may go on from all that another holds (fork), and
+the beams of a search in one another's places (reorder).  Under a sliding window pages that no later token sees go back to the pool.
 
-Device layout of PagedKVCache per layer: k [n_pages, Hkv, 16, D], v [n_pages, Hkv, D, 16] (fp16), one int32 block table
+Device layout of PagedKVCache per layer: k [n_pages, Hkv, 16, D], v [n_pages, Hkv, D, 16] (fp16; in 8 bits that of ops.QuantPages), one int32 block table
 [max_seqs, max_blocks], fp32 RoPE tables [max_pos, D/2].
 """
 from __future__ import annotations
@@ -38,6 +39,7 @@ class PageTable:
     pass.  What lies in a page is up to the subclass."""
 
     shares_pages = True      # whether a page is all that its tokens leave behind
+    plain = True             # whether the native passes and the plans over shared pages read it
 
     def __init__(self, n_pages, max_seqs, max_blocks, max_pos, device, free_pages=None, page_size=PAGE):
         if page_size != PAGE:
@@ -58,6 +60,7 @@ class PageTable:
         self._cur = None
         self._staged = None     # (raw stream, event) of arrays queued last
         self._users = {}        # raw stream -> (stream, event behind the last pass's work or None): streams whose work reads the arrays
+        self._adrift = {}       # sequences -> their slots [n] on the device, of beams whose rows the device has changed since the host read them
 
     # ------------------------------------------------------------------ protocol
     def add_sequence(self, sid):
@@ -72,19 +75,50 @@ class PageTable:
         """Give back the pages and the slot of a finished sequence."""
         if self._cur is not None:
             raise RuntimeError("free_sequence between begin_forward and end_forward")
+        self.settle()
         row = self.slot.pop(sid)
         del self.lens[sid]
         for p in self.table_h[row][self.table_h[row] >= 0].tolist():
-            left = self._owners.get(p, 1) - 1
-            if left == 0:
-                self.free.append(p)
-            elif left == 1:
-                del self._owners[p]
-            else:
-                self._owners[p] = left
+            self._own(p, -1)
         self.table_h[row] = -1
         self.free_slots.insert(0, row)
         self._dirty = True
+
+    def _own(self, page, more):
+        """`more` sequences take a page over, or give it back."""
+        n = self._owners.get(page, 1) + more
+        if n > 1:
+            self._owners[page] = n
+            return
+        self._owners.pop(page, None)
+        if n == 0:
+            self.free.append(page)
+
+    def settle(self):
+        """Reads the rows of the block table back that a search's beams have on the device, where they have changed since: one wait for the device.  Pages
+        that no beam holds any more go back to the pool.  Called by itself ahead of whatever needs the rows here."""
+        if not self._adrift:
+            return
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("paged KV cache: the rows of beams are to be read back, which a capture cannot")
+        self._enter()
+        table = self.block_table.cpu().numpy()
+        for sids, slots in self._adrift.items():
+            self._read_back(sids, slots.cpu().numpy(), table)
+        self._adrift = {}
+
+    def _read_back(self, sids, slots, table):
+        rows = np.asarray([self.slot[s] for s in sids])
+        if not np.array_equal(np.sort(rows), np.sort(slots)):
+            raise RuntimeError(f"paged KV cache: beams of rows {rows.tolist()} in {slots.tolist()}")
+        held = np.concatenate([self.table_h[rows].ravel(), table[rows].ravel()])
+        pages, of = np.unique(held, return_inverse=True)
+        n = held.size // 2
+        for p, more in zip(pages.tolist(), (np.bincount(of.ravel()[n:], minlength=pages.size) - np.bincount(of.ravel()[:n], minlength=pages.size)).tolist()):
+            if p >= 0 and more:
+                self._own(p, more)
+        self.table_h[rows] = table[rows]
+        self.slot.update(zip(sids, slots.tolist()))
 
     def share_prefix(self, sid, of, tokens=None) -> int:
         """Sequence `sid`, added and still empty, begins with the first `tokens` tokens of sequence `of` (None: all that are committed),
@@ -94,16 +128,45 @@ class PageTable:
             raise RuntimeError("share_prefix between begin_forward and end_forward")
         if not self.shares_pages:
             raise ValueError(f"{type(self).__name__}: what a sequence leaves behind lies not in pages alone")
+        self.settle()
         row, src = self.slot[sid], self.slot[of]
         if sid == of or self.lens[sid] or (self.table_h[row] >= 0).any():
             raise ValueError(f"share_prefix: sequence {sid} is not another, empty one")
         n = max(min(self.lens[of] if tokens is None else int(tokens), self.lens[of]), 0) // PAGE
+        n = self._shareable(src, n)
         for p in self.table_h[src, :n].tolist():
-            self._owners[p] = self._owners.get(p, 1) + 1
+            if p >= 0:
+                self._own(p, 1)
         self.table_h[row, :n] = self.table_h[src, :n]
         self.lens[sid] = n * PAGE
         self._dirty = self._dirty or n > 0
         return n * PAGE
+
+    def _shareable(self, row, n):
+        """How many of a row's first n pages another sequence can begin with."""
+        return n
+
+    def _held(self, sid):
+        """Blocks of a sequence that have had their pages."""
+        return int((self.table_h[self.slot[sid]] >= 0).sum())
+
+    def _release(self, seq_ids):
+        """Ahead of a pass of these sequences, whatever of theirs it does not read."""
+
+    def lacks_page(self, sid):
+        """Whether the sequence's next token needs a page that it has not."""
+        j = self.lens[sid] // PAGE
+        return j < self.max_blocks and self.table_h[self.slot[sid], j] < 0
+
+    def reserve(self, seq_ids, tokens):
+        """Pages for the next `tokens` tokens of sequences, as far as their rows go and if the pool has all of them; otherwise none."""
+        self.settle()
+        room = min(self.max_blocks, self.max_pos // PAGE)
+        want = [(self.slot[s], j) for s in seq_ids for j in range(self._held(s), min(-(-(self.lens[s] + tokens) // PAGE), room))]
+        if want and len(want) <= len(self.free):
+            for row, j in want:
+                self.table_h[row, j] = self.free.pop(0)
+            self._dirty = True
 
     def prefix_groups(self, seq_ids):
         """(positions in seq_ids, pages): which of the sequences begin with the same pages, cut so that the pages saved are most; of equal
@@ -174,6 +237,9 @@ class PageTable:
             raise RuntimeError("begin_forward called twice without end_forward")
         if len(seq_ids) != len(append_lens):
             raise ValueError("seq_ids and append_lens differ in length")
+        if self._adrift and (device_meta is None or self._dirty):
+            self.settle()
+        self._release(seq_ids)
         # Which sequences lack a page (they are handed out in order: the last one needed is missing).  us a step without host-made arrays, one by one / all at
         # once: one sequence 2.5 / 15.5, four 3.6 / 16.3, 64 29 / 34, 212 94 / 81
         if len(seq_ids) < AT_ONCE:
@@ -184,7 +250,7 @@ class PageTable:
                 if new_len > self.max_pos or need > self.max_blocks:
                     raise RuntimeError(f"sequence {sid}: length {new_len} exceeds the cache geometry")
                 if need > 0 and self.table_h[row, need - 1] < 0:
-                    short.append((row, need))
+                    short.append((sid, need))
         else:
             rows, base = self._rows_and_lens(seq_ids)
             new_len = base + np.asarray(append_lens, dtype=np.int64)
@@ -193,9 +259,13 @@ class PageTable:
             if beyond.any():
                 i = int(beyond.argmax())
                 raise RuntimeError(f"sequence {seq_ids[i]}: length {new_len[i]} exceeds the cache geometry")
-            short = [(rows[i], int(need[i])) for i in np.flatnonzero((need > 0) & (self.table_h[rows, np.maximum(need, 1) - 1] < 0))]
-        for row, need in short:
-            for j in range(int((self.table_h[row] >= 0).sum()), need):
+            short = [(seq_ids[i], int(need[i])) for i in np.flatnonzero((need > 0) & (self.table_h[rows, np.maximum(need, 1) - 1] < 0))]
+        if short and self._adrift:
+            self.settle()
+            return self.begin_forward(seq_ids, append_lens, device_meta)
+        for sid, need in short:
+            row = self.slot[sid]
+            for j in range(self._held(sid), need):
                 if not self.free:
                     raise RuntimeError("paged KV cache out of pages")
                 self.table_h[row, j] = self.free.pop(0)
@@ -268,6 +338,7 @@ class PageTable:
 
     def __getstate__(self):
         """A copy, or a pickle, is made behind all that the passes have queued and knows no streams (which neither takes)."""
+        self.settle()
         self._enter()
         return {**self.__dict__, "_staged": None, "_users": {}}
 
@@ -286,34 +357,150 @@ class PageTable:
 
     # ------------------------------------------------------------------ helpers
     def pages_of(self, sid):
+        self.settle()
         row = self.table_h[self.slot[sid]]
         return row[row >= 0].tolist()
 
 
 class PagedKVCache(PageTable):
     def __init__(self, n_layers, n_pages, n_kv_heads, head_dim, max_seqs, max_blocks, rope_theta, max_pos,
-                 device="cuda:0", free_pages=None, page_size=PAGE, n_q_heads=None):
-        """n_q_heads: of the model that reads the cache; without them decode steps read shared pages for each sequence anew."""
+                 device="cuda:0", free_pages=None, page_size=PAGE, n_q_heads=None, bits=16, window=None, sinks=0):
+        """n_q_heads: of the model that reads the cache; without them decode steps read shared pages for each sequence anew.
+        bits: 8 holds every page that is complete in 8 bits, at a step per page and head (ops.QuantPages), in little more than half the memory.
+        window: a token sees only the last so many, itself among them, and the first `sinks`; pages in between go back to the pool.
+        A cache of either kind is read by operators of its own, one launch a layer and step (`plain` is false)."""
         super().__init__(n_pages, max_seqs, max_blocks, max_pos, device, free_pages, page_size)
+        if bits not in (8, 16):
+            raise ValueError(f"PagedKVCache: pages of {bits} bits (8 or 16)")
+        self.bits, (self.window, self.sinks) = bits, ops._window("PagedKVCache", window, sinks)
+        self.plain = bits == 16 and not self.window
+        if not self.plain and head_dim not in (64, 128):
+            raise ValueError(f"PagedKVCache: pages of {bits} bits with a window of {window} tokens for heads of {head_dim} (64 or 128)")
+        self.cut = None         # tokens by which attention over a cache that is not plain shares its work out
+        self._gone = {}         # sid -> block in front of which all but the sinks' have gone back
         self.n_layers, self.Hkv, self.D, self.n_q_heads = n_layers, n_kv_heads, head_dim, n_q_heads
         self.plan = None        # of the current decode step
         self._plans = {}        # batch -> SharedPrefixPlan or None, for batches whose sequences are there
         if head_dim % 32:
             raise ValueError("head_dim must be a multiple of 32")
         # keys in matrix-core fragment order: element (token, d) of a page at [d // 32, (d % 32) // 8, token, d % 8]
-        self.k = torch.zeros((n_layers, n_pages, n_kv_heads, head_dim // 32, 4, PAGE, 8), dtype=torch.float16, device=self.device)
-        self.v = torch.zeros((n_layers, n_pages, n_kv_heads, head_dim, PAGE), dtype=torch.float16, device=self.device)
+        zeros = lambda *shape, dtype=torch.float16: torch.zeros((n_layers, *shape), dtype=dtype, device=self.device)      # noqa: E731
+        last = (max_seqs if bits == 8 else n_pages, n_kv_heads)
+        k16, v16 = zeros(*last, head_dim // 32, 4, PAGE, 8), zeros(*last, head_dim, PAGE)
+        if bits == 8:
+            self.tail_k, self.tail_v, self._pages = k16, v16, {}
+            self.k = zeros(n_pages, n_kv_heads, head_dim // 64, 4, PAGE, 2, 8, dtype=torch.int8)
+            self.v = zeros(n_pages, n_kv_heads, head_dim // 64, 4, PAGE, 4, 4, dtype=torch.int8)
+            self.step = zeros(n_pages, n_kv_heads, 2, dtype=torch.float32)
+        else:
+            self.k, self.v = k16, v16
         cos, sin = rope_tables(head_dim, rope_theta, max_pos)
         self.rope_cos = torch.from_numpy(cos).to(self.device)
         self.rope_sin = torch.from_numpy(sin).to(self.device)
 
     def k_rowmajor(self, layer: int) -> torch.Tensor:
-        """The layer's rotated keys as [n_pages, Hkv, 16, D] (a copy, for inspection)."""
+        """The layer's rotated keys as [n_pages, Hkv, 16, D] (a copy, for inspection; of pages in 8 bits what they stand for)."""
+        if self.bits == 8:
+            return self.pages(layer).values(torch.arange(self.n_pages, dtype=torch.int32, device=self.device))[0]
         k = self.k[layer]
         return k.permute(0, 1, 4, 2, 3, 5).reshape(self.n_pages, self.Hkv, PAGE, self.D).contiguous()
 
+    def pages(self, layer) -> ops.QuantPages:
+        """A layer's pages in 8 bits."""
+        if layer not in self._pages:
+            self._pages[layer] = ops.QuantPages(self.k[layer], self.v[layer], self.step[layer], self.tail_k[layer], self.tail_v[layer])
+        return self._pages[layer]
+
+    def __getstate__(self):
+        state = super().__getstate__()
+        return {**state, "_pages": {}} if self.bits == 8 else state
+
+    # Under a window a row has the pages of the sinks, then none, then those from the first one on that its next token sees.
+    def _first_seen(self, length):
+        return max(length - self.window + 1, 0) // PAGE if self.window else 0
+
+    def _release(self, seq_ids):
+        if not self.window:
+            return
+        adrift = {s for sids in self._adrift for s in sids}      # (rows that are not known here keep their pages until they are)
+        for sid in seq_ids:
+            first, gone = self._first_seen(self.lens[sid]), self._gone.get(sid, -(-self.sinks // PAGE))
+            if first > gone and sid not in adrift:
+                blocks = self.table_h[self.slot[sid], gone:first]
+                for p in blocks[blocks >= 0].tolist():
+                    self._own(p, -1)
+                blocks[:] = -1
+                self._gone[sid] = first
+                self._dirty = True
+
+    def _held(self, sid):
+        if not self.window:
+            return super()._held(sid)
+        has = np.flatnonzero(self.table_h[self.slot[sid]] >= 0)
+        return max(int(has[-1]) + 1 if has.size else 0, -(-self.lens[sid] // PAGE))
+
+    def _shareable(self, row, n):
+        if not self.window:
+            return n
+        seen = np.arange(n)
+        seen = seen[(seen < -(-self.sinks // PAGE)) | (seen >= self._first_seen(n * PAGE))]
+        return n if (self.table_h[row, seen] >= 0).all() else 0  # (a row that has gone on may have given back what this one needs)
+
+    def fork(self, sids, of):
+        """Sequences `sids`, which are added here, go on from all the tokens of sequence `of`: its whole pages have them as owners too, the contents of its
+        last page are copied (all sequences and layers in one launch)."""
+        if self._cur is not None:
+            raise RuntimeError("fork between begin_forward and end_forward")
+        sids = list(sids)
+        self.settle()
+        src, n = self.slot[of], self.lens[of]
+        full, part = n // PAGE, n % PAGE > 0
+        if len(set(sids)) < len(sids) or any(s in self.slot for s in sids):
+            raise ValueError("fork: a sequence that has already been added")
+        if len(sids) > len(self.free_slots) or part and len(sids) > len(self.free):
+            raise RuntimeError(f"paged KV cache: {len(self.free_slots)} slots and {len(self.free)} pages left for {len(sids)} sequences")
+        pairs = []
+        for sid in sids:
+            self.add_sequence(sid)
+            row = self.slot[sid]
+            for p in self.table_h[src, :full].tolist():
+                if p >= 0:
+                    self._own(p, 1)
+            self.table_h[row, :full] = self.table_h[src, :full]
+            if part:
+                self.table_h[row, full] = self.free.pop(0)
+                pairs.append((src, row) if self.bits == 8 else (int(self.table_h[src, full]), int(self.table_h[row, full])))
+            self.lens[sid] = n
+            if of in self._gone:
+                self._gone[sid] = self._gone[of]
+        self._dirty = self._dirty or bool(sids)
+        if pairs:
+            self._enter()
+            at = ops.upload(torch.tensor(pairs, dtype=torch.int32).t().contiguous(), self.device)
+            ops.copy_pages([self.tail_k, self.tail_v] if self.bits == 8 else [self.k, self.v], at[0], at[1])
+
+    def reorder(self, sids, parents, slots, ctx):
+        """A step of a beam search: the beams `sids` of requests (an equal number each, one behind the other, of equal length) go on from the tokens of their parents [R, W]
+        int32 (-1: from none), chosen by ops.beam_select.  slots [R * W] int32 are their rows of the block table, and become those that they then have; ctx [R * W] their lengths.
+        All of it stays on the device, can be recorded into a graph, and is one launch for the rows and one for what is to be copied: the contents of last pages
+        that are not complete.  The host learns of it from `adrift`."""
+        new, moves = ops.beam_reorder(parents, slots, self.block_table, ctx)
+        if self.bits == 8:
+            ops.copy_pages([self.tail_k, self.tail_v], moves.src_slot, moves.dst_slot)
+        else:
+            ops.copy_pages([self.k, self.v], moves.src_page, moves.dst_page)
+        slots.copy_(new)
+
+    def adrift(self, sids, slots):
+        """`reorder` of these beams has run, or is queued: their rows are to be read back (`settle`) before they are used here."""
+        sids = tuple(sids)
+        self._adrift[sids] = slots
+        if len(self._plans) > (sids in self._plans):           # (the batch's own plan is of the pages that its requests' beams shared first, and share on)
+            self._plans = {b: p for b, p in self._plans.items() if b == sids or not set(b) & set(sids)}
+
     def free_sequence(self, sid):
         super().free_sequence(sid)
+        self._gone.pop(sid, None)
         self._plans = {b: p for b, p in self._plans.items() if sid not in b}
 
     def share_prefix(self, sid, of, tokens=None):
@@ -328,7 +515,7 @@ class PagedKVCache(PageTable):
         32 heads of 128 over 32, 32 rows, 16 shared pages 16.4 / 14.2, 64 pages 35 / 16, 256 pages 133 / 29; 2 rows, 64 pages 11.2 / 10.4, 256 pages
         38 / 22; 128 rows, 4 pages 36 / 35; 32 heads over 8, 32 rows, 64 pages (130 MB) 12.8 / 14.6, 256 pages 32 / 23, 128 rows, 16 pages (133 MB) 18 / 16,
         64 rows, 64 pages 20 / 17."""
-        if not self._owners or not self.n_q_heads or not 1 <= self.n_q_heads // self.Hkv <= 16:
+        if not self._owners or not self.plain or not self.n_q_heads or not 1 <= self.n_q_heads // self.Hkv <= 16:
             return None
         batch = tuple(seq_ids)
         recorded = self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()      # (a capture takes no arrays from the host)
@@ -353,6 +540,10 @@ class PagedKVCache(PageTable):
 
     def begin_forward(self, seq_ids, append_lens, device_meta=None):
         super().begin_forward(seq_ids, append_lens, device_meta)
+        if not self.plain:
+            # a step's work is cut for the next power of two, so that a recorded one is cut as the others are
+            longest = max((self.lens[s] + n for s, n in zip(seq_ids, append_lens)), default=0)
+            self.cut = min(max(1 << max(longest - 1, 0).bit_length(), 256), self.max_blocks * PAGE) if self._cur[2] else longest
         self.plan = self.shared_plan(seq_ids) if self._cur[2] and self._owners else None
         if self.plan is not None and self.device.type == "cuda" and not torch.cuda.is_current_stream_capturing():
             self.plan.data.record_stream(torch.cuda.current_stream(self.device))      # (it may have been made on another)
@@ -371,6 +562,10 @@ class PagedKVCache(PageTable):
         _, append_lens, decode, tok_seq, tok_pos, ctx = self._cur
         T = sum(append_lens)
         qkv = qkv.view(T, n_q_heads + 2 * self.Hkv, self.D)
+        if not self.plain:
+            if o_shrink is not None:
+                raise ValueError("attention_with_fused_qkv: o_shrink is for plain caches")
+            return self._attention(layer, qkv, n_q_heads, out, frag)
         ops.rope_kv_append(qkv, self.k[layer], self.v[layer], self.block_table, tok_seq, tok_pos,
                            self.rope_cos, self.rope_sin, n_q_heads, self.Hkv, self.D)
         if decode and self.plan is not None and n_q_heads == self.n_q_heads and o_shrink is None:
@@ -384,10 +579,28 @@ class PagedKVCache(PageTable):
         return ops.paged_attn_prefill(qkv, self.k[layer], self.v[layer], self.block_table, tok_seq, tok_pos,
                                       n_q_heads, self.Hkv, self.D, out=out, frag=frag)
 
+    def _attention(self, layer, qkv, n_q_heads, out, frag):
+        """`attention_with_fused_qkv` of a cache in 8 bits, or under a window (which may leave q as it comes)."""
+        _, _, decode, tok_seq, tok_pos, _ = self._cur
+        where, heads = (self.block_table, tok_seq, tok_pos), (n_q_heads, self.Hkv, self.D)
+        seen = {"window": self.window or None, "sinks": self.sinks, "longest": self.cut, "out": out, "frag": frag}
+        rope = (self.rope_cos, self.rope_sin)
+        if self.bits == 8:
+            return (ops.rope_attn_decode_q8 if decode else ops.rope_attn_prefill_q8)(qkv, self.pages(layer), *where, *rope, *heads, **seen)
+        k, v = self.k[layer], self.v[layer]
+        if decode:
+            return ops.rope_attn_decode_window(qkv, k, v, *where, *rope, *heads, **seen)
+        ops.rope_kv_append(qkv, k, v, *where, *rope, *heads)
+        return ops.paged_attn_prefill_window(qkv, k, v, *where, *heads, **seen)
+
     def kv_bytes_read_per_step(self, seq_ids):
         """Algorithmic K+V bytes one decode step reads for these sequences, all layers."""
         per_pos = self.n_layers * 2 * self.Hkv * self.D * 2
-        return int(sum(self.lens[s] + 1 for s in seq_ids)) * per_pos
+        seen = [n if not self.window or n <= self.window + self.sinks else self.window + self.sinks for n in (self.lens[s] + 1 for s in seq_ids)]
+        if self.bits == 8:                       # complete pages at a byte a number and two steps, those ahead of the token's own
+            own = [(self.lens[s] % PAGE) + 1 for s in seq_ids]
+            return int(sum(o * per_pos + (n - o) * (per_pos // 2 + self.n_layers * self.Hkv * 8 // PAGE) for n, o in zip(seen, (min(o, n) for o, n in zip(own, seen)))))
+        return int(sum(seen)) * per_pos
 
 
 class PagedLatentCache(PageTable):

@@ -59,6 +59,7 @@ class LoraType:
 class LlamaForCausalLM(CausalLM):
     dtypes = ("float16",)
     native_step = True
+    cache_forms = True        # caches in 8 bits and under windows, and searches by beams, serve it
     quant_group = None
 
     def __init__(self, shape: LlamaShape, device="cuda:0", quant_group=None):
@@ -244,14 +245,15 @@ class LlamaForCausalLM(CausalLM):
         return out
 
     def create_paged_kv_cache(self, max_batch_size, max_total_seq_len, prefill_chunk_size, page_size,
-                              free_pages=None, max_seq_len=None):
+                              free_pages=None, max_seq_len=None, bits=16, window=None, sinks=0):
         """Same arguments as the reference's VM function (`llama_for_causal_lm.py:148-174`).  The pool holds
-        ceil(max_total_seq_len / page_size) + max_batch_size pages (one partial page per sequence)."""
+        ceil(max_total_seq_len / page_size) + max_batch_size pages (one partial page per sequence).
+        bits, window, sinks: as for PagedKVCache."""
         s = self.shape
         n_pages, max_blocks = self._cache_geometry(max_batch_size, max_total_seq_len, page_size, free_pages, max_seq_len)
         return PagedKVCache(s.num_hidden_layers, n_pages, s.num_key_value_heads, s.head_dim, max_seqs=max_batch_size,
                             max_blocks=max_blocks, rope_theta=s.rope_theta, max_pos=max_blocks * page_size,
-                            device=self.device, free_pages=free_pages, page_size=page_size, n_q_heads=s.num_attention_heads)
+                            device=self.device, free_pages=free_pages, page_size=page_size, n_q_heads=s.num_attention_heads, bits=bits, window=window, sinks=sinks)
 
     @property
     def vocab_size(self):
@@ -427,7 +429,7 @@ class LlamaForCausalLM(CausalLM):
             (tid, ids), = tok_adapter.items()
             near = (self.lora_types[tid], ids, 1 if segs else distinct_adapters(host_ids[tid], self.lora_types[tid].n_adapters))
         o_shares = None
-        if tok_adapter and "multi" not in tok_adapter and len(tok_adapter) == 1 and is_decode and T > 64 and frag and getattr(kv, "plan", None) is None:
+        if tok_adapter and "multi" not in tok_adapter and len(tok_adapter) == 1 and is_decode and T > 64 and frag and getattr(kv, "plan", None) is None and getattr(kv, "plain", True):
             (tid, ids), = tok_adapter.items()
             lt = self.lora_types[tid]
             if ops.o_shrink_served(T, s.num_attention_heads, s.num_key_value_heads, s.head_dim, H, lt.r):
@@ -601,10 +603,10 @@ class LlamaForCausalLM(CausalLM):
 
     # ------------------------------------------------------------------ a prompt pass in one call
     def _native_prefill_serves(self, h, kv):
-        """Whether `mlora_prefill` takes a pass: not a decode step, activations in fragment order, a cache of at least the model's layers, and `forward` is this
+        """Whether `mlora_prefill` takes a pass: not a decode step, activations in fragment order, a plain cache of at least the model's layers, and `forward` is this
         class's (whose launches it queues)."""
         s = self.shape
-        return (self.quant_group is None and getattr(self.forward, "__func__", None) is LlamaForCausalLM.forward and kv._cur is not None and not kv._cur[2] and h.dim() == 2 and h.shape[0] > 0 and h.is_cuda and h.dtype == torch.float32
+        return (self.quant_group is None and getattr(kv, "plain", True) and getattr(self.forward, "__func__", None) is LlamaForCausalLM.forward and kv._cur is not None and not kv._cur[2] and h.dim() == 2 and h.shape[0] > 0 and h.is_cuda and h.dtype == torch.float32
                 and h.is_contiguous() and not s.hidden_size % 32 and not s.q_size % 32 and not s.intermediate_size % 32
                 and tuple(h.shape) == (sum(kv._cur[1]), s.hidden_size) and kv.n_layers >= len(self.layers))
 

@@ -48,6 +48,13 @@ class LlamaExecConfig:
     # their requests share once, where that pays; a batch for which it does runs through the recorded per-operator step.  Shorter
     # prefills take other kernels and summation orders, so a token can differ at a near tie.
     share_prefix: bool = False
+    # The paged cache in 8 bits (of every page that is complete, at a step per page and head) instead of 16, in little more than half the memory.
+    cache_bits: int = 16
+    # A sliding window: a token sees only the last so many, itself among them, and the first `sinks`.  The cache is sized for what is seen.
+    window: int | None = None
+    sinks: int = 0
+    # Beam search instead of greedy decoding: the answer is the best of so many beams by the sum of its tokens' log-probabilities.
+    beams: int = 1
 
 
 class LlamaExecGraph(ExecGraph):
@@ -76,11 +83,22 @@ class LlamaExecGraph(ExecGraph):
         if delete_prev:
             self.kv_cache = None
         self._prompts = {}
-        n = self.seq_info.get_num_sequences()
+        self._first = {}              # sequence -> the logits behind its prompt, of those whose beams have not begun
         c = self.exec_config
+        beams, form = getattr(c, "beams", 1), {}
+        if getattr(c, "cache_bits", 16) != 16 or getattr(c, "window", None) is not None:
+            form = {"bits": c.cache_bits, "window": c.window, "sinks": c.sinks}
+        if (form or beams != 1) and not getattr(self.vm, "cache_forms", False):
+            raise ValueError(f"{type(self.vm).__name__}: no caches in 8 bits or under windows, and no search by beams")
+        if not 1 <= beams <= 16:
+            raise ValueError(f"LlamaExecConfig: {beams} beams (1 to 16)")
+        n, longest = self.seq_info.get_num_sequences() * beams, c.max_prompt_len + c.max_gen_len
+        held = longest                # tokens of a sequence that are in the cache at once
+        if form and c.window is not None:
+            held = min(longest, max(c.max_prompt_len, c.window + c.sinks + 3 * c.page_size))
         self.kv_cache = self.vm["create_paged_kv_cache"](
-            n, n * (c.max_prompt_len + c.max_gen_len), c.max_prompt_len, c.page_size,
-            free_pages=self.free_pages, max_seq_len=c.max_prompt_len + c.max_gen_len)
+            n, n * held, c.max_prompt_len, c.page_size,
+            free_pages=self.free_pages, max_seq_len=longest, **form)
 
     def set_measuring(self, dest):
         """One millisecond value per line, one line per prefill and per decode step (`:48-50,70-74,116-132`)."""
@@ -160,6 +178,8 @@ class LlamaExecGraph(ExecGraph):
 
     def _choose_first(self, sids, logits):
         """The tokens behind the prompts, on the host."""
+        if getattr(self.exec_config, "beams", 1) > 1:
+            self._first.update(zip(sids, logits))
         rules = [self.seq_info.get_rules(sid) for sid in sids]
         if not any(r is not None for r in rules):
             return ops.argmax(logits).cpu().numpy()
@@ -225,16 +245,18 @@ class LlamaExecGraph(ExecGraph):
         if any(outputs[sid][0] < 0 for sid in seqs):        # nothing was left ahead of the first step
             seqs = [sid for sid in seqs if outputs[sid][0] >= 0]
             self.check_seqs_finished([sid for sid in ordered if outputs[sid][0] < 0], outputs)
+        if getattr(self.exec_config, "beams", 1) > 1:
+            outputs, seqs = self._decode_beams(seqs), []
         # As in the reference (`:102-141`), the finish rule (`:94-100`) is applied only after a decode step: every
         # sequence takes at least one step after its prefill, also when its first token is EOS or max_gen_len is 1.
         while seqs:
             method, params = self.seq_info.get_decode_method(seqs)
             ruled = any(self.seq_info.get_rules(sid) is not None for sid in seqs)
             if getattr(self.exec_config, "native_decode", False):
-                # a model without the C decode step, rules, which it does not apply, or shared pages, which it reads for every request:
-                # graph-replayed operators
+                # a model without the C decode step, rules, which it does not apply, a cache that it does not read, or shared pages, which it reads for
+                # every request: graph-replayed operators
                 dense = len(seqs) <= 64 and self._dense_ok(method)       # the dense shrink serves at most 64 sequences
-                if not self.vm.native_step or ruled or self._shared_pays(seqs, dense):
+                if not self.vm.native_step or ruled or not getattr(self.kv_cache, "plain", True) or self._shared_pays(seqs, dense):
                     seqs = self._decode_session(seqs, outputs, method, params)
                     continue
                 seqs = self._decode_native(seqs, outputs, method, params, dense) if dense or not method.startswith("mixed_decode") \
@@ -323,11 +345,7 @@ class LlamaExecGraph(ExecGraph):
         replayed from a graph when enough steps lie ahead.  Same kernels in the same order as the call-per-step path,
         so the same tokens."""
         from .decode_session import DecodeSession
-        tids = self._method_tids(method)
-        if method.startswith("mixed_decode"):
-            pairs = {tid: (params[2 * i], params[2 * i + 1]) for i, tid in enumerate(tids)}
-        else:
-            pairs = {tid: (None, params[0]) for tid in tids}
+        pairs = self._method_pairs(method, params)
         last = [outputs[sid][-1] for sid in seqs]
         ahead = max(1, min(self.seq_info.get_max_gen_len(sid) - len(outputs[sid]) for sid in seqs))
         rules = self._batch_rules(seqs, outputs, ahead)
@@ -352,6 +370,38 @@ class LlamaExecGraph(ExecGraph):
                 return left
             if held:
                 rules.allow([outputs[sid] for sid in seqs])
+
+    def _decode_beams(self, seqs):
+        """The answers of a batch by beam search (`LlamaExecConfig.beams`); requests of one length limit search together."""
+        from .decode_session import BeamSession
+        if any(self.seq_info.get_rules(sid) is not None for sid in seqs):
+            raise ValueError("beam search under token rules is not served")
+        outputs, limits = {}, {}
+        for sid in seqs:
+            limits.setdefault(self.seq_info.get_max_gen_len(sid), []).append(sid)
+        for limit, group in limits.items():
+            method, params = self.seq_info.get_decode_method(group)
+            steps = max(1, limit - 1)                        # (one behind the prefill at least, as in the greedy loop)
+            pairs = self._method_pairs(method, params)
+            sess = BeamSession(self.vm, self.kv_cache, group, self.vm._ids(len(group), pairs), torch.stack([self._first.pop(sid) for sid in group]),
+                               self.exec_config.beams, eos=self.eos_token_id, steps=steps, use_graph=steps >= 8)
+            for _ in range(steps):
+                ev = self._tic()
+                sess.step()
+                self._toc(ev)
+                if self.eos_token_id is not None and sess.done():
+                    break
+            for sid, beams in zip(group, sess.answers()):
+                outputs[sid] = beams[0][1]
+            sess.close()
+        return outputs
+
+    def _method_pairs(self, method, params):
+        """Adapter types of a decode entry point with their rows and weight ids, as `_ids` takes them."""
+        tids = self._method_tids(method)
+        if method.startswith("mixed_decode"):
+            return {tid: (params[2 * i], params[2 * i + 1]) for i, tid in enumerate(tids)}
+        return {tid: (None, params[0]) for tid in tids}
 
     def execute_decode_answer(self, op):
         assert len(op.input_vars) == 1 and len(op.output_vars) == 1 and len(op.seqids) == 1, \

@@ -11,6 +11,7 @@ from . import ops
 class CausalLM:
     dtypes = ("float16",)     # element types the model runs in
     native_step = False       # whether the C decode step (mlora_decode_step) serves it
+    cache_forms = False       # whether caches in 8 bits and under windows, and searches by beams, serve it
 
     lora_types = ()
 
