@@ -697,6 +697,9 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     __syncthreads();                                                  // (the ring begins)
   }
   int unit = 0;                                                       // o is in units of 2^unit
+  const uint32_t page_elems = (uint32_t)a.Hkv * PE;
+  const f16* k_of = (const f16*)a.k + (size_t)kh * PE;
+  const f16* v_of = (const f16*)a.v + (size_t)kh * PE;
 
   for (int c = 0; c < nt;) {
     int next = nt;                                                    // where the run ends
@@ -712,14 +715,19 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     if (!token_ok(a, seq, pc)) continue;
     const int pe = min(pc + next - c0 - 1, min(a.max_pos, a.max_blocks * PAGE) - 1);
     const int32_t* __restrict__ bt = a.block_table + (size_t)seq * a.max_blocks;
-    // blocks of four pages: those of the sinks, then those of the window
+    // Blocks of four of the pages that the run sees: those of the sinks, then those of the window.  fp16: in one row (4096 tokens under a window of 1024 with 4 sinks:
+    // 133 us, 142 with blocks of their own for the sinks).  8 bits: blocks of their own; one row takes registers that are not there (8 prompts of 456 tokens, no window: 170 us for 165)
     const int end = Q8 ? pe / PAGE : pe / PAGE + 1;
     const int from = min(a.window > 0 && pc >= a.window ? (pc - a.window + 1) / PAGE : 0, end);
     const int heads = a.sinks > 0 ? min((a.sinks - 1) / PAGE + 1, from) : 0;
-    const int head_blocks = (heads + 3) / 4, blocks = head_blocks + (end - from + 3) / 4;
+    const int head_blocks = Q8 ? (heads + 3) / 4 : 0, blocks = Q8 ? head_blocks + (end - from + 3) / 4 : (heads + end - from + 3) / 4;
     const int blk0 = (int)((long)blocks * split / a.splits), blk1 = (int)((long)blocks * (split + 1) / a.splits);
-    auto begin_of = [&](int blk) { return blk < head_blocks ? 4 * blk : from + 4 * (blk - head_blocks); };       // a block's first page
-    auto end_of = [&](int blk) { return blk < head_blocks ? heads : end; };                                         // and where its pages end, at most four on
+    auto page_of = [&](int blk, int p) {
+      const int i = 4 * blk + p;
+      if constexpr (Q8) return (blk < head_blocks ? 4 * blk : from + 4 * (blk - head_blocks)) + p;
+      else return i < heads ? i : from + i - heads;
+    };
+    auto end_of = [&](int blk) { return Q8 && blk < head_blocks ? heads : end; };                               // where a block's pages end, at most four on
     int lim[NT], lo[NT], least_lim[NT], most_lim[NT], least_lo[NT], most_lo[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -743,7 +751,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 
     // of the four pages on their way: a lane's id (of page lane % 4), this wave's operands; then what the block needs beside its operands
     auto id_of = [&](int blk) {
-      const int i = begin_of(blk) + (lane & 3);
+      const int i = page_of(blk, lane & 3);
       const int id = blk < blk1 && i < end_of(blk) ? bt[i] : -1;
       return id < a.n_pages ? id : -1;
     };
@@ -757,19 +765,25 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
         const bool values = u / NL & 1;
         if (8 * NL % NW != 0 && u >= 8 * NL) break;
         const int id = __builtin_amdgcn_readlane(ids, p);
-        const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh) * PE;
         if constexpr (Q8) {
+          const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh) * PE;
           piece[i] = *reinterpret_cast<const uint4*>((const uint8_t*)(values ? a.v : a.k) + at + j * 1024 + lane * 16);
         } else {                                                      // straight into the ring
-          const f16* from = values ? (const f16*)a.v + at + j * 512 + (lane & 31) * PAGE + (lane >> 5) * 8 : (const f16*)a.k + at + j * 512 + lane * 8;
+          const f16* from = (values ? v_of + (lane & 31) * PAGE + (lane >> 5) * 8 : k_of + lane * 8) + (size_t)(uint32_t)max(id, 0) * page_elems + j * 512;
           f16* to = lds + buf * 4 * PE + (values ? 8 * PE + (p >> 1) * 2 * PE + (p & 1) * 512 + j * 1024 : p * PE + j * 512);
           __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
         }
       }
       if constexpr (Q8) rstep = *reinterpret_cast<const f32x2*>(a.step + 2 * ((size_t)(ids < 0 ? 0 : ids) * a.Hkv + kh));
     };
+    int there = 0;
+    // fp16: whether somebody may not see all of a block, so that its values are looked at
+    auto checked = [&](int blk) {
+      const int first = page_of(blk, 0) * PAGE;
+      return there != 15 || first + 4 * PAGE > run_lim || (first < run_lo && first + 4 * PAGE > a.sinks);
+    };
     float by[4] = {a.scale, a.scale, a.scale, a.scale}, up[4] = {0.f, 0.f, 0.f, 0.f}, share[4] = {1.f, 1.f, 1.f, 1.f};       // of the block in LDS (uniform)
-    int there = 0, unit_next = unit;
+    int unit_next = unit;
     uint32_t nans = 0;                                                // pages of 8 bits that are NaN
     auto stage = [&](int buf, int blk, int ids) {
       there = (int)(__ballot(ids >= 0) & 15);
@@ -815,7 +829,8 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
           const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
           if ((8 * NL % NW != 0 && u >= 8 * NL) || !(u / NL & 1)) continue;
           uint32_t bad = 0;
-          const int first = (begin_of(blk) + p) * PAGE;
+          const int first = page_of(blk, p) * PAGE;
+          if (!checked(blk)) break;                                   // uniform
           if (!(there >> p & 1) || first + PAGE > run_lim || (first < run_lo && first + PAGE > a.sinks)) {        // uniform
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             f16* at = lds + 8 * PE + buf * 4 * PE + (p >> 1) * 2 * PE + (p & 1) * 512 + j * 1024 + lane * 8;
@@ -854,7 +869,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
           unit = unit_next;
         }
       }
-      const int first0 = begin_of(blk) * PAGE;
+      const int first0 = page_of(blk, 0) * PAGE;                     // (of a block that has pages of both, with others between them, nobody sees all by these comparisons)
       bool sees[NT], whole[NT];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -869,7 +884,10 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           bad[p] = Q8 && (nans >> p & 1) ? 0xffffu : 0u;
-          if constexpr (!Q8) {
+        }
+        if (!Q8 && checked(blk)) {                                    // (148 us for 153, 4096 tokens under a window of 1024: otherwise nothing waits for these)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
             uint32_t x = 0;
 #pragma unroll
             for (int j = 0; j < NL; ++j) x |= odd[buf][p * NL + j];
@@ -910,7 +928,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
               const int page = Q8 ? p : (p & 2) + (gm >> 1), in = Q8 ? 4 * gm : 8 * (gm & 1) + 4 * (p & 1);
-              first[p] = there >> page & 1 ? first0 + page * PAGE + in : 0x3fffffff;
+              first[p] = there >> page & 1 ? (Q8 ? first0 + page * PAGE : page_of(blk, page) * PAGE) + in : 0x3fffffff;
               four[p] = (Q8 ? bad[p] : gm >> 1 ? bad[p | 1] : bad[p & 2]) >> in & 15;
             }
             tile_mask<4>(st[i], first, lim_, lo_, first0 < a.sinks ? a.sinks : 0, four, (bad[0] | bad[1] | bad[2] | bad[3]) != 0);
