@@ -142,7 +142,12 @@ __device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh,
 
 // ---------------------------------------------------------------------------------------------
 // One token a sequence: rotation, the new token's place in the cache, and attention.  A workgroup has a kv head of a sequence, or a share of
-// its pages; its waves take them in turn, in the matrix-core layouts of the decode kernel in attention.hip.
+// its pages; its waves take them in turn, in the matrix-core layouts of the decode kernel in attention.hip.  A wave keeps two pages on their way in registers.
+//
+// Bound by the memory: 256 rows of 128 to 2048 tokens, 8 kv heads of 128, 579 MB in 8 bits, take 141 us (4.1 TB/s), 4 rows of 31000 55 (4.7) and 5 for the join, 48 rows that
+// see 2052 tokens of fp16 pages 78 (5.2).  Equal rows (256 of 1080) take 125, only read 107: what is left are the tokens' own pages, which are dirtied in lines of 64 bytes for
+// 2 or 16 of them, and a workgroup's first reads, which wait for one another.  Three or four pages on their way, loads past the caches, several kv heads a workgroup and an order
+// of workgroups by chiplet: no faster, or slower.
 // ---------------------------------------------------------------------------------------------
 template <int D, bool Q8>
 struct PageRegs {
@@ -442,9 +447,14 @@ __global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Prompts.  A workgroup has 64 NT consecutive tokens of a pass under one query head, a wave NT tiles of 16 of them; the tokens' runs (consecutive
-// positions of one sequence) are worked one behind the other, each over the pages that it sees, four at a time.  A wave brings one of the four from
-// the cache into LDS as fp16 operands while the workgroup multiplies the four before.
+// Prompts.  A workgroup has 16 NT NW rows, each a token of the pass under one of a kv head's query heads, tokens consecutive, a wave NT tiles of 16 of them; the
+// tokens' runs (consecutive positions of one sequence) are worked one behind the other, each over the pages that it sees, four at a time.  The waves bring
+// their pieces of the next four from the cache into LDS as fp16 operands while the workgroup multiplies four.  Tokens' own pages of 8-bit caches come first, unrounded.
+//
+// Bound by what a SIMD's four waves issue and wait for in turn, over the same phases between two barriers (per cent of the time of 4096 tokens under a window of 1024: vector
+// instructions 56, of them products 35, LDS reads 45; taken out one by one, loads, LDS reads, the softmax and the weights' second halves are 15 to 24 % each).  Those 4096 tokens,
+// 32 heads over 8, take 134 us, 450 TFLOP/s; 8 prompts of 456 on 8-bit pages, 32 heads, 99, with 33 + 6 for rounding and storing; 777 tokens behind 3500, 32 heads over 8, 128
+// (340 TFLOP/s) with 22 for storing and joining.  No faster: keys ahead by four or six fragments, values by four; slower: two tiles a wave (below).
 //
 // Of a page's step 2^e f (1 <= f < 2), the power of two goes into the values' operand, relative to the largest so far, where it is exact, and f into the
 // weights, so that two pages with steps of their own fill one matrix instruction.
@@ -990,7 +1000,8 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 }
 
 // Pages that a pass completes, in 8 bits: a wave has the keys or the values of 16 tokens of the pass under a kv head, and of the tokens those that are the first of their page
-// in the pass.  D / 16 lanes take a token's row, so that a load's lines are whole; the codes go by way of LDS into their order.
+// in the pass.  D / 16 lanes take a token's row, so that a load's lines are whole; the codes go by way of LDS into their order.  8 prompts of 456 tokens, 32 heads of 128, 90 MB:
+// 33 us, 2.7 TB/s; a page's steps (its 16 rows, the largest, codes, LDS, the store) wait for one another.  Products instead of divisions: 33 as well.
 template <int D>
 __global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
   constexpr int LD = 20, NCH = D / 16, PER = WAVE / NCH, NP = 16 / PER;       // bytes of a dim's tokens in LDS, apart for the banks; lanes of a row; rows of a load; loads
@@ -1163,6 +1174,8 @@ int launch_decode(const PageAttn& a, hipStream_t s) {
   return mlora_launch_status("page_attn_decode");
 }
 
+// Few workgroups have eight waves, more than fill the device twice four: us with 8 / 4, 1 row of 300 tokens, 16 heads of 64, 5.8 / 7.1; 256 rows of 1080 tokens, 8 kv heads of 128
+// (2048 workgroups), 127 / 125; 128 rows of 570, 32 heads, 149 / 141; 1024 of 1080, 8 heads, 478 / 464.
 template <int D, bool Q8>
 int decode(const PageAttn& a, hipStream_t s) {
   const long wgs = (long)a.T * a.Hkv * a.splits;
@@ -1172,7 +1185,7 @@ int decode(const PageAttn& a, hipStream_t s) {
   return mlora_launch_status("page_attn_decode");
 }
 
-// Eight waves of one tile: four waves on a SIMD.  (Us, so / four waves of two tiles, whose registers leave two: 8 prompts of 456 115 / 128, 777 tokens behind 3500
+// Eight waves of one tile: four waves on a SIMD.  (Us at the time, so / four waves of two tiles, whose registers leave two: 8 prompts of 456 115 / 128, 777 tokens behind 3500
 // 136 / 165, 4096 tokens under a window of 1024 in fp16 185 / 179)
 constexpr int PREFILL_TILES = 1, PREFILL_WAVES = 8, PREFILL_ROWS = 16 * PREFILL_TILES * PREFILL_WAVES;
 
@@ -1204,11 +1217,14 @@ extern "C" int mlora_page_attn_splits(int prompt, int T, int Hq, int Hkv, int pa
   const int G = Hq / Hkv;
   if (prompt) {
     if (G > PREFILL_ROWS) return 1;
+    // as many as run at once, two a compute unit: a round that is not full costs less than partial results do (777 tokens of 32 heads: 13 MB a share, written and read)
     const long wgs = (long)Hkv * ceil_div(T, PREFILL_ROWS / G);
     long n = 512 / wgs;
     n = n < pages / 32 ? n : pages / 32;
     return n < 1 ? 1 : n > 64 ? 64 : (int)n;
   }
+  // Two workgroups a compute unit, and shares of 16 pages at least.  (us with so many / twice: 4 rows of 31000 tokens 64 / 67, 64 of 4345 116 / 121, 48 under a window of 2048
+  // 86 / 93, 64 of 128 to 8192 149 / 133, 16 of 1280 to 20480 105 / 101; shares of 8 pages, one row of 4345: 17 for 14)
   const long wgs = (long)T * Hkv;
   long n = (512 + wgs - 1) / wgs;
   n = n < pages / 16 ? n : pages / 16;
