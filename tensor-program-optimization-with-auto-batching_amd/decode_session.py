@@ -115,10 +115,14 @@ class BeamSession:
         dev = model.device
         i32 = lambda a: (a if isinstance(a, torch.Tensor) else torch.as_tensor(np.asarray(a, dtype=np.int32))).to(dev, torch.int32)      # noqa: E731
         self.seq_ids = []
-        for sid in seq_ids:
-            forks = [("beam", sid, w) for w in range(1, W)]
-            kv.fork(forks, sid)
-            self.seq_ids += [sid, *forks]
+        try:
+            for sid in seq_ids:
+                forks = [("beam", sid, w) for w in range(1, W)]
+                kv.fork(forks, sid)
+                self.seq_ids += [sid, *forks]
+        except Exception:
+            self.close()
+            raise
         self.tok_adapter = {tid: i32(ids).repeat_interleave(W) for tid, ids in tok_adapter.items()}
         if len(self.tok_adapter) > 1:
             self.tok_adapter = model._merge_types(self.tok_adapter)

@@ -495,8 +495,11 @@ class PagedKVCache(PageTable):
         """`reorder` of these beams has run, or is queued: their rows are to be read back (`settle`) before they are used here."""
         sids = tuple(sids)
         self._adrift[sids] = slots
-        if len(self._plans) > (sids in self._plans):           # (the batch's own plan is of the pages that its requests' beams shared first, and share on)
-            self._plans = {b: p for b, p in self._plans.items() if b == sids or not set(b) & set(sids)}
+        if self.plain:
+            # the batch's own plan, if it has one by now, is of the pages that its requests' beams shared first, and share on: none is made of others
+            self._plans.setdefault(sids, None)
+            if len(self._plans) > 1:
+                self._plans = {b: p for b, p in self._plans.items() if b == sids or not set(b) & set(sids)}
 
     def free_sequence(self, sid):
         super().free_sequence(sid)

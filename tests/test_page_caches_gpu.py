@@ -453,3 +453,83 @@ def test_two_streams_fork_and_decode(fp16):
 
     one = torch.cuda.Stream()
     assert torch.equal(run([one, one]), run([torch.cuda.Stream(), torch.cuda.Stream()]))
+
+
+@pytest.mark.parametrize("record", [False, True])
+def test_beams_behind_a_long_prompt_read_it_once(record):
+    """The plan over the prompt's pages serves every step, however the beams' rows change behind them."""
+    print("case long prompt", record, flush=True)
+    W, Hq, Hkv, D, i32 = 5, 4, 2, 64, dict(dtype=torch.int32, device=DEV)
+    m = Mirror({}, Hq, Hkv, D, W, 170, blocks=140, seed=8)
+    m.add(0)
+    m.go([0], [2070])
+    sids = [0, *(("f", w) for w in range(1, W))]
+    m.kv.fork(sids[1:], 0)
+    for s in sids[1:]:
+        m.like(s, 0)
+    kv, rng = m.kv, np.random.default_rng(2)
+    slots, pos = torch.tensor([kv.slot[s] for s in sids], **i32), torch.full((W,), 2070, **i32)
+    ctx, parents, x = pos + 1, torch.zeros(1, W, **i32), torch.zeros(W, Hq + 2 * Hkv, D, dtype=torch.float16, device=DEV)
+    out, graph, plans = torch.zeros(W, Hq * D, dtype=torch.float16, device=DEV), None, set()
+    for i in range(36):
+        if kv.lacks_page(0):
+            kv.reserve(sids, PAGE)
+        new, exp = m.draw(sids, [1] * W)
+        x.copy_(new)
+        chosen = rng.integers(0, W, W).astype(np.int32)
+        parents.copy_(torch.from_numpy(chosen)[None])
+        kv.begin_forward(sids, [1] * W, device_meta=(slots, pos, ctx))
+        plans.add(id(kv.plan))
+        assert kv.plan is not None
+
+        def enqueue():
+            kv.attention_with_fused_qkv(0, x.clone(), Hq, out=out)
+            kv.reorder(sids, parents, slots, ctx)
+            pos.add_(1)
+            ctx.add_(1)
+
+        if record and i > 0:
+            if graph is None:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    enqueue()
+            graph.replay()
+        else:
+            enqueue()
+        kv.end_forward()
+        kv.adrift(sids, slots)
+        close(out, exp)
+        held = [(m.book.k[m.at[s]], m.book.v[m.at[s]]) for s in sids]
+        for j, s in enumerate(sids):
+            m.book.k[m.at[s]], m.book.v[m.at[s]] = held[chosen[j]]
+    assert len(plans) == 1
+    for s in sids:
+        kv.free_sequence(s)
+    assert sorted(kv.free) == list(range(170)) and not kv._owners
+
+
+@pytest.mark.parametrize("form", FORMS[:3])
+def test_a_wide_batch_in_fragment_order(form):
+    print("case wide", form, flush=True)
+    m = Mirror(form, 4, 2, 64, 75, 400, blocks=6, seed=9)
+    for s in range(75):
+        m.add(s)
+    m.go(list(range(75)), [1 + s for s in range(75)], frag=True)
+    for _ in range(2):
+        m.go(list(range(74, -1, -1)), [1] * 75, frag=True)
+
+
+@pytest.mark.parametrize("sinks", [1, 17, 40, 64, 70, 130])
+@pytest.mark.parametrize("quant", [False, True])
+def test_sinks_and_window_in_one_block(sinks, quant):
+    """Sinks of one to nine pages, with pages in between that nobody sees, or that only some tokens of a portion see."""
+    print("case sinks", sinks, quant, flush=True)
+    form = {"window": 45, "sinks": sinks, **({"bits": 8} if quant else {})}
+    m = Mirror(form, 8, 2, 128, 2, 60, blocks=26, seed=sinks)
+    m.add("a")
+    m.add("b")
+    m.go(["a"], [130])
+    m.go(["a", "b"], [77, 200])
+    m.go(["b"], [1])
+    m.go(["b", "a"], [33, 140])
+    m.go(["a"], [1])

@@ -194,6 +194,43 @@ def test_rows_of_beams_are_read_back(kw):
     assert copied.slot != kv.slot and not copied._adrift
 
 
+def test_beams_take_no_plan_from_rows_that_change():
+    """Pages that beams have come to share are not theirs to share for long: no plan is made of them, whatever it would save."""
+    rng = np.random.default_rng(1)
+    kv = cache(pages=1200, seqs=4, blocks=300, n_q_heads=2)
+    kv.add_sequence("p")
+    grow(kv, "p", 3)                                 # (no whole page that the beams share)
+    sids = ["p", "b", "c", "d"]
+    for s in sids[1:]:                               # as forks, whose copies the CPU does not make
+        kv.add_sequence(s)
+        grow(kv, s, 3)
+    beams = Device(kv, sids, 4)
+    kv.reserve(sids, 2320)                           # (so that the host hears of the rows at the end alone)
+    for i in range(2300):
+        beams.step(rng, i)
+    kv.settle()
+    sound(kv)
+    assert max(p for _, p in kv.prefix_groups(sids)) >= 128
+    kv.begin_forward(sids, [1] * 4, device_meta=(beams.slots, None, None))
+    assert kv.plan is None and kv.shared_plan(sids) is None
+
+
+def test_a_search_that_finds_no_room_leaves_nothing():
+    ds = load_pkg("decode_session")
+
+    class Model:
+        cache_forms, device = True, "cpu"
+
+    kv = cache(pages=12, seqs=5)
+    for s in "ab":
+        kv.add_sequence(s)
+        grow(kv, s, 32)
+    with pytest.raises(RuntimeError):                # rows for one more beam of each, not for two
+        ds.BeamSession(Model, kv, ["a", "b"], {}, torch.zeros(2, 50), 3)
+    assert sorted(kv.slot) == ["a", "b"]
+    sound(kv)
+
+
 def test_pages_of_a_copied_cache_are_its_own():
     kv = cache(bits=8)
     kv.pages(0)
