@@ -1368,7 +1368,7 @@ class BeamMoves(typing.NamedTuple):
 def beam_reorder(parents, slots, block_table, tok_pos):
     """Where beams go on whose parents [R, W] int32 `beam_select` has chosen: slots [R * W] int32, the rows of block_table that the beams have, become those returned: a
     parent's first child keeps its slot, further children take those of beams without any, whose rows of the table are changed to the parent's pages up to
-    that of the token appended last (tok_pos [R * W] int32).  -> (slots, BeamMoves): the last pages, and what else a slot holds, are to be copied by the moves."""
+    that of the token appended last (tok_pos [R * W] int32; positions of the next tokens: a page that is complete is taken over as well, not copied).  -> (slots, BeamMoves): the last pages, and what else a slot holds, are to be copied by the moves."""
     dev = _here(parents.device, "beam_reorder")
     if parents.dim() != 2 or block_table.dim() != 2 or slots.shape != (parents.numel(),) or tok_pos.shape != slots.shape:
         raise ValueError(f"beam_reorder: parents{tuple(parents.shape)} slots{tuple(slots.shape)} table{tuple(block_table.shape)} positions{tuple(tok_pos.shape)}")
