@@ -307,3 +307,37 @@ def test_quotients_half_way_between_two_codes(ops):
             step(ops, one, x[t:t + 1], seqs[t:t + 1], poss[t:t + 1])
         one.k, one.v, one.lens = book.k, book.v, book.lens
         one.same_pages(0)
+
+
+@pytest.mark.parametrize("step", [0.4, 1.0, 1.7, 2.5, 40.0, -0.7])
+@pytest.mark.parametrize("quant", [False, True])
+def test_scores_that_climb(ops, quant, step):
+    """The greatest score grows (or falls) from tile to tile by amounts around those for which sums are rescaled, in a prompt and in single tokens behind it."""
+    print("case climb", quant, step, flush=True)
+    Hq, Hkv, D, n = 4, 2, 64, 400
+    b = Book([0], Hq, Hkv, D, quant, seed=4, room=n + 20)
+    t = torch.arange(n + 20, device=b.dev, dtype=torch.float32) / 64
+    if step < 0:
+        t = t.flip(0)
+    u = torch.randn(D, generator=b.g).to(b.dev)
+    u /= u.norm()
+    # a rotation-free direction would need no tables: the tables here are made of ones and zeros, so that scores are what is drawn
+    b.cos.fill_(1)
+    b.sin.fill_(0)
+    size = (t * abs(step) * 0.6931 * D ** 0.5).sqrt()[:, None, None]
+    x = b.draw(n + 20, Hq + 2 * Hkv, D)
+    top = float(size.max())
+    x[:, :Hq] = (x[:, :Hq] * 0.05 + u * top).half()                          # q . k / sqrt(D) / ln 2 = step * token / 64, a little apart
+    x[:, Hq:Hq + Hkv] = (x[:, Hq:Hq + Hkv] * 0.01 + u * size * size / max(top, 1e-3)).half()
+    for new in [n] + [1] * 20:
+        at = b.lens[0]
+        x1, seqs, poss, q = b.take(x[at:at + new].contiguous(), [0], [new], [0] * new, list(range(at, at + new)))
+        if quant:
+            fn = ops.rope_attn_prefill_q8 if new > 1 else ops.rope_attn_decode_q8
+            out = fn(x1, b.pages, b.table, seqs, poss, b.cos, b.sin, Hq, Hkv, D)
+        elif new > 1:
+            ops.rope_kv_append(x1, b.kc, b.vc, b.table, seqs, poss, b.cos, b.sin, Hq, Hkv, D)
+            out = ops.paged_attn_prefill_window(x1, b.kc, b.vc, b.table, seqs, poss, Hq, Hkv, D, window=300)
+        else:
+            out = ops.rope_attn_decode_window(x1, b.kc, b.vc, b.table, seqs, poss, b.cos, b.sin, Hq, Hkv, D, window=300)
+        close(out, b.expect(q, seqs, poss, None if quant else 300))
