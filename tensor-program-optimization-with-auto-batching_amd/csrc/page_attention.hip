@@ -20,6 +20,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Weights enter the matrix cores as two fp16 halves, the greatest as 2^14 (2^15 with a page's factor): 22 bits, and none of them is off by more than 2^-39 of the greatest, where
 // fp16 numbers end.  (With 1 for the greatest it is 2^-25: too much where small weights meet values that are 2^25 times those of the others.)
 constexpr float TOP = 14.f;
+constexpr float NOTHING = -1e30f;             // the maximum of no scores: below every score but -inf, whose weight stays 0
 
 struct PageAttn {
   f16* out;
@@ -144,7 +145,7 @@ __device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh,
 // One token a sequence: rotation, the new token's place in the cache, and attention.  A workgroup has a kv head of a sequence, or a share of
 // its pages; its waves take them in turn, in the matrix-core layouts of the decode kernel in attention.hip.  A wave keeps two pages on their way in registers.
 //
-// Bound by the memory: 256 rows of 128 to 2048 tokens, 8 kv heads of 128, 579 MB in 8 bits, take 141 us (4.1 TB/s), 4 rows of 31000 55 (4.7) and 5 for the join, 48 rows that
+// Bound by the memory: 256 rows of 128 to 2048 tokens, 8 kv heads of 128, 579 MB in 8 bits, take 139 us (4.2 TB/s), 4 rows of 31000 55 (4.7) and 5 for the join, 48 rows that
 // see 2052 tokens of fp16 pages 78 (5.2).  Equal rows (256 of 1080) take 125, only read 107: what is left are the tokens' own pages, which are dirtied in lines of 64 bytes for
 // 2 or 16 of them, and a workgroup's first reads, which wait for one another.  Three or four pages on their way, loads past the caches, several kv heads a workgroup and an order
 // of workgroups by chiplet: no faster, or slower.
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int seq = a.tok_seq[b], pos = a.tok_pos[b];
   const bool ok = token_ok(a, seq, pos);                    // uniform; otherwise no token is seen
-  float m = -INFINITY, l = 0.f;
+  float m = NOTHING, l = 0.f;
   f32x4 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -190,22 +191,21 @@ __global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
 
     // the scores of a page become weights: st, by `scale`, of which a lane has tokens first .. first + 3; EDGE: some may not be seen
     auto weights = [&](f32x4 st, float scale, int first, int end, f16x8& p, bool edge) {
-      float pm = -INFINITY;
+      float pm = NOTHING;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         st[e] *= scale;
         if (edge && (first + e >= end || (first + e < least && first + e >= a.sinks))) st[e] = -INFINITY;
         pm = fmaxf(pm, st[e]);
       }
-      pm = groups_max(pm);
-      if (__any(pm > m)) {
-        const float mn = fmaxf(m, pm), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      if (__any(pm > m + 1.9f)) {                           // (seldom behind the first pages: m may be so far below the greatest, whose weight is below 2^15.9 then)
+        const float mn = fmaxf(m, groups_max(pm)), alpha = __builtin_amdgcn_exp2f(m - mn);
         l *= alpha;
         m = mn;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) o[db] *= alpha;
       }
-      const float base = m == -INFINITY ? 0.f : m - TOP;
+      const float base = m - TOP;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float w = __builtin_amdgcn_exp2f(st[e] - base);
@@ -385,11 +385,10 @@ __global__ __launch_bounds__(NW* WAVE, 4) void page_decode_kernel(PageAttn a) {
     float M = sm[0][qh];
 #pragma unroll
     for (int w = 1; w < NW; ++w) M = fmaxf(M, sm[w][qh]);
-    const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, x = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sm[w][qh] - base);
+      const float f = __builtin_amdgcn_exp2f(sm[w][qh] - M);
       L += sl[w][qh] * f;
       x += sacc[((size_t)w * G + qh) * D + d] * f;
     }
@@ -425,14 +424,14 @@ __global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
     float m = M;
 #pragma unroll
     for (int u = 0; u < 4; ++u) m = fmaxf(m, ml[u][0]);
-    const float base = m == -INFINITY ? 0.f : m, f = __builtin_amdgcn_exp2f(M - base);
+    const float f = __builtin_amdgcn_exp2f(M - m);             // (m is NOTHING at least)
     M = m;
     L *= f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) o[e] *= f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float fu = __builtin_amdgcn_exp2f(ml[u][0] - base);
+      const float fu = __builtin_amdgcn_exp2f(ml[u][0] - m);
       L += ml[u][1] * fu;
 #pragma unroll
       for (int e = 0; e < PER; ++e) o[e] += x[u][e] * fu;
@@ -532,8 +531,6 @@ __device__ __forceinline__ float rest_of(float w, f16x2 h) {
   else asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(x.u), "v"(w));
   return r;
 }
-
-constexpr float NOTHING = -1e30f;             // the maximum of no scores: below every score but -inf, whose weight stays 0
 
 // Scores of P pages under a tile's column, in units by[p] > 0, become weights, as pairs of fp16 halves, and the column's maximum and sum go on.  A page's weights
 // come times 2^up[p] = 1 / share[p].
