@@ -3,8 +3,8 @@
 //   out[t, h] = softmax(scale q[t, h] . K) V  over the tokens that position p sees: j <= p and (j > p - window or j < sinks)
 //
 // Pages of 8 bits: once the 16 tokens of a page are there, its keys and its values are rounded per kv head to code * step, step = fp32(a / 127),
-// a = max |x|, code = rint(127 x / a).  That is exact in fp32: x and a are fp16 numbers, so 127 x / a, where it is below 2^(8 - d), is a ratio whose
-// denominator is below 2^(11 + d): it is half-way between two integers or at least 2^(-12 - d) off, and the division errs by 2^(-16 - d).
+// a = max |x|, code = rint(127 x / a).  That can be had exactly from fp32: x and a are fp16 numbers, so 127 x / a, where it is below 2^(8 - d), is a ratio whose
+// denominator is below 2^(11 + d): it is half-way between two integers or at least 2^(-12 - d) off.
 // A page with an infinity or NaN has a step that is NaN.  The tokens of a sequence's last page lie unrounded in its tail.  A query sees its
 // own page unrounded and the pages ahead of it in 8 bits, so results do not depend on how a prompt is cut into passes.
 //
@@ -100,23 +100,40 @@ __device__ __forceinline__ bool token_ok(const PageAttn& a, int seq, int pos) {
 
 // How a page's keys or values are rounded, of which a wave holds all
 struct Rounding {
-  float most, step;                                        // infinite: codes 0
-  __device__ __forceinline__ uint32_t code(float x) const { return (uint32_t)((int)rintf(127.f * (most == INFINITY ? 0.f : x) / most) & 255); }
+  float by, step;                                          // 127 / a, 0 for a page of zeros
+  uint32_t keep;                                           // 0: codes are 0
+  // A code in the low byte, behind others' bits.  The product by 127 / a is less than 2^-23 of itself off (two roundings).  Rounded to 21 bits it is what the quotient would be, rounded so: a quotient below
+  // 2^(8 - d) is half-way between two integers or 2^(-12 - d) off at least, steps of 21 bits are 2^(-13 - d), and half-way points are among them.  Behind the sum with 1.5 2^23 the whole
+  // number, ties to even, is the last bits.  (Divisions took 15 instructions a code, this takes 5: 8 prompts of 456 tokens, 32 heads, 33 us to 27.)
+  __device__ __forceinline__ uint32_t bits(float x) const {
+    const uint32_t y = (__float_as_uint(x * by) + 4) & ~7u;
+    return __float_as_uint(__fadd_rn(__uint_as_float(y), 12582912.f)) & keep;
+  }
 };
+
+// Four codes of bits() as bytes
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400), __builtin_amdgcn_perm(b, a, 0x0c0c0400), 0x05040100);
+}
+
+// Of a wave's whole page: magnitudes of fp16 numbers are in the order of their bits, infinities and NaN last
 template <class T, int N>
 __device__ __forceinline__ Rounding rounding_of(const T (&x)[N]) {
-  float most = 0.f, odd = 0.f;                             // odd: x - x, which is zero but for infinities and NaN
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
 #pragma unroll
-  for (int i = 0; i < N; ++i)
+  for (int i = 0; i < N; ++i) {
+    union { T h; uint32_t u[sizeof(T) / 4]; } y = {x[i]};
 #pragma unroll
-    for (int e = 0; e < (int)(sizeof(T) / 2); ++e) {
-      const float y = (float)x[i][e];
-      most = fmaxf(most, fabsf(y));
-      odd += y - y;
+    for (int e = 0; e < (int)(sizeof(T) / 4); ++e) {
+      union { uint32_t u; u16x2 h; } z = {y.u[e] & 0x7fff7fffu};
+      most = __builtin_elementwise_max(most, z.h);
     }
-  most = wave_max(most);
-  const bool bad = __any(odd != 0.f);
-  return Rounding{most > 0.f && !bad ? most : INFINITY, bad ? NAN : most / 127.f};
+  }
+  const uint32_t m = (uint32_t)wave_max((float)max(most[0], most[1]));
+  union { uint16_t u; f16 h; } a = {(uint16_t)m};
+  const bool bad = m >= 0x7c00, none = m == 0;
+  return Rounding{bad || none ? 0.f : 127.f / (float)a.h, bad ? NAN : (float)a.h / 127.f, bad ? 0u : ~0u};
 }
 
 // A whole page of a head from a wave's operands - keys: lane (g, token) dims 32 kb + 8 g ..; values: lane (g, col) tokens 4 g .. of dims 16 db + col -
@@ -129,11 +146,14 @@ __device__ __forceinline__ void store_codes(const PageAttn& a, int page, int kh,
   uint8_t* vp = (uint8_t*)a.v + ((size_t)page * a.Hkv + kh) * PAGE * D + lane * 16;
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) {
-    uint32_t x[4] = {}, y[4] = {};
+    uint32_t x[4], y[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[e / 4] |= rk.code((float)k[2 * j + e / 8][e % 8]) << (8 * (e % 4));
-      y[e / 4] |= rv.code((float)v[4 * j + e / 4][e % 4]) << (8 * (e % 4));
+    for (int e = 0; e < 4; ++e) {
+      const f16x8& h = k[2 * j + e / 2];
+      const f16x4& w = v[4 * j + e];
+      const int at = 4 * (e % 2);
+      x[e] = bytes_of(rk.bits(h[at]), rk.bits(h[at + 1]), rk.bits(h[at + 2]), rk.bits(h[at + 3]));
+      y[e] = bytes_of(rv.bits(w[0]), rv.bits(w[1]), rv.bits(w[2]), rv.bits(w[3]));
     }
     *reinterpret_cast<uint4*>(kp + j * 1024) = uint4{x[0], x[1], x[2], x[3]};
     *reinterpret_cast<uint4*>(vp + j * 1024) = uint4{y[0], y[1], y[2], y[3]};
@@ -451,8 +471,8 @@ __global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
 // their pieces of the next four from the cache into LDS as fp16 operands while the workgroup multiplies four.  Tokens' own pages of 8-bit caches come first, unrounded.
 //
 // Bound by what a SIMD's four waves issue and wait for in turn, over the same phases between two barriers (per cent of the time of 4096 tokens under a window of 1024: vector
-// instructions 56, of them products 35, LDS reads 45; taken out one by one, loads, LDS reads, the softmax and the weights' second halves are 15 to 24 % each).  Those 4096 tokens,
-// 32 heads over 8, take 134 us, 450 TFLOP/s; 8 prompts of 456 on 8-bit pages, 32 heads, 99, with 33 + 6 for rounding and storing; 777 tokens behind 3500, 32 heads over 8, 128
+// instructions 50, of them products 36, LDS reads 25; taken out one by one, loads, LDS reads, the softmax and the weights' second halves were 15 to 24 % each).  Those 4096 tokens,
+// 32 heads over 8, take 129 us, 465 TFLOP/s; 8 prompts of 456 on 8-bit pages, 32 heads, 99, with 27 + 6 for rounding and storing; 777 tokens behind 3500, 32 heads over 8, 128
 // (340 TFLOP/s) with 22 for storing and joining.  No faster: keys ahead by four or six fragments, values by four; slower: two tiles a wave (below).
 //
 // Of a page's step 2^e f (1 <= f < 2), the power of two goes into the values' operand, relative to the largest so far, where it is exact, and f into the
@@ -1004,7 +1024,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 
 // Pages that a pass completes, in 8 bits: a wave has the keys or the values of 16 tokens of the pass under a kv head, and of the tokens those that are the first of their page
 // in the pass.  D / 16 lanes take a token's row, so that a load's lines are whole; the codes go by way of LDS into their order.  8 prompts of 456 tokens, 32 heads of 128, 90 MB:
-// 33 us, 2.7 TB/s; a page's steps (its 16 rows, the largest, codes, LDS, the store) wait for one another.  Products instead of divisions: 33 as well.
+// 27 us, 3.3 TB/s; a page's steps (its 16 rows, the largest, codes, LDS, the store) wait for one another.  More waves a SIMD than the five of 97 registers: spills (80 registers: 37).
 template <int D>
 __global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
   constexpr int LD = 20, NCH = D / 16, PER = WAVE / NCH, NP = 16 / PER;       // bytes of a dim's tokens in LDS, apart for the banks; lanes of a row; rows of a load; loads
@@ -1064,13 +1084,13 @@ __global__ __launch_bounds__(4 * WAVE) void page_store_kernel(PageAttn a) {
 #pragma unroll
     for (int i = 0; i < 2 * NP; ++i) {
       const int token = lane / NCH + PER * (i / 2), k8 = ch + (i % 2) * NCH;
-      uint32_t y[2] = {};
+      uint32_t y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e / 4] |= r.code((float)x[i][e]) << (8 * (e % 4));
-      if (!values) *reinterpret_cast<uint2*>(at + (((k8 / 8) * 4 + k8 % 4) * 16 + token) * 16 + (k8 / 4 % 2) * 8) = uint2{y[0], y[1]};
+      for (int e = 0; e < 8; ++e) y[e] = r.bits(x[i][e]);
+      if (!values) *reinterpret_cast<uint2*>(at + (((k8 / 8) * 4 + k8 % 4) * 16 + token) * 16 + (k8 / 4 % 2) * 8) = uint2{bytes_of(y[0], y[1], y[2], y[3]), bytes_of(y[4], y[5], y[6], y[7])};
       else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) at[(k8 * 8 + e) * LD + token] = (uint8_t)(y[e / 4] >> (8 * (e % 4)));
+        for (int e = 0; e < 8; ++e) at[(k8 * 8 + e) * LD + token] = (uint8_t)y[e];
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
