@@ -341,3 +341,28 @@ def test_scores_that_climb(ops, quant, step):
         else:
             out = ops.rope_attn_decode_window(x1, b.kc, b.vc, b.table, seqs, poss, b.cos, b.sin, Hq, Hkv, D, window=300)
         close(out, b.expect(q, seqs, poss, None if quant else 300))
+
+
+@pytest.mark.parametrize("shift", [-24, -20, -14, -7, 0, 6])
+def test_codes_of_every_magnitude(ops, shift):
+    """Pages of fp16 numbers of any bits, down to the smallest there is: every code is the nearest whole number to 127 x / a."""
+    print("case magnitudes", shift, flush=True)
+    T = 2048
+    b = Book([0], 8, 8, 128, True, seed=100 + shift, room=T)
+    b.cos.fill_(1), b.sin.fill_(0)
+    g = torch.Generator().manual_seed(shift + 50)
+    low = max(0, (shift + 24 - 12) << 10) if shift > -14 else 0                # of bits: up to 2^13 below the largest
+    high = (1 << (shift + 24)) + 3 if shift < -14 else (shift + 15) << 10
+    bits = torch.randint(low, high, (T, 24, 128), generator=g, dtype=torch.int32)
+    y = (bits | torch.randint(0, 2, bits.shape, generator=g, dtype=torch.int32) << 15).to(torch.int16).view(torch.float16).to(b.dev)
+    y[:, :8] = 0                                                               # (scores are zero)
+    x, seqs, poss, q = b.take(y, [0], [T], [0] * T, list(range(T)))
+    b.k[0] = x[:, 8:16].clone()
+    out = prompt(ops, b, x, seqs, poss)
+    b.same_pages(0)
+    keys, values = b.pages.values(b.table[0, :T // 16].contiguous())
+    for got, want in ((keys, b.k[0]), (values, b.v[0])):
+        step = want.view(-1, 16, 8, 128).abs().amax((1, 3)).double() / 127
+        d = (got.transpose(1, 2).double() - want.view(-1, 16, 8, 128).double()).abs()
+        # half a step, the step's rounding (up to 127 of them), fp16's rounding of what is given back
+        assert bool((d <= step[:, None, :, None] * (0.5 + 127 * 2.0 ** -24) + want.view(-1, 16, 8, 128).double().abs() * 2.0 ** -10 + 2.0 ** -24).all())
