@@ -614,6 +614,26 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     if (r < nt) b = r == 0 || a.tok_seq[t] != a.tok_seq[t - 1] || a.tok_pos[t] != a.tok_pos[t - 1] + 1 || a.tok_pos[t] == 0;      // (0 behind -1, which is none)
     begins[j] = __ballot(b);
   }
+  // 8 bits: the tokens' own keys and values, on their way to LDS: a thread's pairs of 8 dims of keys, and 8 dims of values
+  constexpr int KI = Q8 ? QB * (D / 16) / (NW * WAVE) : 1, VI = Q8 ? 2 * KI : 1;
+  f16x8 kx[KI], ky[KI], vx[VI];
+  int kpos[KI];
+  if (Q8 && split == 0) {
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int e = threadIdx.x + i * NW * WAVE, rr = e / (D / 16), c = e % (D / 16), tt = t0 + min(rr, nt - 1);
+      const f16* row = a.qkv + ((size_t)tt * HH + a.Hq + kh) * D + (c >> 2) * 32 + (c & 3) * 8;
+      kx[i] = ld8(row);
+      ky[i] = ld8(row + D / 2);
+      const int pos = a.tok_pos[tt];
+      kpos[i] = rr < nt && token_ok(a, a.tok_seq[tt], pos) ? pos : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int e = threadIdx.x + i * NW * WAVE, rr = e / (D / 8), c = e % (D / 8);
+      vx[i] = ld8(a.qkv + ((size_t)(t0 + min(rr, nt - 1)) * HH + a.Hq + a.Hkv + kh) * D + c * 8);
+    }
+  }
   f16x8 q[NT][NKB];
   f32x4 o[NT][NDB];
   float m[NT], l[NT];
@@ -644,20 +664,19 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     // The own pages, unrounded: the tokens' keys and values by way of LDS
     f16* ok = lds;
     f16* ov = lds + 4 * NKB * KLD * 8;
-    for (int i = threadIdx.x; i < nt * (D / 16); i += NW * WAVE) {     // 8 pairs of a key
-      const int r = i / (D / 16), c = i % (D / 16), gg = c & 3, kb = c >> 2, t = t0 + r;
-      const int pos = a.tok_pos[t];
-      if (!token_ok(a, a.tok_seq[t], pos)) continue;
-      const f16* row = a.qkv + ((size_t)t * HH + a.Hq + kh) * D + kb * 32 + gg * 8;
-      const size_t at = (size_t)pos * (D / 2) + kb * 32 + gg * 8;
-      f16x8 x = ld8(row), y = ld8(row + D / 2);
-      rotate8(x, y, a.rope_cos + at, a.rope_sin + at);
-      st8(ok + ((kb * 4 + gg) * KLD + r) * 8, x);
-      st8(ok + (((kb + NKB / 2) * 4 + gg) * KLD + r) * 8, y);
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int e = threadIdx.x + i * NW * WAVE, rr = e / (D / 16), c = e % (D / 16), gg = c & 3, kb = c >> 2;
+      if (kpos[i] < 0) continue;
+      const size_t at = (size_t)kpos[i] * (D / 2) + kb * 32 + gg * 8;
+      rotate8(kx[i], ky[i], a.rope_cos + at, a.rope_sin + at);
+      st8(ok + ((kb * 4 + gg) * KLD + rr) * 8, kx[i]);
+      st8(ok + (((kb + NKB / 2) * 4 + gg) * KLD + rr) * 8, ky[i]);
     }
-    for (int i = threadIdx.x; i < nt * (D / 8); i += NW * WAVE) {      // 8 dims of a value
-      const int r = i / (D / 8), c = i % (D / 8);
-      st8(ov + r * VLD + c * 8, ld8(a.qkv + ((size_t)(t0 + r) * HH + a.Hq + a.Hkv + kh) * D + c * 8));
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int e = threadIdx.x + i * NW * WAVE, rr = e / (D / 8), c = e % (D / 8);
+      if (rr < nt) st8(ov + rr * VLD + c * 8, vx[i]);
     }
     __syncthreads();
 #pragma unroll
@@ -673,7 +692,13 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
         todo &= ~(unsigned)(__ballot(in) & 0xffff);
         f32x4 st[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
         f16x4 v[NDB];
-        if (r0 >= 0 && a.tok_seq[t0 + r0] == s && a.tok_pos[t0 + r0] == p * PAGE) {       // uniform
+        bool whole = r0 >= 0;                                         // uniform: no run begins behind its first token
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int from = max(r0 + 1 - 64 * j, 0), to = row - t0 - 64 * j;     // of begins[j], bits from .. to
+          if (from <= to && from < 64 && (begins[j] >> from << from) & (to < 63 ? (2ull << to) - 1 : ~0ull)) whole = false;
+        }
+        if (whole) {
           const int rk = min(r0 + col, QB - 1);
 #pragma unroll
           for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(ld8(ok + ((kb * 4 + g) * KLD + rk) * 8), q[i][kb], st[0]);
@@ -996,14 +1021,18 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     }
   }
 
+  // Results go by way of LDS, a tile of a wave at a time, so that lines are written whole (everybody is done with the ring: a barrier ends every block)
+  constexpr int OLD = D + 8;
+  static_assert(NW * 16 * OLD <= (RING > OWN ? RING : OWN), "the tiles fit the ring");
+  f16* mine = lds + wave * 16 * OLD;
   const float scale_up = power(unit);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    const int t = t0 + ctok[i], h = kh * G + (wave * 16 * NT + i * 16 + col) % G;
     l[i] += __shfl_xor(l[i], 16, WAVE);
     l[i] += __shfl_xor(l[i], 32, WAVE);
-    if (ctok[i] >= nt) continue;
-    if (a.splits > 1) {
+    if (a.splits > 1) {                                               // uniform
+      if (ctok[i] >= nt) continue;
+      const int t = t0 + ctok[i], h = kh * G + (wave * 16 * NT + i * 16 + col) % G;
       const size_t at = ((size_t)t * a.Hq + h) * a.splits + split;
 #pragma unroll
       for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(a.acc + at * D + db * 16 + 4 * g) = o[i][db] * scale_up;
@@ -1013,11 +1042,19 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     const float f = l[i] == 0.f ? 0.f : scale_up / l[i];
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
-      const int d = h * D + db * 16 + 4 * g;
       f16x4 x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = (f16)(l[i] == 0.f ? 0.f : o[i][db][e] * f);
-      *reinterpret_cast<f16x4*>(a.out + (a.frag_tt ? frag_offset(t, d, a.frag_tt) : (size_t)t * a.Hq * D + d)) = x;
+      *reinterpret_cast<f16x4*>(mine + col * OLD + db * 16 + 4 * g) = x;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const int e = j * WAVE + lane, rr = e / (D / 8), c = e % (D / 8), r = wave * 16 * NT + i * 16 + rr, tok = r / G, d = (kh * G + r % G) * D + c * 8;
+      const f16x8 x = ld8(mine + rr * OLD + c * 8);
+      if (tok < nt) st8(a.out + (a.frag_tt ? frag_offset(t0 + tok, d, a.frag_tt) : (size_t)(t0 + tok) * a.Hq * D + d), x);
     }
   }
 }
