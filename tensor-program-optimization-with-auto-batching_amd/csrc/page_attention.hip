@@ -472,8 +472,8 @@ __global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
 //
 // Bound by what a SIMD's four waves issue and wait for in turn, over the same phases between two barriers (per cent of the time of 4096 tokens under a window of 1024: vector
 // instructions 50, of them products 36, LDS reads 25; taken out one by one, loads, LDS reads, the softmax and the weights' second halves were 15 to 24 % each).  Those 4096 tokens,
-// 32 heads over 8, take 129 us, 465 TFLOP/s; 8 prompts of 456 on 8-bit pages, 32 heads, 99, with 27 + 6 for rounding and storing; 777 tokens behind 3500, 32 heads over 8, 128
-// (340 TFLOP/s) with 22 for storing and joining.  No faster: keys ahead by four or six fragments, values by four; slower: two tiles a wave (below).
+// 32 heads over 8, take 128 us, 470 TFLOP/s; 8 prompts of 456 on 8-bit pages, 32 heads, 97, with 27 + 6 for rounding and storing; 777 tokens behind 3500, 32 heads over 8, 126
+// (350 TFLOP/s) with 20 for storing and joining.  No faster: keys ahead by four or six fragments, values by four; slower: two tiles a wave (below).
 //
 // Of a page's step 2^e f (1 <= f < 2), the power of two goes into the values' operand, relative to the largest so far, where it is exact, and f into the
 // weights, so that two pages with steps of their own fill one matrix instruction.
