@@ -533,3 +533,53 @@ def test_sinks_and_window_in_one_block(sinks, quant):
     m.go(["b"], [1])
     m.go(["b", "a"], [33, 140])
     m.go(["a"], [1])
+
+
+@pytest.mark.parametrize("form", [{}, {"bits": 8}, {"bits": 8, "window": 40, "sinks": 2}])
+@pytest.mark.parametrize("graph", [False, True])
+def test_searches_beside_each_other(fp16, form, graph):
+    """Two searches and a greedy batch take turns on one cache, from which sequences come and go meanwhile: each gives what it gives alone."""
+    print("case beside", form, graph, flush=True)
+    _, model = fp16
+    ds = load_pkg("decode_session")
+    prompts, steps = prompts_of(model, (45, 14, 30, 20), 15), 40
+
+    def made(kv, which):
+        out = {}
+        for i in which:
+            z = begin(model, kv, i, prompts[i])
+            if i < 2:
+                out[i] = ds.BeamSession(model, kv, [i], {}, z, 3 + i, use_graph=graph)
+            elif i == 2:
+                out[i] = ds.DecodeSession(model, kv, [i], {}, z.argmax(-1).int(), use_graph=graph)
+        return out
+
+    def result(s):
+        return s.answers() if isinstance(s, ds.BeamSession) else torch.stack(s.history).tolist()
+
+    make = lambda: model.create_paged_kv_cache(10, 10 * 128, 64, 16, max_seq_len=128, **form)                              # noqa: E731
+    alone = {}
+    for i in range(3):
+        s = made(make(), [i])[i]
+        for _ in range(steps):
+            s.step(**({"keep_history": True} if i == 2 else {}))
+        alone[i] = result(s)
+    kv = make()
+    sessions = made(kv, range(3))
+    for j in range(steps):
+        for i, s in sessions.items():
+            s.step(**({"keep_history": True} if i == 2 else {}))
+        if j % 7 == 3:
+            begin(model, kv, "x", prompts[3])
+        if j % 7 == 5:
+            kv.free_sequence("x")
+    for i, s in sessions.items():
+        got = result(s)
+        if i < 2:
+            assert [[t for _, t in r] for r in got] == [[t for _, t in r] for r in alone[i]] and [[v for v, _ in r] for r in got] == [[v for v, _ in r] for r in alone[i]]
+            s.close()
+        else:
+            assert got == alone[i]
+    for i in list(kv.slot):
+        kv.free_sequence(i)
+    assert sorted(kv.free) == list(range(kv.n_pages)) and not kv._owners
