@@ -2,7 +2,8 @@
 //
 //   value(b, v) = score[b] + z[b, v] - log sum_u exp z[b, u]        candidates of a request: its beams x the vocabulary
 //
-// The k greatest, the lowest b V + v of equal ones.  Within a beam the order is that of the logits, exactly; between beams values are compared in 64 bits.
+// The k greatest, the lowest b V + v of equal ones.  Within a beam the order is that of the logits, exactly; between beams values are compared in 64 bits, of sums of exponentials
+// that were taken in 32 (values closer than those are exact may change places).
 #include "common.h"
 
 namespace {
