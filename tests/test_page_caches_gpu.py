@@ -583,3 +583,22 @@ def test_searches_beside_each_other(fp16, form, graph):
     for i in list(kv.slot):
         kv.free_sequence(i)
     assert sorted(kv.free) == list(range(kv.n_pages)) and not kv._owners
+
+
+def test_all_together_on_a_4_bit_model():
+    """A search by the front end over a model with 4-bit linears and adapters, on a cache in 8 bits under a window, whose prompts begin alike."""
+    print("case together", flush=True)
+    synth = load_pkg("synth")
+    wl = synth.config1()
+    model = load_pkg("llama").LlamaForCausalLM.from_synthetic(wl.seed, wl.shape, [wl.lora], DEV, quant_group=64)
+    prompts = prompts_of(model, (50, 50, 21), 20)
+    prompts[1] = np.concatenate([prompts[0][:40], prompts[1][:10]])
+    form = {"bits": 8, "window": 36, "sinks": 2}
+    got, b = front_end(model, prompts, [1, 1, 1], [24, 24, 24], beams=3, cache_bits=8, window=36, sinks=2, share_prefix=True)
+    order = b.seq_info.order_seqs([0, 1, 2])[0]
+    kv = model.create_paged_kv_cache(20, 20 * 112, 64, 16, max_seq_len=88, **form)
+    # prompts that are prefilled whole: the last ten tokens of the second take other kernels in the front end, so that its logits differ by roundings
+    scores, want = naive_search(model, kv, [prompts[i] for i in order], [1, 1, 1], 3, 23, None)
+    for i, w, s in zip(order, want, scores):
+        assert got[i] == w[0] or i == 1 and len(got[i]) == 24, i
+    assert len(b.graph.kv_cache.slot) == 3 and all(len(b.graph.kv_cache.pages_of(i)) <= 1 + 36 // 16 + 3 for i in range(3))
