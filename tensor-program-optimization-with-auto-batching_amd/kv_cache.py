@@ -237,9 +237,10 @@ class PageTable:
             raise RuntimeError("begin_forward called twice without end_forward")
         if len(seq_ids) != len(append_lens):
             raise ValueError("seq_ids and append_lens differ in length")
-        if self._adrift and (device_meta is None or self._dirty):
-            self.settle()
         self._release(seq_ids)
+        if self._adrift and (device_meta is None or self._dirty):      # (a table that changes is uploaded whole, the beams' rows with it)
+            self.settle()
+            self._release(seq_ids)
         # Which sequences lack a page (they are handed out in order: the last one needed is missing).  us a step without host-made arrays, one by one / all at
         # once: one sequence 2.5 / 15.5, four 3.6 / 16.3, 64 29 / 34, 212 94 / 81
         if len(seq_ids) < AT_ONCE:
