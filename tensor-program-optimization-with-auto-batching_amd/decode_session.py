@@ -114,11 +114,12 @@ class BeamSession:
         self.model, self.kv, self.R, self.W, self.eos, self.left = model, kv, R, W, eos, steps
         dev = model.device
         i32 = lambda a: (a if isinstance(a, torch.Tensor) else torch.as_tensor(np.asarray(a, dtype=np.int32))).to(dev, torch.int32)      # noqa: E731
-        self.seq_ids = []
+        self.seq_ids, self._forks = [], []
         try:
             for sid in seq_ids:
                 forks = [("beam", sid, w) for w in range(1, W)]
                 kv.fork(forks, sid)
+                self._forks += forks
                 self.seq_ids += [sid, *forks]
         except Exception:
             self.close()
@@ -203,9 +204,9 @@ class BeamSession:
 
     def close(self):
         """Gives back the rows and pages of all beams but each request's first, which goes on under its sequence's id (at whatever beam it is)."""
-        for s in self.seq_ids:
-            if isinstance(s, tuple) and s[0] == "beam":
-                self.kv.free_sequence(s)
+        while self._forks:
+            self.kv.free_sequence(self._forks[0])
+            del self._forks[0]
 
 
 class NativeDecodeSession:

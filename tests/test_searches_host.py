@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+from conftest import load_pkg
 from test_page_caches_host import PAGE, Device, cache, grow, sound
 
 
@@ -64,4 +65,89 @@ def test_searches_under_a_window_beside_each_other(window, sinks, lens):
             one.step(rng, i)
             assert i == 0 or torch.equal(visible(kv, other), before), i        # (ahead of its first step a search's rows are on the host alone)
     kv.settle()
+    sound(kv)
+
+
+class Model:
+    """Logits from a table, a row for every token; `fails` raises instead."""
+
+    cache_forms, device = True, "cpu"
+
+    def __init__(self, V=50, seed=0):
+        self.table = torch.randn((V, V), generator=torch.Generator().manual_seed(seed))
+        self.fails = False
+
+    def embed(self, tokens):
+        return self.table[tokens.long()]
+
+    def forward(self, hidden, kv, tok_adapter):
+        if self.fails:
+            raise RuntimeError("a forward pass that fails")
+        return hidden
+
+
+def select(logits, scores, ended=None, eos=None, k=None):
+    """ops.beam_select on the CPU."""
+    (R, W), V = scores.shape, logits.shape[1]
+    k = W if k is None else k
+    value = scores.double()[..., None] + logits.double().log_softmax(-1).view(R, W, V)
+    if ended is not None:
+        only = torch.where(torch.arange(V) == eos, scores.double()[..., None], -torch.inf)
+        value = torch.where(ended[..., None] != 0, only, value)
+    value = torch.where(value > -torch.inf, value, -torch.inf).view(R, W * V)
+    value = torch.nn.functional.pad(value, (0, max(0, k - W * V)), value=-torch.inf)
+    best, at = value.sort(dim=1, descending=True, stable=True)
+    best, at = best[:, :k], at[:, :k].int()
+    none = best == -torch.inf
+    return best.float(), torch.where(none, -1, at % V), torch.where(none, -1, at // V)
+
+
+def reorder(parents, slots, table, ctx):
+    """ops.beam_reorder on the CPU, without the moves."""
+    (R, W), new, old = parents.shape, slots.clone(), table.clone()
+    for r in range(R):
+        p, mine = parents[r].tolist(), slots.view(R, W)[r].tolist()
+        dead, block = [w for w in range(W) if w not in p], int(ctx[r * W]) // PAGE
+        for w in range(W):
+            stays = p[w] >= 0 and p[w] not in p[:w]
+            to = mine[p[w]] if stays else mine[dead.pop(0)]
+            if p[w] >= 0 and not stays:
+                table[to, :block] = old[mine[p[w]], :block]
+            new[r * W + w] = to
+    return new, load_pkg("ops").BeamMoves(new, new, new, new)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    ops = load_pkg("ops")
+    monkeypatch.setattr(ops, "beam_select", select)
+    monkeypatch.setattr(ops, "beam_reorder", reorder)
+    monkeypatch.setattr(ops, "copy_pages", lambda *a: None)
+    return load_pkg("decode_session")
+
+
+def prompts(kv, lens):
+    for sid, n in lens.items():
+        kv.add_sequence(sid)
+        grow(kv, sid, n)
+
+
+def test_a_search_gives_back_its_own_forks_alone(on_cpu):
+    """Whatever the caller's sequences are called, and however often a search is closed."""
+    kv = cache(pages=60, seqs=12)
+    prompts(kv, {0: 32, ("beam", "mine"): 48, ("beam", 7, 1): 16})
+    model = Model()
+    ids = [0, ("beam", "mine"), ("beam", 7, 1)]
+    s = on_cpu.BeamSession(model, kv, ids, {}, model.table[:3], 3)
+    for _ in range(20):
+        s.step()
+    s.close()
+    assert list(kv.slot) == ids
+    sound(kv)
+    s.close()
+    assert list(kv.slot) == ids and [len(kv.pages_of(i)) for i in ids] == [4, 5, 3]
+    again = on_cpu.BeamSession(model, kv, ids, {}, model.table[:3], 4)
+    again.step()
+    again.close()
+    assert list(kv.slot) == ids
     sound(kv)
