@@ -112,8 +112,6 @@ class BeamSession:
         if not 1 <= W <= 16 or logits.shape[0] != R:
             raise ValueError(f"BeamSession: {W} beams (1 to 16) of {R} sequences, logits of {logits.shape[0]}")
         self.model, self.kv, self.R, self.W, self.eos, self.left = model, kv, R, W, eos, steps
-        dev = model.device
-        i32 = lambda a: (a if isinstance(a, torch.Tensor) else torch.as_tensor(np.asarray(a, dtype=np.int32))).to(dev, torch.int32)      # noqa: E731
         self.seq_ids, self._forks = [], []
         try:
             for sid in seq_ids:
@@ -121,9 +119,17 @@ class BeamSession:
                 kv.fork(forks, sid)
                 self._forks += forks
                 self.seq_ids += [sid, *forks]
+            self._begin(tok_adapter, logits)
         except Exception:
             self.close()
             raise
+        self.use_graph, self._eager_steps = use_graph, 0
+        self.graph = self._plan = self._cut = None
+
+    def _begin(self, tok_adapter, logits):
+        """The beams' state on the device, and their first tokens."""
+        model, kv, R, W, dev = self.model, self.kv, self.R, self.W, self.model.device
+        i32 = lambda a: (a if isinstance(a, torch.Tensor) else torch.as_tensor(np.asarray(a, dtype=np.int32))).to(dev, torch.int32)      # noqa: E731
         self.tok_adapter = {tid: i32(ids).repeat_interleave(W) for tid, ids in tok_adapter.items()}
         if len(self.tok_adapter) > 1:
             self.tok_adapter = model._merge_types(self.tok_adapter)
@@ -133,12 +139,10 @@ class BeamSession:
         # of the step before: scores (fp32), tokens, parents (-1: no beam), by request and beam, the best first
         self.state = torch.empty((3, R, W), dtype=torch.int32, device=dev)
         self.scores, self.chosen, self.parents = self.state[0].view(torch.float32), self.state[1], self.state[2]
-        self.ended = None if eos is None else torch.zeros((R, W), dtype=torch.int32, device=dev)
+        self.ended = None if self.eos is None else torch.zeros((R, W), dtype=torch.int32, device=dev)
         self.tokens = torch.empty(R * W, dtype=torch.int32, device=dev)
         self._take(*ops.beam_select(logits, torch.zeros((R, 1), dtype=torch.float32, device=dev), k=W))
         self.history = [self.state.clone()]
-        self.use_graph, self._eager_steps = use_graph, 0
-        self.graph = self._plan = self._cut = None
 
     def _take(self, scores, tokens, parents):
         if self.ended is not None:

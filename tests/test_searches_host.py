@@ -151,3 +151,35 @@ def test_a_search_gives_back_its_own_forks_alone(on_cpu):
     again.close()
     assert list(kv.slot) == ids
     sound(kv)
+
+
+def test_a_search_that_does_not_begin_leaves_nothing(on_cpu, monkeypatch):
+    """Refused logits, adapters that cannot be merged, no memory for what a search holds: the forks go back, and the next search begins."""
+    kv = cache(pages=60, seqs=12)
+    prompts(kv, {0: 32, 1: 48})
+    model, ops, rows = Model(), load_pkg("ops"), torch.zeros(2, dtype=torch.int32)
+
+    def refuse(*a, **k):
+        raise RuntimeError("refused")
+
+    def attempt(adapters):
+        with pytest.raises(RuntimeError):
+            on_cpu.BeamSession(model, kv, [0, 1], adapters, model.table[:2], 4)
+        assert list(kv.slot) == [0, 1]
+        sound(kv)
+
+    model._merge_types = refuse
+    attempt({0: rows, 1: rows})
+    for of, name in ((ops, "beam_select"), (torch, "zeros"), (torch, "empty")):
+        with monkeypatch.context() as m:
+            m.setattr(of, name, refuse)
+            if name != "zeros":                       # (flags of beams that have ended are made where there is an end)
+                attempt({0: rows})
+            else:
+                with pytest.raises(RuntimeError):
+                    on_cpu.BeamSession(model, kv, [0, 1], {0: rows}, model.table[:2], 4, eos=3)
+                assert list(kv.slot) == [0, 1]
+    s = on_cpu.BeamSession(model, kv, [0, 1], {0: rows}, model.table[:2], 4)
+    s.step()
+    s.close()
+    sound(kv)
