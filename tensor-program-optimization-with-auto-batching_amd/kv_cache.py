@@ -476,9 +476,14 @@ class PagedKVCache(PageTable):
                 self._gone[sid] = self._gone[of]
         self._dirty = self._dirty or bool(sids)
         if pairs:
-            self._enter()
-            at = ops.upload(torch.tensor(pairs, dtype=torch.int32).t().contiguous(), self.device)
-            ops.copy_pages([self.tail_k, self.tail_v] if self.bits == 8 else [self.k, self.v], at[0], at[1])
+            try:
+                self._enter()
+                at = ops.upload(torch.tensor(pairs, dtype=torch.int32).t().contiguous(), self.device)
+                ops.copy_pages([self.tail_k, self.tail_v] if self.bits == 8 else [self.k, self.v], at[0], at[1])
+            except Exception:
+                for sid in sids:
+                    self.free_sequence(sid)
+                raise
 
     def reorder(self, sids, parents, slots, ctx):
         """A step of a beam search: the beams `sids` of requests (an equal number each, one behind the other, of equal length) go on from the tokens of their parents [R, W]

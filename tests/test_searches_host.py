@@ -183,3 +183,16 @@ def test_a_search_that_does_not_begin_leaves_nothing(on_cpu, monkeypatch):
     s.step()
     s.close()
     sound(kv)
+
+
+@pytest.mark.parametrize("kw", [{}, {"bits": 8}, {"window": 20, "sinks": 2}])
+def test_a_fork_whose_copy_fails_leaves_nothing(kw):
+    """The copy of the last page's contents is refused where the cache is not on the current device (here on none)."""
+    kv = cache(pages=60, seqs=12, **kw)
+    prompts(kv, {"a": 53})
+    table = kv.table_h.copy()
+    with pytest.raises(ValueError):
+        kv.fork(["b", "c"], "a")
+    assert list(kv.slot) == ["a"] and kv.lens == {"a": 53} and (kv.table_h == table).all() and len(kv.free_slots) == 11
+    assert set(kv._gone) <= {"a"}
+    sound(kv)
