@@ -123,7 +123,7 @@ class BeamSession:
         except Exception:
             self.close()
             raise
-        self.use_graph, self._eager_steps = use_graph, 0
+        self.use_graph, self._eager_steps, self._failed = use_graph, 0, False
         self.graph = self._plan = self._cut = None
 
     def _begin(self, tok_adapter, logits):
@@ -160,14 +160,9 @@ class BeamSession:
         self.pos.add_(1)
         self.ctx.add_(1)
 
-    def step(self):
-        """One step of every beam; returns (scores, tokens, parents) [R, W] on the device, which the next step overwrites."""
-        kv = self.kv
-        if any(kv.lacks_page(s) for s in self.seq_ids[::self.W]):
-            kv.reserve(self.seq_ids, PAGE if self.left is None else max(1, min(PAGE, self.left)))
-        kv.begin_forward(self.seq_ids, [1] * len(self.seq_ids), device_meta=(self.slots, self.pos, self.ctx))
+    def _queue_step(self):
         if self.use_graph and self._eager_steps >= 1:
-            plan, cut = step_form(kv)
+            plan, cut = step_form(self.kv)
             if self.graph is None or plan is not self._plan or cut != self._cut:
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g):
@@ -177,8 +172,24 @@ class BeamSession:
         else:
             self._enqueue()
             self._eager_steps += 1
-        kv.end_forward()
+
+    def step(self):
+        """One step of every beam; returns (scores, tokens, parents) [R, W] on the device, which the next step overwrites.  One that finds no pages can be
+        taken again; one that fails behind that ends the search, which is to be closed, and what its sequences hold is of no use."""
+        if self._failed:
+            raise RuntimeError("BeamSession: a step has failed")
+        kv = self.kv
+        if any(kv.lacks_page(s) for s in self.seq_ids[::self.W]):
+            kv.reserve(self.seq_ids, PAGE if self.left is None else max(1, min(PAGE, self.left)))
+        kv.begin_forward(self.seq_ids, [1] * len(self.seq_ids), device_meta=(self.slots, self.pos, self.ctx))
         kv.adrift(self.seq_ids, self.slots)
+        try:
+            self._queue_step()
+        except Exception:
+            self._failed = True
+            kv.abandon_forward()
+            raise
+        kv.end_forward()
         self.history.append(self.state.clone())
         if self.left is not None:
             self.left -= 1

@@ -351,6 +351,11 @@ class PageTable:
         seq_ids, append_lens = self._cur[0], self._cur[1]
         for sid, n in zip(seq_ids, append_lens):
             self.lens[sid] += n
+        self.abandon_forward()
+
+    def abandon_forward(self):
+        """Ends a pass that failed: its sequences are as long as before.  (What it may have stored behind their ends is written anew; the tokens of an 8-bit
+        cache's last page outlast a step, not a pass that went on to another page.)"""
         self._cur = None
         for raw, (stream, _) in self._users.items():         # (the default stream outlives every pass: no event before one is waited for)
             if raw and not torch.cuda.is_current_stream_capturing():
@@ -498,7 +503,7 @@ class PagedKVCache(PageTable):
         slots.copy_(new)
 
     def adrift(self, sids, slots):
-        """`reorder` of these beams has run, or is queued: their rows are to be read back (`settle`) before they are used here."""
+        """`reorder` of these beams has run, or is queued (or will be, behind the pass that has begun): their rows are to be read back (`settle`) before they are used here."""
         sids = tuple(sids)
         self._adrift[sids] = slots
         if self.plain:

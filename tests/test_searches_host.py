@@ -196,3 +196,61 @@ def test_a_fork_whose_copy_fails_leaves_nothing(kw):
     assert list(kv.slot) == ["a"] and kv.lens == {"a": 53} and (kv.table_h == table).all() and len(kv.free_slots) == 11
     assert set(kv._gone) <= {"a"}
     sound(kv)
+
+
+@pytest.mark.parametrize("where", ["forward", "beam_select", "beam_reorder", "copy_pages"])
+@pytest.mark.parametrize("kw", [{}, {"window": 20, "sinks": 2}])
+def test_a_step_that_fails_ends_the_search(on_cpu, monkeypatch, where, kw):
+    """Wherever it fails, the host knows the rows that the device has, and forks and pages go back."""
+    kv = cache(pages=60, seqs=12, **kw)
+    prompts(kv, {0: 32, 1: 48, "x": 5})
+    model, ops = Model(), load_pkg("ops")
+    s = on_cpu.BeamSession(model, kv, [0, 1], {}, model.table[:2], 4)
+    for _ in range(5):
+        s.step()
+
+    def refuse(*a, **k):
+        raise RuntimeError("refused")
+
+    with monkeypatch.context() as m:
+        if where == "forward":
+            model.fails = True
+        else:
+            m.setattr(ops, where, refuse)
+        with pytest.raises(RuntimeError):
+            s.step()
+    model.fails = False
+    assert kv.lens[0] == 37 and kv.lens[1] == 53
+    with pytest.raises(RuntimeError):                 # (its state may be of half a step)
+        s.step()
+    table = kv.block_table.clone()
+    grow(kv, "x", 1)                                  # another's pass, which reads the rows back
+    kv.settle()
+    rows = [kv.slot[i] for i in s.seq_ids]
+    assert torch.equal(torch.from_numpy(kv.table_h[rows]), table[rows])
+    sound(kv)
+    s.close()
+    assert list(kv.slot) == [0, 1, "x"]
+    sound(kv)
+
+
+def test_a_step_without_room_can_be_taken_again(on_cpu):
+    """No page for the next token: nothing has been queued, and the search goes on when there is one."""
+    kv = cache(pages=10, seqs=6)
+    prompts(kv, {0: 32, "x": 64})
+    model = Model()
+    want = cache(pages=30, seqs=6)
+    prompts(want, {0: 32})
+    both = [on_cpu.BeamSession(model, c, [0], {}, model.table[:1], 4) for c in (kv, want)]
+    for _ in range(16):
+        for s in both:
+            s.step()
+    with pytest.raises(RuntimeError):                 # (four pages are wanted; the four of the first 16 tokens are not all given up)
+        both[0].step()
+    kv.free_sequence("x")
+    for _ in range(9):
+        for s in both:
+            s.step()
+    assert both[0].answers() == both[1].answers()
+    both[0].close()
+    sound(kv)
