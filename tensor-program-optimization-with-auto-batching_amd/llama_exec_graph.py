@@ -385,15 +385,17 @@ class LlamaExecGraph(ExecGraph):
             pairs = self._method_pairs(method, params)
             sess = BeamSession(self.vm, self.kv_cache, group, self.vm._ids(len(group), pairs), torch.stack([self._first.pop(sid) for sid in group]),
                                self.exec_config.beams, eos=self.eos_token_id, steps=steps, use_graph=steps >= 8)
-            for _ in range(steps):
-                ev = self._tic()
-                sess.step()
-                self._toc(ev)
-                if self.eos_token_id is not None and sess.done():
-                    break
-            for sid, beams in zip(group, sess.answers()):
-                outputs[sid] = beams[0][1]
-            sess.close()
+            try:
+                for _ in range(steps):
+                    ev = self._tic()
+                    sess.step()
+                    self._toc(ev)
+                    if self.eos_token_id is not None and sess.done():
+                        break
+                for sid, beams in zip(group, sess.answers()):
+                    outputs[sid] = beams[0][1]
+            finally:
+                sess.close()
         return outputs
 
     def _method_pairs(self, method, params):

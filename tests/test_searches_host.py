@@ -254,3 +254,59 @@ def test_a_step_without_room_can_be_taken_again(on_cpu):
     assert both[0].answers() == both[1].answers()
     both[0].close()
     sound(kv)
+
+
+class Served(dict):
+    """The front end's model: entry points by name."""
+
+    cache_forms, native_step, lora_types, device, vocab_size = True, False, (), "cpu", 50
+
+    def __init__(self, kv, bad=()):
+        super().__init__(create_paged_kv_cache=lambda *a, **k: kv, embed=lambda t: Model.embed(self, t.reshape(-1)), prefill_no_adapter=self.prefill)
+        self.table, self.fails, self.bad, self.kv = Model().table, False, set(bad), kv
+
+    def prefill(self, hidden, kv):
+        logits = hidden[-1:].clone()
+        if kv._cur[0][0] in self.bad:
+            logits[:] = torch.nan
+        return logits, None
+
+    embed, forward = Model.embed, Model.forward
+
+    def _ids(self, n, pairs):
+        return {}
+
+
+def front_end(kv, lens, bad=(), rules=None, **config):
+    """(batcher, answers) of requests of these lengths, whose limits are 20 tokens."""
+    ab, xg = load_pkg("auto_batcher"), load_pkg("llama_exec_graph")
+    b = ab.LlamaAutoBatcherClass()
+    b.set_model(Served(kv, bad))
+    b.set_exec_config(xg.LlamaExecConfig(max_prompt_len=64, max_gen_len=24, page_size=16, native_decode=False, **config))
+    out = []
+    for i, n in enumerate(lens):
+        if rules is not None and rules[i] is not None:
+            b.set_rules(rules[i])
+        out.append(b.generate(b.create_var(np.arange(n, dtype=np.int32) % 50), max_gen_len=20))
+    b.compile()
+    return b, out
+
+
+@pytest.fixture
+def served(on_cpu, monkeypatch):
+    class Eager(on_cpu.BeamSession):
+        def __init__(self, *a, use_graph, **kw):
+            super().__init__(*a, **kw)
+
+    monkeypatch.setattr(on_cpu, "BeamSession", Eager)
+    monkeypatch.setattr(load_pkg("ops"), "argmax", lambda z: z.argmax(-1).int())
+
+
+def test_a_front_end_search_that_fails_leaves_its_requests_alone(served):
+    """Out of pages in the middle: the searches' rows and pages go back."""
+    kv = cache(pages=12, seqs=8)
+    b, _ = front_end(kv, (32, 48), beams=3)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        b.execute()
+    assert sorted(kv.slot) == [0, 1]
+    sound(kv)
