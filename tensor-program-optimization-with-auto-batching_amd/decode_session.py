@@ -200,7 +200,8 @@ class BeamSession:
         return self.ended is not None and bool(self.ended[:, 0].all())
 
     def answers(self):
-        """Per request its beams so far as (score, tokens), the best first, up to `eos`.  Waits for the device."""
+        """Per request its beams so far as (score, tokens), the best first, up to `eos`; none of a request whose beams have
+        all gone, for want of logits that are numbers.  Waits for the device."""
         h = torch.stack(self.history).cpu().numpy()
         scores, out = h[-1, 0].view(np.float32), []
         at, alive = np.broadcast_to(np.arange(self.W), (self.R, self.W)), h[-1, 1] >= 0

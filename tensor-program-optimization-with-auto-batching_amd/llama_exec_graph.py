@@ -393,7 +393,7 @@ class LlamaExecGraph(ExecGraph):
                     if self.eos_token_id is not None and sess.done():
                         break
                 for sid, beams in zip(group, sess.answers()):
-                    outputs[sid] = beams[0][1]
+                    outputs[sid] = beams[0][1] if beams else []           # (no beam is left where every logit was NaN: an empty answer)
             finally:
                 sess.close()
         return outputs

@@ -310,3 +310,20 @@ def test_a_front_end_search_that_fails_leaves_its_requests_alone(served):
         b.execute()
     assert sorted(kv.slot) == [0, 1]
     sound(kv)
+
+
+@pytest.mark.parametrize("eos", [None, 7])
+def test_a_request_without_beams_has_no_answer(served, eos):
+    """Logits that are NaN leave a request no beam: its answer is empty, and the others' are what they are without it."""
+    answers = []
+    for lens, bad in (((32, 48, 16), (1,)), ((32, 16), ())):
+        kv = cache(pages=90, seqs=12)
+        b, out = front_end(kv, lens, bad, beams=3)
+        b.graph.eos_token_id = eos
+        b.execute()
+        assert sorted(kv.slot) == list(range(len(lens)))
+        sound(kv)
+        answers.append([o.var.tolist() for o in out])
+        assert all(o.var.dtype == np.int64 for o in out)
+    assert answers[0] == [answers[1][0], [], answers[1][1]]
+    assert all(len(a) == 20 or a[-1] == eos for a in answers[1])
