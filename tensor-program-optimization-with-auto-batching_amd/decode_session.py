@@ -196,8 +196,9 @@ class BeamSession:
         return self.scores, self.chosen, self.parents
 
     def done(self) -> bool:
-        """Whether every request's best beam has ended: scores only fall, so none overtakes it.  Waits for the device."""
-        return self.ended is not None and bool(self.ended[:, 0].all())
+        """Whether every request's best beam has ended - scores only fall, so none overtakes it - or it has no beam left.  Waits for the device."""
+        over = self.chosen[:, 0] < 0
+        return bool((over if self.ended is None else over | (self.ended[:, 0] != 0)).all())
 
     def answers(self):
         """Per request its beams so far as (score, tokens), the best first, up to `eos`; none of a request whose beams have

@@ -327,3 +327,23 @@ def test_a_request_without_beams_has_no_answer(served, eos):
         assert all(o.var.dtype == np.int64 for o in out)
     assert answers[0] == [answers[1][0], [], answers[1][1]]
     assert all(len(a) == 20 or a[-1] == eos for a in answers[1])
+
+
+def test_a_search_is_done_where_no_beam_is_left(on_cpu):
+    """A request without beams has none that could go on, whether or not there is an end token."""
+    model, eos = Model(), 5
+    model.table[:, eos] = 30.0                        # every beam ends soon
+    logits = model.table[:2].clone()
+    logits[1] = torch.nan
+    kv = cache(pages=60, seqs=12)
+    prompts(kv, {0: 32, 1: 48})
+    s = on_cpu.BeamSession(model, kv, [0, 1], {}, logits, 3, eos=eos)
+    for _ in range(3):
+        s.step()
+    assert s.done() and [len(b) for b in s.answers()] == [3, 0]
+    s.close()
+    for z, want in ((logits, False), (logits[1:].repeat(2, 1), True)):
+        s = on_cpu.BeamSession(model, kv, [0, 1], {}, z, 3)
+        s.step()
+        assert s.done() is want
+        s.close()
