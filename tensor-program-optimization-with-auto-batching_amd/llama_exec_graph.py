@@ -126,6 +126,14 @@ class LlamaExecGraph(ExecGraph):
             self.measure_file.flush()                   # the file stays open across passes: keep it readable meanwhile
 
     # ------------------------------------------------------------------ operations
+    def execute(self):
+        self._check_searches([sid for op in self.op_nodes for sid in op.seqids])
+        super().execute()
+
+    def _check_searches(self, sids):
+        if getattr(self.exec_config, "beams", 1) > 1 and any(self.seq_info.get_rules(sid) is not None for sid in sids):
+            raise ValueError("beam search under token rules is not served")
+
     def execute_encode_prompt(self, op):
         assert len(op.input_vars) == 1 and len(op.output_vars) == 1 and len(op.seqids) == 1, \
             "encode_prompt node must have exactly 1 input var, 1 output var and 1 seqid"
@@ -238,6 +246,7 @@ class LlamaExecGraph(ExecGraph):
     def execute_decode(self, op):
         assert len(op.input_vars) == len(op.output_vars), "decode node needs as many output vars as input vars"
         assert len(op.input_vars) == len(op.seqids), "decode node needs one sequence id per input var"
+        self._check_searches(op.seqids)
         seqs, original_positions = self.seq_info.order_seqs(op.seqids)
         outputs = {sid: [int(op.input_vars[original_positions[i]].var)] for i, sid in enumerate(seqs)}
         ordered = list(seqs)
@@ -246,7 +255,8 @@ class LlamaExecGraph(ExecGraph):
             seqs = [sid for sid in seqs if outputs[sid][0] >= 0]
             self.check_seqs_finished([sid for sid in ordered if outputs[sid][0] < 0], outputs)
         if getattr(self.exec_config, "beams", 1) > 1:
-            outputs, seqs = self._decode_beams(seqs), []
+            outputs.update(self._decode_beams(seqs))
+            seqs = []
         # As in the reference (`:102-141`), the finish rule (`:94-100`) is applied only after a decode step: every
         # sequence takes at least one step after its prefill, also when its first token is EOS or max_gen_len is 1.
         while seqs:
@@ -374,8 +384,6 @@ class LlamaExecGraph(ExecGraph):
     def _decode_beams(self, seqs):
         """The answers of a batch by beam search (`LlamaExecConfig.beams`); requests of one length limit search together."""
         from .decode_session import BeamSession
-        if any(self.seq_info.get_rules(sid) is not None for sid in seqs):
-            raise ValueError("beam search under token rules is not served")
         outputs, limits = {}, {}
         for sid in seqs:
             limits.setdefault(self.seq_info.get_max_gen_len(sid), []).append(sid)

@@ -347,3 +347,37 @@ def test_a_search_is_done_where_no_beam_is_left(on_cpu):
         s.step()
         assert s.done() is want
         s.close()
+
+
+class Ruled:
+    """Rules of which the batch below leaves nothing."""
+
+
+@pytest.mark.parametrize("batch_prefill", [False, True])
+@pytest.mark.parametrize("ruled", [0, 1])
+def test_a_search_under_rules_is_refused_ahead_of_its_prompts(served, monkeypatch, ruled, batch_prefill):
+    """Also where the rules leave a request no token at all."""
+    xg = load_pkg("llama_exec_graph")
+
+    class Nothing:
+        def __init__(self, rules, *a):
+            self.n = len(rules)
+
+        def choose(self, logits):
+            return torch.full((self.n,), -1, dtype=torch.int32)
+
+    monkeypatch.setattr(xg, "BatchRules", Nothing)
+    kv = cache(pages=90, seqs=12)
+    rules = [None, None]
+    rules[ruled] = Ruled()
+    b, _ = front_end(kv, (32, 48), rules=rules, beams=3, batch_prefill=batch_prefill)
+    with pytest.raises(ValueError, match="rules"):
+        b.execute()
+    assert not kv.slot
+    graph = b.graph
+    graph.kv_cache.add_sequence(0), graph.kv_cache.add_sequence(1)
+    decode = graph.op_nodes[[op.op_type for op in graph.op_nodes].index("decode")]
+    for var, first in zip(decode.input_vars, (5, 5)):
+        var.var = -1 if decode.seqids[decode.input_vars.index(var)] == ruled else first
+    with pytest.raises(ValueError, match="rules"):                  # the decode alone
+        graph.execute_decode(decode)
