@@ -86,7 +86,7 @@ class LlamaExecGraph(ExecGraph):
         self._first = {}              # sequence -> the logits behind its prompt, of those whose beams have not begun
         c = self.exec_config
         beams, form = getattr(c, "beams", 1), {}
-        if getattr(c, "cache_bits", 16) != 16 or getattr(c, "window", None) is not None:
+        if getattr(c, "cache_bits", 16) != 16 or getattr(c, "window", None) is not None or getattr(c, "sinks", 0):
             form = {"bits": c.cache_bits, "window": c.window, "sinks": c.sinks}
         if (form or beams != 1) and not getattr(self.vm, "cache_forms", False):
             raise ValueError(f"{type(self.vm).__name__}: no caches in 8 bits or under windows, and no search by beams")

@@ -381,3 +381,21 @@ def test_a_search_under_rules_is_refused_ahead_of_its_prompts(served, monkeypatc
         var.var = -1 if decode.seqids[decode.input_vars.index(var)] == ruled else first
     with pytest.raises(ValueError, match="rules"):                  # the decode alone
         graph.execute_decode(decode)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_sinks_without_a_window_are_refused(bits):
+    """As PagedKVCache refuses them, on caches of 16 bits too."""
+    with pytest.raises(ValueError, match="sinks"):
+        front_end_cache(cache_bits=bits, sinks=4)
+    assert front_end_cache(cache_bits=bits).sinks == 0
+    assert front_end_cache(cache_bits=bits, window=32, sinks=4).sinks == 4
+
+
+def front_end_cache(**config):
+    xg, si = load_pkg("llama_exec_graph"), load_pkg("seq_info")
+    vm = Served(None)
+    vm["create_paged_kv_cache"] = lambda n, total, chunk, page, free_pages, max_seq_len, **form: cache(**form)
+    g = xg.LlamaExecGraph()
+    g.set_exec_vars(vm, "cpu", None, None, si.LlamaSeqInfo(8), xg.LlamaExecConfig(max_prompt_len=64, max_gen_len=24, page_size=16, **config))
+    return g.kv_cache
