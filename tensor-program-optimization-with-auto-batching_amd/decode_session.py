@@ -55,7 +55,7 @@ class DecodeSession:
         if len(self.tok_adapter) > 1:         # several adapter types: merged once here (the check reads back to the host)
             self.tok_adapter = model._merge_types(self.tok_adapter)
         self.tokens = i32(first_tokens).clone()
-        self.rows = i32([kv.slot[s] for s in self.seq_ids])
+        self.rows = i32(kv.rows_of(self.seq_ids))
         self.pos = i32([kv.lens[s] for s in self.seq_ids])
         self.ctx = self.pos + 1
         self.use_graph = use_graph
@@ -133,7 +133,7 @@ class BeamSession:
         self.tok_adapter = {tid: i32(ids).repeat_interleave(W) for tid, ids in tok_adapter.items()}
         if len(self.tok_adapter) > 1:
             self.tok_adapter = model._merge_types(self.tok_adapter)
-        self.slots = i32([kv.slot[s] for s in self.seq_ids])
+        self.slots = i32(kv.rows_of(self.seq_ids))
         self.pos = i32([kv.lens[s] for s in self.seq_ids])
         self.ctx = self.pos + 1
         # of the step before: scores (fp32), tokens, parents (-1: no beam), by request and beam, the best first
@@ -261,7 +261,7 @@ class NativeDecodeSession:
             lt = model.lora_union(tid)[0] if isinstance(tid, tuple) else model.lora_types[tid]
         i32 = lambda a: torch.as_tensor(np.asarray(a, dtype=np.int32)).to(dev)
         self.tokens = i32(first_tokens)
-        self.rows = i32([kv.slot[q] for q in self.seq_ids])
+        self.rows = i32(kv.rows_of(self.seq_ids))
         self.pos = i32([kv.lens[q] for q in self.seq_ids])
         self.ctx = self.pos + 1
         self.tok_adapter = None

@@ -362,6 +362,11 @@ class PageTable:
                 self._users[raw] = (stream, stream.record_event())
 
     # ------------------------------------------------------------------ helpers
+    def rows_of(self, seq_ids):
+        """The rows of the block table that sequences have."""
+        self.settle()
+        return [self.slot[s] for s in seq_ids]
+
     def pages_of(self, sid):
         self.settle()
         row = self.table_h[self.slot[sid]]

@@ -399,3 +399,23 @@ def front_end_cache(**config):
     g = xg.LlamaExecGraph()
     g.set_exec_vars(vm, "cpu", None, None, si.LlamaSeqInfo(8), xg.LlamaExecConfig(max_prompt_len=64, max_gen_len=24, page_size=16, **config))
     return g.kv_cache
+
+
+def test_sessions_take_the_rows_that_beams_have_now(on_cpu):
+    """A sequence of a search that is still open lies in whatever row its beam has come to."""
+    model, moved = Model(seed=3), 0
+    for seed in range(6):
+        kv = cache(pages=60, seqs=12)
+        prompts(kv, {0: 32, 1: 48})
+        s = on_cpu.BeamSession(model, kv, [0, 1], {}, model.table[seed:seed + 2], 4)
+        for _ in range(7):
+            s.step()
+        assert kv._adrift
+        moved += s.slots.tolist() != [kv.slot[i] for i in s.seq_ids]
+        rows = {i: n for i, n in zip(s.seq_ids, s.slots.tolist())}
+        if seed % 2:
+            assert on_cpu.DecodeSession(model, kv, [1, 0], {}, [3, 4]).rows.tolist() == [rows[1], rows[0]]
+        else:
+            assert on_cpu.BeamSession(model, kv, [1, 0], {}, model.table[:2], 1).slots.tolist() == [rows[1], rows[0]]
+        assert kv.rows_of(s.seq_ids) == s.slots.tolist() and not kv._adrift
+    assert moved > 2
