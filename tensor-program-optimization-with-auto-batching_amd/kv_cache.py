@@ -176,6 +176,8 @@ class PageTable:
         goes with the deepest one that it passes: saved are the depths of the sequences' groups, less every group's own.  So from the leaves up,
         for each ancestor that may be the deepest group above a node: the most that its sequences save, with a group of their own at the node
         or without."""
+        if any(s in sids for sids in self._adrift for s in seq_ids):
+            self.settle()
         rows = [self.slot[s] for s in seq_ids]
         full = [self.lens[s] // PAGE for s in seq_ids]
         owned = [i for i, r in enumerate(rows) if full[i] and int(self.table_h[r, 0]) in self._owners]

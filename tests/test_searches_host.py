@@ -419,3 +419,23 @@ def test_sessions_take_the_rows_that_beams_have_now(on_cpu):
             assert on_cpu.BeamSession(model, kv, [1, 0], {}, model.table[:2], 1).slots.tolist() == [rows[1], rows[0]]
         assert kv.rows_of(s.seq_ids) == s.slots.tolist() and not kv._adrift
     assert moved > 2
+
+
+def test_groups_of_shared_pages_are_of_the_rows_that_beams_have_now(on_cpu):
+    model = Model(seed=3)
+    kv = cache(pages=90, seqs=12)
+    prompts(kv, {0: 32})
+    s = on_cpu.BeamSession(model, kv, [0], {}, model.table[:1], 4, steps=60)
+    for _ in range(14):
+        s.step()
+    kv.settle()
+    kv.reserve(s.seq_ids, 48)                         # (so that no step reads the rows back)
+    for _ in range(40):
+        s.step()
+    assert kv._adrift
+    groups = kv.prefix_groups(s.seq_ids)
+    table = kv.block_table[s.slots.long(), :kv.lens[0] // PAGE]
+    for members, pages in groups:
+        assert pages == 0 or (table[members, :pages] == table[members[0], :pages]).all()
+    kv.settle()
+    assert groups == kv.prefix_groups(s.seq_ids) and max(p for _, p in groups) > 2
