@@ -111,6 +111,8 @@ class BeamSession:
         R, W = len(seq_ids), int(beams)
         if not 1 <= W <= 16 or logits.shape[0] != R:
             raise ValueError(f"BeamSession: {W} beams (1 to 16) of {R} sequences, logits of {logits.shape[0]}")
+        if len(set(seq_ids)) < R:
+            raise ValueError("BeamSession: a sequence twice")
         self.model, self.kv, self.R, self.W, self.eos, self.left = model, kv, R, W, eos, steps
         self.seq_ids, self._forks = [], []
         try:

@@ -439,3 +439,16 @@ def test_groups_of_shared_pages_are_of_the_rows_that_beams_have_now(on_cpu):
         assert pages == 0 or (table[members, :pages] == table[members[0], :pages]).all()
     kv.settle()
     assert groups == kv.prefix_groups(s.seq_ids) and max(p for _, p in groups) > 2
+
+
+@pytest.mark.parametrize("W", [1, 3])
+def test_a_sequence_is_searched_once(on_cpu, W):
+    """The same sequence twice would be two rows that store into one page."""
+    model = Model()
+    kv = cache(pages=60, seqs=12)
+    prompts(kv, {0: 32, 1: 48})
+    for ids in ([0, 0], [1, 0, 1]):
+        with pytest.raises(ValueError, match="twice"):
+            on_cpu.BeamSession(model, kv, ids, {}, model.table[:len(ids)], W)
+        assert list(kv.slot) == [0, 1]
+    sound(kv)
