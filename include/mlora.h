@@ -472,8 +472,9 @@ int mlora_copy_pages(const mlora_page_pool* host_pools, int n_pools, const int32
 
 /* A step of a beam search over R requests of W <= 16 beams.
  * mlora_beam_select: the k <= 32 best continuations of every request: candidates (b, v) with value scores[b] + z[b, v] - log sum exp z[b], z = logits [R * W, ld] fp32; a beam
- * with ended[b] != 0 (ended may be NULL) has the one candidate eos, of value scores[b].  Values are formed and compared in 64 bits, of sums of exponentials that
- * are taken in 32 (between beams, values closer than those are exact may change places); the lowest b V + v of equal ones comes first, -inf and NaN are none.  out_scores, tokens, parents (beam within the request) [R, k]; where candidates run out -inf, -1, -1.
+ * with ended[b] != 0 (ended may be NULL) has the one candidate eos, of value scores[b].  A beam's candidates are in the order of their logits, the lower token of equal ones
+ * first; between beams values are formed and compared in 64 bits, of sums of exponentials that are taken in 32 (values closer than those are exact may change places), the lower
+ * beam of equal ones first; -inf and NaN are none.  out_scores, tokens, parents (beam within the request) [R, k]; where candidates run out -inf, -1, -1.
  * mlora_beam_reorder: beam i goes on as a child of parents[i].  slots [R, W]: rows of block_table that the beams have, pos [R * W]: of the tokens they appended last (or of the next
  * ones: a page that is complete is then taken over, not copied).  A parent's first child keeps the parent's slot; the others (and a beam with a parent outside 0..W-1, which copies nothing) take, in order, the slots of beams without children: new_slots.
  * For those, row dst_slot of the table takes over row src_slot's pages ahead of the one of the last token, and dst_page is to become a copy of src_page (and whatever else a

@@ -2,8 +2,8 @@
 //
 //   value(b, v) = score[b] + z[b, v] - log sum_u exp z[b, u]        candidates of a request: its beams x the vocabulary
 //
-// The k greatest, the lowest b V + v of equal ones.  Within a beam the order is that of the logits, exactly; between beams values are compared in 64 bits, of sums of exponentials
-// that were taken in 32 (values closer than those are exact may change places).
+// The k greatest.  Within a beam the order is that of the logits, exactly, the lower token of equal ones first; between beams values are compared in 64 bits, the lower beam of
+// equal ones first, of sums of exponentials that were taken in 32 (values closer than those are exact may change places).
 #include "common.h"
 
 namespace {
@@ -133,14 +133,13 @@ __global__ __launch_bounds__(4 * WAVE) void beam_scan_kernel(Best* __restrict__ 
   if (lane == 0) sums[at] = f32x2{M, s};
 }
 
-// A request, of which a wave each merges a beam's parts.  A candidate's place is then the number of those ahead of it: in its own beam, which is looked through,
-// and in the others, whose values fall, by halving.  9 us for 64 requests of 8 beams, 6 for one of 4 (17 and 9 with four waves a request that take out the
+// A request, of which a wave each merges a beam's parts.  A candidate's place is then the number of those ahead of it: in its own beam the lanes before, for they
+// are in order, and in the others, whose values fall, by halving.  9 us for 64 requests of 8 beams, 6 for one of 4 (17 and 9 with four waves a request that take out the
 // greatest k times): bound by steps that wait for one another, most of them the merge's.
 __global__ __launch_bounds__(MAX_BEAMS* WAVE) void beam_join_kernel(float* __restrict__ out_scores, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
                                                                     const Best* __restrict__ best, const f32x2* __restrict__ sums, const float* __restrict__ scores,
                                                                     const int32_t* __restrict__ ended, int eos, int W, int k, int parts) {
   __shared__ double value[MAX_BEAMS * MAX_BEST];
-  __shared__ int column[MAX_BEAMS * MAX_BEST];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = blockIdx.x, row = r * W + w;
   const int n = parts * k;
   const float score = scores[row];
@@ -177,28 +176,19 @@ __global__ __launch_bounds__(MAX_BEAMS* WAVE) void beam_join_kernel(float* __res
     if (b.z > -INFINITY) val = (double)score + ((double)b.z - lse);
     if (!(val > -INFINITY)) val = -INFINITY;                                    // NaN is no candidate
   }
-  if (lane < k) {
-    value[w * k + lane] = val;
-    column[w * k + lane] = b.v;
-  }
+  if (lane < k) value[w * k + lane] = val;
   __syncthreads();
-  int place = 0;
+  int place = lane;                                                             // (values may be equal in 64 bits where logits are not)
   for (int o = 0; o < W; ++o) {
-    if (o == w) {
-      for (int i = 0; i < k; ++i) {
-        const double x = value[w * k + i];
-        place += x > val || (x == val && column[w * k + i] < b.v);
-      }
-    } else {                                                                    // equal ones of an earlier beam are ahead
-      int n = 0;
+    if (o == w) continue;
+    int n = 0;                                                                  // equal ones of an earlier beam are ahead
 #pragma unroll
-      for (int step = MAX_BEST; step > 0; step >>= 1)
-        if (n + step <= k) {
-          const double x = value[o * k + n + step - 1];
-          if (x > val || (x == val && o < w)) n += step;
-        }
-      place += n;
-    }
+    for (int step = MAX_BEST; step > 0; step >>= 1)
+      if (n + step <= k) {
+        const double x = value[o * k + n + step - 1];
+        if (x > val || (x == val && o < w)) n += step;
+      }
+    place += n;
   }
   const bool in = lane < k && val > -INFINITY;
   if (in && place < k) {

@@ -1325,8 +1325,8 @@ def copy_pages(pools, src, dst):
 def beam_select(logits, scores, ended=None, eos=None, k=None):
     """The k (None: as many as beams) best continuations of R requests of W beams each: of beam b by token v with value scores[b] + logits[b, v] - logsumexp(logits[b]).
     logits [R * W, V] fp32 (any row stride), scores [R, W] fp32 (-inf: no beam there).  ended [R, W] int32: such a beam goes on with `eos` alone, at its score.
-    -> scores [R, k] fp32, tokens [R, k], parents [R, k] int32 (the beam within its request), the best first, of equal values the lower beam and token;
-    -inf, -1, -1 where candidates run out."""
+    -> scores [R, k] fp32, tokens [R, k], parents [R, k] int32 (the beam within its request), the best first - a beam's in the order of their logits,
+    the lower token of equal ones first, and the lower beam of equal values -; -inf, -1, -1 where candidates run out."""
     (N, V), (R, W) = logits.shape, scores.shape
     dev = _here(logits.device, "beam_select")
     k = W if k is None else k
