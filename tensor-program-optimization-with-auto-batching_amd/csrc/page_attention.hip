@@ -466,7 +466,7 @@ __global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Prompts.  A workgroup has 16 NT NW rows, each a token of the pass under one of a kv head's query heads, tokens consecutive, a wave NT tiles of 16 of them; the
+// Prompts.  A workgroup has 16 NW rows, each a token of the pass under one of a kv head's query heads, tokens consecutive, a wave 16 of them; the
 // tokens' runs (consecutive positions of one sequence) are worked one behind the other, each over the pages that it sees, four at a time.  The waves bring
 // their pieces of the next four from the cache into LDS as fp16 operands while the workgroup multiplies four.  Tokens' own pages of 8-bit caches come first, unrounded.
 //
@@ -474,6 +474,7 @@ __global__ __launch_bounds__(4 * WAVE) void page_join_kernel(PageAttn a) {
 // instructions 50, of them products 36, LDS reads 25; taken out one by one, loads, LDS reads, the softmax and the weights' second halves were 15 to 24 % each).  Those 4096 tokens,
 // 32 heads over 8, take 128 us, 470 TFLOP/s; 8 prompts of 456 on 8-bit pages, 32 heads, 97, with 27 + 6 for rounding and storing; 777 tokens behind 3500, 32 heads over 8, 126
 // (350 TFLOP/s) with 20 for storing and joining.  No faster: keys ahead by four or six fragments, values by four; slower: two tiles a wave (below).
+// The form for 8 bits and heads of 128 keeps 17 of its values in scratch memory, which are read back for an own page, ahead of a run's blocks and behind them, not among them.
 //
 // Of a page's step 2^e f (1 <= f < 2), the power of two goes into the values' operand, relative to the largest so far, where it is exact, and f into the
 // weights, so that two pages with steps of their own fill one matrix instruction.
@@ -590,10 +591,11 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&st)[P], const float (
 
 __device__ __forceinline__ f16x8 join(f16x2 a, f16x2 b, f16x2 c, f16x2 d) { return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
 
-template <int D, bool Q8, int NT, int NW>
-__global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel(PageAttn a) {
-  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, QB = 16 * NT * NW, KLD = QB + 1, VLD = D + 8;
-  constexpr int NL = Q8 ? D / 64 : D / 32, NU = (8 * NL + NW - 1) / NW;        // KiB of a page's keys or values; pieces of 1 KiB that a wave brings of four pages
+template <int D, bool Q8, int NW>
+__global__ __launch_bounds__(NW* WAVE, 4) void page_prefill_kernel(PageAttn a) {
+  constexpr int NKB = D / 32, NDB = D / 16, PE = PAGE * D, QB = 16 * NW, KLD = QB + 1, VLD = D + 8;
+  constexpr int NL = Q8 ? D / 64 : D / 32, NU = 8 * NL / NW;          // KiB of a page's keys or values; pieces of 1 KiB that a wave brings of four pages
+  static_assert(NU * NW == 8 * NL, "a wave's pieces are as many as another's");
   // two buffers of four pages: keys [page][kb][lane][8]; values of 8-bit pages [pair of pages][db][lane][page of the pair][4 tokens], of fp16 pages
   // [pair][32 dims][page][half of the tokens][dim][8].  Before that, of pages of 8 bits, the tokens' own keys [kb][g][token][8] and values [token][d]
   // (fp16: keys of odd pages 64 bytes on, for a read that goes over a pair of pages meets a bank once: of the 37 % of the time that LDS reads, a third less)
@@ -618,7 +620,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
   constexpr int KI = Q8 ? QB * (D / 16) / (NW * WAVE) : 1, VI = Q8 ? 2 * KI : 1;
   f16x8 kx[KI], ky[KI], vx[VI];
   int kpos[KI];
-  if (Q8 && split == 0) {
+  if (Q8 && __builtin_expect(split == 0, 1)) {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       const int e = threadIdx.x + i * NW * WAVE, rr = e / (D / 16), c = e % (D / 16), tt = t0 + min(rr, nt - 1);
@@ -634,34 +636,31 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
       vx[i] = ld8(a.qkv + ((size_t)(t0 + min(rr, nt - 1)) * HH + a.Hq + a.Hkv + kh) * D + c * 8);
     }
   }
-  f16x8 q[NT][NKB];
-  f32x4 o[NT][NDB];
-  float m[NT], l[NT];
-  int ctok[NT], cpos[NT];                                             // the column's token, nt: none, and its position, -1: none
+  f16x8 q[NKB];
+  f32x4 o[NDB];
+  float m = NOTHING, l = 0.f;
+  int ctok, cpos;                                                     // the column's token, nt: none, and its position, -1: none
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    m[i] = NOTHING;
-    l[i] = 0.f;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int r = wave * 16 * NT + i * 16 + col;
-    ctok[i] = min(r / G, nt);
-    const int t = t0 + (ctok[i] < nt ? ctok[i] : 0), pos = a.tok_pos[t];
-    cpos[i] = ctok[i] < nt && token_ok(a, a.tok_seq[t], pos) ? pos : -1;
+  for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  {
+    const int r = wave * 16 + col;
+    ctok = min(r / G, nt);
+    const int t = t0 + (ctok < nt ? ctok : 0), pos = a.tok_pos[t];
+    cpos = ctok < nt && token_ok(a, a.tok_seq[t], pos) ? pos : -1;
     const f16* qp = a.qkv + ((size_t)t * HH + kh * G + r % G) * D;
-    if (cpos[i] < 0) {
+    if (cpos < 0) {
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) q[i][kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      for (int kb = 0; kb < NKB; ++kb) q[kb] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
     } else if constexpr (Q8) {
-      load_rotated<D>(q[i], qp, a.rope_cos + (size_t)pos * (D / 2), a.rope_sin + (size_t)pos * (D / 2), g);
+      load_rotated<D>(q, qp, a.rope_cos + (size_t)pos * (D / 2), a.rope_sin + (size_t)pos * (D / 2), g);
     } else {
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) q[i][kb] = ld8(qp + kb * 32 + g * 8);
+      for (int kb = 0; kb < NKB; ++kb) q[kb] = ld8(qp + kb * 32 + g * 8);
     }
   }
 
-  if (Q8 && split == 0) {
-    // The own pages, unrounded: the tokens' keys and values by way of LDS
+  if (Q8 && __builtin_expect(split == 0, 1)) {
+    // The own pages, unrounded: the tokens' keys and values by way of LDS.  (Expected, or the compiler puts this behind the loop: 8 prompts of 456 tokens, all launches, 149 us for 147)
     f16* ok = lds;
     f16* ov = lds + 4 * NKB * KLD * 8;
 #pragma unroll
@@ -679,78 +678,75 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
       if (rr < nt) st8(ov + rr * VLD + c * 8, vx[i]);
     }
     __syncthreads();
+    const int t = t0 + (ctok < nt ? ctok : 0);
+    const int seq = a.tok_seq[t], own = cpos >= 0 ? cpos / PAGE : -1;
+    unsigned todo = (unsigned)(__ballot(cpos >= 0) & 0xffff);
+    while (todo) {                                                    // the pages of a tile's columns one behind the other
+      const int c = __builtin_ctz(todo);
+      const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(own, c), ps = __builtin_amdgcn_readlane(cpos, c);
+      const int row = __builtin_amdgcn_readlane(t, c), r0 = row - t0 - (ps - p * PAGE);       // where the page would begin among the workgroup's tokens
+      const bool in = own == p && seq == s && t - row == cpos - ps;        // (of the same run)
+      todo &= ~(unsigned)(__ballot(in) & 0xffff);
+      f32x4 st[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+      f16x4 v[NDB];
+      bool whole = r0 >= 0;                                           // uniform: no run begins behind its first token
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int t = t0 + (ctok[i] < nt ? ctok[i] : 0);
-      const int seq = a.tok_seq[t], own = cpos[i] >= 0 ? cpos[i] / PAGE : -1;
-      unsigned todo = (unsigned)(__ballot(cpos[i] >= 0) & 0xffff);
-      while (todo) {                                                  // the pages of a tile's columns one behind the other
-        const int c = __builtin_ctz(todo);
-        const int s = __builtin_amdgcn_readlane(seq, c), p = __builtin_amdgcn_readlane(own, c), ps = __builtin_amdgcn_readlane(cpos[i], c);
-        const int row = __builtin_amdgcn_readlane(t, c), r0 = row - t0 - (ps - p * PAGE);       // where the page would begin among the workgroup's tokens
-        const bool in = own == p && seq == s && t - row == cpos[i] - ps;        // (of the same run)
-        todo &= ~(unsigned)(__ballot(in) & 0xffff);
-        f32x4 st[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-        f16x4 v[NDB];
-        bool whole = r0 >= 0;                                         // uniform: no run begins behind its first token
+      for (int j = 0; j < NB; ++j) {
+        const int from = max(r0 + 1 - 64 * j, 0), to = row - t0 - 64 * j;     // of begins[j], bits from .. to
+        if (from <= to && from < 64 && (begins[j] >> from << from) & (to < 63 ? (2ull << to) - 1 : ~0ull)) whole = false;
+      }
+      if (whole) {
+        const int rk = min(r0 + col, QB - 1);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          const int from = max(r0 + 1 - 64 * j, 0), to = row - t0 - 64 * j;     // of begins[j], bits from .. to
-          if (from <= to && from < 64 && (begins[j] >> from << from) & (to < 63 ? (2ull << to) - 1 : ~0ull)) whole = false;
-        }
-        if (whole) {
-          const int rk = min(r0 + col, QB - 1);
-#pragma unroll
-          for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(ld8(ok + ((kb * 4 + g) * KLD + rk) * 8), q[i][kb], st[0]);
-#pragma unroll
-          for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[db][e] = ov[min(r0 + 4 * g + e, QB - 1) * VLD + db * 16 + col];
-        } else {                                                      // tokens ahead of the workgroup's, of the pass or of the tail
-          f16x8 vr[NKB];
-          const int mine = row_of(a, row, ps, s, p * PAGE + col);
-          load_own<D>(a, s, kh, mine, ps, false, vr);
-#pragma unroll
-          for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(vr[kb], q[i][kb], st[0]);
-          load_own<D>(a, s, kh, mine, ps, true, vr);
-          // rows to columns: the lane of (dim 16 db + col, token 4 g + e) asks lane (dim % 32 / 8, token)
-#pragma unroll
-          for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int from = (((db & 1) * 2 + (col >> 3)) << 4) + 4 * g + e;
-              union { f16x8 h; uint32_t u[4]; } x = {vr[db >> 1]};
-              uint32_t y[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) y[j] = __shfl(x.u[j], from, WAVE);
-              const uint32_t w = col & 4 ? (col & 2 ? y[3] : y[2]) : (col & 2 ? y[1] : y[0]);
-              union { uint16_t u; f16 h; } z = {(uint16_t)(col & 1 ? w >> 16 : w)};
-              v[db][e] = z.h;
-            }
-        }
-        uint32_t bad[1] = {0};                                        // tokens whose values are not finite: their scores are NaN where they are seen
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          bool not_finite = false;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) {
-            const bool y = !(fabsf((float)v[db][e]) <= 65504.f);
-            not_finite = not_finite || y;
-            if (y) v[db][e] = (f16)0.f;
-          }
-          const unsigned long long b = __ballot(not_finite);
-          if (b >> (16 * g) & 0xffff) bad[0] |= 1u << e;
-        }
-        const float by[1] = {a.scale}, one[1] = {1.f};
-        const int first[1] = {p * PAGE + 4 * g};
-        f16x2 hi[2], low[2];
-        tile_mask<1>(st, first, in ? cpos[i] + 1 : 0, in && a.window > 0 ? max(cpos[i] - a.window + 1, 0) : 0, a.sinks, bad, __any(bad[0]));
-        tile_weights<D, 1, false>(st, by, one, one, m[i], l[i], o[i], hi, low);
-        const f16x8 w = join(hi[0], hi[1], low[0], low[1]);
+        for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(ld8(ok + ((kb * 4 + g) * KLD + rk) * 8), q[kb], st[0]);
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
-          o[i][db] = mfma_16x16x32(f16x8{v[db][0], v[db][1], v[db][2], v[db][3], v[db][0], v[db][1], v[db][2], v[db][3]}, w, o[i][db]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[db][e] = ov[min(r0 + 4 * g + e, QB - 1) * VLD + db * 16 + col];
+      } else {                                                        // tokens ahead of the workgroup's, of the pass or of the tail
+        f16x8 vr[NKB];
+        const int mine = row_of(a, row, ps, s, p * PAGE + col);
+        load_own<D>(a, s, kh, mine, ps, false, vr);
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) st[0] = mfma_16x16x32(vr[kb], q[kb], st[0]);
+        load_own<D>(a, s, kh, mine, ps, true, vr);
+        // rows to columns: the lane of (dim 16 db + col, token 4 g + e) asks lane (dim % 32 / 8, token)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int from = (((db & 1) * 2 + (col >> 3)) << 4) + 4 * g + e;
+            union { f16x8 h; uint32_t u[4]; } x = {vr[db >> 1]};
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = __shfl(x.u[j], from, WAVE);
+            const uint32_t w = col & 4 ? (col & 2 ? y[3] : y[2]) : (col & 2 ? y[1] : y[0]);
+            union { uint16_t u; f16 h; } z = {(uint16_t)(col & 1 ? w >> 16 : w)};
+            v[db][e] = z.h;
+          }
       }
+      uint32_t bad[1] = {0};                                          // tokens whose values are not finite: their scores are NaN where they are seen
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        bool not_finite = false;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const bool y = !(fabsf((float)v[db][e]) <= 65504.f);
+          not_finite = not_finite || y;
+          if (y) v[db][e] = (f16)0.f;
+        }
+        const unsigned long long b = __ballot(not_finite);
+        if (b >> (16 * g) & 0xffff) bad[0] |= 1u << e;
+      }
+      const float by[1] = {a.scale}, one[1] = {1.f};
+      const int first[1] = {p * PAGE + 4 * g};
+      f16x2 hi[2], low[2];
+      tile_mask<1>(st, first, in ? cpos + 1 : 0, in && a.window > 0 ? max(cpos - a.window + 1, 0) : 0, a.sinks, bad, __any(bad[0]));
+      tile_weights<D, 1, false>(st, by, one, one, m, l, o, hi, low);
+      const f16x8 w = join(hi[0], hi[1], low[0], low[1]);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        o[db] = mfma_16x16x32(f16x8{v[db][0], v[db][1], v[db][2], v[db][3], v[db][0], v[db][1], v[db][2], v[db][3]}, w, o[db]);
     }
     __syncthreads();                                                  // (the ring begins)
   }
@@ -786,25 +782,18 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
       else return i < heads ? i : from + i - heads;
     };
     auto end_of = [&](int blk) { return Q8 && blk < head_blocks ? heads : end; };                               // where a block's pages end, at most four on
-    int lim[NT], lo[NT], least_lim[NT], most_lim[NT], least_lo[NT], most_lo[NT];
+    const bool in_run = ctok >= c0 && ctok < next && cpos >= 0;
+    const int lim = !in_run ? 0 : Q8 ? cpos / PAGE * PAGE : cpos + 1, lo = in_run && a.window > 0 ? max(cpos - a.window + 1, 0) : 0;
+    int ends[4] = {lim, lim, in_run ? lo : 0x7fffffff, lo};
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const bool in = ctok[i] >= c0 && ctok[i] < next && cpos[i] >= 0;
-      lim[i] = !in ? 0 : Q8 ? cpos[i] / PAGE * PAGE : cpos[i] + 1;
-      lo[i] = in && a.window > 0 ? max(cpos[i] - a.window + 1, 0) : 0;
-      int v[4] = {lim[i], lim[i], in ? lo[i] : 0x7fffffff, lo[i]};
-#pragma unroll
-      for (int s = 8; s > 0; s >>= 1) {
-        v[0] = min(v[0], __shfl_xor(v[0], s, WAVE));
-        v[1] = max(v[1], __shfl_xor(v[1], s, WAVE));
-        v[2] = min(v[2], __shfl_xor(v[2], s, WAVE));
-        v[3] = max(v[3], __shfl_xor(v[3], s, WAVE));
-      }
-      least_lim[i] = __builtin_amdgcn_readfirstlane(v[0]);
-      most_lim[i] = __builtin_amdgcn_readfirstlane(v[1]);
-      least_lo[i] = __builtin_amdgcn_readfirstlane(v[2]);
-      most_lo[i] = __builtin_amdgcn_readfirstlane(v[3]);
+    for (int s = 8; s > 0; s >>= 1) {
+      ends[0] = min(ends[0], __shfl_xor(ends[0], s, WAVE));
+      ends[1] = max(ends[1], __shfl_xor(ends[1], s, WAVE));
+      ends[2] = min(ends[2], __shfl_xor(ends[2], s, WAVE));
+      ends[3] = max(ends[3], __shfl_xor(ends[3], s, WAVE));
     }
+    const int least_lim = __builtin_amdgcn_readfirstlane(ends[0]), most_lim = __builtin_amdgcn_readfirstlane(ends[1]);
+    const int least_lo = __builtin_amdgcn_readfirstlane(ends[2]), most_lo = __builtin_amdgcn_readfirstlane(ends[3]);
     const int run_lim = Q8 ? pc / PAGE * PAGE : pc + 1, run_lo = a.window > 0 ? pe - a.window + 1 : 0;
 
     // of the four pages on their way: a lane's id (of page lane % 4), this wave's operands; then what the block needs beside its operands
@@ -821,7 +810,6 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
       for (int i = 0; i < NU; ++i) {
         const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
         const bool values = u / NL & 1;
-        if (8 * NL % NW != 0 && u >= 8 * NL) break;
         const int id = __builtin_amdgcn_readlane(ids, p);
         if constexpr (Q8) {
           const size_t at = ((size_t)(id < 0 ? 0 : id) * a.Hkv + kh) * PE;
@@ -867,8 +855,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
           const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
-          if (8 * NL % NW != 0 && u >= 8 * NL) break;
-          if (u / NL & 1) {                                           // uniform
+            if (u / NL & 1) {                                         // uniform
             const f16 x = (f16)__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mult), p));
             f16* to = lds + VB + buf * 4 * PE + ((p >> 1) * NDB * 64 + lane) * 8 + (p & 1) * 4 + 4 * j * 512;
             const uint32_t y[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
@@ -885,7 +872,7 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
           const int u = wave + i * NW, p = u / (2 * NL), j = u % NL;
-          if ((8 * NL % NW != 0 && u >= 8 * NL) || !(u / NL & 1)) continue;
+          if (!(u / NL & 1)) continue;
           uint32_t bad = 0;
           const int first = page_of(blk, p) * PAGE;
           if (!checked(blk)) break;                                   // uniform
@@ -921,23 +908,14 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
         if (unit_next != unit) {                                      // uniform
           const float f = power(max(unit - unit_next, -126));
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) o[i][db] *= f;
+          for (int db = 0; db < NDB; ++db) o[db] *= f;
           unit = unit_next;
         }
       }
-      const int first0 = page_of(blk, 0) * PAGE;                     // (of a block that has pages of both, with others between them, nobody sees all by these comparisons)
-      bool sees[NT], whole[NT];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        sees[i] = first0 < most_lim[i] && (first0 + 4 * PAGE > least_lo[i] || first0 < a.sinks);
-        whole[i] = there == 15 && first0 + 4 * PAGE <= least_lim[i] && (first0 >= most_lo[i] || first0 + 4 * PAGE <= a.sinks);
-      }
-      bool any = false;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) any = any || sees[i];
-      if (any) {                                                      // uniform over the wave
+      const int first0 = page_of(blk, 0) * PAGE;                      // (of a block that has pages of both, with others between them, nobody sees all by these comparisons)
+      const bool sees = first0 < most_lim && (first0 + 4 * PAGE > least_lo || first0 < a.sinks);
+      bool whole = there == 15 && first0 + 4 * PAGE <= least_lim && (first0 >= most_lo || first0 + 4 * PAGE <= a.sinks);
+      if (sees) {                                                     // uniform over the wave
         uint32_t bad[4];                                              // of the pages
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -952,53 +930,41 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
             bad[p] = __builtin_amdgcn_readfirstlane(x);
           }
         }
-        if (bad[0] | bad[1] | bad[2] | bad[3])
-#pragma unroll
-          for (int i = 0; i < NT; ++i) whole[i] = false;
+        if (bad[0] | bad[1] | bad[2] | bad[3]) whole = false;
         // Four products of scores.  8 bits: of a page each; a lane has tokens 4 g .. + 3, as its values lie.  fp16: two of a pair of pages, so that over both a lane has the
         // eight tokens that are 16 bytes of the values as they come, half g % 2 of page g / 2
-        f32x4 st[NT][4];
+        f32x4 st[4];
         const f16* kl = lds + buf * KB + (Q8 ? lane * 8 : (col >> 3) * (PE + KP) + (g * 16 + (col >> 2 & 1) * 8 + (col & 3)) * 8);
         auto keys = [&](int p, int kb) { return ld8(kl + (Q8 ? p * PE : (p >> 1) * (2 * PE + KP) + (p & 1) * 32) + kb * 512); };
-        constexpr int KR = NT == 1 ? 1 : 2;
-        f16x8 k[KR][NKB];                                             // a page's keys while those of the one before are multiplied
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) k[0][kb] = keys(0, kb);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          if (KR == 2 ? p < 3 : p > 0)
+          f16x8 k[NKB];
 #pragma unroll
-            for (int kb = 0; kb < NKB; ++kb) k[KR == 2 ? (p + 1) & 1 : 0][kb] = keys(KR == 2 ? p + 1 : p, kb);
+          for (int kb = 0; kb < NKB; ++kb) k[kb] = keys(p, kb);
+          st[p] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < NT; ++i) st[i][p] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-            for (int i = 0; i < NT; ++i) st[i][p] = mfma_16x16x32(k[p % KR][kb], q[i][kb], st[i][p]);
+          for (int kb = 0; kb < NKB; ++kb) st[p] = mfma_16x16x32(k[kb], q[kb], st[p]);
         }
-        f16x2 hi[NT][8], low[NT][8];
+        f16x2 hi[8], low[8];
+        if (!whole) {                                                 // uniform
+          int first[4], gm = g, lim_ = lim, lo_ = lo;
+          asm volatile("" : "+v"(gm), "+v"(lim_), "+v"(lo_));         // (or the comparisons are made ahead of the branch that seldom leads here)
+          uint32_t four[4];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if (!whole[i]) {                                            // uniform
-            int first[4], gm = g, lim_ = lim[i], lo_ = lo[i];
-            asm volatile("" : "+v"(gm), "+v"(lim_), "+v"(lo_));       // (or the comparisons are made ahead of the branch that seldom leads here)
-            uint32_t four[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              const int page = Q8 ? p : (p & 2) + (gm >> 1), in = Q8 ? 4 * gm : 8 * (gm & 1) + 4 * (p & 1);
-              first[p] = there >> page & 1 ? (Q8 ? first0 + page * PAGE : page_of(blk, page) * PAGE) + in : 0x3fffffff;
-              four[p] = (Q8 ? bad[p] : gm >> 1 ? bad[p | 1] : bad[p & 2]) >> in & 15;
-            }
-            tile_mask<4>(st[i], first, lim_, lo_, first0 < a.sinks ? a.sinks : 0, four, (bad[0] | bad[1] | bad[2] | bad[3]) != 0);
+          for (int p = 0; p < 4; ++p) {
+            const int page = Q8 ? p : (p & 2) + (gm >> 1), in = Q8 ? 4 * gm : 8 * (gm & 1) + 4 * (p & 1);
+            first[p] = there >> page & 1 ? (Q8 ? first0 + page * PAGE : page_of(blk, page) * PAGE) + in : 0x3fffffff;
+            four[p] = (Q8 ? bad[p] : gm >> 1 ? bad[p | 1] : bad[p & 2]) >> in & 15;
           }
-          tile_weights<D, 4, Q8>(st[i], by, up, share, m[i], l[i], o[i], hi[i], low[i]);
+          tile_mask<4>(st, first, lim_, lo_, first0 < a.sinks ? a.sinks : 0, four, (bad[0] | bad[1] | bad[2] | bad[3]) != 0);
         }
+        tile_weights<D, 4, Q8>(st, by, up, share, m, l, o, hi, low);
         const f16* vl = lds + VB + buf * 4 * PE + (Q8 ? lane * 8 : (g >> 1) * 512 + (g & 1) * 256 + col * 8);
         auto values = [&](int j) {                                    // of pair j / NDB, dims 16 (j % NDB) ..
           const int pair = j / NDB, db = j % NDB;
           return ld8(vl + (Q8 ? (pair * NDB + db) * 512 : pair * 2 * PE + (db >> 1) * 1024 + (db & 1) * 128));
         };
-        constexpr int AHEAD = NT == 1 ? 2 : 4;
+        constexpr int AHEAD = 2;
         f16x8 v[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) v[j] = values(j);
@@ -1007,12 +973,8 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
           const int pair = j / NDB, db = j % NDB;
           const f16x8 x = v[j % AHEAD];
           if (j + AHEAD < 2 * NDB) v[j % AHEAD] = values(j + AHEAD);
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-            o[i][db] = mfma_16x16x32(x, join(hi[i][4 * pair], hi[i][4 * pair + 1], hi[i][4 * pair + 2], hi[i][4 * pair + 3]), o[i][db]);
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-            o[i][db] = mfma_16x16x32(x, join(low[i][4 * pair], low[i][4 * pair + 1], low[i][4 * pair + 2], low[i][4 * pair + 3]), o[i][db]);
+          o[db] = mfma_16x16x32(x, join(hi[4 * pair], hi[4 * pair + 1], hi[4 * pair + 2], hi[4 * pair + 3]), o[db]);
+          o[db] = mfma_16x16x32(x, join(low[4 * pair], low[4 * pair + 1], low[4 * pair + 2], low[4 * pair + 3]), o[db]);
         }
       }
       if (blk + 1 < blk1) stage(buf ^ 1, blk + 1, ids_next);
@@ -1021,41 +983,38 @@ __global__ __launch_bounds__(NW* WAVE, NT == 1 ? 4 : 2) void page_prefill_kernel
     }
   }
 
-  // Results go by way of LDS, a tile of a wave at a time, so that lines are written whole (everybody is done with the ring: a barrier ends every block)
+  // Results go by way of LDS, a wave's tile, so that lines are written whole (everybody is done with the ring: a barrier ends every block)
   constexpr int OLD = D + 8;
   static_assert(NW * 16 * OLD <= (RING > OWN ? RING : OWN), "the tiles fit the ring");
   f16* mine = lds + wave * 16 * OLD;
   const float scale_up = power(unit);
+  l += __shfl_xor(l, 16, WAVE);
+  l += __shfl_xor(l, 32, WAVE);
+  if (a.splits > 1) {                                                 // uniform
+    if (ctok >= nt) return;
+    const int t = t0 + ctok, h = kh * G + (wave * 16 + col) % G;
+    const size_t at = ((size_t)t * a.Hq + h) * a.splits + split;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    l[i] += __shfl_xor(l[i], 16, WAVE);
-    l[i] += __shfl_xor(l[i], 32, WAVE);
-    if (a.splits > 1) {                                               // uniform
-      if (ctok[i] >= nt) continue;
-      const int t = t0 + ctok[i], h = kh * G + (wave * 16 * NT + i * 16 + col) % G;
-      const size_t at = ((size_t)t * a.Hq + h) * a.splits + split;
+    for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(a.acc + at * D + db * 16 + 4 * g) = o[db] * scale_up;
+    if (g == 0) *reinterpret_cast<f32x2*>(a.ml + 2 * at) = f32x2{m, l};
+    return;
+  }
+  const float f = l == 0.f ? 0.f : scale_up / l;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(a.acc + at * D + db * 16 + 4 * g) = o[i][db] * scale_up;
-      if (g == 0) *reinterpret_cast<f32x2*>(a.ml + 2 * at) = f32x2{m[i], l[i]};
-      continue;
-    }
-    const float f = l[i] == 0.f ? 0.f : scale_up / l[i];
+  for (int db = 0; db < NDB; ++db) {
+    f16x4 x;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) {
-      f16x4 x;
+    for (int e = 0; e < 4; ++e) x[e] = (f16)(l == 0.f ? 0.f : o[db][e] * f);
+    *reinterpret_cast<f16x4*>(mine + col * OLD + db * 16 + 4 * g) = x;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (f16)(l[i] == 0.f ? 0.f : o[i][db][e] * f);
-      *reinterpret_cast<f16x4*>(mine + col * OLD + db * 16 + 4 * g) = x;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const int e = j * WAVE + lane, rr = e / (D / 8), c = e % (D / 8), r = wave * 16 * NT + i * 16 + rr, tok = r / G, d = (kh * G + r % G) * D + c * 8;
-      const f16x8 x = ld8(mine + rr * OLD + c * 8);
-      if (tok < nt) st8(a.out + (a.frag_tt ? frag_offset(t0 + tok, d, a.frag_tt) : (size_t)(t0 + tok) * a.Hq * D + d), x);
-    }
+  for (int j = 0; j < D / 32; ++j) {
+    const int e = j * WAVE + lane, rr = e / (D / 8), c = e % (D / 8), row = wave * 16 + rr, tok = row / G, d = (kh * G + row % G) * D + c * 8;
+    const f16x8 x = ld8(mine + rr * OLD + c * 8);
+    if (tok < nt) st8(a.out + (a.frag_tt ? frag_offset(t0 + tok, d, a.frag_tt) : (size_t)(t0 + tok) * a.Hq * D + d), x);
   }
 }
 
@@ -1247,12 +1206,12 @@ int decode(const PageAttn& a, hipStream_t s) {
 
 // Eight waves of one tile: four waves on a SIMD.  (Us at the time, so / four waves of two tiles, whose registers leave two: 8 prompts of 456 115 / 128, 777 tokens behind 3500
 // 136 / 165, 4096 tokens under a window of 1024 in fp16 185 / 179)
-constexpr int PREFILL_TILES = 1, PREFILL_WAVES = 8, PREFILL_ROWS = 16 * PREFILL_TILES * PREFILL_WAVES;
+constexpr int PREFILL_WAVES = 8, PREFILL_ROWS = 16 * PREFILL_WAVES;
 
 template <int D, bool Q8>
 int launch_prefill(const PageAttn& a, hipStream_t s) {
   const int G = a.Hq / a.Hkv;
-  hipLaunchKernelGGL((page_prefill_kernel<D, Q8, PREFILL_TILES, PREFILL_WAVES>), dim3(a.Hkv, ceil_div(a.T, PREFILL_ROWS / G), a.splits), dim3(PREFILL_WAVES * WAVE), 0, s, a);
+  hipLaunchKernelGGL((page_prefill_kernel<D, Q8, PREFILL_WAVES>), dim3(a.Hkv, ceil_div(a.T, PREFILL_ROWS / G), a.splits), dim3(PREFILL_WAVES * WAVE), 0, s, a);
   if (int e = mlora_launch_status("page_attn_prefill")) return e;
   if (a.splits == 1) return MLORA_OK;
   hipLaunchKernelGGL(page_join_kernel<D>, dim3(ceil_div(a.Hq, 4), a.T), dim3(4 * WAVE), 0, s, a);
