@@ -214,3 +214,125 @@ def test_together_on_a_4_bit_model_that_shares_prefixes():
         kv.end_forward()
     _, paths = one_type_search(model, kv, order, torch.cat([z[i] for i in order]), model._ids(3, {0: (None, [1, 1, 1])})[0], 3, 23)
     assert [got[i] for i in order] == [p[0] for p in paths]
+
+
+def searched(ds, model, kv, prompts, W, steps, **kw):
+    z = torch.cat([begin(model, kv, i, p) for i, p in enumerate(prompts)])
+    return ds.BeamSession(model, kv, range(len(prompts)), {}, z, W, steps=steps, **kw)
+
+
+@pytest.mark.parametrize("form", [{}, {"bits": 8, "window": 40, "sinks": 2}])
+def test_searches_whose_prompts_ran_at_once(two_types, form):
+    """The front end with batch_prefill, against a search behind the same pass over all prompts."""
+    model, W, limit = two_types, 3, 20
+    prompts, wids = prompts_of(model, (60, 20, 45), 41), [0, 2, 0]
+    config = {"cache_bits": form.get("bits", 16), "window": form.get("window"), "sinks": form.get("sinks", 0)}
+    got, b = front_end(model, prompts, wids, [limit] * 3, beams=W, batch_prefill=True, **config)
+    order = b.seq_info.order_seqs([0, 1, 2])[0]
+    kv = model.create_paged_kv_cache(2 * 3 * W, 2 * 3 * W * 112, 64, 16, max_seq_len=88, **form)
+    lens = [len(p) for p in prompts]
+    for i in range(3):
+        kv.add_sequence(i)
+    kv.begin_forward([0, 1, 2], lens)
+    ids = model._ids(sum(lens), {0: (None, np.repeat(np.array(wids, np.int32), lens))})
+    z = model.forward(model.embed(torch.from_numpy(np.concatenate(prompts))), kv, ids, model._last_rows(kv))
+    kv.end_forward()
+    _, paths = one_type_search(model, kv, order, z[torch.tensor(order, device=DEV)], model._ids(3, {0: (None, [wids[i] for i in order])})[0], W, limit - 1)
+    assert [got[i] for i in order] == [p[0] for p in paths]
+
+
+@pytest.mark.parametrize("form", [{}, {"bits": 8}, {"window": 40, "sinks": 2}])
+@pytest.mark.parametrize("graph", [False, True])
+def test_searches_on_another_stream_and_again(two_types, form, graph):
+    """On a stream of their own, with the default stream's passes and closed searches in between: the same answers."""
+    model, steps, W = two_types, 36, 4
+    ds = load_pkg("decode_session")
+    prompts = prompts_of(model, (47, 30), 43)
+    make = lambda: model.create_paged_kv_cache(10, 10 * 112, 64, 16, max_seq_len=112, **form)                              # noqa: E731
+    s = searched(ds, model, make(), prompts, W, steps)
+    for _ in range(steps):
+        s.step()
+    want = s.answers()
+    side, kv = torch.cuda.Stream(), make()
+    for again in range(2):
+        with torch.cuda.stream(side):
+            s = searched(ds, model, kv, prompts, W, steps, use_graph=graph)
+        for j in range(steps):
+            with torch.cuda.stream(side):
+                s.step()
+            if j % 9 == 4:
+                begin(model, kv, "x", prompts[1][:20 + j])
+            if j % 9 == 7:
+                kv.free_sequence("x")
+        with torch.cuda.stream(side):
+            got = s.answers()
+        assert got == want, again
+        s.close()
+        for i in (0, 1):
+            kv.free_sequence(i)
+    assert sorted(kv.free) == list(range(kv.n_pages)) and not kv._owners
+
+
+def test_a_step_that_fails_on_the_device_s_side(two_types, monkeypatch):
+    """Behind the reordering's launch: the rows are read back, the forks go, and the cache serves the next search as a new one does."""
+    model, steps, W = two_types, 20, 4
+    ds, ops = load_pkg("decode_session"), load_pkg("ops")
+    prompts = prompts_of(model, (47, 30), 45)
+    answers = []
+    for broken in (True, False):
+        kv = model.create_paged_kv_cache(10, 10 * 112, 64, 16, max_seq_len=112)
+        if broken:
+            s = searched(ds, model, kv, prompts, W, steps)
+            for _ in range(5):
+                s.step()
+
+            def refuse(*a):
+                raise RuntimeError("refused")
+
+            with monkeypatch.context() as m:
+                m.setattr(ops, "copy_pages", refuse)
+                with pytest.raises(RuntimeError, match="refused"):
+                    s.step()
+            with pytest.raises(RuntimeError):
+                s.step()
+            s.close()
+            table = kv.block_table[torch.tensor(kv.rows_of([0, 1]), device=DEV).long()].cpu().numpy()
+            assert (table == kv.table_h[kv.rows_of([0, 1])]).all()
+            for i in (0, 1):
+                kv.free_sequence(i)
+            assert sorted(kv.free) == list(range(kv.n_pages)) and not kv._owners
+        s = searched(ds, model, kv, prompts, W, steps)
+        for _ in range(steps):
+            s.step()
+        answers.append(s.answers())
+    assert answers[0] == answers[1]
+
+
+def test_requests_whose_numbers_are_gone(two_types):
+    """Logits that are NaN, or infinite in every row: no beams, no answer, and the other request's is its own."""
+    model, steps = two_types, 12
+    ds = load_pkg("decode_session")
+    prompts = prompts_of(model, (47, 30, 12), 47)
+    make = lambda: model.create_paged_kv_cache(12, 12 * 112, 64, 16, max_seq_len=112)                                      # noqa: E731
+    s = searched(ds, model, make(), prompts[:1], 3, steps, eos=5)
+    for _ in range(steps):
+        s.step()
+    want = s.answers()
+    kv = make()
+    z = torch.cat([begin(model, kv, i, p) for i, p in enumerate(prompts)])
+    z[1], z[2, 77] = torch.nan, torch.inf
+    for graph in (False, True):
+        kv2 = make()
+        for i, p in enumerate(prompts):
+            begin(model, kv2, i, p)
+        s = ds.BeamSession(model, kv2, range(3), {}, z, 3, eos=5, steps=steps, use_graph=graph)
+        for _ in range(steps):
+            s.step()
+        assert not s.done()
+        got = s.answers()
+        assert [t for _, t in got[0]] == [t for _, t in want[0]] and got[1:] == [[], []]
+        s.close()
+        assert sorted(kv2.slot) == [0, 1, 2]
+    s = ds.BeamSession(model, kv, [1, 2], {}, z[1:], 3)
+    s.step()
+    assert s.done()

@@ -452,3 +452,26 @@ def test_a_sequence_is_searched_once(on_cpu, W):
             on_cpu.BeamSession(model, kv, ids, {}, model.table[:len(ids)], W)
         assert list(kv.slot) == [0, 1]
     sound(kv)
+
+
+@pytest.mark.parametrize("sinks", [0, 1, 16, 33])
+@pytest.mark.parametrize("window", [1, 15, 16, 17, 30, 33, 48])
+def test_the_front_end_s_cache_has_room_for_its_searches(served, window, sinks):
+    """The pool is sized for what is seen, not for what is written: no search runs out of it, whatever its prompts' lengths."""
+    for lens, limit, beams in (((64, 63, 1), 200, 4), ((33, 48), 90, 3), ((17,), 150, 16)):
+        ab, xg, made = load_pkg("auto_batcher"), load_pkg("llama_exec_graph"), []
+        b = ab.LlamaAutoBatcherClass()
+        vm = Served(None)
+
+        def create(n, total, chunk, page, free_pages, max_seq_len, **form):
+            made.append(cache(-(-total // page) + n, n, -(-max_seq_len // page), **form))
+            return made[-1]
+
+        vm["create_paged_kv_cache"] = create
+        b.set_model(vm)
+        b.set_exec_config(xg.LlamaExecConfig(max_prompt_len=64, max_gen_len=limit, page_size=16, native_decode=False, window=window, sinks=sinks, beams=beams))
+        out = [b.generate(b.create_var(np.arange(n, dtype=np.int32) % 50)) for n in lens]
+        b.compile()
+        b.execute()
+        assert [len(o.var) for o in out] == [limit] * len(lens)
+        sound(made[-1])
