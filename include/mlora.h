@@ -432,7 +432,8 @@ int mlora_paged_attn_decode_shared(void* out, int out_layout, const void* qkv, c
  * is rounded once, when its 16 tokens are there: step = fp32(a / 127), c = rint(127 x / a) (ties to even), a = the largest magnitude; a = 0: codes 0; where it holds an
  * infinity or NaN: codes 0 and a step that is NaN.  tail_k, tail_v [n_seq, ...]: a page of each sequence in the layouts of fp16 pages, which holds the tokens of the
  * sequence's last page unrounded.  Every slot may hold anything ahead of its first use.
- * A token at position p sees positions j <= p, with window > 0 only those with j > p - window or j < sinks; of pages of 8 bits, its own page unrounded.
+ * A token at position p sees positions j <= p, with window > 0 only those with j > p - window or j < sinks (positions, and with them rotations, are the text's); of pages of 8 bits, its own page
+ * unrounded.
  * Pages that nobody sees need not be there (ids outside [0, n_pages) are not seen either), and what nobody sees may be infinite or NaN.  A sequence or position that is out of
  * range sees nothing (the result is 0) and is not stored.
  *

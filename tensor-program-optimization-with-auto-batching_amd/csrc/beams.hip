@@ -134,7 +134,7 @@ __global__ __launch_bounds__(4 * WAVE) void beam_scan_kernel(Best* __restrict__ 
 }
 
 // A request, of which a wave each merges a beam's parts.  A candidate's place is then the number of those ahead of it: in its own beam the lanes before, for they
-// are in order, and in the others, whose values fall, by halving.  9 us for 64 requests of 8 beams, 6 for one of 4 (17 and 9 with four waves a request that take out the
+// are in order, and in the others, whose values fall, by halving.  8.5 us for 64 requests of 8 beams, 5.6 for one of 4 (17 and 9 with four waves a request that take out the
 // greatest k times): bound by steps that wait for one another, most of them the merge's.
 __global__ __launch_bounds__(MAX_BEAMS* WAVE) void beam_join_kernel(float* __restrict__ out_scores, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
                                                                     const Best* __restrict__ best, const f32x2* __restrict__ sums, const float* __restrict__ scores,

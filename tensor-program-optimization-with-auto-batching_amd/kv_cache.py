@@ -380,7 +380,7 @@ class PagedKVCache(PageTable):
                  device="cuda:0", free_pages=None, page_size=PAGE, n_q_heads=None, bits=16, window=None, sinks=0):
         """n_q_heads: of the model that reads the cache; without them decode steps read shared pages for each sequence anew.
         bits: 8 holds every page that is complete in 8 bits, at a step per page and head (ops.QuantPages), in little more than half the memory.
-        window: a token sees only the last so many, itself among them, and the first `sinks`; pages in between go back to the pool.
+        window: a token sees only the last so many, itself among them, and the first `sinks`; pages in between go back to the pool.  Positions stay those of the text.
         A cache of either kind is read by operators of its own, one launch a layer and step (`plain` is false)."""
         super().__init__(n_pages, max_seqs, max_blocks, max_pos, device, free_pages, page_size)
         if bits not in (8, 16):

@@ -48,12 +48,16 @@ class LlamaExecConfig:
     # their requests share once, where that pays; a batch for which it does runs through the recorded per-operator step.  Shorter
     # prefills take other kernels and summation orders, so a token can differ at a near tie.
     share_prefix: bool = False
-    # The paged cache in 8 bits (of every page that is complete, at a step per page and head) instead of 16, in little more than half the memory.
+    # The paged cache in 8 bits (of every page that is complete, at a step per page and head) instead of 16, in little more than half the memory.  It has no
+    # native step; its steps are faster where the cache is what they read (32 kv heads, 32 rows of 2060 tokens, us a layer: 203 for 321), and up to 9 % slower for short rows
+    # with adapters of few kv heads.
     cache_bits: int = 16
-    # A sliding window: a token sees only the last so many, itself among them, and the first `sinks`.  The cache is sized for what is seen.
+    # A sliding window: a token sees only the last so many, itself among them, and the first `sinks`, which keep their places in the text.  The cache is sized
+    # for what is seen.
     window: int | None = None
     sinks: int = 0
-    # Beam search instead of greedy decoding: the answer is the best of so many beams by the sum of its tokens' log-probabilities.
+    # Beam search instead of greedy decoding: the answer is the best of so many beams by the sum of its tokens' log-probabilities (empty where logits that are no
+    # numbers leave a request none).
     beams: int = 1
 
 
