@@ -336,3 +336,35 @@ def test_requests_whose_numbers_are_gone(two_types):
     s = ds.BeamSession(model, kv, [1, 2], {}, z[1:], 3)
     s.step()
     assert s.done()
+
+
+@pytest.mark.parametrize("form", [{}, {"bits": 8}, {"window": 24, "sinks": 1}])
+def test_wide_searches(two_types, form):
+    """96 rows, for which a step takes its forms for wide batches: requests of 16 beams, with adapters."""
+    model, W, steps = two_types, 16, 18
+    ds = load_pkg("decode_session")
+    prompts, wids = prompts_of(model, (40, 31, 3, 25, 16, 64), 51), [0, 1, 2, 3, 0, 1]
+
+    def prefilled():
+        kv = model.create_paged_kv_cache(2 * 6 * W, 2 * 6 * W * 112, 64, 16, max_seq_len=112, **form)
+        z = []
+        for i, (p, w) in enumerate(zip(prompts, wids)):
+            kv.add_sequence(i)
+            kv.begin_forward([i], [len(p)])
+            z.append(model["prefill_a0"](model.embed(torch.from_numpy(p)), kv, [w])[0])
+            kv.end_forward()
+        return kv, torch.cat(z)
+
+    ids = model._ids(6, {0: (None, wids)})
+    kv, z = prefilled()
+    scores, paths = one_type_search(model, kv, range(6), z, ids[0], W, steps)
+    for graph in (False, True):
+        kv, z = prefilled()
+        s = ds.BeamSession(model, kv, range(6), ids, z, W, steps=steps, use_graph=graph)
+        for _ in range(steps):
+            s.step()
+        alike(model, s.answers(), scores, paths, steps)
+        s.close()
+        for i in range(6):
+            kv.free_sequence(i)
+        assert sorted(kv.free) == list(range(kv.n_pages)) and not kv._owners
